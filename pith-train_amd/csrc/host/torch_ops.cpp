@@ -1122,6 +1122,8 @@ TORCH_LIBRARY_IMPL(pithtrain_amd, Autograd, m) {
   m.impl("mla_assemble_bwd", &BackwardOp<&mla_assemble_bwd>::call<kMlaAssembleBwd>);
 }
 
+#include "latent_ops.h"
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   TORCH_CHECK(pith_version() == PITH_VERSION, "_pith_torch.so was built for interface version ", PITH_VERSION, " of libpith_hip.so, found ",
               pith_version(), ": build both again");

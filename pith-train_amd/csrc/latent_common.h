@@ -1,0 +1,65 @@
+// What the kernels of the latent cache (include/pith_latent.h) share.
+#pragma once
+
+#include "pith_common.h"
+#include "pith_latent.h"
+
+namespace pith {
+
+constexpr int kLatent = PITH_LATENT_DIM, kRope = PITH_LATENT_ROPE_DIM, kNope = PITH_LATENT_NOPE_DIM, kValue = PITH_LATENT_VALUE_DIM;
+constexpr float kFp8Max = 448.f;
+
+struct LatentCache {
+  char* latent;
+  __bf16* k_pe;
+  float* scale;
+  int64_t latent_ps, k_pe_ps, scale_ps;  // latent_ps in bytes, the others in elements
+  int pages, page_shift;
+};
+
+inline LatentCache to_device(const pith_latent_cache& c) {
+  LatentCache d = {};
+  d.latent = (char*)c.latent;
+  d.k_pe = (__bf16*)c.k_pe;
+  d.scale = c.scale;
+  d.latent_ps = c.latent_ps * (c.dtype == PITH_FP8_E4M3 ? 1 : 2);
+  d.k_pe_ps = c.k_pe_ps;
+  d.scale_ps = c.scale_ps;
+  d.pages = (int)c.pages;
+  d.page_shift = __builtin_ctzll((unsigned long long)c.page_size);
+  return d;
+}
+
+inline int check_cache(const pith_latent_cache& c, const char* who) {
+  if (c.dtype != PITH_BF16 && c.dtype != PITH_FP8_E4M3) return fail(PITH_ERR_BAD_DTYPE, "%s: cache dtype %d is neither bf16 nor e4m3", who, c.dtype);
+  const bool fp8 = c.dtype == PITH_FP8_E4M3;
+  if (!c.latent || !c.k_pe || (fp8 && !c.scale)) return fail(PITH_ERR_NULL_POINTER, "%s: a cache pointer is NULL", who);
+  if (c.page_size < 16 || c.page_size > 65536 || (c.page_size & (c.page_size - 1)))
+    return fail(PITH_ERR_BAD_SHAPE, "%s: page size %lld is not a power of two from 16 to 65536", who, (long long)c.page_size);
+  if (c.pages < 1 || c.pages > ((int64_t)1 << 31) / c.page_size - 1)
+    return fail(PITH_ERR_BAD_SHAPE, "%s: %lld pages of %lld rows: at least one, and fewer than 2^31 rows", who, (long long)c.pages, (long long)c.page_size);
+  if (c.latent_ps < c.page_size * kLatent || c.k_pe_ps < c.page_size * kRope || (fp8 && c.scale_ps < c.page_size))
+    return fail(PITH_ERR_BAD_SHAPE, "%s: a page stride is shorter than a page", who);
+  if (!aligned16(c.latent) || !aligned16(c.k_pe) || c.latent_ps % (fp8 ? 16 : 8) || c.k_pe_ps % 8 || (fp8 && (uintptr_t)c.scale % 4))
+    return fail(PITH_ERR_MISALIGNED, "%s: the cache breaks the 16-byte alignment", who);
+  return PITH_OK;
+}
+
+// Page number of a table entry, kept inside the cache.
+__device__ __forceinline__ int safe_page(int page, int pages) { return min(max(page, 0), pages - 1); }
+
+// Two e4m3 values (the low or the high half of `word`) -> two bf16, exact.
+template <bool HIGH>
+__device__ __forceinline__ bf16x2 fp8x2_to_bf16(uint32_t word) {
+  return __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(word, 1.0f, HIGH);
+}
+
+// Rotated pair j (0..31) of a rotary vector whose interleaved elements 2j, 2j+1 are `pair` (bf16 x 2): features j and 32 + j of the result.
+__device__ __forceinline__ void rotate_pair(uint32_t pair, const __bf16* cos_row, const __bf16* sin_row, int j, float& first, float& second) {
+  const float even = bf16lo_to_f32(pair), odd = bf16hi_to_f32(pair);
+  first = even * (float)cos_row[j] - odd * (float)sin_row[j];
+  second = odd * (float)cos_row[kRope / 2 + j] + even * (float)sin_row[kRope / 2 + j];
+}
+__device__ __forceinline__ int64_t clamped_position(int64_t pos, int64_t P) { return pos < 0 ? 0 : (pos >= P ? P - 1 : pos); }
+
+}  // namespace pith

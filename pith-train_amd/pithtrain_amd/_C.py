@@ -1,4 +1,4 @@
-"""ctypes binding of libpith_hip.so (declarations in include/pith_hip.h).
+"""ctypes binding of libpith_hip.so (declarations in include/pith_hip.h and include/pith_latent.h).
 
 There is no fallback: if the library has not been built, or a call returns an error code, an
 exception is raised. PyTorch is used only for device memory and streams; every tensor argument
@@ -14,8 +14,9 @@ import torch
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "lib", "libpith_hip.so")
 
 PITH_VERSION = 202  # of include/pith_hip.h, whose structs are declared below
+PITH_LATENT_VERSION = 100  # of include/pith_latent.h
 
-PITH_BF16, PITH_F32 = 0, 1
+PITH_BF16, PITH_F32, PITH_FP8_E4M3 = 0, 1, 2
 PITH_BASE_2, PITH_BASE_E = 0, 1
 
 PITH_OK = 0
@@ -131,6 +132,45 @@ class DeviceInfo(Structure):
     ]  # fmt: skip
 
 
+class LatentCacheArgs(Structure):
+    _fields_ = [
+        ("latent", c_void_p), ("k_pe", c_void_p), ("scale", c_void_p), ("pages", c_int64), ("page_size", c_int64),
+        ("latent_ps", c_int64), ("k_pe_ps", c_int64), ("scale_ps", c_int64), ("dtype", c_int32), ("reserved0", c_int32),
+    ]  # fmt: skip
+
+
+class LatentAppendArgs(Structure):
+    _fields_ = [
+        ("kv_a", c_void_p), ("weight", c_void_p), ("cos", c_void_p), ("sin", c_void_p), ("position_ids", c_void_p), ("slots", c_void_p),
+        ("T", c_int64), ("P", c_int64), ("kv_a_rs", c_int64), ("eps", c_float), ("weight_dtype", c_int32), ("cache", LatentCacheArgs),
+    ]  # fmt: skip
+
+
+class LatentGatherArgs(Structure):
+    _fields_ = [
+        ("cache", LatentCacheArgs), ("page_table", c_void_p), ("cu_rows", c_void_p), ("latent_out", c_void_p), ("k_pe_out", c_void_p),
+        ("B", c_int64), ("rows", c_int64), ("table_rs", c_int64), ("table_width", c_int64), ("latent_rs", c_int64), ("k_pe_rs", c_int64),
+    ]  # fmt: skip
+
+
+class LatentAbsorbArgs(Structure):
+    _fields_ = [
+        ("x", c_void_p), ("weight", c_void_p), ("out", c_void_p), ("q_pe", c_void_p), ("cos", c_void_p), ("sin", c_void_p),
+        ("position_ids", c_void_p), ("T", c_int64), ("H", c_int64), ("P", c_int64), ("x_ts", c_int64), ("x_hs", c_int64),
+        ("out_ts", c_int64), ("out_hs", c_int64), ("q_pe_ts", c_int64), ("q_pe_hs", c_int64),
+    ]  # fmt: skip
+
+
+class LatentAttnArgs(Structure):
+    _fields_ = [
+        ("q_latent", c_void_p), ("q_pe", c_void_p), ("cache", LatentCacheArgs), ("page_table", c_void_p), ("lengths", c_void_p), ("cu_q", c_void_p),
+        ("tree_mask", c_void_p), ("o", c_void_p), ("lse", c_void_p), ("workspace", c_void_p), ("workspace_bytes", c_int64),
+        ("T", c_int64), ("B", c_int64), ("H", c_int64), ("table_rs", c_int64), ("table_width", c_int64),
+        ("q_ts", c_int64), ("q_hs", c_int64), ("q_pe_ts", c_int64), ("q_pe_hs", c_int64), ("o_ts", c_int64), ("o_hs", c_int64), ("lse_hs", c_int64),
+        ("scale", c_float), ("reserved0", c_int32),
+    ]  # fmt: skip
+
+
 # name -> (restype, argtypes); must list every symbol declared in include/pith_hip.h
 SYMBOLS = {
     "pith_version": (c_int, []),
@@ -164,6 +204,17 @@ SYMBOLS = {
     "pith_mla_assemble_bwd": (c_int, [POINTER(MlaAssembleArgs), c_void_p]),
 }
 
+# the same for include/pith_latent.h
+LATENT_SYMBOLS = {
+    "pith_latent_version": (c_int, []),
+    "pith_latent_append": (c_int, [POINTER(LatentAppendArgs), c_void_p]),
+    "pith_latent_gather": (c_int, [POINTER(LatentGatherArgs), c_void_p]),
+    "pith_latent_absorb_query": (c_int, [POINTER(LatentAbsorbArgs), c_void_p]),
+    "pith_latent_absorb_value": (c_int, [POINTER(LatentAbsorbArgs), c_void_p]),
+    "pith_latent_attn_workspace_bytes": (c_int64, [POINTER(LatentAttnArgs)]),
+    "pith_latent_attn": (c_int, [POINTER(LatentAttnArgs), c_void_p]),
+}
+
 _lib = None
 
 
@@ -177,12 +228,14 @@ def lib() -> ctypes.CDLL:
                 "(there is no non-HIP fallback for these operators)"
             )
         handle = ctypes.CDLL(LIB_PATH)
-        for name, (restype, argtypes) in SYMBOLS.items():
+        for name, (restype, argtypes) in {**SYMBOLS, **LATENT_SYMBOLS}.items():
             fn = getattr(handle, name)
             fn.restype = restype
             fn.argtypes = argtypes
         if handle.pith_version() != PITH_VERSION:
             raise ImportError(f"{LIB_PATH} has interface version {handle.pith_version()}, this package needs {PITH_VERSION}: build it again")
+        if handle.pith_latent_version() != PITH_LATENT_VERSION:
+            raise ImportError(f"{LIB_PATH} has latent interface version {handle.pith_latent_version()}, this package needs {PITH_LATENT_VERSION}: build it again")
         _lib = handle
     return _lib
 
@@ -247,5 +300,6 @@ def bhs_strides(t: torch.Tensor, what: str):
 
 __all__ = [
     "lib", "check", "PithError", "CombineArgs", "AttnFwdArgs", "KeyChunk", "AttnDeltaArgs", "AttnBwdArgs", "AttnBwdPlan", "NormRopeArgs", "MlaAssembleArgs", "DeviceInfo", "SYMBOLS",
+    "LatentCacheArgs", "LatentAppendArgs", "LatentGatherArgs", "LatentAbsorbArgs", "LatentAttnArgs", "LATENT_SYMBOLS",
     "dtype_code", "current_stream", "require_device", "bshd_batch_stride", "bshd_head_range_strides", "bhs_strides", "byref",
 ]  # fmt: skip

@@ -503,6 +503,17 @@ class MLA(nn.Module):
         o, _ = _attn_fwd_op(q, k, v, self.softmax_scale, True)
         return o
 
+    def decode(self, q, kv_a, norm_weight, kv_b_weight, cos, sin, position_ids, slots, cache, page_table, lengths, cu_q,
+               eps: float = 1e-6, tree_mask: torch.Tensor = None) -> torch.Tensor:  # fmt: skip
+        """The same attention for new tokens of sequences whose earlier ones lie in a latent cache (absorbed form, one or a few tokens a
+        sequence): o [T, h, dv] of q [T, h, dq] and kv_a [T, 576]. Arguments as in pithtrain_amd.operators.mla.latent.latent_decode."""
+        from pithtrain_amd.operators.mla.latent import latent_decode
+
+        assert (self.dq, self.dv) == (192, 128), f"the latent cache goes with dq=192 and dv=128, got dq={self.dq} and dv={self.dv}"
+        assert q.dim() == 3 and tuple(q.shape[1:]) == (self.h, self.dq), f"q must be [tokens, {self.h}, {self.dq}], got {list(q.shape)}"
+        return latent_decode(q, kv_a, norm_weight, kv_b_weight, cos, sin, position_ids, slots, cache, page_table, lengths, cu_q,
+                             self.softmax_scale, eps, tree_mask)  # fmt: skip
+
 
 __all__ = [
     "MLA", "attention_func", "_mla_fwd", "_mla_bwd_preprocess", "_mla_bwd_dk_dv", "_mla_bwd_dq",
