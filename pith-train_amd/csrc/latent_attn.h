@@ -1,7 +1,7 @@
 // Attention to the latent cache: what its kernels share. The work list, the tiles and the join.
 //
 // Work list. A sequence of n new tokens and L rows is ceil(n H / M) row blocks (row = token * H + head; M of them share a workgroup's tiles) times
-// ceil(L / 32) tiles of 32 keys, and the tiles of all row blocks of all sequences, one behind the other, are dealt to the workgroups in equal
+// ceil(L / 64) tiles of 64 keys, and the tiles of all row blocks of all sequences, one behind the other, are dealt to the workgroups in equal
 // ranges. Lengths are read on the device, so nothing depends on the host knowing them: a captured call follows its sequences as they grow, and one
 // long sequence among short ones is spread over as many workgroups as its share of the tiles. A workgroup whose range covers a row block wholly
 // writes its rows; parts of a row block leave (sum, maximum, unnormalised result) in fp32 in the workspace, and a second kernel joins them in the
@@ -13,7 +13,7 @@
 
 namespace pith {
 
-constexpr int kLatentKeys = 32;  // keys of a tile
+constexpr int kLatentKeys = 64;  // keys of a tile
 
 // load_lds16 from an address of each lane's own.
 __device__ __forceinline__ void load_lds16_at(const void* src, char* dst_wave) {
