@@ -1,11 +1,13 @@
 // Attention to the latent cache: what its kernels share. The work list, the tiles and the join.
 //
-// Work list. A sequence of n new tokens and L rows is ceil(n H / M) row blocks (row = token * H + head; M of them share a workgroup's tiles) times
-// ceil(L / 64) tiles of 64 keys, and the tiles of all row blocks of all sequences, one behind the other, are dealt to the workgroups in equal
-// ranges. Lengths are read on the device, so nothing depends on the host knowing them: a captured call follows its sequences as they grow, and one
-// long sequence among short ones is spread over as many workgroups as its share of the tiles. A workgroup whose range covers a row block wholly
-// writes its rows; parts of a row block leave (sum, maximum, unnormalised result) in fp32 in the workspace, and a second kernel joins them in the
-// order of the keys (results do not depend on scheduling).
+// Work list. A sequence of n new tokens and L rows is R = ceil(n H / M) row blocks of M rows (row = token * H + head) times
+// N = ceil(L / K) tiles of K keys, and the R N tiles of all sequences, one sequence behind the other, are dealt to the workgroups in equal ranges.
+// Lengths are read on the device, so nothing depends on the host knowing them: a captured call follows its sequences as they grow, and one long
+// sequence among short ones is spread over as many workgroups as its share of the tiles. With several row blocks the tiles of a sequence are cut into
+// the fewest equal chunks that are no longer than a range, and come chunk by chunk, in each all row blocks one behind the other: neighbouring
+// workgroups, which share an XCD, then walk the same tiles of different row blocks in step, and its cache fetches them once.
+// A workgroup whose range covers a row block wholly writes its rows; parts of a row block leave (maximum, sum, unnormalised result) in fp32 in the
+// workspace, and a second kernel joins them in the order of the keys (results do not depend on scheduling).
 #pragma once
 
 #include "attn_tiles.h"
@@ -13,13 +15,14 @@
 
 namespace pith {
 
-constexpr int kLatentKeys = 64;  // keys of a tile
-
-// load_lds16 from an address of each lane's own.
-__device__ __forceinline__ void load_lds16_at(const void* src, char* dst_wave) {
-  const uint32_t lds_addr = (uint32_t)(uintptr_t)(lds_char*)dst_wave;
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" : : "s"(lds_addr), "v"(src) : "memory");
-}
+// What the join needs of a row block: its rows (token * H + head of the whole call) and where its parts lie. chunks = 0: nothing to join.
+struct LatentJoin {
+  int row0, rows;
+  int first;          // place of the sequence's first tile in the work list
+  int blocks, block;  // its row blocks, and which this is
+  int tiles, chunks;
+  int per;            // length of a workgroup's range
+};
 
 struct LatentAttnParams {
   const __bf16* q_latent;
@@ -36,38 +39,450 @@ struct LatentAttnParams {
   int max_len;  // table_width * page_size
   float kappa;  // scale * log2(e)
   // workspace
-  int* items;    // number of row blocks of this call
-  int4* joins;   // [row blocks] what the join needs of each: first row (token * H + head of the whole call), rows, first and last slot (equal: nothing)
-  float2* stats; // [slots][M] running maximum (in bits) and sum
-  float* parts;  // [slots][M][512]
-  int max_items; // capacity of joins
-  int min_tiles; // of a workgroup's range
+  int* items;         // number of row blocks of this call
+  LatentJoin* joins;  // [row blocks]
+  float2* stats;      // [slots][M] running maximum (in bits) and sum
+  float* parts;       // [slots][M][512]
+  int max_items;      // capacity of joins
 };
 
 struct SeqWork {
-  int tok0, n, len;       // first token, new tokens, cached rows
-  int blocks, tiles;      // row blocks, tiles of each
+  int tok0, n, len;   // first token, new tokens, cached rows
+  int blocks, tiles;  // row blocks, tiles of each
 };
 
-__device__ __forceinline__ SeqWork seq_work(const LatentAttnParams& p, int b, int rows_per_block) {
+// Chunks of a sequence's tiles, and the first tile of chunk k (k = chunks: behind the last).
+__device__ __forceinline__ int chunks_of(int blocks, int tiles, int per) { return blocks > 1 ? (tiles + per - 1) / per : 1; }
+__device__ __forceinline__ int chunk_start(int k, int tiles, int chunks) { return (int)((int64_t)k * tiles / chunks); }
+
+// Where the part [x, y) of the work list of workgroup id lies, which is not a whole row block. A range holds at most three such parts: one from its
+// first tile on, one up to its last, and one whole chunk in between (chunks are at least half a range long).
+constexpr int kSlots = 3;
+__device__ __forceinline__ int64_t slot_of(int id, int x, int y, int per) {
+  return (int64_t)kSlots * id + (x == id * per ? 0 : y == (id + 1) * per ? 2 : 1);
+}
+
+template <int M, int KEYS>
+__device__ __forceinline__ SeqWork seq_work(const LatentAttnParams& p, int b) {
   SeqWork s;
   const int c0 = min(max(p.cu_q[b], 0), p.T), c1 = min(max(p.cu_q[b + 1], c0), p.T);
   s.tok0 = c0;
   s.n = c1 - c0;
   s.len = min(max(p.lengths[b], 0), p.max_len);
-  s.blocks = (s.n * p.H + rows_per_block - 1) / rows_per_block;
-  s.tiles = max((s.len + kLatentKeys - 1) / kLatentKeys, 1);  // rows without keys get their zeros from an empty tile
+  s.blocks = (s.n * p.H + M - 1) / M;
+  s.tiles = max((s.len + KEYS - 1) / KEYS, 1);  // rows without keys get their zeros from an empty tile
   return s;
 }
 
 // Inclusive sums over the lanes of a wavefront.
-__device__ __forceinline__ int wave_scan(int x, int lane) {
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const int y = __shfl_up(x, d);
-    x += lane >= d ? y : 0;
-  }
-  return x;
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int add_dpp(int x) {
+  return x + __builtin_amdgcn_update_dpp(0, x, CTRL, ROWS, 0xf, false);
 }
+__device__ __forceinline__ int wave_scan(int x) {
+  x = add_dpp<0x111, 0xf>(x);  // from 1, 2, 4, 8 lanes below in the row of 16
+  x = add_dpp<0x112, 0xf>(x);
+  x = add_dpp<0x114, 0xf>(x);
+  x = add_dpp<0x118, 0xf>(x);
+  x = add_dpp<0x142, 0xa>(x);  // lane 15 of a row to the next row, then lane 31 to the upper half
+  return add_dpp<0x143, 0xc>(x);
+}
+
+// A workgroup's way through its range of the work list, segment by segment (tiles of one chunk of one row block). Every wave walks for itself; all of it
+// is wave-uniform.
+template <int M, int KEYS>
+struct Walk {
+  int id, per, at, end;               // workgroup's number in the list, length of a range, place, end of the range
+  int b, before, item;                // sequence, tiles and row blocks in front of it
+  int chunks, chunk, tile0, tile1;    // chunk and its tiles
+  int block, tile;                    // row block, first tile of the segment
+  SeqWork s;
+
+  // False: nothing to do. IN_STEP: see the chunks above; short lists are spread over the XCDs all the same.
+  template <bool IN_STEP>
+  __device__ __forceinline__ bool start(const LatentAttnParams& p, int lane) {
+    int w = 0, k = 0, sw = 0, sk = 0, total = 0, blocks_total = 0;
+    const auto sums = [&](int b0) __attribute__((always_inline)) {  // over 64 sequences
+      w = k = 0;
+      if (b0 + lane < p.B) {
+        const SeqWork x = seq_work<M, KEYS>(p, b0 + lane);
+        w = x.blocks * x.tiles;
+        k = x.blocks;
+      }
+      sw = wave_scan(w);
+      sk = wave_scan(k);
+    };
+    for (int b0 = 0; b0 < p.B; b0 += 64) {
+      sums(b0);
+      total += __builtin_amdgcn_readlane(sw, 63);
+      blocks_total += __builtin_amdgcn_readlane(sk, 63);
+    }
+    if (blockIdx.x == 0 && threadIdx.x == 0) *p.items = min(blocks_total, p.max_items);
+    const int groups = gridDim.x;
+    per = (total + groups - 1) / groups;
+    const bool in_step = IN_STEP && total >= 2 * groups;  // workgroups are dealt to the eight XCDs in turn
+    id = in_step ? (blockIdx.x & 7) * (groups >> 3) + (blockIdx.x >> 3) : blockIdx.x;
+    at = id * per;
+    end = min(at + per, total);  // (the host has bounded total + gridDim.x)
+    if (at >= end) return false;
+    before = item = 0;
+    for (int b0 = 0;; b0 += 64) {
+      if (p.B > 64) sums(b0);
+      const uint64_t beyond = __ballot(before + sw > at);
+      if (beyond != 0) {
+        const int i = __builtin_ctzll(beyond);
+        b = b0 + i;
+        before += __builtin_amdgcn_readlane(sw - w, i);
+        item += __builtin_amdgcn_readlane(sk - k, i);
+        break;
+      }
+      before += __builtin_amdgcn_readlane(sw, 63);
+      item += __builtin_amdgcn_readlane(sk, 63);
+    }
+    s = seq_work<M, KEYS>(p, b);
+    chunks = chunks_of(s.blocks, s.tiles, per);
+    chunk = 0;
+    if (chunks > 1) chunk = (int)((((int64_t)((at - before) / s.blocks) + 1) * chunks - 1) / s.tiles);  // the last that begins at or before this tile
+    enter_chunk();
+    block = (at - before - tile0 * s.blocks) / (tile1 - tile0);
+    tile = at - before - tile0 * s.blocks - block * (tile1 - tile0) + tile0;
+    return true;
+  }
+  __device__ __forceinline__ void enter_chunk() {
+    tile0 = chunks > 1 ? chunk_start(chunk, s.tiles, chunks) : 0;
+    tile1 = chunks > 1 ? chunk_start(chunk + 1, s.tiles, chunks) : s.tiles;
+  }
+  __device__ __forceinline__ int n_tiles() const { return min(tile1 - tile, end - at); }
+  __device__ __forceinline__ int rows(const LatentAttnParams& p) const { return min(s.n * p.H - block * M, M); }
+  __device__ __forceinline__ bool whole() const { return n_tiles() == s.tiles; }
+  __device__ __forceinline__ int64_t slot() const { return slot_of(id, at, at + n_tiles(), per); }
+  // Who ends a row block says how it was cut.
+  __device__ __forceinline__ void leave_join(const LatentAttnParams& p) const {
+    if (tile + n_tiles() == s.tiles && threadIdx.x == 0 && item + block < p.max_items)
+      p.joins[item + block] = LatentJoin{s.tok0 * p.H + block * M, rows(p), before, s.blocks, block, s.tiles, whole() ? 0 : chunks, per};
+  }
+  // On to the next segment. False: the range is done.
+  __device__ __forceinline__ bool next(const LatentAttnParams& p) {
+    at += n_tiles();
+    if (at >= end) return false;
+    if (++block == s.blocks) {
+      block = 0;
+      if (++chunk == chunks) {
+        before += s.blocks * s.tiles;
+        item += s.blocks;
+        do s = seq_work<M, KEYS>(p, ++b); while (s.blocks == 0);
+        chunks = chunks_of(s.blocks, s.tiles, per);
+        chunk = 0;
+      }
+      enter_chunk();
+    }
+    tile = tile0;
+    return true;
+  }
+};
+
+// ---------------------------------------------------------------------------------------------
+// Tiles
+
+template <bool FP8, int KEYS>
+struct LatentTile {
+  static constexpr int kLatentRow = FP8 ? kLatent : 2 * kLatent;  // bytes
+  static constexpr int kPe = KEYS * kLatentRow;                   // offsets in a tile
+  static constexpr int kScale = kPe + KEYS * 2 * kRope;           // [KEYS] fp32
+  static constexpr int kBytes = kScale + (FP8 ? KEYS * 4 : 0);
+  static constexpr int kLoads = FP8 ? 6 : 9;  // direct loads of a wave: eight rows
+};
+
+// Piece (16 bytes) swizzles: piece q of a row lies at q ^ swizzle(row). Latent rows are whole multiples of 256 bytes; the low four bits of the piece
+// are swizzled so that sixteen consecutive rows read at one piece hit different banks (tile_swizzle, attn_tiles.h). Rotary rows lie two to a 256-byte
+// LDS row: row 8 w + i and 8 w + 4 + i (i < 4) in pieces 0-7 and 8-15 of LDS row 4 w + i, so that a wave's eight rows are one instruction.
+__device__ __forceinline__ int pe_row(int row) { return ((row >> 3) << 2) | (row & 3); }
+__device__ __forceinline__ int pe_swizzle(int lds_row) { return ((lds_row & 3) << 1) | ((lds_row >> 2) & 1); }
+
+// Page of the sixteen rows from key on (a multiple of 16); rows behind the sequence's last one are read as that one.
+// Read as constant memory (nobody writes tables while the kernel runs): a scalar load, which the counted waits for tiles do not see.
+typedef const __attribute__((address_space(4))) int32_t* ScalarTable;
+__device__ __forceinline__ int page_of(const LatentAttnParams& p, ScalarTable table, int key, int last) {
+  return safe_page(table[min(key, last) >> p.cache.page_shift], p.cache.pages);
+}
+
+// Wave w's direct loads of a tile: rows 8 w .. 8 w + 7 of it, which are half of the sixteen from key16 = key0 + 16 (w >> 1) on. Rows behind the sequence's
+// last one are read as that one. The loads are asked for one by one, where the caller has room between its products.
+template <bool FP8, int KEYS>
+struct TileLoads {
+  using T = LatentTile<FP8, KEYS>;
+  const char *base, *pe;  // of the wave's first row
+  const float* scale;
+  char* slot;
+  int left;  // rows behind the wave's first that exist (below zero: none, nor that one)
+  int wave;
+  __device__ __forceinline__ TileLoads(const LatentAttnParams& p, int page, int key16, int last, char* slot_, int wave_) : slot(slot_), wave(wave_) {
+    const int first = min(key16, last) & ~15;  // the page's sixteen rows
+    const int r0 = 8 * (wave & 1);             // of the sixteen
+    const int in_page = (first & ((1 << p.cache.page_shift) - 1)) + r0;
+    left = last - first - r0;
+    base = p.cache.latent + page * p.cache.latent_ps + (int64_t)in_page * T::kLatentRow;
+    pe = reinterpret_cast<const char*>(p.cache.k_pe + page * p.cache.k_pe_ps + (int64_t)in_page * kRope);
+    scale = FP8 ? p.cache.scale + page * p.cache.scale_ps + in_page : nullptr;
+  }
+  // Load n of T::kLoads.
+  __device__ __forceinline__ void issue(int n, int lane) const {
+    constexpr int kLatentLoads = FP8 ? 4 : 8;
+    if (n < kLatentLoads) {
+      char* const dst = slot + 8 * wave * T::kLatentRow + n * 1024;
+      if constexpr (FP8) {  // two rows an instruction
+        const int r = 2 * n + (lane >> 5);
+        load_lds16(base + min(left, 0) * T::kLatentRow, max(min(r, left), 0) * T::kLatentRow + 16 * ((lane & 31) ^ tile_swizzle(8 * wave + r)), dst);
+      } else {
+        load_lds16(base + min(n, left) * T::kLatentRow, (16 * lane) ^ (16 * tile_swizzle(8 * wave + n)), dst);
+      }
+    } else if (n == kLatentLoads) {
+      const int piece = (lane & 15) ^ pe_swizzle(4 * wave + (lane >> 4));
+      const int r = 4 * (piece >> 3) + (lane >> 4);
+      load_lds16(pe + min(left, 0) * (2 * kRope), max(min(r, left), 0) * (2 * kRope) + 16 * (piece & 7), slot + T::kPe + wave * 1024);
+    } else {
+      if (lane < 8) load_lds4(scale + min(lane, left), slot + T::kScale + 32 * wave);
+    }
+  }
+  __device__ __forceinline__ void issue_all(int lane) const {
+    asm volatile("" : "+v"(lane));  // the rows' offsets are formed on the spot, not kept (and spilled) from tile to tile
+#pragma unroll
+    for (int n = 0; n < T::kLoads; ++n) issue(n, lane);
+  }
+};
+
+__device__ __forceinline__ f32x4 mfma16(bf16x8 a, bf16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+
+// max / sum over the eight lanes of a row of the 32-row softmax (lane % 8 = 0 .. 7), in all of them
+template <int CTRL>
+__device__ __forceinline__ float dpp(float x) {
+  return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(x), CTRL, 0xf, 0xf, true));
+}
+constexpr int kQuadXor1 = 0xB1, kQuadXor2 = 0x4E, kHalfMirror = 0x141;
+__device__ __forceinline__ float eight_max(float x) {
+  x = fmaxf(x, dpp<kQuadXor1>(x));
+  x = fmaxf(x, dpp<kQuadXor2>(x));
+  return fmaxf(x, dpp<kHalfMirror>(x));
+}
+__device__ __forceinline__ float eight_sum(float x) {
+  x += dpp<kQuadXor1>(x);
+  x += dpp<kQuadXor2>(x);
+  return x + dpp<kHalfMirror>(x);
+}
+
+// max / sum over the four lanes c, c + 16, c + 32, c + 48 that share a query row
+__device__ __forceinline__ float quad_max(float x) {
+  const int i = __float_as_int(x);
+  const auto r = __builtin_amdgcn_permlane16_swap(i, i, false, false);
+  return pair_max(fmaxf(__int_as_float(r[0]), __int_as_float(r[1])));
+}
+__device__ __forceinline__ float quad_sum(float x) {
+  const int i = __float_as_int(x);
+  const auto r = __builtin_amdgcn_permlane16_swap(i, i, false, false);
+  return pair_sum(__int_as_float(r[0]) + __int_as_float(r[1]));
+}
+
+template <int LATER>
+__device__ __forceinline__ void wait_loads() {
+  static_assert(LATER < 64, "vmcnt has six bits");
+  __builtin_amdgcn_s_waitcnt(0x0F70 | (LATER & 15) | ((LATER >> 4) << 14));
+  asm volatile("" ::: "memory");
+}
+
+// Eight e4m3 values (two words) -> bf16, exact.
+__device__ __forceinline__ bf16x8 widen(uint32_t w0, uint32_t w1) {
+  const bf16x2 a = fp8x2_to_bf16<false>(w0), b = fp8x2_to_bf16<true>(w0), c = fp8x2_to_bf16<false>(w1), d = fp8x2_to_bf16<true>(w1);
+  return bf16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+
+// Scores of 16 keys against J groups of query rows: STEPS times 64 latent features, then with_pe the 64 rotary ones; between(i) is called in step i. `at` is the place of the lane's
+// first piece (its row, piece g of the swizzled 256 bytes) of the tile; piece 4 k + g lies at ^ (64 k), as rows are multiples of 256 bytes.
+template <bool FP8, int J, int STEPS, int Q, typename Between>
+__device__ __forceinline__ void score(const char* tile, int at, int pe_at, bool with_pe, f32x4 scale, const bf16x8 (&q)[J][Q], f32x4 (&s)[J], Between between) {
+#pragma unroll
+  for (int j = 0; j < J; ++j) s[j] = f32x4{};
+#pragma unroll
+  for (int i = 0; i < STEPS; ++i) {
+    bf16x8 k0, k1;
+    if constexpr (FP8) {  // sixteen features a lane: two steps
+      const u32x4 raw = *reinterpret_cast<const u32x4*>(tile + (at ^ (64 * (i & 3))) + 256 * (i >> 2));
+      k0 = widen(raw[0], raw[1]);
+      k1 = widen(raw[2], raw[3]);
+    } else {
+      k0 = *reinterpret_cast<const bf16x8*>(tile + (at ^ (128 * (i & 1))) + 256 * (i >> 1));
+      k1 = *reinterpret_cast<const bf16x8*>(tile + (at ^ (128 * (i & 1) + 64)) + 256 * (i >> 1));
+    }
+#pragma unroll
+    for (int j = 0; j < J; ++j) s[j] = mfma16(k0, q[j][2 * i], s[j]);
+    between(i);
+#pragma unroll
+    for (int j = 0; j < J; ++j) s[j] = mfma16(k1, q[j][2 * i + 1], s[j]);
+  }
+  if constexpr (FP8) {
+#pragma unroll
+    for (int j = 0; j < J; ++j) s[j] *= scale;
+  }
+  if (with_pe) {
+    const bf16x8 k0 = *reinterpret_cast<const bf16x8*>(tile + pe_at), k1 = *reinterpret_cast<const bf16x8*>(tile + (pe_at ^ 64));
+#pragma unroll
+    for (int j = 0; j < J; ++j) s[j] = mfma16(k0, q[j][Q - 2], s[j]);
+#pragma unroll
+    for (int j = 0; j < J; ++j) s[j] = mfma16(k1, q[j][Q - 1], s[j]);
+  }
+}
+
+// Which of a wave's features (64 or 128, 16 a product) result 0 of product n is in a lane of group g; results 1 to 3 follow it. Transposed reads take their columns in groups of four (bf16) or eight
+// (e4m3) from wherever a lane points; as bf16 the groups of two products are dealt so that a lane's results of both are eight consecutive ones.
+template <bool FP8>
+__device__ __forceinline__ int feature_of(int n, int g) {
+  return FP8 ? 16 * n + 4 * g : 32 * (n >> 1) + 8 * g + 4 * (n & 1);
+}
+
+// Place of the lane's transposed reads of FEATURES features in a tile, rows 0-31, wave w's from feature FEATURES w on; those of other pieces and rows are
+// ^ and + from there.
+template <bool FP8, int FEATURES>
+__device__ __forceinline__ int value_place(int wave, int c, int g) {
+  const int r = 8 * g + (FP8 ? c >> 1 : c >> 2);
+  const int piece = FP8 ? FEATURES / 16 * wave : FEATURES / 8 * wave + (c & 3);
+  return r * (FP8 ? kLatent : 2 * kLatent) + ((piece ^ tile_swizzle(r)) << 4) + (FP8 ? 8 * (c & 1) : 0);
+}
+
+// Operand A of product n over keys 8 g + e.
+template <bool FP8>
+__device__ __forceinline__ bf16x8 value_fragment(const char* tile, int at, int n) {
+  if constexpr (FP8) {
+    typedef __attribute__((ext_vector_type(2))) int i32x2;
+    typedef __attribute__((address_space(3))) i32x2 lds_i32x2;
+    const i32x2 raw = __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_i32x2*)(tile + (at ^ (16 * n))));
+    return widen((uint32_t)raw[0], (uint32_t)raw[1]);
+  } else {  // four rows further on the swizzle differs in its lowest bit
+    return lds_read_transposed_at(tile + (at ^ (64 * (n >> 1))) + 8 * (n & 1), tile + (at ^ (64 * (n >> 1) + 16)) + 4 * (2 * kLatent) + 8 * (n & 1));
+  }
+}
+
+// Infinities and NaN of a tile's latent rows -> 0, in place, by all threads. For tiles that some rows see in part only: a row's weight of a key it does
+// not see is 0, and must stay so against whatever the key holds. A row that sees such a key has a score of the same kind.
+template <bool FP8, int KEYS, int THREADS>
+__device__ __forceinline__ void clean_tile(char* tile) {
+  for (int at = 16 * threadIdx.x; at < LatentTile<FP8, KEYS>::kPe; at += 16 * THREADS) {
+    u32x4 x = *reinterpret_cast<const u32x4*>(tile + at);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if constexpr (FP8) {
+#pragma unroll
+        for (int k = 0; k < 32; k += 8)
+          if (((x[e] >> k) & 0x7fu) == 0x7fu) x[e] &= ~(0xffu << k);
+      } else {
+        if ((x[e] & 0x7f80u) == 0x7f80u) x[e] &= 0xffff0000u;
+        if ((x[e] & 0x7f800000u) == 0x7f800000u) x[e] &= 0xffffu;
+      }
+    }
+    *reinterpret_cast<u32x4*>(tile + at) = x;
+  }
+}
+
+// A weight times its row's scale; 0 stays 0, also against a scale that is not finite.
+__device__ __forceinline__ float scaled(float weight, float scale) { return weight == 0.f ? 0.f : weight * scale; }
+
+// x *= f in place: as a plain product under a branch the accumulators are copied on the other way, which doubles their registers. The compiler does not
+// look into the statement for hazards: f may come from v_exp_f32 right before it (one wait state), and x from products of the tile before (two barriers
+// away).
+__device__ __forceinline__ void scale_in_place(f32x4& x, float f) {
+  float a = x[0], b = x[1], c = x[2], d = x[3];
+  asm("s_nop 1\n\tv_mul_f32 %0, %4, %0\n\tv_mul_f32 %1, %4, %1\n\tv_mul_f32 %2, %4, %2\n\tv_mul_f32 %3, %4, %3" : "+v"(a), "+v"(b), "+v"(c), "+v"(d) : "v"(f));
+  x = f32x4{a, b, c, d};
+}
+
+// Scores x[0 .. N-1] of keys key0 .. against a row of token tok: those of keys that it does not see -> -infinity. In the last tiles of a sequence only, so
+// what a token sees is looked up anew there. (In words and without branches: hipcc 7.2 lost the selected score behind nested conditions on a shift of
+// 64 bits.)
+template <bool TREE, int N, typename X>
+__device__ __forceinline__ void mask_scores(const LatentAttnParams& p, const SeqWork& s, X& x, int tok, int key0) {
+  uint32_t lo = 0, hi = 0;
+  if constexpr (TREE) {
+    const uint64_t word = (uint64_t)p.tree[s.tok0 + tok];
+    lo = (uint32_t)word;
+    hi = (uint32_t)(word >> 32);
+  }
+  const int ctx = s.len - s.n;  // rows in front of the new ones (below zero only where the lengths contradict each other)
+#pragma unroll
+  for (int v = 0; v < N; ++v) {
+    const int key = key0 + v, draft = key - ctx;
+    int seen;
+    if constexpr (TREE) {
+      const uint32_t bits = draft < 32 ? lo : hi;
+      seen = (draft < 0) | ((draft < 64) & (int)((bits >> (draft & 31)) & 1u));
+    } else {
+      seen = draft <= tok;
+    }
+    seen &= key < s.len;
+    x[v] = seen ? x[v] : -INFINITY;
+  }
+}
+
+// Whether some row may not see all of the tile from key0 on.
+template <bool TREE, int KEYS>
+__device__ __forceinline__ bool partial_tile(const SeqWork& s, int key0) { return key0 + KEYS > s.len - s.n + (TREE ? 0 : 1); }
+
+// Operand B fragments of a query row: 32 latent features a step from `latent` on (e4m3 keys are read 16 features at a time: steps 2 i, 2 i + 1 then contract
+// features 64 i + 16 g + {0..7, 8..15}), then two rotary steps.
+template <bool FP8, int Q>
+__device__ __forceinline__ void load_query(const LatentAttnParams& p, const SeqWork& s, int row, int latent, int g, bf16x8 (&q)[Q]) {
+  const int tok = row / p.H, head = row - tok * p.H;
+  const __bf16* ql = p.q_latent + (int64_t)(s.tok0 + tok) * p.q_ts + head * p.q_hs + latent;
+  const __bf16* qp = p.q_pe + (int64_t)(s.tok0 + tok) * p.q_pe_ts + head * p.q_pe_hs;
+#pragma unroll
+  for (int i = 0; i < Q - 2; ++i) q[i] = *reinterpret_cast<const bf16x8*>(ql + (FP8 ? 64 * (i >> 1) + 16 * g + 8 * (i & 1) : 32 * i + 8 * g));
+#pragma unroll
+  for (int i = 0; i < 2; ++i) q[Q - 2 + i] = *reinterpret_cast<const bf16x8*>(qp + 32 * i + 8 * g);
+}
+
+// The queries have to be there before a walk: left to their first use, the compiler's waits for them would stand in its loop and wait for the tiles in
+// flight in every turn.
+template <int J, int Q>
+__device__ __forceinline__ void pin_queries(bf16x8 (&q)[J][Q]) {
+#pragma unroll
+  for (int j = 0; j < J; ++j)
+#pragma unroll
+    for (int i = 0; i < Q; ++i) asm volatile("" : "+v"(q[j][i]));
+}
+
+// Results of one row (16 N features of the wave from f0 on) as bf16, and its lse by one lane; or, where the segment is a part, sums, maximum and
+// unnormalised results in the workspace.
+template <bool FP8, int M, int N, typename W>
+__device__ __forceinline__ void store_row(const LatentAttnParams& p, const W& walk, const f32x4 (&acc)[N], float top, float sum, int row, int f0, int g, bool first) {
+  if (row >= walk.rows(p)) return;
+  if (walk.whole()) {
+    const int at = walk.block * M + row, tok = walk.s.tok0 + at / p.H, head = at % p.H;
+    const float inv = 1.f / sum;
+    __bf16* const dst = p.o + (int64_t)tok * p.o_ts + head * p.o_hs + f0;
+#pragma unroll
+    for (int n = 0; n < N; n += 2) {
+      const f32x4 a = sum == 0.f ? f32x4{} : acc[n] * inv, d = sum == 0.f ? f32x4{} : acc[n + 1] * inv;
+      const u32x2 lo = {pack_bf16x2(a[0], a[1]), pack_bf16x2(a[2], a[3])}, hi = {pack_bf16x2(d[0], d[1]), pack_bf16x2(d[2], d[3])};
+      if constexpr (FP8) {
+        *reinterpret_cast<u32x2*>(dst + feature_of<true>(n, g)) = lo;
+        *reinterpret_cast<u32x2*>(dst + feature_of<true>(n + 1, g)) = hi;
+      } else {
+        *reinterpret_cast<u32x4*>(dst + feature_of<false>(n, g)) = u32x4{lo[0], lo[1], hi[0], hi[1]};
+      }
+    }
+    if (first) p.lse[head * p.lse_hs + tok] = sum == 0.f ? -INFINITY : top + __builtin_amdgcn_logf(sum);
+  } else {
+    const int64_t part = walk.slot();
+    float* const dst = p.parts + (part * M + row) * kLatent + f0;
+#pragma unroll
+    for (int n = 0; n < N; ++n) *reinterpret_cast<f32x4*>(dst + feature_of<FP8>(n, g)) = acc[n];
+    if (first) p.stats[part * M + row] = make_float2(top, sum);
+  }
+}
+
+// Where a score may exceed the reference of its row's weights, in bits, before the reference is moved: weights stay below 2^8, far from the end of
+// their range, and neither they nor the sums lose precision by it.
+constexpr float kSlack = 8.f;
+
+// The attention kernel for 64 rows to a workgroup (latent_attn_wide.hip).
+constexpr int kWideRows = 64, kWideKeys = 64;
+void launch_latent_wide(const LatentAttnParams& p, bool fp8, bool tree, int groups, hipStream_t stream);
 
 }  // namespace pith
