@@ -1,12 +1,11 @@
 // Attention to the latent cache: what its kernels share. The work list, the tiles and the join.
 //
-// Work list. A sequence of n new tokens and L rows is R = ceil(n H / M) row blocks of M rows (row = token * H + head) times
-// N = ceil(L / K) tiles of K keys, and the R N tiles of all sequences, one sequence behind the other, are dealt to the workgroups in equal ranges.
-// Lengths are read on the device, so nothing depends on the host knowing them: a captured call follows its sequences as they grow, and one long
-// sequence among short ones is spread over as many workgroups as its share of the tiles. With several row blocks the tiles of a sequence are cut into
-// the fewest equal chunks that are no longer than a range, and come chunk by chunk, in each all row blocks one behind the other: neighbouring
-// workgroups, which share an XCD, then walk the same tiles of different row blocks in step, and its cache fetches them once.
-// A workgroup whose range covers a row block wholly writes its rows; parts of a row block leave (maximum, sum, unnormalised result) in fp32 in the
+// Work list. A sequence of n new tokens and L rows is R = ceil(n H / M) row blocks of M rows (row = token * H + head) times N = ceil(L / K) tiles of K keys,
+// and the tiles of all row blocks of all sequences, one behind the other, are dealt to the workgroups in equal ranges. Lengths are read on the device,
+// so nothing depends on the host knowing them: a captured call follows its sequences as they grow, and one long sequence among short ones is spread over
+// as many workgroups as its share of the tiles. (Tiles of all row blocks in step on one XCD, chunk by chunk, so that its cache fetches them once, was
+// slower: 128 heads 119 us against 100, trees of 48 drafts 272 against 250; the ranges are cut more often, and the kernels do not wait for these bytes.)
+// A workgroup whose range covers a row block wholly writes its rows; parts of a row block leave (reference, sum, unnormalised result) in fp32 in the
 // workspace, and a second kernel joins them in the order of the keys (results do not depend on scheduling).
 #pragma once
 
@@ -15,13 +14,10 @@
 
 namespace pith {
 
-// What the join needs of a row block: its rows (token * H + head of the whole call) and where its parts lie. chunks = 0: nothing to join.
+// What the join needs of a row block: its rows (token * H + head of the whole call) and the slots of its parts, the first and, of the workgroups behind
+// that one, the last (equal: nothing to join).
 struct LatentJoin {
-  int row0, rows;
-  int first;          // place of the sequence's first tile in the work list
-  int blocks, block;  // its row blocks, and which this is
-  int tiles, chunks;
-  int per;            // length of a workgroup's range
+  int row0, rows, first, last;
 };
 
 struct LatentAttnParams {
@@ -41,8 +37,8 @@ struct LatentAttnParams {
   // workspace
   int* items;         // number of row blocks of this call
   LatentJoin* joins;  // [row blocks]
-  float2* stats;      // [slots][M] running maximum (in bits) and sum
-  float* parts;       // [slots][M][512]
+  float2* stats;      // [slots][M] reference (in bits) and sum
+  float* parts;       // [slots][M][512]; slot 2 i: workgroup i's part that begins with its range, 2 i + 1: one that begins later
   int max_items;      // capacity of joins
 };
 
@@ -50,17 +46,6 @@ struct SeqWork {
   int tok0, n, len;   // first token, new tokens, cached rows
   int blocks, tiles;  // row blocks, tiles of each
 };
-
-// Chunks of a sequence's tiles, and the first tile of chunk k (k = chunks: behind the last).
-__device__ __forceinline__ int chunks_of(int blocks, int tiles, int per) { return blocks > 1 ? (tiles + per - 1) / per : 1; }
-__device__ __forceinline__ int chunk_start(int k, int tiles, int chunks) { return (int)((int64_t)k * tiles / chunks); }
-
-// Where the part [x, y) of the work list of workgroup id lies, which is not a whole row block. A range holds at most three such parts: one from its
-// first tile on, one up to its last, and one whole chunk in between (chunks are at least half a range long).
-constexpr int kSlots = 3;
-__device__ __forceinline__ int64_t slot_of(int id, int x, int y, int per) {
-  return (int64_t)kSlots * id + (x == id * per ? 0 : y == (id + 1) * per ? 2 : 1);
-}
 
 template <int M, int KEYS>
 __device__ __forceinline__ SeqWork seq_work(const LatentAttnParams& p, int b) {
@@ -88,18 +73,16 @@ __device__ __forceinline__ int wave_scan(int x) {
   return add_dpp<0x143, 0xc>(x);
 }
 
-// A workgroup's way through its range of the work list, segment by segment (tiles of one chunk of one row block). Every wave walks for itself; all of it
-// is wave-uniform.
+// A workgroup's way through its range of the work list, segment by segment (tiles of one row block). Every wave walks for itself; all of it is
+// wave-uniform.
 template <int M, int KEYS>
 struct Walk {
-  int id, per, at, end;               // workgroup's number in the list, length of a range, place, end of the range
-  int b, before, item;                // sequence, tiles and row blocks in front of it
-  int chunks, chunk, tile0, tile1;    // chunk and its tiles
-  int block, tile;                    // row block, first tile of the segment
+  int per, begin, at, end;  // length of a range, begin of this one, place, end
+  int b, item;              // sequence, row blocks in front of it
+  int block, tile;          // row block, first tile of the segment
   SeqWork s;
 
-  // False: nothing to do. IN_STEP: see the chunks above; short lists are spread over the XCDs all the same.
-  template <bool IN_STEP>
+  // False: nothing to do.
   __device__ __forceinline__ bool start(const LatentAttnParams& p, int lane) {
     int w = 0, k = 0, sw = 0, sk = 0, total = 0, blocks_total = 0;
     const auto sums = [&](int b0) __attribute__((always_inline)) {  // over 64 sequences
@@ -118,14 +101,12 @@ struct Walk {
       blocks_total += __builtin_amdgcn_readlane(sk, 63);
     }
     if (blockIdx.x == 0 && threadIdx.x == 0) *p.items = min(blocks_total, p.max_items);
-    const int groups = gridDim.x;
-    per = (total + groups - 1) / groups;
-    const bool in_step = IN_STEP && total >= 2 * groups;  // workgroups are dealt to the eight XCDs in turn
-    id = in_step ? (blockIdx.x & 7) * (groups >> 3) + (blockIdx.x >> 3) : blockIdx.x;
-    at = id * per;
+    per = (total + (int)gridDim.x - 1) / (int)gridDim.x;
+    begin = at = blockIdx.x * per;
     end = min(at + per, total);  // (the host has bounded total + gridDim.x)
     if (at >= end) return false;
-    before = item = 0;
+    int before = 0;  // tiles in front of the sequence
+    item = 0;
     for (int b0 = 0;; b0 += 64) {
       if (p.B > 64) sums(b0);
       const uint64_t beyond = __ballot(before + sw > at);
@@ -140,43 +121,36 @@ struct Walk {
       item += __builtin_amdgcn_readlane(sk, 63);
     }
     s = seq_work<M, KEYS>(p, b);
-    chunks = chunks_of(s.blocks, s.tiles, per);
-    chunk = 0;
-    if (chunks > 1) chunk = (int)((((int64_t)((at - before) / s.blocks) + 1) * chunks - 1) / s.tiles);  // the last that begins at or before this tile
-    enter_chunk();
-    block = (at - before - tile0 * s.blocks) / (tile1 - tile0);
-    tile = at - before - tile0 * s.blocks - block * (tile1 - tile0) + tile0;
+    block = (at - before) / s.tiles;
+    tile = at - before - block * s.tiles;
     return true;
   }
-  __device__ __forceinline__ void enter_chunk() {
-    tile0 = chunks > 1 ? chunk_start(chunk, s.tiles, chunks) : 0;
-    tile1 = chunks > 1 ? chunk_start(chunk + 1, s.tiles, chunks) : s.tiles;
-  }
-  __device__ __forceinline__ int n_tiles() const { return min(tile1 - tile, end - at); }
+  __device__ __forceinline__ int n_tiles() const { return min(s.tiles - tile, end - at); }
   __device__ __forceinline__ int rows(const LatentAttnParams& p) const { return min(s.n * p.H - block * M, M); }
   __device__ __forceinline__ bool whole() const { return n_tiles() == s.tiles; }
-  __device__ __forceinline__ int64_t slot() const { return slot_of(id, at, at + n_tiles(), per); }
+  __device__ __forceinline__ int slot() const { return 2 * blockIdx.x + (at == begin ? 0 : 1); }
   // Who ends a row block says how it was cut.
   __device__ __forceinline__ void leave_join(const LatentAttnParams& p) const {
-    if (tile + n_tiles() == s.tiles && threadIdx.x == 0 && item + block < p.max_items)
-      p.joins[item + block] = LatentJoin{s.tok0 * p.H + block * M, rows(p), before, s.blocks, block, s.tiles, whole() ? 0 : chunks, per};
+    if (tile + n_tiles() != s.tiles || threadIdx.x != 0 || item + block >= p.max_items) return;
+    int first = 0, last = 0;
+    if (!whole()) {
+      const int from = at - tile;  // of the row block in the work list
+      const int id = from / per;
+      first = 2 * id + (from == id * per ? 0 : 1);
+      last = 2 * blockIdx.x;
+    }
+    p.joins[item + block] = LatentJoin{s.tok0 * p.H + block * M, rows(p), first, last};
   }
   // On to the next segment. False: the range is done.
   __device__ __forceinline__ bool next(const LatentAttnParams& p) {
     at += n_tiles();
     if (at >= end) return false;
+    tile = 0;
     if (++block == s.blocks) {
       block = 0;
-      if (++chunk == chunks) {
-        before += s.blocks * s.tiles;
-        item += s.blocks;
-        do s = seq_work<M, KEYS>(p, ++b); while (s.blocks == 0);
-        chunks = chunks_of(s.blocks, s.tiles, per);
-        chunk = 0;
-      }
-      enter_chunk();
+      item += s.blocks;
+      do s = seq_work<M, KEYS>(p, ++b); while (s.blocks == 0);
     }
-    tile = tile0;
     return true;
   }
 };

@@ -39,7 +39,7 @@ __global__ __launch_bounds__(kThreads, 2) void latent_attn_kernel(LatentAttnPara
   const int c = lane & 15, g = lane >> 4;
   const int kg = wave & 1, half = wave >> 1;
   Walk<kM, kKeys> walk;
-  if (!walk.start<false>(p, lane)) return;
+  if (!walk.start(p, lane)) return;
 
   const int key_row = 16 * kg + c;  // the key this lane brings
   const int key_at = key_row * T::kLatentRow + half * (T::kLatentRow / 2) + ((g ^ tile_swizzle(key_row)) << 4);
@@ -136,94 +136,77 @@ __global__ __launch_bounds__(kThreads, 2) void latent_attn_kernel(LatentAttnPara
 }
 
 constexpr int kJoinThreads = 256;
-constexpr int kMaxGroups = 1024;  // workgroups of the attention kernel, at most
-constexpr int kMaxParts = 2 * kMaxGroups + 2;  // of a row block: two of each chunk
+constexpr int kMaxGroups = 512;  // workgroups of the attention kernel, at most: kMaxGroups + 1 parts of a row block
 
 // Joins the parts of a row block: o = sum_i w_i O_i / sum_i w_i l_i, w_i = 2^(m_i - max m). blockIdx.x: row block, blockIdx.y: which of gridDim.y
-// equal shares of its m_rows * 512 results. The weights of a row are formed first, in one pass over its maxima and sums, so that the loads of the sums
-// over the parts do not wait for one another; where a share has fewer pieces of four features than there are threads, several groups of threads take
-// every other part and add up in LDS.
+// equal shares of its m_rows * 512 results, 1024 of them at most. The weights of a row are formed first, in one pass over its references and sums, so that the loads of the
+// sums over the parts do not wait for one another; where a share has fewer pieces of four features than there are threads, several groups of threads
+// take every other part and add up in LDS.
 __global__ __launch_bounds__(kJoinThreads) void latent_join_kernel(LatentAttnParams p, int m_rows) {
   __shared__ __attribute__((aligned(16))) float sum_o[kJoinThreads][4];
-  __shared__ float w_part[2][kMaxParts], l_part[2][kMaxParts];
+  __shared__ float w_part[2][kMaxGroups + 1], l_part[2][kMaxGroups + 1];
   __shared__ float of_wave[2][kJoinThreads / 64];
-  __shared__ int place[kMaxParts];
-  if ((int)blockIdx.x >= *p.items) return;
-  const LatentJoin join = p.joins[blockIdx.x];
-  if (join.chunks == 0) return;
-  // the parts: of one chunk as many as it meets ranges, of several two each, of which the second may be missing
-  const int g0 = (join.first + join.block * join.tiles) / join.per;
-  const int n = min(join.chunks > 1 ? 2 * join.chunks : (join.first + (join.block + 1) * join.tiles - 1) / join.per - g0 + 1, kMaxParts);
-  const auto slot = [&](int i) -> int64_t {
-    const int chunk = join.chunks > 1 ? i >> 1 : 0;
-    const int t0 = chunk_start(chunk, join.tiles, join.chunks), t1 = chunk_start(chunk + 1, join.tiles, join.chunks);
-    const int x = join.first + t0 * join.blocks + join.block * (t1 - t0), y = x + t1 - t0;
-    const int id = join.chunks > 1 ? x / join.per + (i & 1) : g0 + i;
-    const int from = max(x, id * join.per), to = min(y, (id + 1) * join.per);
-    return from < to ? slot_of(id, from, to, join.per) : -1;
-  };
+  const int items = *p.items;
+  const LatentJoin join = p.joins[blockIdx.x];  // (beyond `items` it is whatever the workspace held)
+  if ((int)blockIdx.x >= items || join.first == join.last) return;
+  const int n = min(join.last / 2 - join.first / 2 + 1, kMaxGroups + 1);  // parts: the first slot, then the even ones up to the last
+  const auto slot = [&](int i) { return (int64_t)(i == 0 ? join.first : 2 * (join.first / 2 + i)); };
   const int pieces = m_rows * (kLatent / 4) / gridDim.y;  // of this share: a power of two
-  const int lanes = min(pieces, kJoinThreads), groups = kJoinThreads / lanes;
-  const int mine = threadIdx.x % lanes, group = threadIdx.x / lanes;
-  const int n_rows = lanes > kLatent / 4 ? 2 : 1, per_row = kJoinThreads / n_rows;  // rows of a pass, threads that form the weights of each
+  const int groups = kJoinThreads / pieces, mine = threadIdx.x % pieces, group = threadIdx.x / pieces;
+  const int n_rows = pieces > kLatent / 4 ? 2 : 1, per_row = kJoinThreads / n_rows;  // rows of the share, threads that form the weights of each
   const int r = threadIdx.x / per_row, u = threadIdx.x % per_row, waves = per_row / 64;
-  for (int piece0 = 0; piece0 < pieces; piece0 += lanes) {
-    const int first = blockIdx.y * pieces + piece0;
-    const int row = (first + mine) / (kLatent / 4), feature = 4 * ((first + mine) % (kLatent / 4));
-    __syncthreads();  // the pass before is through with the shared arrays
-    float top = -INFINITY;
-    for (int i = u; i < n; i += per_row) {
-      const int64_t sl = slot(i);
-      const float2 st = sl < 0 ? make_float2(-INFINITY, 0.f) : p.stats[sl * m_rows + first / (kLatent / 4) + r];
-      place[i] = (int)(sl < 0 ? slot(i - 1) : sl);  // (a second part that is missing is read as the first one, with weight 0)
-      w_part[r][i] = st.x;
-      l_part[r][i] = st.y;
-      top = fmaxf(top, st.x);
-    }
+  const int first = blockIdx.y * pieces;
+  const int row = (first + mine) / (kLatent / 4), feature = 4 * ((first + mine) % (kLatent / 4));
+  float top = -INFINITY;
+  for (int i = u; i < n; i += per_row) {
+    const float2 st = p.stats[slot(i) * m_rows + first / (kLatent / 4) + r];
+    w_part[r][i] = st.x;
+    l_part[r][i] = st.y;
+    top = fmaxf(top, st.x);
+  }
 #pragma unroll
-    for (int d = 1; d < 64; d <<= 1) top = fmaxf(top, __shfl_xor(top, d));
-    of_wave[0][threadIdx.x >> 6] = top;
+  for (int d = 1; d < 64; d <<= 1) top = fmaxf(top, __shfl_xor(top, d));
+  of_wave[0][threadIdx.x >> 6] = top;
+  __syncthreads();
+  for (int k = 0; k < waves; ++k) top = fmaxf(top, of_wave[0][r * waves + k]);
+  const float ref = top == -INFINITY ? 0.f : top;
+  float sum = 0.f;
+  for (int i = u; i < n; i += per_row) {
+    const float w = __builtin_amdgcn_exp2f(w_part[r][i] - ref);
+    w_part[r][i] = w;
+    sum += w * l_part[r][i];
+  }
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) sum += __shfl_xor(sum, d);
+  of_wave[1][threadIdx.x >> 6] = sum;
+  __syncthreads();
+  const int rr = n_rows == 2 ? mine / (kLatent / 4) : 0;  // the row of this thread's piece
+  sum = 0.f;
+  top = -INFINITY;
+  for (int k = 0; k < waves; ++k) sum += of_wave[1][rr * waves + k], top = fmaxf(top, of_wave[0][rr * waves + k]);
+  f32x4 o = {};
+  const float* const src = p.parts + (int64_t)row * kLatent + feature;
+  int i = group;
+  for (; i + 3 * groups < n; i += 4 * groups) {
+    f32x4 x[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) x[k] = *reinterpret_cast<const f32x4*>(src + slot(i + k * groups) * m_rows * kLatent);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) o += x[k] * w_part[rr][i + k * groups];
+  }
+  for (; i < n; i += groups) o += *reinterpret_cast<const f32x4*>(src + slot(i) * m_rows * kLatent) * w_part[rr][i];
+  if (groups > 1) {
+    *reinterpret_cast<f32x4*>(sum_o[threadIdx.x]) = o;
     __syncthreads();
-    for (int k = 0; k < waves; ++k) top = fmaxf(top, of_wave[0][r * waves + k]);
-    const float ref = top == -INFINITY ? 0.f : top;
-    float sum = 0.f;
-    for (int i = u; i < n; i += per_row) {
-      const float w = __builtin_amdgcn_exp2f(w_part[r][i] - ref);
-      w_part[r][i] = w;
-      sum += w * l_part[r][i];
-    }
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) sum += __shfl_xor(sum, d);
-    of_wave[1][threadIdx.x >> 6] = sum;
-    __syncthreads();
-    const int rr = n_rows == 2 ? mine / (kLatent / 4) : 0;  // the row of this thread's piece
-    sum = 0.f;
-    top = -INFINITY;
-    for (int k = 0; k < waves; ++k) sum += of_wave[1][rr * waves + k], top = fmaxf(top, of_wave[0][rr * waves + k]);
-    f32x4 o = {};
-    const float* const src = p.parts + (int64_t)row * kLatent + feature;
-    int i = group;
-    for (; i + 3 * groups < n; i += 4 * groups) {
-      f32x4 x[4];
-#pragma unroll
-      for (int k = 0; k < 4; ++k) x[k] = *reinterpret_cast<const f32x4*>(src + (int64_t)place[i + k * groups] * m_rows * kLatent);
-#pragma unroll
-      for (int k = 0; k < 4; ++k) o += x[k] * w_part[rr][i + k * groups];
-    }
-    for (; i < n; i += groups) o += *reinterpret_cast<const f32x4*>(src + (int64_t)place[i] * m_rows * kLatent) * w_part[rr][i];
-    if (groups > 1) {
-      *reinterpret_cast<f32x4*>(sum_o[threadIdx.x]) = o;
-      __syncthreads();
-      if (group == 0)
-        for (int k = 1; k < groups; ++k) o += *reinterpret_cast<const f32x4*>(sum_o[k * lanes + mine]);
-    }
-    if (group == 0 && row < join.rows) {
-      const int at = join.row0 + row, tok = at / p.H, head = at - tok * p.H;
-      o = sum == 0.f ? f32x4{} : o * (1.f / sum);
-      const u32x2 out = {pack_bf16x2(o[0], o[1]), pack_bf16x2(o[2], o[3])};
-      *reinterpret_cast<u32x2*>(p.o + (int64_t)tok * p.o_ts + head * p.o_hs + feature) = out;
-      if (feature == 0) p.lse[head * p.lse_hs + tok] = sum == 0.f ? -INFINITY : (top == -INFINITY ? 0.f : top) + __builtin_amdgcn_logf(sum);
-    }
+    if (group == 0)
+      for (int k = 1; k < groups; ++k) o += *reinterpret_cast<const f32x4*>(sum_o[k * pieces + mine]);
+  }
+  if (group == 0 && row < join.rows) {
+    const int at = join.row0 + row, tok = at / p.H, head = at - tok * p.H;
+    o = sum == 0.f ? f32x4{} : o * (1.f / sum);
+    const u32x2 out = {pack_bf16x2(o[0], o[1]), pack_bf16x2(o[2], o[3])};
+    *reinterpret_cast<u32x2*>(p.o + (int64_t)tok * p.o_ts + head * p.o_hs + feature) = out;
+    if (feature == 0) p.lse[head * p.lse_hs + tok] = sum == 0.f ? -INFINITY : (top == -INFINITY ? 0.f : top) + __builtin_amdgcn_logf(sum);
   }
 }
 
@@ -244,14 +227,14 @@ LatentPlan plan_of(const pith_latent_attn_args* a) {
   pl.max_items = (int)items;
   const int units = (m == kM ? 2 : 1) * compute_units_or_default() & ~7;  // two workgroups a compute unit, or one
   pl.groups = units < 8 ? 8 : units > kMaxGroups ? kMaxGroups : units;
-  int shares = 1;
+  int shares = m / 2;  // a share is what the threads of a workgroup hold, or less where there are few row blocks
   while (shares < 4 * m && shares * items < 1024) shares *= 2;
   pl.join_shares = shares;
   const auto up = [](int64_t x) { return (x + 255) & ~(int64_t)255; };
   pl.joins_at = 256;
   pl.stats_at = pl.joins_at + up(items * (int64_t)sizeof(LatentJoin));
-  pl.parts_at = pl.stats_at + up((int64_t)kSlots * pl.groups * m * sizeof(float2));
-  pl.bytes = pl.parts_at + (int64_t)kSlots * pl.groups * m * kLatent * 4;
+  pl.parts_at = pl.stats_at + up((int64_t)2 * pl.groups * m * sizeof(float2));
+  pl.bytes = pl.parts_at + (int64_t)2 * pl.groups * m * kLatent * 4;
   return pl;
 }
 

@@ -34,7 +34,7 @@ __global__ __launch_bounds__(kThreads, 2) void latent_attn_wide_kernel(LatentAtt
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int kg = wave & 3, set = wave >> 2;
   Walk<kM, kKeys> walk;
-  if (!walk.start<true>(p, lane)) return;
+  if (!walk.start(p, lane)) return;
 
   do {
     const SeqWork& s = walk.s;
@@ -87,8 +87,8 @@ __global__ __launch_bounds__(kThreads, 2) void latent_attn_wide_kernel(LatentAtt
         const TileLoads<FP8, kKeys> loads(p, next_page, key, last, lds + into * T::kBytes, wave);
         score<FP8, J, kSteps>(kt, key_at, pe_at, true, sc, q, x, [&](int step) __attribute__((always_inline)) {
           if (!more) return;  // (wave-uniform)
-          if (step < T::kLoads) loads.issue(step, ln);
-          if (step == 7 && T::kLoads == 9) loads.issue(8, ln);
+          if (2 * step < T::kLoads) loads.issue(2 * step, ln);
+          if (2 * step + 1 < T::kLoads) loads.issue(2 * step + 1, ln);
         });
         if (more) next_page = page_of(p, table, key + kKeys, last);
       }
