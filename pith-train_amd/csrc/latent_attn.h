@@ -38,7 +38,7 @@ struct LatentAttnParams {
   int* items;         // number of row blocks of this call
   LatentJoin* joins;  // [row blocks]
   float2* stats;      // [slots][M] reference (in bits) and sum
-  float* parts;       // [slots][M][512]; slot 2 i: workgroup i's part that begins with its range, 2 i + 1: one that begins later
+  float* parts;       // [slots][M * 512] (part_at); slot 2 i: workgroup i's part that begins with its range, 2 i + 1: one that begins later
   int max_items;      // capacity of joins
 };
 
@@ -101,7 +101,7 @@ struct Walk {
       blocks_total += __builtin_amdgcn_readlane(sk, 63);
     }
     if (blockIdx.x == 0 && threadIdx.x == 0) *p.items = min(blocks_total, p.max_items);
-    per = (total + (int)gridDim.x - 1) / (int)gridDim.x;
+    per = __builtin_amdgcn_readfirstlane((total + (int)gridDim.x - 1) / (int)gridDim.x);  // (divisions leave the scalar registers)
     begin = at = blockIdx.x * per;
     end = min(at + per, total);  // (the host has bounded total + gridDim.x)
     if (at >= end) return false;
@@ -121,7 +121,7 @@ struct Walk {
       item += __builtin_amdgcn_readlane(sk, 63);
     }
     s = seq_work<M, KEYS>(p, b);
-    block = (at - before) / s.tiles;
+    block = __builtin_amdgcn_readfirstlane((at - before) / s.tiles);
     tile = at - before - block * s.tiles;
     return true;
   }
@@ -157,6 +157,12 @@ struct Walk {
 
 // ---------------------------------------------------------------------------------------------
 // Tiles
+
+// load_lds16 from an address of each lane's own.
+__device__ __forceinline__ void load_lds16_at(const void* src, char* dst_wave) {
+  const uint32_t lds_addr = (uint32_t)(uintptr_t)(lds_char*)dst_wave;
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" : : "s"(lds_addr), "v"(src) : "memory");
+}
 
 template <bool FP8, int KEYS>
 struct LatentTile {
@@ -398,38 +404,74 @@ __device__ __forceinline__ void mask_scores(const LatentAttnParams& p, const Seq
 template <bool TREE, int KEYS>
 __device__ __forceinline__ bool partial_tile(const SeqWork& s, int key0) { return key0 + KEYS > s.len - s.n + (TREE ? 0 : 1); }
 
-// Operand B fragments of a query row: 32 latent features a step from `latent` on (e4m3 keys are read 16 features at a time: steps 2 i, 2 i + 1 then contract
-// features 64 i + 16 g + {0..7, 8..15}), then two rotary steps.
-template <bool FP8, int Q>
-__device__ __forceinline__ void load_query(const LatentAttnParams& p, const SeqWork& s, int row, int latent, int g, bf16x8 (&q)[Q]) {
-  const int tok = row / p.H, head = row - tok * p.H;
-  const __bf16* ql = p.q_latent + (int64_t)(s.tok0 + tok) * p.q_ts + head * p.q_hs + latent;
-  const __bf16* qp = p.q_pe + (int64_t)(s.tok0 + tok) * p.q_pe_ts + head * p.q_pe_hs;
-#pragma unroll
-  for (int i = 0; i < Q - 2; ++i) q[i] = *reinterpret_cast<const bf16x8*>(ql + (FP8 ? 64 * (i >> 1) + 16 * g + 8 * (i & 1) : 32 * i + 8 * g));
-#pragma unroll
-  for (int i = 0; i < 2; ++i) q[Q - 2 + i] = *reinterpret_cast<const bf16x8*>(qp + 32 * i + 8 * g);
+// The lane's number, formed on the spot: it (and what follows from it) takes no register from tile to tile.
+__device__ __forceinline__ int lane_here() {
+  int lane;
+  asm volatile("v_mbcnt_lo_u32_b32 %0, -1, 0\n\tv_mbcnt_hi_u32_b32 %0, -1, %0" : "=v"(lane));
+  return lane;
 }
 
-// The queries have to be there before a walk: left to their first use, the compiler's waits for them would stand in its loop and wait for the tiles in
-// flight in every turn.
-template <int J, int Q>
-__device__ __forceinline__ void pin_queries(bf16x8 (&q)[J][Q]) {
-#pragma unroll
-  for (int j = 0; j < J; ++j)
-#pragma unroll
-    for (int i = 0; i < Q; ++i) asm volatile("" : "+v"(q[j][i]));
+// A wave-uniform address that the compiler formed in vector registers.
+__device__ __forceinline__ const char* scalar_pointer(const void* x) {
+  const uint64_t a = reinterpret_cast<uint64_t>(x);
+  const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)a), hi = __builtin_amdgcn_readfirstlane((uint32_t)(a >> 32));
+  return reinterpret_cast<const char*>((uint64_t)hi << 32 | lo);
 }
 
-// Results of one row (16 N features of the wave from f0 on) as bf16, and its lse by one lane; or, where the segment is a part, sums, maximum and
-// unnormalised results in the workspace.
+// Query rows row0 .. of the walk's row block into LDS, laid out like the rows of a bf16 tile of M keys: wave w brings rows 8 w .. 8 w + 7 (M = 16: the first
+// two waves). Fetched straight into registers, a fragment touches 16 rows, every lane of a quad on a line of its own, which the address unit serves
+// at one lane a cycle: the 36 fragments of 64 rows took a workgroup 9 us in front of its first tile. Rows behind the block's last one are that one.
+template <int M, typename W>
+__device__ __forceinline__ void stage_queries(const LatentAttnParams& p, const W& walk, char* area, int wave, int lane) {
+  using T = LatentTile<false, M>;
+  if (8 * wave >= M) return;
+  const int last = walk.rows(p) - 1, row0 = walk.block * M;
+  int tok = __builtin_amdgcn_readfirstlane((row0 + min(8 * wave, last)) / p.H), head = row0 + min(8 * wave, last) - tok * p.H;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    load_lds16(scalar_pointer(p.q_latent + (int64_t)(walk.s.tok0 + tok) * p.q_ts + head * p.q_hs), (16 * lane) ^ (16 * tile_swizzle(8 * wave + i)),
+               area + (8 * wave + i) * T::kLatentRow);
+    if (8 * wave + i < last && ++head == p.H) head = 0, ++tok;
+  }
+  const int piece = (lane & 15) ^ pe_swizzle(4 * wave + (lane >> 4));
+  const int row = row0 + min(8 * wave + 4 * (piece >> 3) + (lane >> 4), last);
+  const int t = row / p.H, h = row - t * p.H;
+  load_lds16_at(p.q_pe + (int64_t)(walk.s.tok0 + t) * p.q_pe_ts + h * p.q_pe_hs + 8 * (piece & 7), area + T::kPe + wave * 1024);
+}
+
+// Operand B fragments of staged row `row`: 32 latent features a step from `latent` on (e4m3 keys are read 16 features at a time: steps 2 i, 2 i + 1 then
+// contract features 64 i + 16 g + {0..7, 8..15}), then two rotary steps.
+template <bool FP8, int M, int Q>
+__device__ __forceinline__ void read_query(const char* area, int row, int latent, int g, bf16x8 (&q)[Q]) {
+  using T = LatentTile<false, M>;
+  asm volatile("" : "+v"(row), "+v"(g));  // the places are formed here, not kept (and spilled) from segment to segment
+  const char* const rows = area + row * T::kLatentRow + 2 * latent;
+#pragma unroll
+  for (int i = 0; i < Q - 2; ++i) {
+    const int piece = FP8 ? 8 * (i >> 1) + 2 * g + (i & 1) : 4 * i + g;
+    q[i] = *reinterpret_cast<const bf16x8*>(rows + ((piece ^ tile_swizzle(row)) << 4));
+  }
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+    q[Q - 2 + i] = *reinterpret_cast<const bf16x8*>(area + T::kPe + pe_row(row) * 256 + (((8 * ((row >> 2) & 1) + 4 * i + g) ^ pe_swizzle(pe_row(row))) << 4));
+}
+
+// Results of a lane's row of group r (16 N features of the wave from 16 N wave on) as bf16, and its lse by one lane; or, where the segment is a part,
+// reference, sum and unnormalised results in the workspace: there result vector n of a wave lies as the wave holds it, 16 bytes a lane (part_at),
+// because row by row an instruction would touch 16 of them.
+template <int M>
+__device__ __forceinline__ int64_t part_at(int64_t slot, int group, int vector, int lane) {  // vector: N wave + n; in floats
+  return ((slot * (M / 16) + group) * (kLatent / 16) + vector) * 256 + 4 * lane;
+}
 template <bool FP8, int M, int N, typename W>
-__device__ __forceinline__ void store_row(const LatentAttnParams& p, const W& walk, const f32x4 (&acc)[N], float top, float sum, int row, int f0, int g, bool first) {
-  if (row >= walk.rows(p)) return;
+__device__ __forceinline__ void store_row(const LatentAttnParams& p, const W& walk, const f32x4 (&acc)[N], float top, float sum, int r, int wave, int lane) {
+  const int row = 16 * r + (lane & 15), g = lane >> 4;
+  const bool first = wave == 0 && g == 0;
   if (walk.whole()) {
+    if (row >= walk.rows(p)) return;
     const int at = walk.block * M + row, tok = walk.s.tok0 + at / p.H, head = at % p.H;
     const float inv = 1.f / sum;
-    __bf16* const dst = p.o + (int64_t)tok * p.o_ts + head * p.o_hs + f0;
+    __bf16* const dst = p.o + (int64_t)tok * p.o_ts + head * p.o_hs + 16 * N * wave;
 #pragma unroll
     for (int n = 0; n < N; n += 2) {
       const f32x4 a = sum == 0.f ? f32x4{} : acc[n] * inv, d = sum == 0.f ? f32x4{} : acc[n + 1] * inv;
@@ -443,11 +485,10 @@ __device__ __forceinline__ void store_row(const LatentAttnParams& p, const W& wa
     }
     if (first) p.lse[head * p.lse_hs + tok] = sum == 0.f ? -INFINITY : top + __builtin_amdgcn_logf(sum);
   } else {
-    const int64_t part = walk.slot();
-    float* const dst = p.parts + (part * M + row) * kLatent + f0;
+    const int64_t slot = walk.slot();
 #pragma unroll
-    for (int n = 0; n < N; ++n) *reinterpret_cast<f32x4*>(dst + feature_of<FP8>(n, g)) = acc[n];
-    if (first) p.stats[part * M + row] = make_float2(top, sum);
+    for (int n = 0; n < N; ++n) *reinterpret_cast<f32x4*>(p.parts + part_at<M>(slot, r, N * wave + n, lane)) = acc[n];
+    if (first) p.stats[slot * M + row] = make_float2(top, sum);
   }
 }
 

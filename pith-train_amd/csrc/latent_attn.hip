@@ -50,20 +50,26 @@ __global__ __launch_bounds__(kThreads, 2) void latent_attn_kernel(LatentAttnPara
     const int n_tiles = walk.n_tiles(), last = max(s.len - 1, 0);
     const int row = walk.block * kM + min(c, walk.rows(p) - 1);
     const ScalarTable table = (ScalarTable)(uintptr_t)(p.table + walk.b * p.table_rs);
-    bf16x8 q[1][Q];
-    load_query<FP8>(p, s, row, half * (kLatent / 2), g, q[0]);
     f32x4 acc[8] = {};
     float m = -INFINITY, l = 0.f;  // reference and sum (this lane's keys) of the row
 
     __syncthreads();  // the ring's slots and the exchange are free: every wave is through with the segment before
     const int key16 = walk.tile * kKeys + 16 * (wave >> 1);  // this wave's sixteen of the first tile
-#pragma unroll 1
-    for (int i = 0; i < min(kRing, n_tiles); ++i) {
+    const auto request = [&](int i) __attribute__((always_inline)) {
       const int key = key16 + i * kKeys;
       TileLoads<FP8, kKeys>(p, page_of(p, table, key, last), key, last, lds + i * T::kBytes, wave).issue_all(lane);
-    }
+    };
+    bf16x8 q[1][Q];
+    char* const staged = lds + T::kBytes;  // the slots behind the first tile's
+    stage_queries<kM>(p, walk, staged, wave, lane);
+    request(0);
     int next_page = page_of(p, table, key16 + kRing * kKeys, last);
-    pin_queries(q);
+    wait_loads<T::kLoads>();  // the queries, of the waves that brought some
+    __syncthreads();
+    read_query<FP8, kM>(staged, c, half * (kLatent / 2), g, q[0]);
+    __syncthreads();
+#pragma unroll 1
+    for (int i = 1; i < min(kRing, n_tiles); ++i) request(i);
     int slot = 0;
     for (int i = 0; i < n_tiles; ++i) {
       const int key0 = (walk.tile + i) * kKeys;
@@ -130,91 +136,96 @@ __global__ __launch_bounds__(kThreads, 2) void latent_attn_kernel(LatentAttnPara
       }
       slot = slot + 1 == kRing ? 0 : slot + 1;
     }
-    store_row<FP8, kM>(p, walk, acc, m, quad_sum(l), c, 128 * wave, g, wave == 0 && g == 0);
+    store_row<FP8, kM>(p, walk, acc, m, quad_sum(l), 0, wave, lane);
     walk.leave_join(p);
   } while (walk.next(p));
 }
 
-constexpr int kJoinThreads = 256;
+constexpr int kJoinThreads = 512;
 constexpr int kMaxGroups = 512;  // workgroups of the attention kernel, at most: kMaxGroups + 1 parts of a row block
 
-// Joins the parts of a row block: o = sum_i w_i O_i / sum_i w_i l_i, w_i = 2^(m_i - max m). blockIdx.x: row block, blockIdx.y: which of gridDim.y
-// equal shares of its m_rows * 512 results, 1024 of them at most. The weights of a row are formed first, in one pass over its references and sums, so that the loads of the
-// sums over the parts do not wait for one another; where a share has fewer pieces of four features than there are threads, several groups of threads
-// take every other part and add up in LDS.
-__global__ __launch_bounds__(kJoinThreads) void latent_join_kernel(LatentAttnParams p, int m_rows) {
-  __shared__ __attribute__((aligned(16))) float sum_o[kJoinThreads][4];
-  __shared__ float w_part[2][kMaxGroups + 1], l_part[2][kMaxGroups + 1];
-  __shared__ float of_wave[2][kJoinThreads / 64];
+// Joins the parts of a row block: o = sum_i w_i O_i / sum_i w_i l_i, w_i = 2^(m_i - max m). blockIdx.x: row block; blockIdx.y: group of 16 rows of it,
+// and which `vectors` of its 32 result vectors (part_at). The weights of the rows are formed first, in one pass over their references and sums, so that
+// the loads of the sums over the parts do not wait for one another; where a workgroup has fewer vectors than waves, several waves take every other
+// part and add up in LDS.
+template <bool FP8, int M>
+__global__ __launch_bounds__(kJoinThreads) void latent_join_kernel(LatentAttnParams p, int vectors) {
+  constexpr int kWaves = kJoinThreads / 64, N = M == kM ? 8 : 4;  // N: vectors of a wave of the attention kernel
+  constexpr int kPerRow = kJoinThreads / 16;                     // threads that form the weights of a row
+  __shared__ __attribute__((aligned(16))) f32x4 sum_o[kJoinThreads];
+  __shared__ float weights[16][kMaxGroups + 1];
+  __shared__ float inverse[16];  // of the rows' sums (0: nothing seen)
   const int items = *p.items;
   const LatentJoin join = p.joins[blockIdx.x];  // (beyond `items` it is whatever the workspace held)
-  if ((int)blockIdx.x >= items || join.first == join.last) return;
+  const int shares = kLatent / 16 / vectors, r = blockIdx.y / shares;
+  if ((int)blockIdx.x >= items || join.first == join.last || 16 * r >= join.rows) return;
   const int n = min(join.last / 2 - join.first / 2 + 1, kMaxGroups + 1);  // parts: the first slot, then the even ones up to the last
   const auto slot = [&](int i) { return (int64_t)(i == 0 ? join.first : 2 * (join.first / 2 + i)); };
-  const int pieces = m_rows * (kLatent / 4) / gridDim.y;  // of this share: a power of two
-  const int groups = kJoinThreads / pieces, mine = threadIdx.x % pieces, group = threadIdx.x / pieces;
-  const int n_rows = pieces > kLatent / 4 ? 2 : 1, per_row = kJoinThreads / n_rows;  // rows of the share, threads that form the weights of each
-  const int r = threadIdx.x / per_row, u = threadIdx.x % per_row, waves = per_row / 64;
-  const int first = blockIdx.y * pieces;
-  const int row = (first + mine) / (kLatent / 4), feature = 4 * ((first + mine) % (kLatent / 4));
-  float top = -INFINITY;
-  for (int i = u; i < n; i += per_row) {
-    const float2 st = p.stats[slot(i) * m_rows + first / (kLatent / 4) + r];
-    w_part[r][i] = st.x;
-    l_part[r][i] = st.y;
-    top = fmaxf(top, st.x);
-  }
+  {
+    const int row = threadIdx.x / kPerRow, u = threadIdx.x % kPerRow;
+    float top = -INFINITY, sum = 0.f;
+    for (int i = u; i < n; i += kPerRow) {
+      const float m = p.stats[slot(i) * M + 16 * r + row].x;
+      weights[row][i] = m;
+      top = fmaxf(top, m);
+    }
 #pragma unroll
-  for (int d = 1; d < 64; d <<= 1) top = fmaxf(top, __shfl_xor(top, d));
-  of_wave[0][threadIdx.x >> 6] = top;
-  __syncthreads();
-  for (int k = 0; k < waves; ++k) top = fmaxf(top, of_wave[0][r * waves + k]);
-  const float ref = top == -INFINITY ? 0.f : top;
-  float sum = 0.f;
-  for (int i = u; i < n; i += per_row) {
-    const float w = __builtin_amdgcn_exp2f(w_part[r][i] - ref);
-    w_part[r][i] = w;
-    sum += w * l_part[r][i];
-  }
+    for (int d = 1; d < kPerRow; d <<= 1) top = fmaxf(top, __shfl_xor(top, d));
+    const float ref = top == -INFINITY ? 0.f : top;
+    for (int i = u; i < n; i += kPerRow) {
+      const float w = __builtin_amdgcn_exp2f(weights[row][i] - ref);
+      weights[row][i] = w;
+      sum += w * p.stats[slot(i) * M + 16 * r + row].y;
+    }
 #pragma unroll
-  for (int d = 1; d < 64; d <<= 1) sum += __shfl_xor(sum, d);
-  of_wave[1][threadIdx.x >> 6] = sum;
+    for (int d = 1; d < kPerRow; d <<= 1) sum += __shfl_xor(sum, d);
+    if (u == 0) {
+      inverse[row] = sum == 0.f ? 0.f : 1.f / sum;
+      if (blockIdx.y % shares == 0 && 16 * r + row < join.rows) {
+        const int at = join.row0 + 16 * r + row, tok = at / p.H;
+        p.lse[(at - tok * p.H) * p.lse_hs + tok] = sum == 0.f ? -INFINITY : ref + __builtin_amdgcn_logf(sum);
+      }
+    }
+  }
   __syncthreads();
-  const int rr = n_rows == 2 ? mine / (kLatent / 4) : 0;  // the row of this thread's piece
-  sum = 0.f;
-  top = -INFINITY;
-  for (int k = 0; k < waves; ++k) sum += of_wave[1][rr * waves + k], top = fmaxf(top, of_wave[0][rr * waves + k]);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 15;
+  const int mine = wave % vectors, group = wave / vectors, groups = kWaves / vectors;
+  const int vector = blockIdx.y % shares * vectors + mine;
   f32x4 o = {};
-  const float* const src = p.parts + (int64_t)row * kLatent + feature;
   int i = group;
   for (; i + 3 * groups < n; i += 4 * groups) {
     f32x4 x[4];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) x[k] = *reinterpret_cast<const f32x4*>(src + slot(i + k * groups) * m_rows * kLatent);
+    for (int k = 0; k < 4; ++k) x[k] = *reinterpret_cast<const f32x4*>(p.parts + part_at<M>(slot(i + k * groups), r, vector, lane));
 #pragma unroll
-    for (int k = 0; k < 4; ++k) o += x[k] * w_part[rr][i + k * groups];
+    for (int k = 0; k < 4; ++k) o += x[k] * weights[c][i + k * groups];
   }
-  for (; i < n; i += groups) o += *reinterpret_cast<const f32x4*>(src + slot(i) * m_rows * kLatent) * w_part[rr][i];
+  for (; i < n; i += groups) o += *reinterpret_cast<const f32x4*>(p.parts + part_at<M>(slot(i), r, vector, lane)) * weights[c][i];
   if (groups > 1) {
-    *reinterpret_cast<f32x4*>(sum_o[threadIdx.x]) = o;
+    sum_o[threadIdx.x] = o;
     __syncthreads();
-    if (group == 0)
-      for (int k = 1; k < groups; ++k) o += *reinterpret_cast<const f32x4*>(sum_o[k * pieces + mine]);
+    if (group > 0) return;
+    for (int k = 1; k < groups; ++k) o += sum_o[64 * (k * vectors + mine) + lane];
   }
-  if (group == 0 && row < join.rows) {
-    const int at = join.row0 + row, tok = at / p.H, head = at - tok * p.H;
-    o = sum == 0.f ? f32x4{} : o * (1.f / sum);
-    const u32x2 out = {pack_bf16x2(o[0], o[1]), pack_bf16x2(o[2], o[3])};
-    *reinterpret_cast<u32x2*>(p.o + (int64_t)tok * p.o_ts + head * p.o_hs + feature) = out;
-    if (feature == 0) p.lse[head * p.lse_hs + tok] = sum == 0.f ? -INFINITY : (top == -INFINITY ? 0.f : top) + __builtin_amdgcn_logf(sum);
-  }
+  if (16 * r + c >= join.rows) return;
+  const int at = join.row0 + 16 * r + c, tok = at / p.H, head = at - tok * p.H;
+  o = inverse[c] == 0.f ? f32x4{} : o * inverse[c];
+  *reinterpret_cast<u32x2*>(p.o + (int64_t)tok * p.o_ts + head * p.o_hs + 16 * N * (vector / N) + feature_of<FP8>(vector % N, lane >> 4)) =
+      u32x2{pack_bf16x2(o[0], o[1]), pack_bf16x2(o[2], o[3])};
+}
+
+template <int M>
+void launch_join(const LatentAttnParams& p, bool fp8, int vectors, hipStream_t s) {
+  const dim3 grid(p.max_items, M / 16 * (kLatent / 16 / vectors));
+  if (fp8) latent_join_kernel<true, M><<<grid, kJoinThreads, 0, s>>>(p, vectors);
+  else latent_join_kernel<false, M><<<grid, kJoinThreads, 0, s>>>(p, vectors);
 }
 
 struct LatentPlan {
   int rows;        // of a workgroup: 16 or 64
   int groups;      // workgroups of the attention kernel, a multiple of 8
   int max_items;   // row blocks at most
-  int join_shares;
+  int join_vectors;  // of a workgroup of the join, see there
   int64_t joins_at, stats_at, parts_at, bytes;  // workspace
 };
 
@@ -227,9 +238,8 @@ LatentPlan plan_of(const pith_latent_attn_args* a) {
   pl.max_items = (int)items;
   const int units = (m == kM ? 2 : 1) * compute_units_or_default() & ~7;  // two workgroups a compute unit, or one
   pl.groups = units < 8 ? 8 : units > kMaxGroups ? kMaxGroups : units;
-  int shares = m / 2;  // a share is what the threads of a workgroup hold, or less where there are few row blocks
-  while (shares < 4 * m && shares * items < 1024) shares *= 2;
-  pl.join_shares = shares;
+  pl.join_vectors = 8;  // a vector a wave, or fewer where there are few row blocks
+  while (pl.join_vectors > 1 && items * (m / 16) * (kLatent / 16 / pl.join_vectors) < 512) pl.join_vectors /= 2;
   const auto up = [](int64_t x) { return (x + 255) & ~(int64_t)255; };
   pl.joins_at = 256;
   pl.stats_at = pl.joins_at + up(items * (int64_t)sizeof(LatentJoin));
@@ -302,8 +312,12 @@ extern "C" int pith_latent_attn(const pith_latent_attn_args* a, pith_stream_t st
   const bool fp8 = a->cache.dtype == PITH_FP8_E4M3, tree = a->tree_mask != nullptr;
   hipStream_t s = (hipStream_t)stream;
   begin_launch();
-  if (pl.rows == kM) launch_narrow(p, fp8, tree, pl.groups, s);
-  else launch_latent_wide(p, fp8, tree, pl.groups, s);
-  latent_join_kernel<<<dim3(pl.max_items, pl.join_shares), kJoinThreads, 0, s>>>(p, pl.rows);
+  if (pl.rows == kM) {
+    launch_narrow(p, fp8, tree, pl.groups, s);
+    launch_join<kM>(p, fp8, pl.join_vectors, s);
+  } else {
+    launch_latent_wide(p, fp8, tree, pl.groups, s);
+    launch_join<kWideRows>(p, fp8, pl.join_vectors, s);
+  }
   return check_launch(who);
 }

@@ -31,18 +31,15 @@ __global__ __launch_bounds__(kThreads, 2) void latent_attn_wide_kernel(LatentAtt
   __shared__ __attribute__((aligned(1024))) char lds[kRing * T::kBytes + kExchangeBytes];
   char* const exchange = lds + kRing * T::kBytes;
   int* const stamp = reinterpret_cast<int*>(exchange + kStamp);
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int kg = wave & 3, set = wave >> 2;
   Walk<kM, kKeys> walk;
-  if (!walk.start(p, lane)) return;
+  if (!walk.start(p, threadIdx.x & 63)) return;
 
   do {
     const SeqWork& s = walk.s;
     const int n_tiles = walk.n_tiles(), last = max(s.len - 1, 0);
     const ScalarTable table = (ScalarTable)(uintptr_t)(p.table + walk.b * p.table_rs);
-    bf16x8 q[J][Q];
-#pragma unroll
-    for (int j = 0; j < J; ++j) load_query<FP8>(p, s, walk.block * kM + min(16 * (J * set + j) + (lane & 15), walk.rows(p) - 1), 0, lane >> 4, q[j]);
     f32x4 acc[kGroups][4] = {};
     float m[kGroups], l[J];  // references of the lane's row of every group, sums (this lane's keys) of those it scores
 #pragma unroll
@@ -53,13 +50,23 @@ __global__ __launch_bounds__(kThreads, 2) void latent_attn_wide_kernel(LatentAtt
     __syncthreads();  // the ring's slots and the exchange are free: every wave is through with the segment before
     if (threadIdx.x == 0) *stamp = 0;
     const int key16 = walk.tile * kKeys + 16 * (wave >> 1);  // this wave's sixteen of the first tile
-#pragma unroll 1
-    for (int i = 0; i < min(kRing - 1, n_tiles); ++i) {
+    const int lane = lane_here();
+    const auto request = [&](int i) __attribute__((always_inline)) {
       const int key = key16 + i * kKeys;
       TileLoads<FP8, kKeys>(p, page_of(p, table, key, last), key, last, lds + i * T::kBytes, wave).issue_all(lane);
-    }
+    };
+    bf16x8 q[J][Q];
+    char* const staged = lds + T::kBytes;  // the slots behind the first tile's
+    static_assert((kRing - 1) * T::kBytes >= LatentTile<false, kM>::kBytes, "the queries are staged in what the first tile leaves of the ring");
+    stage_queries<kM>(p, walk, staged, wave, lane);
+    request(0);
     int next_page = page_of(p, table, key16 + (kRing - 1) * kKeys, last);
-    pin_queries(q);
+    wait_loads<T::kLoads>();
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < J; ++j) read_query<FP8, kM>(staged, 16 * (J * set + j) + (lane & 15), 0, lane >> 4, q[j]);
+    __syncthreads();
+    if (kRing > 2 && n_tiles > 1) request(1);
     int slot = 0;
     for (int i = 0; i < n_tiles; ++i) {
       const int key0 = (walk.tile + i) * kKeys;
@@ -72,8 +79,7 @@ __global__ __launch_bounds__(kThreads, 2) void latent_attn_wide_kernel(LatentAtt
       slot = slot + 1 == kRing ? 0 : slot + 1;
       const bool partial = partial_tile<TREE, kKeys>(s, key0);
       // What the lane's number gives is formed anew in every tile: kept across the loop it would be spilled.
-      int ln = lane;
-      asm volatile("" : "+v"(ln));
+      const int ln = lane_here();
       const int c = ln & 15, g = ln >> 4;
 
       f32x4 x[J], sc = {};
@@ -161,7 +167,7 @@ __global__ __launch_bounds__(kThreads, 2) void latent_attn_wide_kernel(LatentAtt
       }
     }
 
-    const int c = lane & 15, g = lane >> 4;
+    const int ln = lane_here(), c = ln & 15, g = ln >> 4;
     __syncthreads();  // the last maxima have been read
 #pragma unroll
     for (int j = 0; j < J; ++j) {
@@ -172,7 +178,7 @@ __global__ __launch_bounds__(kThreads, 2) void latent_attn_wide_kernel(LatentAtt
 #pragma unroll
     for (int r = 0; r < kGroups; ++r) {
       const f32x4 k = *reinterpret_cast<const f32x4*>(exchange + kMaxima + 16 * (16 * r + c));
-      store_row<FP8, kM>(p, walk, acc[r], m[r], (k[0] + k[1]) + (k[2] + k[3]), 16 * r + c, 64 * wave, g, wave == 0 && g == 0);
+      store_row<FP8, kM>(p, walk, acc[r], m[r], (k[0] + k[1]) + (k[2] + k[3]), r, wave, ln);
     }
     walk.leave_join(p);
   } while (walk.next(p));
