@@ -169,7 +169,7 @@ struct LatentTile {
   static constexpr int kLatentRow = FP8 ? kLatent : 2 * kLatent;  // bytes
   static constexpr int kPe = KEYS * kLatentRow;                   // offsets in a tile
   static constexpr int kScale = kPe + KEYS * 2 * kRope;           // [KEYS] fp32
-  static constexpr int kBytes = kScale + (FP8 ? KEYS * 4 : 0);
+  static constexpr int kBytes = kScale + (FP8 ? 256 : 0);  // (tiles begin at multiples of 256)
   static constexpr int kLoads = FP8 ? 6 : 9;  // direct loads of a wave: eight rows
 };
 
@@ -275,22 +275,30 @@ __device__ __forceinline__ bf16x8 widen(uint32_t w0, uint32_t w1) {
   return bf16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
 
+__device__ __forceinline__ uint32_t lds_address(const char* x) { return (uint32_t)(uintptr_t)(const lds_char*)x; }
+template <typename V>
+__device__ __forceinline__ const __attribute__((address_space(3))) V* lds_at(uint32_t address) {
+  return (const __attribute__((address_space(3))) V*)(uintptr_t)address;
+}
+
 // Scores of 16 keys against J groups of query rows: STEPS times 64 latent features, then with_pe the 64 rotary ones; between(i) is called in step i. `at` is the place of the lane's
 // first piece (its row, piece g of the swizzled 256 bytes) of the tile; piece 4 k + g lies at ^ (64 k), as rows are multiples of 256 bytes.
 template <bool FP8, int J, int STEPS, int Q, typename Between>
 __device__ __forceinline__ void score(const char* tile, int at, int pe_at, bool with_pe, f32x4 scale, const bf16x8 (&q)[J][Q], f32x4 (&s)[J], Between between) {
+  // XORs on whole addresses: tiles begin at multiples of 256 bytes
+  const uint32_t first = lds_address(tile) + at, pe_first = lds_address(tile) + pe_at;
 #pragma unroll
   for (int j = 0; j < J; ++j) s[j] = f32x4{};
 #pragma unroll
   for (int i = 0; i < STEPS; ++i) {
     bf16x8 k0, k1;
     if constexpr (FP8) {  // sixteen features a lane: two steps
-      const u32x4 raw = *reinterpret_cast<const u32x4*>(tile + (at ^ (64 * (i & 3))) + 256 * (i >> 2));
+      const u32x4 raw = *lds_at<u32x4>((first ^ (64 * (i & 3))) + 256 * (i >> 2));
       k0 = widen(raw[0], raw[1]);
       k1 = widen(raw[2], raw[3]);
     } else {
-      k0 = *reinterpret_cast<const bf16x8*>(tile + (at ^ (128 * (i & 1))) + 256 * (i >> 1));
-      k1 = *reinterpret_cast<const bf16x8*>(tile + (at ^ (128 * (i & 1) + 64)) + 256 * (i >> 1));
+      k0 = *lds_at<bf16x8>((first ^ (128 * (i & 1))) + 256 * (i >> 1));
+      k1 = *lds_at<bf16x8>((first ^ (128 * (i & 1) + 64)) + 256 * (i >> 1));
     }
 #pragma unroll
     for (int j = 0; j < J; ++j) s[j] = mfma16(k0, q[j][2 * i], s[j]);
@@ -303,7 +311,7 @@ __device__ __forceinline__ void score(const char* tile, int at, int pe_at, bool 
     for (int j = 0; j < J; ++j) s[j] *= scale;
   }
   if (with_pe) {
-    const bf16x8 k0 = *reinterpret_cast<const bf16x8*>(tile + pe_at), k1 = *reinterpret_cast<const bf16x8*>(tile + (pe_at ^ 64));
+    const bf16x8 k0 = *lds_at<bf16x8>(pe_first), k1 = *lds_at<bf16x8>(pe_first ^ 64);
 #pragma unroll
     for (int j = 0; j < J; ++j) s[j] = mfma16(k0, q[j][Q - 2], s[j]);
 #pragma unroll
@@ -327,16 +335,20 @@ __device__ __forceinline__ int value_place(int wave, int c, int g) {
   return r * (FP8 ? kLatent : 2 * kLatent) + ((piece ^ tile_swizzle(r)) << 4) + (FP8 ? 8 * (c & 1) : 0);
 }
 
-// Operand A of product n over keys 8 g + e.
+// Operand A of product n over keys 8 g + e; `first`: lds_address of the tile + value_place.
 template <bool FP8>
-__device__ __forceinline__ bf16x8 value_fragment(const char* tile, int at, int n) {
+__device__ __forceinline__ bf16x8 value_fragment(uint32_t first, int n) {
   if constexpr (FP8) {
     typedef __attribute__((ext_vector_type(2))) int i32x2;
     typedef __attribute__((address_space(3))) i32x2 lds_i32x2;
-    const i32x2 raw = __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_i32x2*)(tile + (at ^ (16 * n))));
+    const i32x2 raw = __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_i32x2*)(uintptr_t)(first ^ (16 * n)));
     return widen((uint32_t)raw[0], (uint32_t)raw[1]);
   } else {  // four rows further on the swizzle differs in its lowest bit
-    return lds_read_transposed_at(tile + (at ^ (64 * (n >> 1))) + 8 * (n & 1), tile + (at ^ (64 * (n >> 1) + 16)) + 4 * (2 * kLatent) + 8 * (n & 1));
+    typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(uintptr_t)((first ^ (64 * (n >> 1))) + 8 * (n & 1)));
+    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(uintptr_t)((first ^ (64 * (n >> 1) + 16)) + 4 * (2 * kLatent) + 8 * (n & 1)));
+    typedef __attribute__((ext_vector_type(8))) short s16x8;
+    return __builtin_bit_cast(bf16x8, s16x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]});
   }
 }
 

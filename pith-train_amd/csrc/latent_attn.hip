@@ -126,7 +126,7 @@ __global__ __launch_bounds__(kThreads, 2) void latent_attn_kernel(LatentAttnPara
       }
       const bf16x8 weight = to_bf16x8(y[0], y[1], y[2], y[3], y[4], y[5], y[6], y[7]);  // keys 8 g + e
 #pragma unroll
-      for (int n = 0; n < 8; ++n) acc[n] = mfma16(value_fragment<FP8>(kt, value_at, n), weight, acc[n]);
+      for (int n = 0; n < 8; ++n) acc[n] = mfma16(value_fragment<FP8>(lds_address(kt) + value_at, n), weight, acc[n]);
 
       if (i + kRing < n_tiles) {
         __syncthreads();  // nobody reads this tile any more: its slot is asked to be filled before the next tile is waited for

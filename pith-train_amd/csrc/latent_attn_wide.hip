@@ -88,15 +88,17 @@ __global__ __launch_bounds__(kThreads, 2) void latent_attn_wide_kernel(LatentAtt
         const int key_at = key_row * T::kLatentRow + ((g ^ tile_swizzle(key_row)) << 4);
         const int pe_at = T::kPe + pe_row(key_row) * 256 + (((8 * ((key_row >> 2) & 1) + g) ^ pe_swizzle(pe_row(key_row))) << 4);
         if constexpr (FP8) sc = *reinterpret_cast<const f32x4*>(kt + T::kScale + (16 * kg + 4 * g) * 4);
-        const bool more = i + kRing - 1 < n_tiles;
-        const int key = key16 + (i + kRing - 1) * kKeys;
-        const TileLoads<FP8, kKeys> loads(p, next_page, key, last, lds + into * T::kBytes, wave);
-        score<FP8, J, kSteps>(kt, key_at, pe_at, true, sc, q, x, [&](int step) __attribute__((always_inline)) {
-          if (!more) return;  // (wave-uniform)
-          if (2 * step < T::kLoads) loads.issue(2 * step, ln);
-          if (2 * step + 1 < T::kLoads) loads.issue(2 * step + 1, ln);
-        });
-        if (more) next_page = page_of(p, table, key + kKeys, last);
+        if (i + kRing - 1 < n_tiles) {
+          const int key = key16 + (i + kRing - 1) * kKeys;
+          const TileLoads<FP8, kKeys> loads(p, next_page, key, last, lds + into * T::kBytes, wave);
+          score<FP8, J, kSteps>(kt, key_at, pe_at, true, sc, q, x, [&](int step) __attribute__((always_inline)) {
+            if (2 * step < T::kLoads) loads.issue(2 * step, ln);
+            if (2 * step + 1 < T::kLoads) loads.issue(2 * step + 1, ln);
+          });
+          next_page = page_of(p, table, key + kKeys, last);
+        } else {
+          score<FP8, J, kSteps>(kt, key_at, pe_at, true, sc, q, x, [](int) {});
+        }
       }
       // weights against the references as they are, and whether they will do
       bool beyond = false;
@@ -152,7 +154,7 @@ __global__ __launch_bounds__(kThreads, 2) void latent_attn_wide_kernel(LatentAtt
         clean_tile<FP8, kKeys, kThreads>(kt);
         __syncthreads();
       }
-      const int value_at = value_place<FP8, 64>(wave, c, g);
+      const uint32_t values = lds_address(kt) + value_place<FP8, 64>(wave, c, g);
 #pragma unroll
       for (int ks = 0; ks < 2; ++ks) {
         bf16x8 weight[kGroups];  // keys 32 ks + 8 g + e of the lane's row of each group
@@ -160,7 +162,7 @@ __global__ __launch_bounds__(kThreads, 2) void latent_attn_wide_kernel(LatentAtt
         for (int r = 0; r < kGroups; ++r) weight[r] = *reinterpret_cast<const bf16x8*>(exchange + weight_at(16 * r + c, 4 * ks + g));
 #pragma unroll
         for (int n = 0; n < 4; ++n) {
-          const bf16x8 v = value_fragment<FP8>(kt + 32 * ks * T::kLatentRow, value_at, n);
+          const bf16x8 v = value_fragment<FP8>(values + 32 * ks * T::kLatentRow, n);
 #pragma unroll
           for (int r = 0; r < kGroups; ++r) acc[r][n] = mfma16(v, weight[r], acc[r][n]);
         }
