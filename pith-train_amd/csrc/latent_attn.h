@@ -158,12 +158,6 @@ struct Walk {
 // ---------------------------------------------------------------------------------------------
 // Tiles
 
-// load_lds16 from an address of each lane's own.
-__device__ __forceinline__ void load_lds16_at(const void* src, char* dst_wave) {
-  const uint32_t lds_addr = (uint32_t)(uintptr_t)(lds_char*)dst_wave;
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" : : "s"(lds_addr), "v"(src) : "memory");
-}
-
 template <bool FP8, int KEYS>
 struct LatentTile {
   static constexpr int kLatentRow = FP8 ? kLatent : 2 * kLatent;  // bytes
@@ -231,8 +225,6 @@ struct TileLoads {
   }
 };
 
-__device__ __forceinline__ f32x4 mfma16(bf16x8 a, bf16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
-
 // max / sum over the eight lanes of a row of the 32-row softmax (lane % 8 = 0 .. 7), in all of them
 template <int CTRL>
 __device__ __forceinline__ float dpp(float x) {
@@ -262,23 +254,10 @@ __device__ __forceinline__ float quad_sum(float x) {
   return pair_sum(__int_as_float(r[0]) + __int_as_float(r[1]));
 }
 
-template <int LATER>
-__device__ __forceinline__ void wait_loads() {
-  static_assert(LATER < 64, "vmcnt has six bits");
-  __builtin_amdgcn_s_waitcnt(0x0F70 | (LATER & 15) | ((LATER >> 4) << 14));
-  asm volatile("" ::: "memory");
-}
-
 // Eight e4m3 values (two words) -> bf16, exact.
 __device__ __forceinline__ bf16x8 widen(uint32_t w0, uint32_t w1) {
   const bf16x2 a = fp8x2_to_bf16<false>(w0), b = fp8x2_to_bf16<true>(w0), c = fp8x2_to_bf16<false>(w1), d = fp8x2_to_bf16<true>(w1);
   return bf16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
-}
-
-__device__ __forceinline__ uint32_t lds_address(const char* x) { return (uint32_t)(uintptr_t)(const lds_char*)x; }
-template <typename V>
-__device__ __forceinline__ const __attribute__((address_space(3))) V* lds_at(uint32_t address) {
-  return (const __attribute__((address_space(3))) V*)(uintptr_t)address;
 }
 
 // Scores of 16 keys against J groups of query rows: STEPS times 64 latent features, then with_pe the 64 rotary ones; between(i) is called in step i. `at` is the place of the lane's

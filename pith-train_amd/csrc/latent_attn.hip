@@ -88,7 +88,7 @@ __global__ __launch_bounds__(kThreads, 2) void latent_attn_kernel(LatentAttnPara
         *reinterpret_cast<f32x4*>(exchange + exchange_at(half * kM + c, 4 * kg + g)) = x[0];
       }
       __syncthreads();
-      if (partial && s.n > 1) {
+      if (partial && (TREE || s.n > 1)) {
         clean_tile<FP8, kKeys, kThreads>(kt);
         __syncthreads();
       }
@@ -229,22 +229,28 @@ struct LatentPlan {
   int64_t joins_at, stats_at, parts_at, bytes;  // workspace
 };
 
+// Workgroups of the attention kernel for m rows each: two a compute unit, or one.
+int groups_of(int m) {
+  const int units = (m == kM ? 2 : 1) * compute_units_or_default() & ~7;
+  return units < 8 ? 8 : units > kMaxGroups ? kMaxGroups : units;
+}
+
 LatentPlan plan_of(const pith_latent_attn_args* a) {
   LatentPlan pl = {};
   const int64_t rows = a->T * a->H;
   pl.rows = rows <= kM * a->B ? kM : kWideRows;
-  const int m = pl.rows;
-  const int64_t items = (rows + m - 1) / m + (a->B < a->T ? a->B : a->T);
-  pl.max_items = (int)items;
-  const int units = (m == kM ? 2 : 1) * compute_units_or_default() & ~7;  // two workgroups a compute unit, or one
-  pl.groups = units < 8 ? 8 : units > kMaxGroups ? kMaxGroups : units;
+  pl.groups = groups_of(pl.rows);
+  const auto items = [&](int m) { return (rows + m - 1) / m + (a->B < a->T ? a->B : a->T); };
+  pl.max_items = (int)items(pl.rows);
   pl.join_vectors = 8;  // a vector a wave, or fewer where there are few row blocks
-  while (pl.join_vectors > 1 && items * (m / 16) * (kLatent / 16 / pl.join_vectors) < 512) pl.join_vectors /= 2;
+  while (pl.join_vectors > 1 && pl.max_items * (pl.rows / 16) * (kLatent / 16 / pl.join_vectors) < 512) pl.join_vectors /= 2;
+  // Laid out for whichever kernel needs more: who keeps a workspace from call to call keeps one size.
   const auto up = [](int64_t x) { return (x + 255) & ~(int64_t)255; };
+  const int64_t slot_rows = 2 * std::max<int64_t>(groups_of(kM) * kM, groups_of(kWideRows) * kWideRows);
   pl.joins_at = 256;
-  pl.stats_at = pl.joins_at + up(items * (int64_t)sizeof(LatentJoin));
-  pl.parts_at = pl.stats_at + up((int64_t)2 * pl.groups * m * sizeof(float2));
-  pl.bytes = pl.parts_at + (int64_t)2 * pl.groups * m * kLatent * 4;
+  pl.stats_at = pl.joins_at + up(items(kM) * (int64_t)sizeof(LatentJoin));
+  pl.parts_at = pl.stats_at + up(slot_rows * (int64_t)sizeof(float2));
+  pl.bytes = pl.parts_at + slot_rows * kLatent * 4;
   return pl;
 }
 
@@ -257,7 +263,7 @@ int check_attn(const pith_latent_attn_args* a, const char* who) {
   const int64_t most = a->table_width > 0 && a->table_width > 0x7fffffff / a->cache.page_size ? -1 : a->table_width * a->cache.page_size;
   if (most < 0 || most > 0x7fffffff - 4096) return fail(PITH_ERR_UNSUPPORTED, "%s: page tables of 2^31 rows or more", who);
   const int64_t items = (a->T * a->H + kM - 1) / kM + a->B;
-  if (items * (most / kKeys + 1) > 0x7fffffff - 65536) return fail(PITH_ERR_UNSUPPORTED, "%s: too many row blocks for page tables of that width: call it with fewer tokens at a time", who);
+  if (items > 1 << 22 || items * (most / kKeys + 1) > 0x7fffffff - 65536) return fail(PITH_ERR_UNSUPPORTED, "%s: too many row blocks for page tables of that width: call it with fewer tokens at a time", who);
   return PITH_OK;
 }
 

@@ -150,7 +150,7 @@ __global__ __launch_bounds__(kThreads, 2) void latent_attn_wide_kernel(LatentAtt
       }
 #pragma unroll
       for (int j = 0; j < J; ++j) l[j] += sum[j];
-      if (partial && s.n > 1) {
+      if (partial && (TREE || s.n > 1)) {
         clean_tile<FP8, kKeys, kThreads>(kt);
         __syncthreads();
       }

@@ -1,7 +1,7 @@
 // What the kernels of the latent cache (include/pith_latent.h) share.
 #pragma once
 
-#include "pith_common.h"
+#include "attn_tiles.h"
 #include "pith_latent.h"
 
 namespace pith {
@@ -61,5 +61,28 @@ __device__ __forceinline__ void rotate_pair(uint32_t pair, const __bf16* cos_row
   second = odd * (float)cos_row[kRope / 2 + j] + even * (float)sin_row[kRope / 2 + j];
 }
 __device__ __forceinline__ int64_t clamped_position(int64_t pos, int64_t P) { return pos < 0 ? 0 : (pos >= P ? P - 1 : pos); }
+
+__device__ __forceinline__ f32x4 mfma16(bf16x8 a, bf16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+
+// load_lds16 from an address of each lane's own.
+__device__ __forceinline__ void load_lds16_at(const void* src, char* dst_wave) {
+  const uint32_t lds_addr = (uint32_t)(uintptr_t)(lds_char*)dst_wave;
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" : : "s"(lds_addr), "v"(src) : "memory");
+}
+
+// Until all but the wave's last LATER requests are there.
+template <int LATER>
+__device__ __forceinline__ void wait_loads() {
+  static_assert(LATER < 64, "vmcnt has six bits");
+  __builtin_amdgcn_s_waitcnt(0x0F70 | (LATER & 15) | ((LATER >> 4) << 14));
+  asm volatile("" ::: "memory");
+}
+
+// LDS addresses as numbers, for places that are the XOR of a lane's first one and a constant.
+__device__ __forceinline__ uint32_t lds_address(const char* x) { return (uint32_t)(uintptr_t)(const lds_char*)x; }
+template <typename V>
+__device__ __forceinline__ const __attribute__((address_space(3))) V* lds_at(uint32_t address) {
+  return (const __attribute__((address_space(3))) V*)(uintptr_t)address;
+}
 
 }  // namespace pith

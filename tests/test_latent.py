@@ -269,7 +269,7 @@ def test_direct_loads_are_the_only_users_of_m0(tmp_path):
     """csrc/attn_tiles.h sets M0 inside inline assembly, which the compiler cannot be told about: it must not use the register itself."""
     from pithtrain_amd import build as B
 
-    for src in ("latent_attn.hip", "latent_absorb.hip"):
+    for src in ("latent_attn.hip", "latent_attn_wide.hip", "latent_absorb.hip"):
         out = tmp_path / (src + ".s")
         cmd = [B._hipcc(), *B.HIPCC_FLAGS, *B.SOURCE_FLAGS.get(src, []), "-I", B.INCLUDE_DIR, "-I", B.SRC_DIR, "--cuda-device-only", "-S", os.path.join(B.SRC_DIR, src), "-o", str(out)]
         subprocess.run(cmd, check=True, capture_output=True)

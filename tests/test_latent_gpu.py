@@ -214,6 +214,40 @@ def test_a_row_that_a_token_does_not_see_cannot_reach_it(gpu, bad, tree):
     assert torch.isnan(o[~blind].float()).any()
 
 
+@pytest.mark.parametrize("h", [16, 40])
+@pytest.mark.parametrize("bad", ["latent", "scale", "infinite scale"])
+def test_a_row_of_e4m3_that_a_token_does_not_see_cannot_reach_it(gpu, bad, h):
+    b = Batch(gpu, [3, 3], [70, 3], h, page=16, fp8=True, seed=13)
+    want_o, want_lse = b.attention()
+    for i in range(2):
+        j = b.lengths[i] - 1
+        page, row = b.table[i, j // 16].long(), j % 16
+        if bad == "latent":
+            b.latent.view(torch.uint8)[page, row, 40:] = 0x7F
+        else:
+            b.scale[page, row] = math.nan if bad == "scale" else math.inf
+    blind = torch.tensor([True, True, False] * 2)
+    o, lse = b.attention()
+    assert torch.equal(o[blind], want_o[blind]) and torch.equal(lse[:, blind], want_lse[:, blind])
+    assert torch.isnan(o[~blind].float()).any()
+
+
+@pytest.mark.parametrize("h", [16, 40])
+@pytest.mark.parametrize("fp8", [False, True], ids=["bf16", "fp8"])
+def test_a_single_draft_that_does_not_see_itself_is_not_reached_by_its_row(gpu, fp8, h):
+    b = Batch(gpu, [1, 1], [90, 1], h, page=16, fp8=fp8, tree="tree", seed=14)
+    b.words.zero_()
+    want_o, want_lse = b.attention()
+    b.check(want_o, want_lse)
+    for i in range(2):
+        j = b.lengths[i] - 1
+        page, row = b.table[i, j // 16].long(), j % 16
+        b.latent[page, row] = math.nan
+        b.k_pe[page, row] = math.nan
+    o, lse = b.attention()
+    assert torch.equal(o, want_o) and torch.equal(lse, want_lse)
+
+
 def test_tokens_behind_the_last_sequence_are_left_alone(gpu):
     b = Batch(gpu, [2, 1], [40, 300], 16, seed=10, extra_tokens=5)
     o = torch.full((8, 16, 512), 7.0, dtype=BF, device=gpu)
@@ -375,9 +409,7 @@ def test_gather_returns_the_rows_in_order(gpu, lengths, page, fp8):
 # absorbed products
 
 
-@pytest.mark.parametrize("h", [1, 16, 37])
-@pytest.mark.parametrize("tokens", [1, 15, 16, 17, 300])
-def test_absorbed_products_match_the_oracle(gpu, tokens, h):
+def _absorbed_products(gpu, tokens, h):
     g = torch.Generator().manual_seed(tokens * 100 + h)
     q = torch.randn(tokens, h, 200, generator=g).to(BF)[..., 8:]
     w = (torch.randn(h * 256, 512, generator=g) * 512**-0.5).to(BF)
@@ -392,6 +424,18 @@ def test_absorbed_products_match_the_oracle(gpu, tokens, h):
     got = L.absorb_value(x.to(gpu), w.to(gpu))
     want, mass = O.absorb_value(x, w)
     _within(got, want, U * want.abs() + 514 * 2.0**-24 * mass, "o")
+
+
+@pytest.mark.parametrize("h", [1, 16, 37])
+@pytest.mark.parametrize("tokens", [1, 15, 16, 17, 300])
+def test_absorbed_products_match_the_oracle(gpu, tokens, h):
+    _absorbed_products(gpu, tokens, h)
+
+
+# Many tiles a compute unit, and workgroups whose tokens are more tiles than their ring has slots.
+@pytest.mark.parametrize("tokens, h", [(90, 150), (200, 130), (270, 128), (580, 257)])
+def test_absorbed_products_of_many_heads_match_the_oracle(gpu, tokens, h):
+    _absorbed_products(gpu, tokens, h)
 
 
 # ---------------------------------------------------------------------------------------------
