@@ -81,7 +81,7 @@ __global__ __launch_bounds__(64 * WAVES) void absorb_query_kernel(AbsorbParams p
 #pragma unroll
     for (int k = 0; k < kLoads; ++k) {
       const int region = kLoads * wave + k, r = 4 * region + (lane >> 4);
-      load_lds16_at(p.x + (int64_t)min(t0 + kTokens * i + r, t1 - 1) * p.x_ts + h * p.x_hs + 8 * ((lane & 15) ^ tile_swizzle(r)), lds + slot * kTile + 1024 * region);
+      load_lds16_at(p.x + (int64_t)min(t0 + kTokens * i + r, t1 - 1) * p.x_ts + h * p.x_hs + 8 * ((lane & 15) ^ row_swizzle(r)), lds + slot * kTile + 1024 * region);
     }
   };
   {
@@ -123,7 +123,7 @@ __global__ __launch_bounds__(64 * WAVES) void absorb_query_kernel(AbsorbParams p
       f32x4 acc[4] = {};
 #pragma unroll
       for (int st = 0; st < 4; ++st) {
-        const bf16x8 q = *reinterpret_cast<const bf16x8*>(tile + swizzled_offset(16 * half + c, 4 * st + g));
+        const bf16x8 q = *reinterpret_cast<const bf16x8*>(tile + (16 * half + c) * kRowBytes128 + (((4 * st + g) ^ row_swizzle(c)) << 4));
 #pragma unroll
         for (int n = 0; n < 4; ++n) acc[n] = mfma16(w[n][st], q, acc[n]);
       }
@@ -153,7 +153,7 @@ __global__ __launch_bounds__(64 * WAVES) void absorb_value_kernel(AbsorbParams p
   const int c = lane & 15, g = lane >> 4;
   const int first = 16 * (WAVES * blockIdx.x + wave);  // of the wave's features
   const auto row = [&](const __bf16* src, char* tile, int r) __attribute__((always_inline)) {
-    load_lds16(reinterpret_cast<const char*>(src), (16 * lane) ^ (16 * tile_swizzle(r)), tile + r * 2 * kLatent);
+    load_lds16(reinterpret_cast<const char*>(src), (16 * lane) ^ (16 * row_swizzle(r)), tile + r * 2 * kLatent);
   };
   const auto request = [&](int i, int slot) __attribute__((always_inline)) {
 #pragma unroll
@@ -163,7 +163,7 @@ __global__ __launch_bounds__(64 * WAVES) void absorb_value_kernel(AbsorbParams p
     }
   };
   const auto fragment = [&](const char* tile, int st) __attribute__((always_inline)) {
-    const uint32_t at = lds_address(tile) + c * 2 * kLatent + ((g ^ tile_swizzle(c)) << 4);
+    const uint32_t at = lds_address(tile) + c * 2 * kLatent + ((g ^ row_swizzle(c)) << 4);
     return *lds_at<bf16x8>((at ^ (64 * (st & 3))) + 256 * (st >> 2));
   };
 #pragma unroll

@@ -100,7 +100,8 @@ struct Walk {
       total += __builtin_amdgcn_readlane(sw, 63);
       blocks_total += __builtin_amdgcn_readlane(sk, 63);
     }
-    if (blockIdx.x == 0 && threadIdx.x == 0) *p.items = min(blocks_total, p.max_items);
+    // (named as global memory: with a store to anywhere behind it, all waits for LDS in the kernel would be waits for everything)
+    if (blockIdx.x == 0 && threadIdx.x == 0) *(__attribute__((address_space(1))) int*)(uintptr_t)p.items = min(blocks_total, p.max_items);
     per = __builtin_amdgcn_readfirstlane((total + (int)gridDim.x - 1) / (int)gridDim.x);  // (divisions leave the scalar registers)
     begin = at = blockIdx.x * per;
     end = min(at + per, total);  // (the host has bounded total + gridDim.x)
@@ -163,65 +164,52 @@ struct LatentTile {
   static constexpr int kLatentRow = FP8 ? kLatent : 2 * kLatent;  // bytes
   static constexpr int kPe = KEYS * kLatentRow;                   // offsets in a tile
   static constexpr int kScale = kPe + KEYS * 2 * kRope;           // [KEYS] fp32
-  static constexpr int kBytes = kScale + (FP8 ? 256 : 0);  // (tiles begin at multiples of 256)
-  static constexpr int kLoads = FP8 ? 6 : 9;  // direct loads of a wave: eight rows
+  static constexpr int kBytes = kScale + (FP8 ? 256 : 0);         // (tiles begin at multiples of 256)
 };
 
-// Piece (16 bytes) swizzles: piece q of a row lies at q ^ swizzle(row). Latent rows are whole multiples of 256 bytes; the low four bits of the piece
-// are swizzled so that sixteen consecutive rows read at one piece hit different banks (tile_swizzle, attn_tiles.h). Rotary rows lie two to a 256-byte
-// LDS row: row 8 w + i and 8 w + 4 + i (i < 4) in pieces 0-7 and 8-15 of LDS row 4 w + i, so that a wave's eight rows are one instruction.
+// Latent rows are swizzled by row_swizzle. Rotary rows lie two to a 256-byte LDS row: row 8 w + i and 8 w + 4 + i (i < 4) in pieces 0-7 and 8-15 of LDS
+// row 4 w + i, so that eight rows are one instruction; there the fragment reads have no conflict with this swizzle.
 __device__ __forceinline__ int pe_row(int row) { return ((row >> 3) << 2) | (row & 3); }
-__device__ __forceinline__ int pe_swizzle(int lds_row) { return ((lds_row & 3) << 1) | ((lds_row >> 2) & 1); }
+__device__ __forceinline__ int pe_swizzle(int lds_row) { return (lds_row & 3) << 1; }
 
-// Page of the sixteen rows from key on (a multiple of 16); rows behind the sequence's last one are read as that one.
-// Read as constant memory (nobody writes tables while the kernel runs): a scalar load, which the counted waits for tiles do not see.
+// Page of the sixteen rows from key on (a multiple of 16), the sequence's last ones where that is behind them. Read as constant memory (nobody writes
+// tables while the kernel runs): a scalar load, which the counted waits for tiles do not see.
 typedef const __attribute__((address_space(4))) int32_t* ScalarTable;
-__device__ __forceinline__ int page_of(const LatentAttnParams& p, ScalarTable table, int key, int last) {
-  return safe_page(table[min(key, last) >> p.cache.page_shift], p.cache.pages);
-}
+__device__ __forceinline__ int page_at(const LatentAttnParams& p, ScalarTable table, int key, int last) { return table[min(key, last) >> p.cache.page_shift]; }
 
-// Wave w's direct loads of a tile: rows 8 w .. 8 w + 7 of it, which are half of the sixteen from key16 = key0 + 16 (w >> 1) on. Rows behind the sequence's
-// last one are read as that one. The loads are asked for one by one, where the caller has room between its products.
+// Wave w's (of KEYS / 8) direct loads of a tile: rows 8 w .. 8 w + 7, which are half of the sixteen from key16 = key0 + 16 (w / 2) on; `page`: page_at that.
+// Rows behind the sequence's last one come as the page holds them, or the last sixteen again: nobody sees them, and clean_tile takes out what is not finite.
 template <bool FP8, int KEYS>
 struct TileLoads {
   using T = LatentTile<FP8, KEYS>;
+  static constexpr int kLatentLoads = FP8 ? 4 : 8, kLoads = kLatentLoads + (FP8 ? 2 : 1);
   const char *base, *pe;  // of the wave's first row
   const float* scale;
   char* slot;
-  int left;  // rows behind the wave's first that exist (below zero: none, nor that one)
   int wave;
   __device__ __forceinline__ TileLoads(const LatentAttnParams& p, int page, int key16, int last, char* slot_, int wave_) : slot(slot_), wave(wave_) {
-    const int first = min(key16, last) & ~15;  // the page's sixteen rows
-    const int r0 = 8 * (wave & 1);             // of the sixteen
-    const int in_page = (first & ((1 << p.cache.page_shift) - 1)) + r0;
-    left = last - first - r0;
+    page = safe_page(__builtin_amdgcn_readfirstlane(page), p.cache.pages);
+    const int in_page = (min(key16, last) & ((1 << p.cache.page_shift) - 16)) + 8 * (wave & 1);
     base = p.cache.latent + page * p.cache.latent_ps + (int64_t)in_page * T::kLatentRow;
     pe = reinterpret_cast<const char*>(p.cache.k_pe + page * p.cache.k_pe_ps + (int64_t)in_page * kRope);
     scale = FP8 ? p.cache.scale + page * p.cache.scale_ps + in_page : nullptr;
   }
-  // Load n of T::kLoads.
+  // Load n of kLoads.
   __device__ __forceinline__ void issue(int n, int lane) const {
-    constexpr int kLatentLoads = FP8 ? 4 : 8;
-    if (n < kLatentLoads) {
-      char* const dst = slot + 8 * wave * T::kLatentRow + n * 1024;
-      if constexpr (FP8) {  // two rows an instruction
-        const int r = 2 * n + (lane >> 5);
-        load_lds16(base + min(left, 0) * T::kLatentRow, max(min(r, left), 0) * T::kLatentRow + 16 * ((lane & 31) ^ tile_swizzle(8 * wave + r)), dst);
-      } else {
-        load_lds16(base + min(n, left) * T::kLatentRow, (16 * lane) ^ (16 * tile_swizzle(8 * wave + n)), dst);
-      }
+    if (n < kLatentLoads) {  // a row, or two of e4m3
+      const int r = FP8 ? 2 * n + (lane >> 5) : n;
+      load_lds16(base, r * T::kLatentRow + (16 * (FP8 ? lane & 31 : lane) ^ 16 * row_swizzle(8 * wave + r)), slot + 8 * wave * T::kLatentRow + n * 1024);
     } else if (n == kLatentLoads) {
       const int piece = (lane & 15) ^ pe_swizzle(4 * wave + (lane >> 4));
-      const int r = 4 * (piece >> 3) + (lane >> 4);
-      load_lds16(pe + min(left, 0) * (2 * kRope), max(min(r, left), 0) * (2 * kRope) + 16 * (piece & 7), slot + T::kPe + wave * 1024);
+      load_lds16(pe, (4 * (piece >> 3) + (lane >> 4)) * (2 * kRope) + 16 * (piece & 7), slot + T::kPe + wave * 1024);
     } else {
-      if (lane < 8) load_lds4(scale + min(lane, left), slot + T::kScale + 32 * wave);
+      if (lane < 8) load_lds4(scale + lane, slot + T::kScale + 32 * wave);
     }
   }
   __device__ __forceinline__ void issue_all(int lane) const {
     asm volatile("" : "+v"(lane));  // the rows' offsets are formed on the spot, not kept (and spilled) from tile to tile
 #pragma unroll
-    for (int n = 0; n < T::kLoads; ++n) issue(n, lane);
+    for (int n = 0; n < kLoads; ++n) issue(n, lane);
   }
 };
 
@@ -298,20 +286,15 @@ __device__ __forceinline__ void score(const char* tile, int at, int pe_at, bool 
   }
 }
 
-// Which of a wave's features (64 or 128, 16 a product) result 0 of product n is in a lane of group g; results 1 to 3 follow it. Transposed reads take their columns in groups of four (bf16) or eight
-// (e4m3) from wherever a lane points; as bf16 the groups of two products are dealt so that a lane's results of both are eight consecutive ones.
+// A wave's products of values: product n's result v in a lane of group g is feature 16 n + 4 g + v of its 128. (Dealt so that a lane's results of two
+// products are eight consecutive features, the transposed bf16 reads take halves of four pieces of a row and conflict in the banks.)
+// Place of the lane's transposed reads of 128 features in a tile, rows 0-31, wave w's from feature 128 w on; those of other products and rows are
+// ^ and + from there. A read brings four columns (bf16) or eight (e4m3) of a row.
 template <bool FP8>
-__device__ __forceinline__ int feature_of(int n, int g) {
-  return FP8 ? 16 * n + 4 * g : 32 * (n >> 1) + 8 * g + 4 * (n & 1);
-}
-
-// Place of the lane's transposed reads of FEATURES features in a tile, rows 0-31, wave w's from feature FEATURES w on; those of other pieces and rows are
-// ^ and + from there.
-template <bool FP8, int FEATURES>
 __device__ __forceinline__ int value_place(int wave, int c, int g) {
   const int r = 8 * g + (FP8 ? c >> 1 : c >> 2);
-  const int piece = FP8 ? FEATURES / 16 * wave : FEATURES / 8 * wave + (c & 3);
-  return r * (FP8 ? kLatent : 2 * kLatent) + ((piece ^ tile_swizzle(r)) << 4) + (FP8 ? 8 * (c & 1) : 0);
+  const int piece = FP8 ? 8 * wave : 16 * wave + ((c >> 1) & 1);
+  return r * (FP8 ? kLatent : 2 * kLatent) + ((piece ^ row_swizzle(r)) << 4) + 8 * (c & 1);
 }
 
 // Operand A of product n over keys 8 g + e; `first`: lds_address of the tile + value_place.
@@ -322,21 +305,25 @@ __device__ __forceinline__ bf16x8 value_fragment(uint32_t first, int n) {
     typedef __attribute__((address_space(3))) i32x2 lds_i32x2;
     const i32x2 raw = __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_i32x2*)(uintptr_t)(first ^ (16 * n)));
     return widen((uint32_t)raw[0], (uint32_t)raw[1]);
-  } else {  // four rows further on the swizzle differs in its lowest bit
+  } else {  // four rows further on the swizzle differs in its highest bit
     typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
-    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(uintptr_t)((first ^ (64 * (n >> 1))) + 8 * (n & 1)));
-    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(uintptr_t)((first ^ (64 * (n >> 1) + 16)) + 4 * (2 * kLatent) + 8 * (n & 1)));
+    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(uintptr_t)(first ^ (32 * n)));
+    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(uintptr_t)((first ^ (32 * n ^ 128)) + 4 * (2 * kLatent)));
     typedef __attribute__((ext_vector_type(8))) short s16x8;
     return __builtin_bit_cast(bf16x8, s16x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]});
   }
 }
 
-// Infinities and NaN of a tile's latent rows -> 0, in place, by all threads. For tiles that some rows see in part only: a row's weight of a key it does
-// not see is 0, and must stay so against whatever the key holds. A row that sees such a key has a score of the same kind.
-template <bool FP8, int KEYS, int THREADS>
-__device__ __forceinline__ void clean_tile(char* tile) {
-  for (int at = 16 * threadIdx.x; at < LatentTile<FP8, KEYS>::kPe; at += 16 * THREADS) {
-    u32x4 x = *reinterpret_cast<const u32x4*>(tile + at);
+// Infinities and NaN of a wave's 128 features from 128 w on, in all 32 rows of a tile -> 0, in place. For tiles that some rows see in part only: a row's weight
+// of a key it does not see is 0, and must stay so against whatever the key holds. A row that sees such a key has a score of the same kind.
+template <bool FP8>
+__device__ __forceinline__ void clean_tile(char* tile, int w, int lane) {
+  constexpr int kPieces = FP8 ? 8 : 16;  // of a row
+#pragma unroll 1
+  for (int i = lane; i < 32 * kPieces; i += 64) {
+    const int row = i / kPieces, piece = kPieces * w + i % kPieces;
+    u32x4* const at = reinterpret_cast<u32x4*>(tile + row * LatentTile<FP8, 32>::kLatentRow + ((piece ^ row_swizzle(row)) << 4));
+    u32x4 x = *at;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       if constexpr (FP8) {
@@ -348,7 +335,7 @@ __device__ __forceinline__ void clean_tile(char* tile) {
         if ((x[e] & 0x7f800000u) == 0x7f800000u) x[e] &= 0xffffu;
       }
     }
-    *reinterpret_cast<u32x4*>(tile + at) = x;
+    *at = x;
   }
 }
 
@@ -420,7 +407,7 @@ __device__ __forceinline__ void stage_queries(const LatentAttnParams& p, const W
   int tok = __builtin_amdgcn_readfirstlane((row0 + min(8 * wave, last)) / p.H), head = row0 + min(8 * wave, last) - tok * p.H;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    load_lds16(scalar_pointer(p.q_latent + (int64_t)(walk.s.tok0 + tok) * p.q_ts + head * p.q_hs), (16 * lane) ^ (16 * tile_swizzle(8 * wave + i)),
+    load_lds16(scalar_pointer(p.q_latent + (int64_t)(walk.s.tok0 + tok) * p.q_ts + head * p.q_hs), (16 * lane) ^ (16 * row_swizzle(8 * wave + i)),
                area + (8 * wave + i) * T::kLatentRow);
     if (8 * wave + i < last && ++head == p.H) head = 0, ++tok;
   }
@@ -440,45 +427,39 @@ __device__ __forceinline__ void read_query(const char* area, int row, int latent
 #pragma unroll
   for (int i = 0; i < Q - 2; ++i) {
     const int piece = FP8 ? 8 * (i >> 1) + 2 * g + (i & 1) : 4 * i + g;
-    q[i] = *reinterpret_cast<const bf16x8*>(rows + ((piece ^ tile_swizzle(row)) << 4));
+    q[i] = *reinterpret_cast<const bf16x8*>(rows + ((piece ^ row_swizzle(row)) << 4));
   }
 #pragma unroll
   for (int i = 0; i < 2; ++i)
     q[Q - 2 + i] = *reinterpret_cast<const bf16x8*>(area + T::kPe + pe_row(row) * 256 + (((8 * ((row >> 2) & 1) + 4 * i + g) ^ pe_swizzle(pe_row(row))) << 4));
 }
 
-// Results of a lane's row of group r (16 N features of the wave from 16 N wave on) as bf16, and its lse by one lane; or, where the segment is a part,
-// reference, sum and unnormalised results in the workspace: there result vector n of a wave lies as the wave holds it, 16 bytes a lane (part_at),
-// because row by row an instruction would touch 16 of them.
+// Results of a lane's row of group r (the wave's 128 features) as bf16, and its lse by one lane; or, where the segment is a part, reference, sum and
+// unnormalised results in the workspace: there result vector n of a wave (features 16 (8 wave + n) ..) lies as the wave holds it, 16 bytes a lane
+// (part_at), because row by row an instruction would touch 16 of them.
 template <int M>
-__device__ __forceinline__ int64_t part_at(int64_t slot, int group, int vector, int lane) {  // vector: N wave + n; in floats
+__device__ __forceinline__ int64_t part_at(int64_t slot, int group, int vector, int lane) {  // vector: 8 wave + n; in floats
   return ((slot * (M / 16) + group) * (kLatent / 16) + vector) * 256 + 4 * lane;
 }
-template <bool FP8, int M, int N, typename W>
-__device__ __forceinline__ void store_row(const LatentAttnParams& p, const W& walk, const f32x4 (&acc)[N], float top, float sum, int r, int wave, int lane) {
+template <int M, typename W>
+__device__ __forceinline__ void store_row(const LatentAttnParams& p, const W& walk, const f32x4 (&acc)[8], float top, float sum, int r, int wave, int lane) {
   const int row = 16 * r + (lane & 15), g = lane >> 4;
   const bool first = wave == 0 && g == 0;
   if (walk.whole()) {
     if (row >= walk.rows(p)) return;
     const int at = walk.block * M + row, tok = walk.s.tok0 + at / p.H, head = at % p.H;
     const float inv = 1.f / sum;
-    __bf16* const dst = p.o + (int64_t)tok * p.o_ts + head * p.o_hs + 16 * N * wave;
+    __bf16* const dst = p.o + (int64_t)tok * p.o_ts + head * p.o_hs + 128 * wave + 4 * g;
 #pragma unroll
-    for (int n = 0; n < N; n += 2) {
-      const f32x4 a = sum == 0.f ? f32x4{} : acc[n] * inv, d = sum == 0.f ? f32x4{} : acc[n + 1] * inv;
-      const u32x2 lo = {pack_bf16x2(a[0], a[1]), pack_bf16x2(a[2], a[3])}, hi = {pack_bf16x2(d[0], d[1]), pack_bf16x2(d[2], d[3])};
-      if constexpr (FP8) {
-        *reinterpret_cast<u32x2*>(dst + feature_of<true>(n, g)) = lo;
-        *reinterpret_cast<u32x2*>(dst + feature_of<true>(n + 1, g)) = hi;
-      } else {
-        *reinterpret_cast<u32x4*>(dst + feature_of<false>(n, g)) = u32x4{lo[0], lo[1], hi[0], hi[1]};
-      }
+    for (int n = 0; n < 8; ++n) {
+      const f32x4 x = sum == 0.f ? f32x4{} : acc[n] * inv;
+      *reinterpret_cast<u32x2*>(dst + 16 * n) = u32x2{pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3])};
     }
     if (first) p.lse[head * p.lse_hs + tok] = sum == 0.f ? -INFINITY : top + __builtin_amdgcn_logf(sum);
   } else {
     const int64_t slot = walk.slot();
 #pragma unroll
-    for (int n = 0; n < N; ++n) *reinterpret_cast<f32x4*>(p.parts + part_at<M>(slot, r, N * wave + n, lane)) = acc[n];
+    for (int n = 0; n < 8; ++n) *reinterpret_cast<f32x4*>(p.parts + part_at<M>(slot, r, 8 * wave + n, lane)) = acc[n];
     if (first) p.stats[slot * M + row] = make_float2(top, sum);
   }
 }
@@ -488,7 +469,7 @@ __device__ __forceinline__ void store_row(const LatentAttnParams& p, const W& wa
 constexpr float kSlack = 8.f;
 
 // The attention kernel for 64 rows to a workgroup (latent_attn_wide.hip).
-constexpr int kWideRows = 64, kWideKeys = 64;
+constexpr int kWideRows = 64;
 void launch_latent_wide(const LatentAttnParams& p, bool fp8, bool tree, int groups, hipStream_t stream);
 
 }  // namespace pith

@@ -30,6 +30,7 @@ __device__ __forceinline__ int exchange_at(int row, int piece) { return row * (k
 template <bool FP8, bool TREE>
 __global__ __launch_bounds__(kThreads, 2) void latent_attn_kernel(LatentAttnParams p) {
   using T = LatentTile<FP8, kKeys>;
+  using Loads = TileLoads<FP8, kKeys>;
   constexpr int kRing = FP8 ? 3 : 2;
   constexpr int kSteps = 4;          // of 64 latent features, in each half
   constexpr int Q = 2 * kSteps + 2;  // query fragments, the last two rotary (of the second half)
@@ -42,9 +43,9 @@ __global__ __launch_bounds__(kThreads, 2) void latent_attn_kernel(LatentAttnPara
   if (!walk.start(p, lane)) return;
 
   const int key_row = 16 * kg + c;  // the key this lane brings
-  const int key_at = key_row * T::kLatentRow + half * (T::kLatentRow / 2) + ((g ^ tile_swizzle(key_row)) << 4);
+  const int key_at = key_row * T::kLatentRow + half * (T::kLatentRow / 2) + ((g ^ row_swizzle(key_row)) << 4);
   const int pe_at = T::kPe + pe_row(key_row) * 256 + (((8 * ((key_row >> 2) & 1) + g) ^ pe_swizzle(pe_row(key_row))) << 4);
-  const int value_at = value_place<FP8, 128>(wave, c, g);
+  const int value_at = value_place<FP8>(wave, c, g);
   do {
     const SeqWork& s = walk.s;
     const int n_tiles = walk.n_tiles(), last = max(s.len - 1, 0);
@@ -57,14 +58,14 @@ __global__ __launch_bounds__(kThreads, 2) void latent_attn_kernel(LatentAttnPara
     const int key16 = walk.tile * kKeys + 16 * (wave >> 1);  // this wave's sixteen of the first tile
     const auto request = [&](int i) __attribute__((always_inline)) {
       const int key = key16 + i * kKeys;
-      TileLoads<FP8, kKeys>(p, page_of(p, table, key, last), key, last, lds + i * T::kBytes, wave).issue_all(lane);
+      Loads(p, page_at(p, table, key, last), key, last, lds + i * T::kBytes, wave).issue_all(lane);
     };
     bf16x8 q[1][Q];
     char* const staged = lds + T::kBytes;  // the slots behind the first tile's
     stage_queries<kM>(p, walk, staged, wave, lane);
     request(0);
-    int next_page = page_of(p, table, key16 + kRing * kKeys, last);
-    wait_loads<T::kLoads>();  // the queries, of the waves that brought some
+    int next_page = page_at(p, table, key16 + kRing * kKeys, last);
+    wait_loads<Loads::kLoads>();  // the queries, of the waves that brought some
     __syncthreads();
     read_query<FP8, kM>(staged, c, half * (kLatent / 2), g, q[0]);
     __syncthreads();
@@ -75,8 +76,8 @@ __global__ __launch_bounds__(kThreads, 2) void latent_attn_kernel(LatentAttnPara
       const int key0 = (walk.tile + i) * kKeys;
       // the tiles behind this one, up to a whole ring less one, stay in flight
       const int later = min(kRing - 1, n_tiles - 1 - i);
-      if (later == 2) wait_loads<2 * T::kLoads>();
-      else if (later == 1) wait_loads<T::kLoads>();
+      if (later == 2) wait_loads<2 * Loads::kLoads>();
+      else if (later == 1) wait_loads<Loads::kLoads>();
       else wait_loads<0>();
       __syncthreads();
       char* const kt = lds + slot * T::kBytes;
@@ -88,11 +89,7 @@ __global__ __launch_bounds__(kThreads, 2) void latent_attn_kernel(LatentAttnPara
         *reinterpret_cast<f32x4*>(exchange + exchange_at(half * kM + c, 4 * kg + g)) = x[0];
       }
       __syncthreads();
-      if (partial && (TREE || s.n > 1)) {
-        clean_tile<FP8, kKeys, kThreads>(kt);
-        __syncthreads();
-      }
-
+      if (partial) clean_tile<FP8>(kt, wave, lane);
       float y[8];
       {
         const auto sum = [&](int piece) { return *reinterpret_cast<const f32x4*>(exchange + exchange_at(c, piece)) + *reinterpret_cast<const f32x4*>(exchange + exchange_at(kM + c, piece)); };
@@ -131,12 +128,12 @@ __global__ __launch_bounds__(kThreads, 2) void latent_attn_kernel(LatentAttnPara
       if (i + kRing < n_tiles) {
         __syncthreads();  // nobody reads this tile any more: its slot is asked to be filled before the next tile is waited for
         const int key = key16 + (i + kRing) * kKeys;
-        TileLoads<FP8, kKeys>(p, next_page, key, last, kt, wave).issue_all(lane);
-        next_page = page_of(p, table, key + kKeys, last);
+        Loads(p, next_page, key, last, kt, wave).issue_all(lane);
+        next_page = page_at(p, table, key + kKeys, last);
       }
       slot = slot + 1 == kRing ? 0 : slot + 1;
     }
-    store_row<FP8, kM>(p, walk, acc, m, quad_sum(l), 0, wave, lane);
+    store_row<kM>(p, walk, acc, m, quad_sum(l), 0, wave, lane);
     walk.leave_join(p);
   } while (walk.next(p));
 }
@@ -148,9 +145,9 @@ constexpr int kMaxGroups = 512;  // workgroups of the attention kernel, at most:
 // and which `vectors` of its 32 result vectors (part_at). The weights of the rows are formed first, in one pass over their references and sums, so that
 // the loads of the sums over the parts do not wait for one another; where a workgroup has fewer vectors than waves, several waves take every other
 // part and add up in LDS.
-template <bool FP8, int M>
+template <int M>
 __global__ __launch_bounds__(kJoinThreads) void latent_join_kernel(LatentAttnParams p, int vectors) {
-  constexpr int kWaves = kJoinThreads / 64, N = M == kM ? 8 : 4;  // N: vectors of a wave of the attention kernel
+  constexpr int kWaves = kJoinThreads / 64;
   constexpr int kPerRow = kJoinThreads / 16;                     // threads that form the weights of a row
   __shared__ __attribute__((aligned(16))) f32x4 sum_o[kJoinThreads];
   __shared__ float weights[16][kMaxGroups + 1];
@@ -210,15 +207,14 @@ __global__ __launch_bounds__(kJoinThreads) void latent_join_kernel(LatentAttnPar
   if (16 * r + c >= join.rows) return;
   const int at = join.row0 + 16 * r + c, tok = at / p.H, head = at - tok * p.H;
   o = inverse[c] == 0.f ? f32x4{} : o * inverse[c];
-  *reinterpret_cast<u32x2*>(p.o + (int64_t)tok * p.o_ts + head * p.o_hs + 16 * N * (vector / N) + feature_of<FP8>(vector % N, lane >> 4)) =
+  *reinterpret_cast<u32x2*>(p.o + (int64_t)tok * p.o_ts + head * p.o_hs + 16 * vector + 4 * (lane >> 4)) =
       u32x2{pack_bf16x2(o[0], o[1]), pack_bf16x2(o[2], o[3])};
 }
 
 template <int M>
-void launch_join(const LatentAttnParams& p, bool fp8, int vectors, hipStream_t s) {
+void launch_join(const LatentAttnParams& p, int vectors, hipStream_t s) {
   const dim3 grid(p.max_items, M / 16 * (kLatent / 16 / vectors));
-  if (fp8) latent_join_kernel<true, M><<<grid, kJoinThreads, 0, s>>>(p, vectors);
-  else latent_join_kernel<false, M><<<grid, kJoinThreads, 0, s>>>(p, vectors);
+  latent_join_kernel<M><<<grid, kJoinThreads, 0, s>>>(p, vectors);
 }
 
 struct LatentPlan {
@@ -320,10 +316,10 @@ extern "C" int pith_latent_attn(const pith_latent_attn_args* a, pith_stream_t st
   begin_launch();
   if (pl.rows == kM) {
     launch_narrow(p, fp8, tree, pl.groups, s);
-    launch_join<kM>(p, fp8, pl.join_vectors, s);
+    launch_join<kM>(p, pl.join_vectors, s);
   } else {
     launch_latent_wide(p, fp8, tree, pl.groups, s);
-    launch_join<kWideRows>(p, fp8, pl.join_vectors, s);
+    launch_join<kWideRows>(p, pl.join_vectors, s);
   }
   return check_launch(who);
 }

@@ -64,6 +64,13 @@ __device__ __forceinline__ int64_t clamped_position(int64_t pos, int64_t P) { re
 
 __device__ __forceinline__ f32x4 mfma16(bf16x8 a, bf16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
 
+// Swizzle of rows that are whole multiples of 256 bytes: piece (16 bytes) q of row r lies at q ^ row_swizzle(r). LDS serves 256 bytes a cycle, and a
+// wavefront's 16-byte reads as lanes 0-3 12-15 20-27, then 4-11 16-19 28-31, and the upper half alike (measured with the counter of bank conflicts, two
+// lanes at a time on one bank); 8-byte reads as its halves. So the fragment reads of 16x16x32 products (lane c + 16 g: row c, piece q + g) want rows
+// {0-3, 12-15} and {4-11} each in pairs that differ in the last bit, and the transposed ones (lane: row 8 g + c / 4 or four more, half a piece of a
+// pair) want the pairs of rows {0-3, 8-11} to differ, and of {4-7, 12-15}: this has no conflict in either. (tile_swizzle serves 32-row products.)
+__device__ __forceinline__ int row_swizzle(int row) { return ((((row >> 3) ^ (row >> 2)) & 1) << 3) | ((row & 3) << 1) | ((row >> 3) & 1); }
+
 // load_lds16 from an address of each lane's own.
 __device__ __forceinline__ void load_lds16_at(const void* src, char* dst_wave) {
   const uint32_t lds_addr = (uint32_t)(uintptr_t)(lds_char*)dst_wave;
