@@ -3,8 +3,11 @@
 // Work list. A sequence of n new tokens and L rows is R = ceil(n H / M) row blocks of M rows (row = token * H + head) times N = ceil(L / K) tiles of K keys,
 // and the tiles of all row blocks of all sequences, one behind the other, are dealt to the workgroups in equal ranges. Lengths are read on the device,
 // so nothing depends on the host knowing them: a captured call follows its sequences as they grow, and one long sequence among short ones is spread over
-// as many workgroups as its share of the tiles. (Tiles of all row blocks in step on one XCD, chunk by chunk, so that its cache fetches them once, was
-// slower: 128 heads 119 us against 100, trees of 48 drafts 272 against 250; the ranges are cut more often, and the kernels do not wait for these bytes.)
+// as many workgroups as its share of the tiles.
+// To begin and end a row block costs a workgroup the time of several tiles (START: queries, first tile, parts). Where there are fewer row blocks than
+// workgroups, ranges can therefore be a little longer and each lie in one row block: every row block is taken for as many tiles as fill whole ranges, LEAST
+// tiles or more. The row blocks of a sequence are then cut alike, and as an XCD's workgroups take ranges that follow one another, its cache fetches their
+// tiles about once: 128 heads 73 us at best against 68, trees of up to 48 drafts 194 against 172.
 // A workgroup whose range covers a row block wholly writes its rows; parts of a row block leave (reference, sum, unnormalised result) in fp32 in the
 // workspace, and a second kernel joins them in the order of the keys (results do not depend on scheduling).
 #pragma once
@@ -75,61 +78,86 @@ __device__ __forceinline__ int wave_scan(int x) {
 
 // A workgroup's way through its range of the work list, segment by segment (tiles of one row block). Every wave walks for itself; all of it is
 // wave-uniform.
-template <int M, int KEYS>
+template <int M, int KEYS, int START, int LEAST>
 struct Walk {
+  int range;                // this workgroup's
   int per, begin, at, end;  // length of a range, begin of this one, place, end
   int b, item;              // sequence, row blocks in front of it
   int block, tile;          // row block, first tile of the segment
+  bool single;              // one segment a range
   SeqWork s;
+
+  __device__ __forceinline__ int taken(int tiles) const { return single ? (tiles + per - 1) / per * per : tiles; }  // tiles that a row block is taken for
 
   // False: nothing to do.
   __device__ __forceinline__ bool start(const LatentAttnParams& p, int lane) {
+    SeqWork x = {};
     int w = 0, k = 0, sw = 0, sk = 0, total = 0, blocks_total = 0;
-    const auto sums = [&](int b0) __attribute__((always_inline)) {  // over 64 sequences
-      w = k = 0;
-      if (b0 + lane < p.B) {
-        const SeqWork x = seq_work<M, KEYS>(p, b0 + lane);
-        w = x.blocks * x.tiles;
-        k = x.blocks;
-      }
+    const auto load = [&](int b0) __attribute__((always_inline)) {  // of 64 sequences
+      x.blocks = x.tiles = 0;
+      if (b0 + lane < p.B) x = seq_work<M, KEYS>(p, b0 + lane);
+    };
+    const auto sums = [&]() __attribute__((always_inline)) {
+      k = x.blocks;
+      w = k * taken(x.tiles);
       sw = wave_scan(w);
       sk = wave_scan(k);
     };
+    single = false;
     for (int b0 = 0; b0 < p.B; b0 += 64) {
-      sums(b0);
+      load(b0);
+      sums();
       total += __builtin_amdgcn_readlane(sw, 63);
       blocks_total += __builtin_amdgcn_readlane(sk, 63);
     }
     // (named as global memory: with a store to anywhere behind it, all waits for LDS in the kernel would be waits for everything)
     if (blockIdx.x == 0 && threadIdx.x == 0) *(__attribute__((address_space(1))) int*)(uintptr_t)p.items = min(blocks_total, p.max_items);
-    per = __builtin_amdgcn_readfirstlane((total + (int)gridDim.x - 1) / (int)gridDim.x);  // (divisions leave the scalar registers)
-    begin = at = blockIdx.x * per;
-    end = min(at + per, total);  // (the host has bounded total + gridDim.x)
-    if (at >= end) return false;
+    const int groups = gridDim.x;
+    range = (blockIdx.x & 7) * (groups >> 3) + (blockIdx.x >> 3);  // an XCD's workgroups (every eighth) take ranges that follow one another
+    per = __builtin_amdgcn_readfirstlane((total + groups - 1) / groups);  // (divisions leave the scalar registers)
+    if (blocks_total < groups) {
+      const int free = groups - blocks_total, longer = __builtin_amdgcn_readfirstlane((total + free - 1) / free);
+      if (longer <= per + START) {  // (a row block's last range is not full: at most total / longer + blocks_total ranges)
+        per = max(longer, LEAST);
+        single = true;
+        if (p.B <= 64) sums();
+      }
+    }
+    begin = at = range * per;
+    end = at + per;  // (the host has bounded total + gridDim.x)
     int before = 0;  // tiles in front of the sequence
     item = 0;
-    for (int b0 = 0;; b0 += 64) {
-      if (p.B > 64) sums(b0);
+    for (int b0 = 0; b0 < p.B; b0 += 64) {
+      if (p.B > 64) {
+        load(b0);
+        sums();
+      }
       const uint64_t beyond = __ballot(before + sw > at);
       if (beyond != 0) {
         const int i = __builtin_ctzll(beyond);
         b = b0 + i;
         before += __builtin_amdgcn_readlane(sw - w, i);
         item += __builtin_amdgcn_readlane(sk - k, i);
-        break;
+        s.tok0 = __builtin_amdgcn_readlane(x.tok0, i);
+        s.n = __builtin_amdgcn_readlane(x.n, i);
+        s.len = __builtin_amdgcn_readlane(x.len, i);
+        s.blocks = __builtin_amdgcn_readlane(x.blocks, i);
+        s.tiles = __builtin_amdgcn_readlane(x.tiles, i);
+        const int each = __builtin_amdgcn_readfirstlane(taken(s.tiles));
+        block = __builtin_amdgcn_readfirstlane((at - before) / each);
+        tile = at - before - block * each;
+        if (!single) end = min(end, total);
+        return true;
       }
       before += __builtin_amdgcn_readlane(sw, 63);
       item += __builtin_amdgcn_readlane(sk, 63);
     }
-    s = seq_work<M, KEYS>(p, b);
-    block = __builtin_amdgcn_readfirstlane((at - before) / s.tiles);
-    tile = at - before - block * s.tiles;
-    return true;
+    return false;
   }
   __device__ __forceinline__ int n_tiles() const { return min(s.tiles - tile, end - at); }
   __device__ __forceinline__ int rows(const LatentAttnParams& p) const { return min(s.n * p.H - block * M, M); }
   __device__ __forceinline__ bool whole() const { return n_tiles() == s.tiles; }
-  __device__ __forceinline__ int slot() const { return 2 * blockIdx.x + (at == begin ? 0 : 1); }
+  __device__ __forceinline__ int slot() const { return 2 * range + (at == begin ? 0 : 1); }
   // Who ends a row block says how it was cut.
   __device__ __forceinline__ void leave_join(const LatentAttnParams& p) const {
     if (tile + n_tiles() != s.tiles || threadIdx.x != 0 || item + block >= p.max_items) return;
@@ -138,14 +166,14 @@ struct Walk {
       const int from = at - tile;  // of the row block in the work list
       const int id = from / per;
       first = 2 * id + (from == id * per ? 0 : 1);
-      last = 2 * blockIdx.x;
+      last = 2 * range;
     }
     p.joins[item + block] = LatentJoin{s.tok0 * p.H + block * M, rows(p), first, last};
   }
   // On to the next segment. False: the range is done.
   __device__ __forceinline__ bool next(const LatentAttnParams& p) {
     at += n_tiles();
-    if (at >= end) return false;
+    if (single || at >= end) return false;
     tile = 0;
     if (++block == s.blocks) {
       block = 0;
@@ -194,11 +222,16 @@ struct TileLoads {
     pe = reinterpret_cast<const char*>(p.cache.k_pe + page * p.cache.k_pe_ps + (int64_t)in_page * kRope);
     scale = FP8 ? p.cache.scale + page * p.cache.scale_ps + in_page : nullptr;
   }
-  // Load n of kLoads.
+  // Load n of kLoads, in their order (four latent ones share an M0).
   __device__ __forceinline__ void issue(int n, int lane) const {
-    if (n < kLatentLoads) {  // a row, or two of e4m3
+    if (n < kLatentLoads) {  // a row, or two of e4m3: 1 KB
       const int r = FP8 ? 2 * n + (lane >> 5) : n;
-      load_lds16(base, r * T::kLatentRow + (16 * (FP8 ? lane & 31 : lane) ^ 16 * row_swizzle(8 * wave + r)), slot + 8 * wave * T::kLatentRow + n * 1024);
+      const int at = (FP8 ? (lane >> 5) * T::kLatentRow : 0) + (16 * (FP8 ? lane & 31 : lane) ^ 16 * row_swizzle(8 * wave + r));
+      const char* const four = base + (n & ~3) * 1024;
+      if ((n & 3) == 0) load_lds16(four, at, slot + 8 * wave * T::kLatentRow + n * 1024);
+      else if ((n & 3) == 1) load_lds16_next<1024>(four, at);
+      else if ((n & 3) == 2) load_lds16_next<2048>(four, at);
+      else load_lds16_next<3072>(four, at);
     } else if (n == kLatentLoads) {
       const int piece = (lane & 15) ^ pe_swizzle(4 * wave + (lane >> 4));
       load_lds16(pe, (4 * (piece >> 3) + (lane >> 4)) * (2 * kRope) + 16 * (piece & 7), slot + T::kPe + wave * 1024);
@@ -467,6 +500,8 @@ __device__ __forceinline__ void store_row(const LatentAttnParams& p, const W& wa
 // Where a score may exceed the reference of its row's weights, in bits, before the reference is moved: weights stay below 2^8, far from the end of
 // their range, and neither they nor the sums lose precision by it.
 constexpr float kSlack = 8.f;
+// A row's reference behind scores of up to `top`; it stands unless they are beyond the slack, whatever other rows do (no row's result depends on another's).
+__device__ __forceinline__ float moved(float reference, float top) { return top > reference + kSlack ? top : reference; }
 
 // The attention kernel for 64 rows to a workgroup (latent_attn_wide.hip).
 constexpr int kWideRows = 64;

@@ -20,7 +20,7 @@
 namespace pith {
 namespace {
 
-constexpr int kThreads = 256, kM = 16, kKeys = 32;
+constexpr int kThreads = 256, kM = 16, kKeys = 32, kStart = 3, kLeast = 1;
 
 // Scores [2 halves][16 rows][32 keys] fp32: piece k (16 bytes) of a row lies at k ^ (row % 8), so that sixteen rows of 128 bytes read or written at one
 // piece spread over all banks.
@@ -39,7 +39,7 @@ __global__ __launch_bounds__(kThreads, 2) void latent_attn_kernel(LatentAttnPara
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int c = lane & 15, g = lane >> 4;
   const int kg = wave & 1, half = wave >> 1;
-  Walk<kM, kKeys> walk;
+  Walk<kM, kKeys, kStart, kLeast> walk;
   if (!walk.start(p, lane)) return;
 
   const int key_row = 16 * kg + c;  // the key this lane brings
@@ -102,7 +102,7 @@ __global__ __launch_bounds__(kThreads, 2) void latent_attn_kernel(LatentAttnPara
 #pragma unroll
       for (int e = 1; e < 8; ++e) top = fmaxf(top, y[e]);
       if (__any(top > m + kSlack)) {  // (the same for all waves: they hold the same scores)
-        const float m_new = fmaxf(m, quad_max(top));
+        const float m_new = moved(m, quad_max(top));
         const float alpha = m_new == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - m_new);
         l *= alpha;
 #pragma unroll

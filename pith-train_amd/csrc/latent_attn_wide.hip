@@ -12,10 +12,14 @@
 // barriers more, to move it.
 #include "latent_attn.h"
 
+#include <type_traits>
+
 namespace pith {
 namespace {
 
-constexpr int kThreads = 512, kM = kWideRows, kKeys = 32, kGroups = kM / 16;
+// kLeast: parts are 128 KB each, written and read again: drafts of four sequences of 1500 e4m3 rows took 19.2 + 6.6 us (kernel + join) with ranges of 2 tiles,
+// 18.5 + 4.9 of 4, 20.5 + 4.7 of 8.
+constexpr int kThreads = 512, kM = kWideRows, kKeys = 32, kGroups = kM / 16, kStart = 8, kLeast = 4;
 
 // Two buffers of weights [64 rows][32 keys] bf16, pieces of a row swizzled so that neither the reads (16 rows, piece g or g ^ 1: row_swizzle) nor the
 // writes conflict; maxima (or sums) [64 rows][2 key groups] fp32; two stamps: the tile whose scores went beyond their slack.
@@ -38,7 +42,7 @@ __global__ __launch_bounds__(kThreads, 2) void latent_attn_wide_kernel(LatentAtt
   char* const exchange = lds + kRing * T::kBytes;
   int* const stamp = reinterpret_cast<int*>(exchange + kStamp);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  Walk<kM, kKeys> walk;
+  Walk<kM, kKeys, kStart, kLeast> walk;
   if (!walk.start(p, threadIdx.x & 63)) return;
 
   do {
@@ -46,9 +50,9 @@ __global__ __launch_bounds__(kThreads, 2) void latent_attn_wide_kernel(LatentAtt
     const int n_tiles = walk.n_tiles();
     __syncthreads();  // the ring's slots and the exchange are free: every wave is through with the segment before
     if (threadIdx.x < 2) stamp[threadIdx.x] = -1;
-    stage_queries<kM>(p, walk, staged, wave, lane_here());
 
     if (wave < 4) {
+      stage_queries<kM>(p, walk, staged, wave, lane_here());
       // Scores and weights of keys 16 kg .. of every tile, rows 32 set ..
       const int lane = lane_here(), c = lane & 15, g = lane >> 4;  // (formed in each role: what follows from it takes no register in the other)
       const int kg = wave & 1, set = wave >> 1;
@@ -152,7 +156,7 @@ __global__ __launch_bounds__(kThreads, 2) void latent_attn_wide_kernel(LatentAtt
 #pragma unroll
           for (int j = 0; j < J; ++j) {
             const f32x2 k = *reinterpret_cast<const f32x2*>(exchange + kMaxima + 8 * (16 * (J * set + j) + c));
-            const float m_new = fmaxf(fmaxf(k[0], k[1]), m[j]);
+            const float m_new = moved(m[j], fmaxf(k[0], k[1]));
             l[j] *= m_new == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m[j] - m_new);
             m[j] = m_new;
           }
@@ -190,7 +194,8 @@ __global__ __launch_bounds__(kThreads, 2) void latent_attn_wide_kernel(LatentAtt
       float m[kGroups];  // references of the lane's row of every group
 #pragma unroll
       for (int r = 0; r < kGroups; ++r) m[r] = -INFINITY;
-      wait_loads<Loads::kLoads>();
+      stage_queries<kM>(p, walk, staged, wave, lane_here());
+      wait_loads<0>();
       __syncthreads();  // (1)
       __syncthreads();  // (2)
 #pragma unroll 1
@@ -200,21 +205,26 @@ __global__ __launch_bounds__(kThreads, 2) void latent_attn_wide_kernel(LatentAtt
       __syncthreads();  // (3)
       const int value_at = value_place<FP8>(w, c, g);
       int slot = 0;
-      for (int i = 0; i < n_tiles; ++i) {
-        if (i + kRing - 2 < n_tiles) wait_loads<(kRing - 3) * Loads::kLoads>();
-        else wait_loads<0>();
-        __syncthreads();  // (4) nobody reads tile i - 1 any more
+      const auto add = [&](int i, auto more) __attribute__((always_inline)) {  // tile i
         char* const kt = lds + slot * T::kBytes;
         char* const into = lds + (slot == 0 ? kRing - 1 : slot - 1) * T::kBytes;
         slot = slot + 1 == kRing ? 0 : slot + 1;
+        const int key = key16 + (i + kRing - 1) * kKeys;
+        const Loads loads(p, next_page, key, last, into, w);
+        if (more || i + kRing - 2 < n_tiles) wait_loads<(kRing - 3) * Loads::kLoads>();
+        else wait_loads<0>();
+        __syncthreads();  // (4) nobody reads tile i - 1 any more
         const int marked = stamp[i & 1];
-        bf16x8 weight[kGroups];  // keys 8 g + e of the lane's row of each group
-        const auto read_weights = [&]() __attribute__((always_inline)) {
+        constexpr int kAhead = 4;  // products whose values are read ahead
+        const uint32_t values = lds_address(kt) + value_at;
+        bf16x8 weight[kGroups], v[kAhead];  // weights: keys 8 g + e of the lane's row of each group
+        const auto read_first = [&]() __attribute__((always_inline)) {
 #pragma unroll
           for (int r = 0; r < kGroups; ++r) weight[r] = *reinterpret_cast<const bf16x8*>(exchange + (i & 1) * kWeights + weight_at(c, g) + 16 * r * (kKeys * 2));
+#pragma unroll
+          for (int n = 0; n < kAhead; ++n) v[n] = value_fragment<FP8>(values, n);
         };
-        read_weights();
-        const uint32_t values = lds_address(kt) + value_at;
+        read_first();
         const bool clean = partial_tile<TREE, kKeys>(s, (walk.tile + i) * kKeys), beyond = __builtin_amdgcn_readfirstlane(marked) == i;
         if (beyond || clean) {
           if (beyond) {
@@ -222,38 +232,33 @@ __global__ __launch_bounds__(kThreads, 2) void latent_attn_wide_kernel(LatentAtt
 #pragma unroll
             for (int r = 0; r < kGroups; ++r) {
               const f32x2 k = *reinterpret_cast<const f32x2*>(exchange + kMaxima + 8 * (16 * r + c));
-              const float m_new = fmaxf(fmaxf(k[0], k[1]), m[r]);
+              const float m_new = moved(m[r], fmaxf(k[0], k[1]));
               const float alpha = m_new == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m[r] - m_new);
 #pragma unroll
               for (int n = 0; n < 8; ++n) scale_in_place(acc[r][n], alpha);
               m[r] = m_new;
             }
             __syncthreads();  // (6)
-            read_weights();
           }
           if (clean) clean_tile<FP8>(kt, w, lane);
+          read_first();
         }
-        const bool more = i + kRing - 1 < n_tiles;
-        const int key = key16 + (i + kRing - 1) * kKeys;
-        const Loads loads(p, next_page, key, last, into, w);
-        int ln = lane;
-        asm volatile("" : "+v"(ln));  // the requests' offsets are formed here, not kept (and spilled)
-        bf16x8 v[2] = {value_fragment<FP8>(values, 0), value_fragment<FP8>(values, 1)};
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int n = 0; n < 8; ++n) {
-          const bf16x8 now = v[n & 1];
+          const bf16x8 now = v[n % kAhead];
 #pragma unroll
           for (int r = 0; r < kGroups; ++r) acc[r][n] = mfma16(now, weight[r], acc[r][n]);
-          if (n + 2 < 8) v[n & 1] = value_fragment<FP8>(values, n + 2);
-          if (more) {  // (branches around the requests alone: two versions of the products would hold the results twice)
-            if (n < Loads::kLoads) loads.issue(n, ln);
-            if (n + 8 < Loads::kLoads) loads.issue(n + 8, ln);
-          }
+          if (n + kAhead < 8) v[n % kAhead] = value_fragment<FP8>(values, n + kAhead);
+          if (more && n < Loads::kLoads) loads.issue(n, lane);
+          if (more && n == 7 && Loads::kLoads > 8) loads.issue(8, lane);
           __builtin_amdgcn_sched_barrier(0);
         }
         if (more) next_page = page_at(p, table, key + kKeys, last);
-      }
+      };
+      int i = 0;
+      for (; i + kRing - 1 < n_tiles; ++i) add(i, std::true_type{});
+      for (; i < n_tiles; ++i) add(i, std::false_type{});
       __syncthreads();  // (7)
       __syncthreads();  // (8) the sums are there
 #pragma unroll

@@ -77,6 +77,13 @@ __device__ __forceinline__ void load_lds16_at(const void* src, char* dst_wave) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" : : "s"(lds_addr), "v"(src) : "memory");
 }
 
+// The next of a row of load_lds16's: `OFFSET` behind the last one's global base and LDS place alike (M0 stays as that statement left it: nothing else in
+// these kernels writes it).
+template <int OFFSET>
+__device__ __forceinline__ void load_lds16_next(const char* base, int offset) {
+  asm volatile("global_load_lds_dwordx4 %0, %1 offset:%2" : : "v"(offset), "s"(base), "n"(OFFSET) : "memory");
+}
+
 // Until all but the wave's last LATER requests are there.
 template <int LATER>
 __device__ __forceinline__ void wait_loads() {
