@@ -87,7 +87,7 @@ struct Walk {
   bool single;              // one segment a range
   SeqWork s;
 
-  __device__ __forceinline__ int taken(int tiles) const { return single ? (tiles + per - 1) / per * per : tiles; }  // tiles that a row block is taken for
+  __device__ __forceinline__ int taken(int tiles) const { return single && per > 1 ? (tiles + per - 1) / per * per : tiles; }  // tiles that a row block is taken for
 
   // False: nothing to do.
   __device__ __forceinline__ bool start(const LatentAttnParams& p, int lane) {
@@ -114,13 +114,13 @@ struct Walk {
     if (blockIdx.x == 0 && threadIdx.x == 0) *(__attribute__((address_space(1))) int*)(uintptr_t)p.items = min(blocks_total, p.max_items);
     const int groups = gridDim.x;
     range = (blockIdx.x & 7) * (groups >> 3) + (blockIdx.x >> 3);  // an XCD's workgroups (every eighth) take ranges that follow one another
-    per = __builtin_amdgcn_readfirstlane((total + groups - 1) / groups);  // (divisions leave the scalar registers)
+    per = total <= groups ? 1 : __builtin_amdgcn_readfirstlane((total + groups - 1) / groups);  // (divisions leave the scalar registers)
     if (blocks_total < groups) {
-      const int free = groups - blocks_total, longer = __builtin_amdgcn_readfirstlane((total + free - 1) / free);
+      const int free = groups - blocks_total, longer = total <= free ? 1 : __builtin_amdgcn_readfirstlane((total + free - 1) / free);
       if (longer <= per + START) {  // (a row block's last range is not full: at most total / longer + blocks_total ranges)
         per = max(longer, LEAST);
         single = true;
-        if (p.B <= 64) sums();
+        if (p.B <= 64 && per > 1) sums();
       }
     }
     begin = at = range * per;

@@ -158,21 +158,32 @@ __global__ __launch_bounds__(kJoinThreads) void latent_join_kernel(LatentAttnPar
   if ((int)blockIdx.x >= items || join.first == join.last || 16 * r >= join.rows) return;
   const int n = min(join.last / 2 - join.first / 2 + 1, kMaxGroups + 1);  // parts: the first slot, then the even ones up to the last
   const auto slot = [&](int i) { return (int64_t)(i == 0 ? join.first : 2 * (join.first / 2 + i)); };
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 15;
+  const int mine = wave % vectors, group = wave / vectors, groups = kWaves / vectors;
+  const int vector = blockIdx.y % shares * vectors + mine;
+  const auto part = [&](int i) { return *reinterpret_cast<const f32x4*>(p.parts + part_at<M>(slot(i), r, vector, lane)); };
+  f32x4 x[4];  // the first ones are on their way while the weights are formed (those behind the last one: that one, not used)
+#pragma unroll
+  for (int k = 0; k < 4; ++k) x[k] = part(min(group + k * groups, n - 1));
   {
     const int row = threadIdx.x / kPerRow, u = threadIdx.x % kPerRow;
-    float top = -INFINITY, sum = 0.f;
-    for (int i = u; i < n; i += kPerRow) {
-      const float m = p.stats[slot(i) * M + 16 * r + row].x;
+    const auto stat = [&](int i) { return p.stats[slot(i) * M + 16 * r + row]; };
+    const float2 one = u < n ? stat(u) : make_float2(-INFINITY, 0.f);  // (most often the thread's only one)
+    float top = one.x;
+    for (int i = u + kPerRow; i < n; i += kPerRow) {
+      const float m = stat(i).x;
       weights[row][i] = m;
       top = fmaxf(top, m);
     }
 #pragma unroll
     for (int d = 1; d < kPerRow; d <<= 1) top = fmaxf(top, __shfl_xor(top, d));
-    const float ref = top == -INFINITY ? 0.f : top;
-    for (int i = u; i < n; i += kPerRow) {
+    const float ref = top == -INFINITY ? 0.f : top, w = __builtin_amdgcn_exp2f(one.x - ref);
+    float sum = w * one.y;
+    if (u < n) weights[row][u] = w;
+    for (int i = u + kPerRow; i < n; i += kPerRow) {
       const float w = __builtin_amdgcn_exp2f(weights[row][i] - ref);
       weights[row][i] = w;
-      sum += w * p.stats[slot(i) * M + 16 * r + row].y;
+      sum += w * stat(i).y;
     }
 #pragma unroll
     for (int d = 1; d < kPerRow; d <<= 1) sum += __shfl_xor(sum, d);
@@ -185,19 +196,18 @@ __global__ __launch_bounds__(kJoinThreads) void latent_join_kernel(LatentAttnPar
     }
   }
   __syncthreads();
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 15;
-  const int mine = wave % vectors, group = wave / vectors, groups = kWaves / vectors;
-  const int vector = blockIdx.y % shares * vectors + mine;
   f32x4 o = {};
-  int i = group;
-  for (; i + 3 * groups < n; i += 4 * groups) {
-    f32x4 x[4];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) x[k] = *reinterpret_cast<const f32x4*>(p.parts + part_at<M>(slot(i + k * groups), r, vector, lane));
+  for (int k = 0; k < 4; ++k)
+    if (group + k * groups < n) o += x[k] * weights[c][group + k * groups];
+  int i = group + 4 * groups;
+  for (; i + 3 * groups < n; i += 4 * groups) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) x[k] = part(i + k * groups);
 #pragma unroll
     for (int k = 0; k < 4; ++k) o += x[k] * weights[c][i + k * groups];
   }
-  for (; i < n; i += groups) o += *reinterpret_cast<const f32x4*>(p.parts + part_at<M>(slot(i), r, vector, lane)) * weights[c][i];
+  for (; i < n; i += groups) o += part(i) * weights[c][i];
   if (groups > 1) {
     sum_o[threadIdx.x] = o;
     __syncthreads();
