@@ -246,23 +246,6 @@ struct TileLoads {
   }
 };
 
-// max / sum over the eight lanes of a row of the 32-row softmax (lane % 8 = 0 .. 7), in all of them
-template <int CTRL>
-__device__ __forceinline__ float dpp(float x) {
-  return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(x), CTRL, 0xf, 0xf, true));
-}
-constexpr int kQuadXor1 = 0xB1, kQuadXor2 = 0x4E, kHalfMirror = 0x141;
-__device__ __forceinline__ float eight_max(float x) {
-  x = fmaxf(x, dpp<kQuadXor1>(x));
-  x = fmaxf(x, dpp<kQuadXor2>(x));
-  return fmaxf(x, dpp<kHalfMirror>(x));
-}
-__device__ __forceinline__ float eight_sum(float x) {
-  x += dpp<kQuadXor1>(x);
-  x += dpp<kQuadXor2>(x);
-  return x + dpp<kHalfMirror>(x);
-}
-
 // max / sum over the four lanes c, c + 16, c + 32, c + 48 that share a query row
 __device__ __forceinline__ float quad_max(float x) {
   const int i = __float_as_int(x);
@@ -279,44 +262,6 @@ __device__ __forceinline__ float quad_sum(float x) {
 __device__ __forceinline__ bf16x8 widen(uint32_t w0, uint32_t w1) {
   const bf16x2 a = fp8x2_to_bf16<false>(w0), b = fp8x2_to_bf16<true>(w0), c = fp8x2_to_bf16<false>(w1), d = fp8x2_to_bf16<true>(w1);
   return bf16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
-}
-
-// Scores of 16 keys against J groups of query rows: STEPS times 64 latent features, then with_pe the 64 rotary ones; between(i) is called in step i. `at` is the place of the lane's
-// first piece (its row, piece g of the swizzled 256 bytes) of the tile; piece 4 k + g lies at ^ (64 k), as rows are multiples of 256 bytes.
-template <bool FP8, int J, int STEPS, int Q, typename Between>
-__device__ __forceinline__ void score(const char* tile, int at, int pe_at, bool with_pe, f32x4 scale, const bf16x8 (&q)[J][Q], f32x4 (&s)[J], Between between) {
-  // XORs on whole addresses: tiles begin at multiples of 256 bytes
-  const uint32_t first = lds_address(tile) + at, pe_first = lds_address(tile) + pe_at;
-#pragma unroll
-  for (int j = 0; j < J; ++j) s[j] = f32x4{};
-#pragma unroll
-  for (int i = 0; i < STEPS; ++i) {
-    bf16x8 k0, k1;
-    if constexpr (FP8) {  // sixteen features a lane: two steps
-      const u32x4 raw = *lds_at<u32x4>((first ^ (64 * (i & 3))) + 256 * (i >> 2));
-      k0 = widen(raw[0], raw[1]);
-      k1 = widen(raw[2], raw[3]);
-    } else {
-      k0 = *lds_at<bf16x8>((first ^ (128 * (i & 1))) + 256 * (i >> 1));
-      k1 = *lds_at<bf16x8>((first ^ (128 * (i & 1) + 64)) + 256 * (i >> 1));
-    }
-#pragma unroll
-    for (int j = 0; j < J; ++j) s[j] = mfma16(k0, q[j][2 * i], s[j]);
-    between(i);
-#pragma unroll
-    for (int j = 0; j < J; ++j) s[j] = mfma16(k1, q[j][2 * i + 1], s[j]);
-  }
-  if constexpr (FP8) {
-#pragma unroll
-    for (int j = 0; j < J; ++j) s[j] *= scale;
-  }
-  if (with_pe) {
-    const bf16x8 k0 = *lds_at<bf16x8>(pe_first), k1 = *lds_at<bf16x8>(pe_first ^ 64);
-#pragma unroll
-    for (int j = 0; j < J; ++j) s[j] = mfma16(k0, q[j][Q - 2], s[j]);
-#pragma unroll
-    for (int j = 0; j < J; ++j) s[j] = mfma16(k1, q[j][Q - 1], s[j]);
-  }
 }
 
 // A wave's products of values: product n's result v in a lane of group g is feature 16 n + 4 g + v of its 128. (Dealt so that a lane's results of two

@@ -27,6 +27,34 @@ constexpr int kThreads = 256, kM = 16, kKeys = 32, kStart = 3, kLeast = 1;
 constexpr int kExchangeBytes = 2 * kM * kKeys * 4;
 __device__ __forceinline__ int exchange_at(int row, int piece) { return row * (kKeys * 4) + ((piece ^ (row & 7)) << 4); }
 
+// Scores of 16 keys against the query rows: STEPS times 64 latent features, then with_pe the 64 rotary ones. `at` is the place of the lane's first piece
+// (its row, piece g of the swizzled 256 bytes) of the tile; piece 4 k + g lies at ^ (64 k), on whole addresses, as tiles and rows are multiples of 256 bytes.
+template <bool FP8, int STEPS, int Q>
+__device__ __forceinline__ f32x4 score(const char* tile, int at, int pe_at, bool with_pe, f32x4 scale, const bf16x8 (&q)[Q]) {
+  const uint32_t first = lds_address(tile) + at, pe_first = lds_address(tile) + pe_at;
+  f32x4 s = {};
+#pragma unroll
+  for (int i = 0; i < STEPS; ++i) {
+    bf16x8 k0, k1;
+    if constexpr (FP8) {  // sixteen features a lane: two steps
+      const u32x4 raw = *lds_at<u32x4>((first ^ (64 * (i & 3))) + 256 * (i >> 2));
+      k0 = widen(raw[0], raw[1]);
+      k1 = widen(raw[2], raw[3]);
+    } else {
+      k0 = *lds_at<bf16x8>((first ^ (128 * (i & 1))) + 256 * (i >> 1));
+      k1 = *lds_at<bf16x8>((first ^ (128 * (i & 1) + 64)) + 256 * (i >> 1));
+    }
+    s = mfma16(k0, q[2 * i], s);
+    s = mfma16(k1, q[2 * i + 1], s);
+  }
+  if constexpr (FP8) s *= scale;
+  if (with_pe) {
+    s = mfma16(*lds_at<bf16x8>(pe_first), q[Q - 2], s);
+    s = mfma16(*lds_at<bf16x8>(pe_first ^ 64), q[Q - 1], s);
+  }
+  return s;
+}
+
 template <bool FP8, bool TREE>
 __global__ __launch_bounds__(kThreads, 2) void latent_attn_kernel(LatentAttnParams p) {
   using T = LatentTile<FP8, kKeys>;
@@ -60,14 +88,14 @@ __global__ __launch_bounds__(kThreads, 2) void latent_attn_kernel(LatentAttnPara
       const int key = key16 + i * kKeys;
       Loads(p, page_at(p, table, key, last), key, last, lds + i * T::kBytes, wave).issue_all(lane);
     };
-    bf16x8 q[1][Q];
+    bf16x8 q[Q];
     char* const staged = lds + T::kBytes;  // the slots behind the first tile's
     stage_queries<kM>(p, walk, staged, wave, lane);
     request(0);
     int next_page = page_at(p, table, key16 + kRing * kKeys, last);
     wait_loads<Loads::kLoads>();  // the queries, of the waves that brought some
     __syncthreads();
-    read_query<FP8, kM>(staged, c, half * (kLatent / 2), g, q[0]);
+    read_query<FP8, kM>(staged, c, half * (kLatent / 2), g, q);
     __syncthreads();
 #pragma unroll 1
     for (int i = 1; i < min(kRing, n_tiles); ++i) request(i);
@@ -83,10 +111,9 @@ __global__ __launch_bounds__(kThreads, 2) void latent_attn_kernel(LatentAttnPara
       char* const kt = lds + slot * T::kBytes;
       const bool partial = partial_tile<TREE, kKeys>(s, key0);
       {
-        f32x4 sc = {}, x[1];
+        f32x4 sc = {};
         if constexpr (FP8) sc = *reinterpret_cast<const f32x4*>(kt + T::kScale + (16 * kg + 4 * g) * 4);
-        score<FP8, 1, kSteps>(kt, key_at, pe_at, half == 1, sc, q, x, [](int) {});
-        *reinterpret_cast<f32x4*>(exchange + exchange_at(half * kM + c, 4 * kg + g)) = x[0];
+        *reinterpret_cast<f32x4*>(exchange + exchange_at(half * kM + c, 4 * kg + g)) = score<FP8, kSteps>(kt, key_at, pe_at, half == 1, sc, q);
       }
       __syncthreads();
       if (partial) clean_tile<FP8>(kt, wave, lane);
@@ -244,7 +271,12 @@ int groups_of(int m) {
 LatentPlan plan_of(const pith_latent_attn_args* a) {
   LatentPlan pl = {};
   const int64_t rows = a->T * a->H;
-  pl.rows = rows <= kM * a->B ? kM : kWideRows;
+  // Blocks of 64 rows where sequences bring more than 16, unless the work list is short even with full page tables: two tiles a compute unit. In us (kernel +
+  // join), 16 / 64 rows: 32 sequences of 4096 rows, 16 query rows each 29.4 + 5.9 / 35.1 + 5.1, 32 rows 36.8 + 5.5 / 35.3 + 6.0, 48 rows 73.3 + 6.2 /
+  // 34.8 + 6.6; 4 sequences of 1500 rows, 64 query rows each 13.8 + 5.6 / 17.1 + 5.1, 128 rows (e4m3) 17.5 + 5.2 / 18.6 + 4.9.
+  const int64_t sequences = a->B < a->T ? a->B : a->T, blocks = (rows + kWideRows - 1) / kWideRows;
+  const int64_t tiles = (blocks > sequences ? blocks : sequences) * ((a->table_width * a->cache.page_size + kKeys - 1) / kKeys);
+  pl.rows = rows <= kM * a->B || tiles <= 2 * compute_units_or_default() ? kM : kWideRows;
   pl.groups = groups_of(pl.rows);
   const auto items = [&](int m) { return (rows + m - 1) / m + (a->B < a->T ? a->B : a->T); };
   pl.max_items = (int)items(pl.rows);

@@ -12,6 +12,7 @@ Bounds are elementwise and come from the arithmetic, u = 2^-8 being bf16's half 
 """
 
 import math
+import sys
 
 import pytest
 import torch
@@ -39,6 +40,9 @@ def _within(got, want, bound, what):
     assert over.numel() == 0 or over.max() <= 0, f"{what}: off by {((got - want).abs() / bound.clamp_min(1e-300))[fine].max():.3f} times the bound"
 
 
+MIN_WIDTH = 0  # of page tables: blocks of 64 query rows are for those that are wide
+
+
 class Batch:
     """Sequences in a cache. counts: new tokens of each, lengths: cached rows of each. Everything that no sequence owns (rows behind the last one of a
     page, pages of nobody, table entries that are not needed) holds NaN or nonsense."""
@@ -49,7 +53,7 @@ class Batch:
         self.counts, self.lengths, self.h, self.dev, self.page = counts, lengths, h, dev, page
         t = sum(counts) + extra_tokens
         need = [-(-n // page) for n in lengths]
-        pages, width = sum(need) + 3, max(max(need), 1) + 1
+        pages, width = sum(need) + 3, max(max(need), 1, MIN_WIDTH) + 1
         order = torch.randperm(pages, generator=g)
         table = torch.randint(-5, 2 * pages, (len(counts), width), generator=g).to(I32)  # entries behind a sequence's pages are never followed
         at = 0
@@ -246,6 +250,51 @@ def test_a_single_draft_that_does_not_see_itself_is_not_reached_by_its_row(gpu, 
         b.k_pe[page, row] = math.nan
     o, lse = b.attention()
     assert torch.equal(o, want_o) and torch.equal(lse, want_lse)
+
+
+@pytest.mark.parametrize("fp8", [False, True], ids=["bf16", "fp8"])
+@pytest.mark.parametrize("name", LENGTH_SETS)
+@pytest.mark.parametrize("h", [16, 37])
+def test_blocks_of_64_rows_match_the_oracle(gpu, monkeypatch, name, h, fp8):
+    monkeypatch.setattr(sys.modules[__name__], "MIN_WIDTH", 2048)
+    test_attention_matches_the_oracle(gpu, name, h, fp8)
+
+
+@pytest.mark.parametrize("fp8", [False, True], ids=["bf16", "fp8"])
+@pytest.mark.parametrize("kind", ["tree", "holes"])
+@pytest.mark.parametrize("counts,lengths,h", [([1], [1], 40), ([8, 8], [517, 8], 16), ([64, 1, 33], [64, 300, 1000], 3), ([7, 0, 12], [40, 5, 12], 16), ([64], [63], 2)])
+def test_trees_in_blocks_of_64_rows_match_the_oracle(gpu, monkeypatch, counts, lengths, h, kind, fp8):
+    monkeypatch.setattr(sys.modules[__name__], "MIN_WIDTH", 4096)
+    test_tree_attention_matches_the_oracle(gpu, counts, lengths, h, kind, fp8)
+
+
+# One row block over many workgroups; row blocks that are cut wherever the ranges end; more sequences than a wavefront scans at once.
+@pytest.mark.parametrize("fp8", [False, True], ids=["bf16", "fp8"])
+@pytest.mark.parametrize("counts,lengths,h", [([4, 1], [20011, 3], 16), ([63], [3001], 128), ([2, 0, 1] * 40, list(range(7, 127)), 24)])
+def test_work_lists_of_blocks_of_64_rows(gpu, monkeypatch, counts, lengths, h, fp8):
+    monkeypatch.setattr(sys.modules[__name__], "MIN_WIDTH", 2048)
+    b = Batch(gpu, counts, lengths, h, page=16, fp8=fp8, seed=15, q_std=1.0)
+    b.check(*b.attention())
+
+
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("tree", [None, "tree"])
+def test_blocks_of_64_rows_are_not_reached_by_rows_that_they_do_not_see(gpu, monkeypatch, bad, tree):
+    monkeypatch.setattr(sys.modules[__name__], "MIN_WIDTH", 4096)
+    test_a_row_that_a_token_does_not_see_cannot_reach_it(gpu, bad, tree)
+
+
+@pytest.mark.parametrize("bad", ["latent", "scale", "infinite scale"])
+def test_blocks_of_64_rows_are_not_reached_by_rows_of_e4m3_that_they_do_not_see(gpu, monkeypatch, bad):
+    monkeypatch.setattr(sys.modules[__name__], "MIN_WIDTH", 4096)
+    test_a_row_of_e4m3_that_a_token_does_not_see_cannot_reach_it(gpu, bad, 40)
+    for fp8 in (False, True):
+        test_a_single_draft_that_does_not_see_itself_is_not_reached_by_its_row(gpu, fp8, 40)
+
+
+def test_large_scores_in_blocks_of_64_rows_do_not_overflow(gpu, monkeypatch):
+    monkeypatch.setattr(sys.modules[__name__], "MIN_WIDTH", 2048)
+    test_large_scores_do_not_overflow(gpu)
 
 
 def test_tokens_behind_the_last_sequence_are_left_alone(gpu):
