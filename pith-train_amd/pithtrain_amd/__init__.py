@@ -3,6 +3,7 @@ hot path: hand-written HIP kernels behind a flat C ABI (libpith_hip.so), called 
 host code that keeps the reference operators' Python signatures.
 
 Layout (mirrors pithtrain/operators/ of the reference):
+    operators/mla/latent.py              latent cache and absorbed attention of the MLA layer (LatentCache, latent_attention, ...)
     operators/mla/hip.py                 _mla_fwd, _mla_bwd_preprocess, _mla_bwd_dk_dv, _mla_bwd_dq, MLA
     operators/ring_attention/mla.py      _online_softmax_combine_log2, RingMLAAttentionFunc, ring_mla_attention_func
     operators/ring_attention/standard.py _online_softmax_combine, RingAttentionFunc, ring_attention_func
