@@ -107,10 +107,11 @@ int pith_latent_absorb_value(const pith_latent_absorb_args* args, pith_stream_t 
  * Tokens cu_q[b] .. cu_q[b+1]-1 are sequence b's, its last n = cu_q[b+1]-cu_q[b] rows of lengths[b]. Token i of them sees rows up to
  * lengths[b]-n+i (causal); with tree_mask all rows in front of the n newest, and of those row j where bit j of tree_mask[token] is set (sequences
  * with n > 64 are then computed with their first 64 new rows visible by bits and none behind: keep n <= 64). A token that sees nothing gets o = 0
- * and lse = -inf. Tokens from cu_q[B] on are left alone. Lengths are clamped to table_width * page_size, page numbers to the cache.
+ * and lse = -inf. Tokens from cu_q[B] on are left alone. Lengths are clamped to table_width * page_size, page numbers to the cache, and offsets of
+ * cu_q count as their maximum so far, so that a token belongs to one sequence.
  * q_latent [T,H,512], q_pe [T,H,64], o [T,H,512] bf16 with token and head strides (multiples of 8); lse [H,T] fp32 (head stride lse_hs).
  * lengths [B], cu_q [B+1], page_table [B, table_width] int32; tree_mask [T] int64 or NULL. All of them are read by the kernels only: a call that
- * was captured into a graph can be replayed after their contents, and those of the cache, have changed.
+ * was captured into a graph can be replayed after their contents, and those of the cache, have changed. They must not change while it runs.
  * workspace: pith_latent_attn_workspace_bytes of the same arguments, 256-byte aligned, used by the call's kernels only. Calls that may overlap in
  * time need one each. */
 typedef struct {

@@ -57,7 +57,7 @@ __global__ __launch_bounds__(kRotateThreads) void absorb_rotate_kernel(AbsorbPar
   rotate_queries<kRotateThreads>(p, blockIdx.x);
 }
 
-// The first `products` workgroups: q_latent features [64 WAVES x, + 64 WAVES) of a head, a block of tokens; the others rotate. W_uk's rows are the
+// The first `products` workgroups: q_latent features [64 WAVES x, + 64 WAVES) of a head, a block of tokens; the others (WAVES = 2) rotate. W_uk's rows are the
 // contraction (d), so its fragments come transposed out of LDS, where it lies in slices of 128 features, 256 bytes a row; wave w's 64 features are four
 // products whose rows are dealt so that a lane's results of two are eight consecutive features (product n, row 4 g + v: feature
 // 32 (n / 2) + 8 g + 4 (n % 2) + v). Then the ring of tiles of 32 tokens takes that place. Fetched as fragments, queries took the address unit 64
@@ -69,7 +69,9 @@ __global__ __launch_bounds__(64 * WAVES) void absorb_query_kernel(AbsorbParams p
   constexpr int kTokens = 32, kTile = kTokens * kRowBytes128, kRing = kSlices * 128 * kRowBytes128 / kTile + 1, kLoads = kTokens / 4 / WAVES;
   __shared__ __attribute__((aligned(1024))) char lds[kRing * kTile];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  if ((int)blockIdx.x >= products) return rotate_queries<64 * WAVES>(p, blockIdx.x - products);
+  if constexpr (WAVES == 2) {
+    if ((int)blockIdx.x >= products) return rotate_queries<64 * WAVES>(p, blockIdx.x - products);
+  }
   const int of = blockIdx.x / (8 * kColumns) * 8 + (blockIdx.x & 7), x = (blockIdx.x >> 3) % kColumns;  // head and block, column
   const int h = __builtin_amdgcn_readfirstlane(of / blocks);
   if (h >= p.H) return;

@@ -50,17 +50,20 @@ struct SeqWork {
   int blocks, tiles;  // row blocks, tiles of each
 };
 
+// Of tokens c0 .. c1 - 1 and a cached length as the caller gave it.
 template <int M, int KEYS>
-__device__ __forceinline__ SeqWork seq_work(const LatentAttnParams& p, int b) {
+__device__ __forceinline__ SeqWork seq_work(const LatentAttnParams& p, int c0, int c1, int length) {
   SeqWork s;
-  const int c0 = min(max(p.cu_q[b], 0), p.T), c1 = min(max(p.cu_q[b + 1], c0), p.T);
   s.tok0 = c0;
   s.n = c1 - c0;
-  s.len = min(max(p.lengths[b], 0), p.max_len);
+  s.len = min(max(length, 0), p.max_len);
   s.blocks = (s.n * p.H + M - 1) / M;
   s.tiles = max((s.len + KEYS - 1) / KEYS, 1);  // rows without keys get their zeros from an empty tile
   return s;
 }
+// Token offsets are taken as their maximum so far, so that whatever they hold no token belongs to two sequences, and the work list is no longer than the
+// host has made sure of.
+__device__ __forceinline__ int token_offset(const LatentAttnParams& p, int i) { return min(max(p.cu_q[i], 0), p.T); }
 
 // Inclusive sums over the lanes of a wavefront.
 template <int CTRL, int ROWS>
@@ -74,6 +77,20 @@ __device__ __forceinline__ int wave_scan(int x) {
   x = add_dpp<0x118, 0xf>(x);
   x = add_dpp<0x142, 0xa>(x);  // lane 15 of a row to the next row, then lane 31 to the upper half
   return add_dpp<0x143, 0xc>(x);
+}
+
+// Inclusive maxima of values from 0 on.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int max_dpp(int x) {
+  return max(x, __builtin_amdgcn_update_dpp(0, x, CTRL, ROWS, 0xf, false));
+}
+__device__ __forceinline__ int wave_scan_max(int x) {
+  x = max_dpp<0x111, 0xf>(x);
+  x = max_dpp<0x112, 0xf>(x);
+  x = max_dpp<0x114, 0xf>(x);
+  x = max_dpp<0x118, 0xf>(x);
+  x = max_dpp<0x142, 0xa>(x);
+  return max_dpp<0x143, 0xc>(x);
 }
 
 // A workgroup's way through its range of the work list, segment by segment (tiles of one row block). Every wave walks for itself; all of it is
@@ -93,9 +110,13 @@ struct Walk {
   __device__ __forceinline__ bool start(const LatentAttnParams& p, int lane) {
     SeqWork x = {};
     int w = 0, k = 0, sw = 0, sk = 0, total = 0, blocks_total = 0;
-    const auto load = [&](int b0) __attribute__((always_inline)) {  // of 64 sequences
-      x.blocks = x.tiles = 0;
-      if (b0 + lane < p.B) x = seq_work<M, KEYS>(p, b0 + lane);
+    int behind = 0;  // the sequences that were loaded: their last offset
+    const auto load = [&](int b0) __attribute__((always_inline)) {  // 64 sequences
+      if (b0 == 0) behind = token_offset(p, 0);
+      const bool some = b0 + lane < p.B;
+      const int c1 = max(wave_scan_max(some ? token_offset(p, b0 + lane + 1) : 0), behind);  // (lanes without one: no tokens)
+      x = seq_work<M, KEYS>(p, __builtin_amdgcn_update_dpp(behind, c1, 0x138, 0xf, 0xf, false), c1, some ? p.lengths[b0 + lane] : 0);  // from the lane below
+      behind = __builtin_amdgcn_readlane(c1, 63);
     };
     const auto sums = [&]() __attribute__((always_inline)) {
       k = x.blocks;
@@ -178,7 +199,11 @@ struct Walk {
     if (++block == s.blocks) {
       block = 0;
       item += s.blocks;
-      do s = seq_work<M, KEYS>(p, ++b); while (s.blocks == 0);
+      do {
+        ++b;
+        const int c0 = s.tok0 + s.n;
+        s = seq_work<M, KEYS>(p, c0, max(token_offset(p, b + 1), c0), p.lengths[b]);
+      } while (s.blocks == 0);
     }
     return true;
   }

@@ -326,6 +326,22 @@ def test_pages_and_lengths_out_of_range_stay_in_memory(gpu):
     torch.cuda.synchronize()
 
 
+@pytest.mark.parametrize("width", [0, 2048])
+def test_no_token_belongs_to_two_sequences(gpu, monkeypatch, width):
+    """Token offsets that go back are taken as their maximum so far."""
+    monkeypatch.setattr(sys.modules[__name__], "MIN_WIDTH", width)
+    n = 70
+    b = Batch(gpu, [3, 0] + [0] * (n - 3) + [5], [40] * n, 16, seed=16)
+    want = b.attention()
+    b.check(*want)
+    down = b.cu_q.clone()
+    down[2:-1] = torch.tensor([0, 3, 1, -7], dtype=I32, device=gpu).repeat(n)[: n - 2]
+    assert not torch.equal(down, b.cu_q)
+    b.cu_q.copy_(down)
+    for x, y in zip(b.attention(), want):
+        assert torch.equal(x, y)
+
+
 @pytest.mark.parametrize("fp8", [False, True], ids=["bf16", "fp8"])
 def test_strided_queries_caches_and_tables(gpu, fp8):
     """Queries and page tables as slices, a cache that is one layer of an allocation for several, results into slices: the same bits."""
