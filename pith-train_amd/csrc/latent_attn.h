@@ -6,8 +6,10 @@
 // as many workgroups as its share of the tiles.
 // To begin and end a row block costs a workgroup the time of several tiles (START: queries, first tile, parts). Where there are fewer row blocks than
 // workgroups, ranges can therefore be a little longer and each lie in one row block: every row block is taken for as many tiles as fill whole ranges, LEAST
-// tiles or more. The row blocks of a sequence are then cut alike, and as an XCD's workgroups take ranges that follow one another, its cache fetches their
-// tiles about once: 128 heads 73 us at best against 68, trees of up to 48 drafts 194 against 172.
+// tiles or more, the ranges as short as the workgroups allow. The row blocks of a sequence are then cut alike, and as an XCD's workgroups take ranges that
+// follow one another, they go through the same tiles at the same time, which its cache fetches about once. Blocks of 64 rows (several a sequence) gain by
+// that up to a quarter of their time, so ranges may be a quarter longer: a call for 128 heads took 80 us with ranges cut anywhere and takes 72, one for trees of
+// up to 48 drafts 192 and 166 (with all tiles in the caches, 67 and 146).
 // A workgroup whose range covers a row block wholly writes its rows; parts of a row block leave (reference, sum, unnormalised result) in fp32 in the
 // workspace, and a second kernel joins them in the order of the keys (results do not depend on scheduling).
 #pragma once
@@ -136,12 +138,17 @@ struct Walk {
     const int groups = gridDim.x;
     range = (blockIdx.x & 7) * (groups >> 3) + (blockIdx.x >> 3);  // an XCD's workgroups (every eighth) take ranges that follow one another
     per = total <= groups ? 1 : __builtin_amdgcn_readfirstlane((total + groups - 1) / groups);  // (divisions leave the scalar registers)
-    if (blocks_total < groups) {
-      const int free = groups - blocks_total, longer = total <= free ? 1 : __builtin_amdgcn_readfirstlane((total + free - 1) / free);
-      if (longer <= per + START) {  // (a row block's last range is not full: at most total / longer + blocks_total ranges)
-        per = max(longer, LEAST);
-        single = true;
-        if (p.B <= 64 && per > 1) sums();
+    if (blocks_total < groups && p.B <= 64 && total < 1 << 30) {  // (more sequences are not looked up twice)
+      const int most = per + START + (M > 16 ? per / 4 : 0);
+      int longer = max(per, LEAST);
+      for (int ranges; longer <= most; longer = max(longer + 1, __builtin_amdgcn_readfirstlane((int)(longer * ((float)ranges / groups))))) {
+        ranges = __builtin_amdgcn_readlane(wave_scan(k * (longer > 1 ? (x.tiles + longer - 1) / longer : x.tiles)), 63);
+        if (ranges <= groups) {
+          per = longer;
+          single = true;
+          if (per > 1) sums();
+          break;
+        }
       }
     }
     begin = at = range * per;
