@@ -262,8 +262,8 @@ struct TileLoads {
       const char* const four = base + (n & ~3) * 1024;
       if ((n & 3) == 0) load_lds16(four, at, slot + 8 * wave * T::kLatentRow + n * 1024);
       else if ((n & 3) == 1) load_lds16_next<1024>(four, at);
-      else if ((n & 3) == 2) load_lds16_next<2048>(four, at);
-      else load_lds16_next<3072>(four, at);
+      else if ((n & 3) == 2) load_lds16_next<2 * 1024>(four, at);
+      else load_lds16_next<3 * 1024>(four, at);
     } else if (n == kLatentLoads) {
       const int piece = (lane & 15) ^ pe_swizzle(4 * wave + (lane >> 4));
       load_lds16(pe, (4 * (piece >> 3) + (lane >> 4)) * (2 * kRope) + 16 * (piece & 7), slot + T::kPe + wave * 1024);

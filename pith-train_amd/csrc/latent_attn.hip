@@ -15,6 +15,8 @@
 //            exchange and barrier)
 //   result   wave w: features 128 w ..
 // Every fragment of a tile is read from LDS once for its keys and once for its values.
+// 32 sequences of up to 8192 rows, 16 heads: 37 us (171 MB, 4.7 TB/s) and 6.5 for the join; 8 of up to 131072 e4m3 rows: 106 us (536 MB, 5.1 TB/s) and 8; one of 517 rows:
+// 7.2 and 4.2. Memory bounds the first two, the chain from work list to first tile the last.
 #include "latent_attn.h"
 
 namespace pith {
@@ -170,8 +172,8 @@ constexpr int kMaxGroups = 512;  // workgroups of the attention kernel, at most:
 
 // Joins the parts of a row block: o = sum_i w_i O_i / sum_i w_i l_i, w_i = 2^(m_i - max m). blockIdx.x: row block; blockIdx.y: group of 16 rows of it,
 // and which `vectors` of its 32 result vectors (part_at). The weights of the rows are formed first, in one pass over their references and sums, so that
-// the loads of the sums over the parts do not wait for one another; where a workgroup has fewer vectors than waves, several waves take every other
-// part and add up in LDS.
+// the loads of the sums over the parts do not wait for one another (the first of them are on their way by then); where a workgroup has fewer vectors than
+// waves, several waves take every other part and add up in LDS. 17 MB of parts: 6.5 us, 33 MB: 9.6; parts of one row block: 4.2, two latencies and a launch.
 template <int M>
 __global__ __launch_bounds__(kJoinThreads) void latent_join_kernel(LatentAttnParams p, int vectors) {
   constexpr int kWaves = kJoinThreads / 64;
