@@ -2,6 +2,7 @@
 // layers: what is not of ordinary layout, or rejected by the library, goes to the Python body, nothing having been launched.
 #pragma once
 
+#include <ATen/hip/EmptyTensor.h>
 #include <c10/hip/HIPGuard.h>
 
 #include "pith_latent.h"
@@ -21,6 +22,9 @@ void token_strides(const Tensor& t, int64_t* ts, int64_t* hs) {
   *ts = t.size(0) > 1 ? t.stride(0) : t.size(1) * t.size(2);
   *hs = t.size(1) > 1 ? t.stride(1) : t.size(2);
 }
+
+// A new tensor on the device of `like`, past the dispatcher: nothing between this op and the allocator wants to see it.
+Tensor fresh(const Tensor& like, at::IntArrayRef shape, at::ScalarType dtype) { return at::detail::empty_cuda(shape, dtype, like.device(), std::nullopt); }
 
 bool checking_positions() {
   const char* e = std::getenv("PITHTRAIN_AMD_CHECK_POSITIONS");
@@ -90,7 +94,7 @@ Two latent_gather(const Tensor& latent, const Tensor& k_pe, const OptTensor& sca
     a.rows = rows;
     if (latent_cache_args(a.cache, latent, latent, k_pe, scale) && is_index(cu_rows, latent, at::kInt, {a.B + 1}) &&
         page_table_args(table, latent, a.B, &a.page_table, &a.table_rs, &a.table_width)) {
-      Tensor out = empty_like_shape(latent, {rows, PITH_LATENT_DIM}, at::kBFloat16), pe = empty_like_shape(latent, {rows, PITH_LATENT_ROPE_DIM}, at::kBFloat16);
+      Tensor out = fresh(latent, {rows, PITH_LATENT_DIM}, at::kBFloat16), pe = fresh(latent, {rows, PITH_LATENT_ROPE_DIM}, at::kBFloat16);
       a.cu_rows = cu_rows.data_ptr<int32_t>();
       a.latent_out = out.data_ptr(); a.k_pe_out = pe.data_ptr();
       a.latent_rs = PITH_LATENT_DIM; a.k_pe_rs = PITH_LATENT_ROPE_DIM;
@@ -114,7 +118,7 @@ bool absorb_args(pith_latent_absorb_args& a, const Tensor& x, const Tensor& weig
 Two latent_absorb_query(const Tensor& q, const Tensor& weight, const Tensor& cos, const Tensor& sin, const Tensor& pos) {
   if (q.is_cuda() && q.dim() == 3 && !checking_positions()) {
     const c10::hip::HIPGuard guard(q.device().index());
-    Tensor out = empty_like_shape(q, {q.size(0), q.size(1), PITH_LATENT_DIM}, q.scalar_type()), pe = empty_like_shape(q, {q.size(0), q.size(1), PITH_LATENT_ROPE_DIM}, q.scalar_type());
+    Tensor out = fresh(q, {q.size(0), q.size(1), PITH_LATENT_DIM}, q.scalar_type()), pe = fresh(q, {q.size(0), q.size(1), PITH_LATENT_ROPE_DIM}, q.scalar_type());
     pith_latent_absorb_args a = {};
     if (absorb_args(a, q, weight, out, PITH_LATENT_NOPE_DIM + PITH_LATENT_ROPE_DIM) && rotary_tables(cos, sin, q, &a.P) && is_index(pos, q, at::kLong, {a.T})) {
       a.q_pe = pe.data_ptr();
@@ -129,7 +133,7 @@ Two latent_absorb_query(const Tensor& q, const Tensor& weight, const Tensor& cos
 Tensor latent_absorb_value(const Tensor& x, const Tensor& weight) {
   if (x.is_cuda() && x.dim() == 3) {
     const c10::hip::HIPGuard guard(x.device().index());
-    Tensor out = empty_like_shape(x, {x.size(0), x.size(1), PITH_LATENT_VALUE_DIM}, x.scalar_type());
+    Tensor out = fresh(x, {x.size(0), x.size(1), PITH_LATENT_VALUE_DIM}, x.scalar_type());
     pith_latent_absorb_args a = {};
     if (absorb_args(a, x, weight, out, PITH_LATENT_DIM) && accepted(pith_latent_absorb_value(&a, stream_of(x)))) return out;
   }
@@ -145,7 +149,7 @@ Two latent_attention(const Tensor& q_latent, const Tensor& q_pe, const Tensor& l
     if (rows_of(q_pe, q_latent, 3, PITH_LATENT_ROPE_DIM) && q_pe.size(0) == a.T && q_pe.size(1) == a.H && latent_cache_args(a.cache, q_latent, latent, k_pe, scale) &&
         page_table_args(table, q_latent, a.B, &a.page_table, &a.table_rs, &a.table_width) && is_index(lengths, q_latent, at::kInt, {a.B}) &&
         is_index(cu_q, q_latent, at::kInt, {a.B + 1}) && (!tree || is_index(*tree, q_latent, at::kLong, {a.T}))) {
-      Tensor o = empty_like_shape(q_latent, {a.T, a.H, PITH_LATENT_DIM}, at::kBFloat16), lse = empty_like_shape(q_latent, {a.H, a.T}, at::kFloat);
+      Tensor o = fresh(q_latent, {a.T, a.H, PITH_LATENT_DIM}, at::kBFloat16), lse = fresh(q_latent, {a.H, a.T}, at::kFloat);
       a.q_latent = q_latent.data_ptr(); a.q_pe = q_pe.data_ptr(); a.o = o.data_ptr(); a.lse = lse.data_ptr<float>();
       a.lengths = lengths.data_ptr<int32_t>(); a.cu_q = cu_q.data_ptr<int32_t>();
       a.tree_mask = tree ? tree->data_ptr<int64_t>() : nullptr;
@@ -155,7 +159,7 @@ Two latent_attention(const Tensor& q_latent, const Tensor& q_pe, const Tensor& l
       a.lse_hs = a.T;
       a.scale = (float)softmax_scale;
       a.workspace_bytes = pith_latent_attn_workspace_bytes(&a);
-      Tensor ws = empty_like_shape(q_latent, {a.workspace_bytes}, at::kByte);
+      Tensor ws = fresh(q_latent, {a.workspace_bytes}, at::kByte);
       a.workspace = ws.data_ptr();
       if (accepted(pith_latent_attn(&a, stream_of(q_latent)))) return {o, lse};
     }
@@ -164,22 +168,20 @@ Two latent_attention(const Tensor& q_latent, const Tensor& q_pe, const Tensor& l
 }
 
 // No gradients: a call that would have to record one is refused rather than cut off from the graph.
-void collect(variable_list&, const std::optional<double>&) {}
+bool records(const Tensor& t) { return t.requires_grad(); }
+bool records(const OptTensor& t) { return t.has_value() && t->requires_grad(); }
+bool records(double) { return false; }
+bool records(int64_t) { return false; }
 template <auto BODY>
 struct ServingOp;
 template <typename R, typename... Args, R (*BODY)(Args...)>
 struct ServingOp<BODY> {
   template <const char* NAME>
-  static R call(Args... args) {
+  static R call(c10::DispatchKeySet keys, Args... args) {
     static const auto op = op_handle<R(Args...)>(NAME);
-    if (at::GradMode::is_enabled()) {
-      variable_list inputs;
-      (collect(inputs, args), ...);
-      for (const Tensor& t : inputs)
-        TORCH_CHECK(!t.requires_grad(), NAME, " has no backward: call it under torch.no_grad(), or detach what requires a gradient");
-    }
+    TORCH_CHECK(!at::GradMode::is_enabled() || !(records(args) || ...), NAME, " has no backward: call it under torch.no_grad(), or detach what requires a gradient");
     at::AutoDispatchBelowADInplaceOrView guard;
-    return op.call(args...);
+    return op.redispatch(keys & c10::after_ADInplaceOrView_keyset, args...);
   }
 };
 
