@@ -330,22 +330,30 @@ template <bool FP8>
 __device__ __forceinline__ void clean_tile(char* tile, int w, int lane) {
   constexpr int kPieces = FP8 ? 8 : 16;  // of a row
 #pragma unroll 1
-  for (int i = lane; i < 32 * kPieces; i += 64) {
-    const int row = i / kPieces, piece = kPieces * w + i % kPieces;
-    u32x4* const at = reinterpret_cast<u32x4*>(tile + row * LatentTile<FP8, 32>::kLatentRow + ((piece ^ row_swizzle(row)) << 4));
-    u32x4 x = *at;
+  for (int i0 = lane; i0 < 32 * kPieces; i0 += 4 * 64) {  // four a lane at a time
+    u32x4 x[4];
+    char* at[4];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      if constexpr (FP8) {
-#pragma unroll
-        for (int k = 0; k < 32; k += 8)
-          if (((x[e] >> k) & 0x7fu) == 0x7fu) x[e] &= ~(0xffu << k);
-      } else {
-        if ((x[e] & 0x7f80u) == 0x7f80u) x[e] &= 0xffff0000u;
-        if ((x[e] & 0x7f800000u) == 0x7f800000u) x[e] &= 0xffffu;
-      }
+    for (int j = 0; j < 4; ++j) {
+      const int i = i0 + 64 * j, row = i / kPieces, piece = kPieces * w + i % kPieces;
+      at[j] = tile + row * LatentTile<FP8, 32>::kLatentRow + ((piece ^ row_swizzle(row)) << 4);
+      x[j] = *reinterpret_cast<const u32x4*>(at[j]);
     }
-    *at = x;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if constexpr (FP8) {
+#pragma unroll
+          for (int k = 0; k < 32; k += 8)
+            if (((x[j][e] >> k) & 0x7fu) == 0x7fu) x[j][e] &= ~(0xffu << k);
+        } else {
+          if ((x[j][e] & 0x7f80u) == 0x7f80u) x[j][e] &= 0xffff0000u;
+          if ((x[j][e] & 0x7f800000u) == 0x7f800000u) x[j][e] &= 0xffffu;
+        }
+      }
+      *reinterpret_cast<u32x4*>(at[j]) = x[j];
+    }
   }
 }
 
