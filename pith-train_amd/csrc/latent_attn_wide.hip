@@ -69,10 +69,11 @@ __global__ __launch_bounds__(kThreads, 2) void latent_attn_wide_kernel(LatentAtt
       for (int j = 0; j < J; ++j) read_query<FP8, kM>(staged, 16 * (J * set + j) + c, 0, g, q[j]);
       __syncthreads();  // (2) and have been read
 
-      f32x4 x[J], sc = {};  // scores of a tile, scales of its keys
-      float m[J], l[J];     // references of the lane's rows, and sums over its keys
+      f32x4 x[J], sc = {};       // scores of a tile, scales of its keys
+      float factor = p.kappa;    // what the scores are still to be multiplied by
+      float m[J], ref[J], l[J];  // references of the lane's rows, the same to subtract (0 while there is none), and sums over its keys
 #pragma unroll
-      for (int j = 0; j < J; ++j) m[j] = -INFINITY, l[j] = 0.f;
+      for (int j = 0; j < J; ++j) m[j] = -INFINITY, ref[j] = l[j] = 0.f;
       const auto tile_scores = [&](const char* kt, f32x4 (&y)[J]) __attribute__((always_inline)) {
         constexpr int kLatentReads = FP8 ? kLatent / 64 : kLatent / 32, kReads = kLatentReads + 2, kAhead = 6;  // fragments read ahead of their products
         const uint32_t first = lds_address(kt) + key_at, pe_first = lds_address(kt) + pe_at;
@@ -110,10 +111,9 @@ __global__ __launch_bounds__(kThreads, 2) void latent_attn_wide_kernel(LatentAtt
       const auto leave_weights = [&](int i, float (&sum)[J], const f32x4& scale) __attribute__((always_inline)) {
 #pragma unroll
         for (int j = 0; j < J; ++j) {
-          const float ref = m[j] == -INFINITY ? 0.f : m[j];
           f32x4 w;
 #pragma unroll
-          for (int v = 0; v < 4; ++v) w[v] = __builtin_amdgcn_exp2f(x[j][v] - ref);
+          for (int v = 0; v < 4; ++v) w[v] = __builtin_amdgcn_exp2f(fmaf(x[j][v], factor, -ref[j]));
           sum[j] = (w[0] + w[1]) + (w[2] + w[3]);
           if constexpr (FP8) {
 #pragma unroll
@@ -126,13 +126,18 @@ __global__ __launch_bounds__(kThreads, 2) void latent_attn_wide_kernel(LatentAtt
       const auto weigh = [&](int i, float (&sum)[J]) __attribute__((always_inline)) {  // scores x of tile i
         const int key0 = (walk.tile + i) * kKeys;
         bool beyond = false;
+        factor = p.kappa;
+        if (partial_tile<TREE, kKeys>(s, key0) || p.kappa < 0.f) {  // (below zero the largest score is not the largest product)
+          factor = 1.f;
 #pragma unroll
-        for (int j = 0; j < J; ++j) {
-          x[j] *= p.kappa;
-          if (partial_tile<TREE, kKeys>(s, key0))
-            mask_scores<TREE, 4>(p, s, x[j], (walk.block * kM + min(16 * (J * set + j) + c, walk.rows(p) - 1)) / p.H, key0 + 16 * kg + 4 * g);
-          beyond |= fmaxf(fmaxf(x[j][0], x[j][1]), fmaxf(x[j][2], x[j][3])) > m[j] + kSlack;
+          for (int j = 0; j < J; ++j) {
+            x[j] *= p.kappa;
+            if (partial_tile<TREE, kKeys>(s, key0))
+              mask_scores<TREE, 4>(p, s, x[j], (walk.block * kM + min(16 * (J * set + j) + c, walk.rows(p) - 1)) / p.H, key0 + 16 * kg + 4 * g);
+          }
         }
+#pragma unroll
+        for (int j = 0; j < J; ++j) beyond |= fmaxf(fmaxf(x[j][0], x[j][1]), fmaxf(x[j][2], x[j][3])) * factor > m[j] + kSlack;
         leave_weights(i, sum, sc);
         if (__any(beyond) && lane == 0) stamp[i & 1] = i;
       };
@@ -152,7 +157,7 @@ __global__ __launch_bounds__(kThreads, 2) void latent_attn_wide_kernel(LatentAtt
         if (__builtin_amdgcn_readfirstlane(marked) == i) {
 #pragma unroll
           for (int j = 0; j < J; ++j) {
-            const float top = quad_max(fmaxf(fmaxf(x[j][0], x[j][1]), fmaxf(x[j][2], x[j][3])));
+            const float top = quad_max(fmaxf(fmaxf(x[j][0], x[j][1]), fmaxf(x[j][2], x[j][3]))) * factor;
             if (g == 0) *reinterpret_cast<float*>(exchange + kMaxima + 8 * (16 * (J * set + j) + c) + 4 * kg) = top;
           }
           __syncthreads();  // (5)
@@ -162,6 +167,7 @@ __global__ __launch_bounds__(kThreads, 2) void latent_attn_wide_kernel(LatentAtt
             const float m_new = moved(m[j], fmaxf(k[0], k[1]));
             l[j] *= m_new == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m[j] - m_new);
             m[j] = m_new;
+            ref[j] = m_new == -INFINITY ? 0.f : m_new;
           }
           leave_weights(i, sum, scale);
           __syncthreads();  // (6)

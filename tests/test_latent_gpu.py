@@ -297,6 +297,22 @@ def test_large_scores_in_blocks_of_64_rows_do_not_overflow(gpu, monkeypatch):
     test_large_scores_do_not_overflow(gpu)
 
 
+@pytest.mark.parametrize("width", [0, 2048])
+@pytest.mark.parametrize("fp8", [False, True], ids=["bf16", "fp8"])
+def test_scales_below_zero_and_of_zero(gpu, monkeypatch, fp8, width):
+    monkeypatch.setattr(sys.modules[__name__], "MIN_WIDTH", width)
+    b = Batch(gpu, [1, 5], [300, 97], 24, fp8=fp8, seed=17)
+    b.check(*L.latent_attention(-b.q_latent, -b.q_pe, b.cache, b.table, b.lens, b.cu_q, -SCALE))
+    # scale 0: the mean of the rows that are seen, each weight 1 exactly
+    o, lse = L.latent_attention(b.q_latent, b.q_pe, b.cache, b.table, b.lens, b.cu_q, 0.0)
+    for t, i, seen in [(0, 0, 300)] + [(1 + k, 1, 93 + k) for k in range(5)]:
+        rows = b.rows(i)[0][:seen]
+        mean, mass = rows.mean(0), rows.abs().mean(0)
+        # (e4m3: a weight is its row's scale, rounded to bf16)
+        _within(o[t], mean.expand(24, 512), (U * mean.abs() + ((U if fp8 else 0) + 2.0**-14) * mass).expand(24, 512), f"mean of token {t}")
+        _within(lse[:, t], torch.full((24,), math.log2(seen)), torch.full((24,), 2.0**-17), f"lse of token {t}")
+
+
 def test_tokens_behind_the_last_sequence_are_left_alone(gpu):
     b = Batch(gpu, [2, 1], [40, 300], 16, seed=10, extra_tokens=5)
     o = torch.full((8, 16, 512), 7.0, dtype=BF, device=gpu)
