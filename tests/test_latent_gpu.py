@@ -608,6 +608,36 @@ def test_two_streams_and_two_calls_at_once(gpu):
             assert all(torch.equal(x, y) for x, y in zip(pair, want[k]))
 
 
+def test_blocks_of_64_rows_over_runs_streams_and_replays(gpu, monkeypatch):
+    """The same bits from call to call, from two calls at once on two streams, and from a graph whose lengths change in place between its replays."""
+    monkeypatch.setattr(sys.modules[__name__], "MIN_WIDTH", 2048)
+    a, b = (Batch(gpu, [3] * 9, [2000 + 37 * i for i in range(9)], 16, seed=40 + s, fp8=bool(s), page=16) for s in (0, 1))
+    want = a.attention(), b.attention()
+    a.check(*want[0])
+    streams = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(4):
+        for k, (s, x) in enumerate(zip(streams, (a, b))):
+            with torch.cuda.stream(s):
+                got[k].append(x.attention())
+    torch.cuda.synchronize()
+    for k in range(2):
+        for pair in got[k]:
+            assert all(torch.equal(x, y) for x, y in zip(pair, want[k]))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = a.attention()
+    for step in (0, 1000, 1990, 3):
+        a.lens.copy_(torch.tensor(a.lengths, dtype=I32) - step)
+        for t in out:
+            t.fill_(math.nan)
+        graph.replay()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for x, y in zip(out, a.attention())), step
+
+
 @pytest.mark.parametrize("fp8", [False, True], ids=["bf16", "fp8"])
 def test_a_captured_step_follows_its_sequences(gpu, fp8):
     """One graph of a decoding step, replayed while lengths, slots, pages and tokens change in place (padded sequences among them), with eager work and
