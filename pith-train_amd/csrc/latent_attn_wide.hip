@@ -8,9 +8,10 @@
 // tiles, one request behind every four products. One barrier a tile. So a key fragment is read from LDS by two waves and a value fragment by one, either
 // kind of wave fills the other's latencies, and its registers are one operand's. (All eight waves doing both, 16 rows and 64 features each, waited for
 // one another and read each key fragment four times: 128 heads 81 us against 74, trees of up to 48 drafts 246 against 217.)
-// A scoring wave is busy for 1700 of a tile's 1850 cycles (half in products, half in softmax), an adding one for 1500. Trees of up to 48 drafts over 16 sequences of up
-// to 16384 rows, 16 heads (147 GF): 152 us and 10.5 for the join; 128 heads over 32 sequences of up to 8192 rows (46 GF, 201 MB): 62 and 9.6. Sixteen waves of half the
-// size were no faster (188 us against 190 at the time).
+// Trees of up to 48 drafts over 16 sequences of up to 16384 rows, 16 heads (147 GF): 150 us and 10.5 for the join; 128 heads over 32 sequences of up to 8192 rows
+// (46 GF, 201 MB): 62 and 9.6. A scoring wave is busy for 1700 of a tile's 1850 cycles (half in products, half in softmax), an adding one for 1500; but sixteen
+// waves of half the size, a higher priority for the scoring ones, and 4, 6 or 8 fragments read ahead all take the same time within 1 %, at a clock that falls to
+// 1.4 to 1.6 GHz: what is left is the card's power.
 // Weights are formed against a reference of each row that all waves know from earlier tiles; only a score beyond its slack (kSlack) makes them meet, two
 // barriers more, to move it.
 #include "latent_attn.h"
@@ -75,7 +76,7 @@ __global__ __launch_bounds__(kThreads, 2) void latent_attn_wide_kernel(LatentAtt
 #pragma unroll
       for (int j = 0; j < J; ++j) m[j] = -INFINITY, ref[j] = l[j] = 0.f;
       const auto tile_scores = [&](const char* kt, f32x4 (&y)[J]) __attribute__((always_inline)) {
-        constexpr int kLatentReads = FP8 ? kLatent / 64 : kLatent / 32, kReads = kLatentReads + 2, kAhead = 6;  // fragments read ahead of their products
+        constexpr int kLatentReads = FP8 ? kLatent / 64 : kLatent / 32, kReads = kLatentReads + 2, kAhead = 4;  // fragments read ahead of their products
         const uint32_t first = lds_address(kt) + key_at, pe_first = lds_address(kt) + pe_at;
         const auto read = [&](int n) __attribute__((always_inline)) {
           return n < kLatentReads ? *lds_at<u32x4>((first ^ (64 * (n & 3))) + 256 * (n >> 2)) : *lds_at<u32x4>(pe_first ^ (64 * (n - kLatentReads)));
