@@ -110,7 +110,7 @@ def _launch(name: str, args, like: torch.Tensor) -> None:
 def _aligned_rows(t: torch.Tensor) -> torch.Tensor:
     """t, or a copy whose rows the kernels can read 16 bytes at a time."""
     ok = t.data_ptr() % 16 == 0 and all(st % 8 == 0 for n, st in zip(t.shape[:-1], t.stride()[:-1]) if n > 1) and (t.shape[-1] == 1 or t.stride(-1) == 1)
-    return t if ok else t.contiguous()
+    return t if ok else t.clone(memory_format=torch.contiguous_format)  # (contiguous() would be t itself where only its beginning is off)
 
 
 def _strides(t: torch.Tensor) -> Tuple[int, int]:

@@ -2,6 +2,7 @@
 refuse, and their shape propagation."""
 
 import ctypes
+import math
 import os
 import re
 import subprocess
@@ -254,6 +255,17 @@ def test_a_cache_of_another_type_is_refused():
         L.LatentCache.empty(2, dtype=torch.float16, device="cpu")
     c = L.LatentCache.empty(2, 32, L.FP8, "cpu")
     assert c.latent.shape == (2, 32, 512) and c.scale.shape == (2, 32) and L.LatentCache.empty(2, device="cpu").scale is None
+
+
+@pytest.mark.parametrize("dtype", [BF, torch.float32])
+@pytest.mark.parametrize("shape", [(512,), (3, 576), (3, 2, 192)])
+@pytest.mark.parametrize("offset", [0, 1, 4])
+def test_rows_that_begin_off_the_alignment_are_copied(offset, shape, dtype):
+    """Also where they lie one behind the other already, as slices of a flat buffer do."""
+    x = torch.arange(offset + math.prod(shape)).to(dtype)[offset:].view(shape)
+    got = L._aligned_rows(x)
+    assert got.data_ptr() % 16 == 0 and got.is_contiguous() and torch.equal(got, x)
+    assert (got.data_ptr() == x.data_ptr()) == (x.data_ptr() % 16 == 0)
 
 
 def test_decode_is_for_the_layers_head_dims():

@@ -389,6 +389,38 @@ def test_strided_queries_caches_and_tables(gpu, fp8):
         assert torch.equal(x, y)
 
 
+@pytest.mark.parametrize("offset", [1, 4])
+def test_contiguous_rows_off_their_alignment(gpu, offset):
+    """Every input that may begin anywhere, as a contiguous slice of a flat buffer that is 2 or 8 bytes off: the aligned call's bits."""
+
+    def off(t):
+        at = max(2 * offset // t.element_size(), 1)  # (fp32: 4 or 8 bytes)
+        x = torch.empty(t.numel() + 8, dtype=t.dtype, device=gpu)[at : at + t.numel()].view(t.shape)
+        x.copy_(t)
+        assert x.is_contiguous() and x.data_ptr() % 16 != 0
+        return x
+
+    g, w, kv_b, cos, sin = _layer(5, 50, gpu)
+    b = Batch(gpu, [1, 3], [150, 70], 5, seed=51)
+    idx = torch.arange(4, device=gpu)
+    attention = lambda f: L.latent_attention(f(b.q_latent), f(b.q_pe), b.cache, b.table, b.lens, b.cu_q, SCALE)  # noqa: E731
+    q, kv_a = torch.randn(4, 5, 192, generator=g).to(BF).to(gpu), torch.randn(4, 576, generator=g).to(BF).to(gpu)
+    query = lambda f: L.absorb_query(f(q), f(kv_b), f(cos), f(sin), idx)  # noqa: E731
+    value = lambda f: [L.absorb_value(f(b.q_latent), f(kv_b))]  # noqa: E731
+
+    def append(weight):
+        def call(f):
+            cache = L.LatentCache(*(torch.zeros(1, 16, n, dtype=BF, device=gpu) for n in (512, 64)))
+            L.latent_cache_append(f(kv_a), f(weight), f(cos), f(sin), idx, idx, cache)
+            return cache[:2]
+
+        return call
+
+    for call in (attention, query, value, append(w), append(w.float())):
+        for x, y in zip(call(off), call(lambda t: t)):
+            assert torch.equal(x, y)
+
+
 def test_rows_beyond_32_bit_offsets(gpu):
     """A cache of 5 GB whose sequences lie in its last pages."""
     b = Batch(gpu, [1, 1], [100, 300], 16, seed=13)
