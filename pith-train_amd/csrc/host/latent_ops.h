@@ -180,14 +180,31 @@ struct ServingOp<BODY> {
   static R call(c10::DispatchKeySet keys, Args... args) {
     static const auto op = op_handle<R(Args...)>(NAME);
     TORCH_CHECK(!at::GradMode::is_enabled() || !(records(args) || ...), NAME, " has no backward: call it under torch.no_grad(), or detach what requires a gradient");
-    at::AutoDispatchBelowADInplaceOrView guard;
-    return op.redispatch(keys & c10::after_ADInplaceOrView_keyset, args...);
+    at::AutoDispatchBelowAutograd guard;
+    return op.redispatch(keys & c10::after_autograd_keyset, args...);
   }
 };
 
 constexpr char kLatentAppend[] = "pithtrain_amd::latent_append", kLatentGather[] = "pithtrain_amd::latent_gather",
                kLatentAbsorbQuery[] = "pithtrain_amd::latent_absorb_query", kLatentAbsorbValue[] = "pithtrain_amd::latent_absorb_value",
                kLatentAttention[] = "pithtrain_amd::latent_attention";
+
+// Below autograd, also where no gradient is recorded: the tensors that append writes count as changed, so that a backward which saved one of them (or a view)
+// notices. Those made in inference mode have no such count and are never saved.
+void latent_append_counted(c10::DispatchKeySet keys, const Tensor& kv_a, const Tensor& weight, const Tensor& cos, const Tensor& sin, const Tensor& pos,
+                           const Tensor& slots, const Tensor& latent, const Tensor& k_pe, const OptTensor& scale, double eps) {
+  static const auto op = op_handle<decltype(latent_append)>(kLatentAppend);
+  {
+    at::AutoDispatchBelowADInplaceOrView guard;
+    op.redispatch(keys & c10::after_ADInplaceOrView_keyset, kv_a, weight, cos, sin, pos, slots, latent, k_pe, scale, eps);
+  }
+  const auto changed = [](const Tensor& t) {
+    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+  };
+  changed(latent);
+  changed(k_pe);
+  if (scale) changed(*scale);
+}
 
 }  // namespace
 
@@ -212,6 +229,8 @@ TORCH_LIBRARY_FRAGMENT(pithtrain_amd, m) {
 PITH_LATENT_IMPL(CUDA)
 PITH_LATENT_IMPL(CPU)
 #undef PITH_LATENT_IMPL
+
+TORCH_LIBRARY_IMPL(pithtrain_amd, ADInplaceOrView, m) { m.impl("latent_append", &latent_append_counted); }
 
 TORCH_LIBRARY_IMPL(pithtrain_amd, Autograd, m) {
   m.impl("latent_append", &ServingOp<&latent_append>::call<kLatentAppend>);

@@ -168,6 +168,7 @@ def latent_cache_gather_into(cache: LatentCache, page_table: torch.Tensor, cu_ro
                                latent_rs=latent_out.stride(0) if rows > 1 else LATENT, k_pe_rs=k_pe_out.stride(0) if rows > 1 else ROPE)  # fmt: skip
     args.page_table, args.table_rs, args.table_width = _table_args(page_table, b)
     _launch("pith_latent_gather", args, latent_out)
+    torch.autograd.graph.increment_version((latent_out, k_pe_out))
 
 
 def _gather_body(latent, k_pe, scale, page_table, cu_rows, rows):
@@ -265,6 +266,7 @@ def latent_attention_into(
         workspace = torch.empty(need, dtype=torch.uint8, device=q_latent.device)
         args.workspace, args.workspace_bytes = workspace.data_ptr(), need
         _C.check(_C.lib().pith_latent_attn(_C.byref(args), _C.current_stream(q_latent)))
+    torch.autograd.graph.increment_version((o, lse))  # (a backward that saved one of them notices)
 
 
 def _attention_body(q_latent, q_pe, latent, k_pe, scale, page_table, lengths, cu_q, softmax_scale, tree_mask):

@@ -250,6 +250,29 @@ def test_arguments_that_require_a_gradient_are_refused():
         L.absorb_value(x, w)
 
 
+@pytest.mark.parametrize("mode", [torch.no_grad, torch.enable_grad, torch.inference_mode])
+@pytest.mark.parametrize("dtype", [BF, L.FP8])
+def test_appending_counts_as_a_change_of_the_cache(dtype, mode):
+    """A backward that saved a tensor of the cache (or a view that shares it) must not take its new rows for the old ones."""
+    layers = L.LatentCache.empty(8, 16, dtype, "meta")
+    cache = L.LatentCache(*(None if t is None else t[::2] for t in layers))
+    gradient = torch.ones(4, 16, 64, dtype=BF, device="meta", requires_grad=True)
+    y = gradient * cache.k_pe
+    before = [t._version for t in layers if t is not None]
+    with mode():
+        L.latent_cache_append(*(t.to("meta") for t in (_zeros(3, 576), _zeros(512), _zeros(8, 64), _zeros(8, 64), _zeros(3, d=torch.int64), _zeros(3, d=torch.int64))), cache)
+    assert all(t._version > v for t, v in zip([t for t in layers if t is not None], before))
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+
+
+def test_a_cache_made_in_inference_mode_can_be_written_outside_it():
+    with torch.inference_mode():
+        cache = L.LatentCache.empty(4, 16, device="meta")
+    with torch.no_grad():
+        L.latent_cache_append(*(t.to("meta") for t in (_zeros(3, 576), _zeros(512), _zeros(8, 64), _zeros(8, 64), _zeros(3, d=torch.int64), _zeros(3, d=torch.int64))), cache)
+
+
 def test_a_cache_of_another_type_is_refused():
     with pytest.raises(AssertionError, match="bfloat16 or float8_e4m3fn"):
         L.LatentCache.empty(2, dtype=torch.float16, device="cpu")

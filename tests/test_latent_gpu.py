@@ -723,6 +723,29 @@ def test_a_captured_step_follows_its_sequences(gpu, fp8):
         assert all((out[i] == 0).all() for i, n in enumerate(lengths) if n == 0)
 
 
+def test_what_is_written_counts_as_changed(gpu):
+    """A backward that saved a tensor which one of the operators has written since is refused, in place of computing with the new contents."""
+    b = Batch(gpu, [1, 2], [150, 40], 16, seed=34)
+    o, lse = torch.zeros(3, 16, 512, dtype=BF, device=gpu), torch.zeros(16, 3, device=gpu)
+    rows, pe = torch.zeros(190, 512, dtype=BF, device=gpu), torch.zeros(190, 64, dtype=BF, device=gpu)
+    cos, sin = _tables(8, gpu)
+    kv_a, ones, idx = torch.zeros(3, 576, dtype=BF, device=gpu), torch.ones(512, device=gpu), torch.arange(3, device=gpu)
+    cu = torch.tensor([0, 150, 190], dtype=I32, device=gpu)
+    calls = [
+        (b.cache[:2], lambda: L.latent_cache_append(kv_a, ones, cos, sin, idx, idx, b.cache)),
+        ((rows, pe), lambda: L.latent_cache_gather_into(b.cache, b.table, cu, rows, pe)),
+        ((o, lse), lambda: L.latent_attention_into(b.q_latent, b.q_pe, b.cache, b.table, b.lens, b.cu_q, SCALE, None, o, lse)),
+    ]
+    for written, call in calls:
+        for t in written:
+            x = torch.ones_like(t, requires_grad=True)
+            y = x * t
+            with torch.no_grad():
+                call()
+            with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+                y.sum().backward()
+
+
 def test_compiled_operators_match_eager(gpu):
     b = Batch(gpu, [1, 2], [150, 40], 16, seed=34)
     f = torch.compile(lambda q, p, c, k: L.latent_attention(q, p, L.LatentCache(c, k), b.table, b.lens, b.cu_q, SCALE), backend="aot_eager", fullgraph=True)
