@@ -167,11 +167,16 @@ Two latent_attention(const Tensor& q_latent, const Tensor& q_pe, const Tensor& l
   return python_body<Two>("latent_attention", q_latent, q_pe, latent, k_pe, scale, table, lengths, cu_q, softmax_scale, tree);
 }
 
-// No gradients: a call that would have to record one is refused rather than cut off from the graph.
+// No gradients: a call that would have to record one, or to carry a forward-mode tangent on, is refused rather than cut off from the graph. (While
+// forward mode is off, as in inference mode, there are no tangents.)
 bool records(const Tensor& t) { return t.requires_grad(); }
 bool records(const OptTensor& t) { return t.has_value() && t->requires_grad(); }
 bool records(double) { return false; }
 bool records(int64_t) { return false; }
+bool tangent(const Tensor& t) { return t._fw_grad(0).defined(); }
+bool tangent(const OptTensor& t) { return t.has_value() && tangent(*t); }
+bool tangent(double) { return false; }
+bool tangent(int64_t) { return false; }
 template <auto BODY>
 struct ServingOp;
 template <typename R, typename... Args, R (*BODY)(Args...)>
@@ -180,6 +185,7 @@ struct ServingOp<BODY> {
   static R call(c10::DispatchKeySet keys, Args... args) {
     static const auto op = op_handle<R(Args...)>(NAME);
     TORCH_CHECK(!at::GradMode::is_enabled() || !(records(args) || ...), NAME, " has no backward: call it under torch.no_grad(), or detach what requires a gradient");
+    TORCH_CHECK(!(tangent(args) || ...), NAME, " has no forward-mode derivative");
     at::AutoDispatchBelowAutograd guard;
     return op.redispatch(keys & c10::after_autograd_keyset, args...);
   }

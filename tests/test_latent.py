@@ -250,6 +250,29 @@ def test_arguments_that_require_a_gradient_are_refused():
         L.absorb_value(x, w)
 
 
+@pytest.mark.parametrize("name", _calls("cpu"))
+def test_tangents_are_refused(name):
+    """Forward-mode derivatives would be left out of the result in silence."""
+    forward_ad = torch.autograd.forward_ad
+    with forward_ad.dual_level():
+        dual = lambda *s, d=BF: forward_ad.make_dual(_zeros(*s, d=d, dev="meta"), _zeros(*s, d=d, dev="meta"))  # noqa: E731
+        z = lambda *s, d=BF: _zeros(*s, d=d, dev="meta")  # noqa: E731
+        i32, i64 = torch.int32, torch.int64
+        cache = L.LatentCache(z(4, 16, 512), dual(4, 16, 64))
+        call = {
+            "append": lambda: L.latent_cache_append(dual(3, 576), z(512), z(8, 64), z(8, 64), z(3, d=i64), z(3, d=i64), L.LatentCache(z(4, 16, 512), z(4, 16, 64))),
+            "gather": lambda: L.latent_cache_gather(cache, z(2, 2, d=i32), z(3, d=i32), 5),
+            "query": lambda: L.absorb_query(z(3, 2, 192), dual(512, 512), z(8, 64), z(8, 64), z(3, d=i64)),
+            "value": lambda: L.absorb_value(dual(3, 2, 512), z(512, 512)),
+            "attention": lambda: L.latent_attention(z(3, 2, 512), z(3, 2, 64), cache, z(2, 2, d=i32), z(2, d=i32), z(3, d=i32), 0.1),
+        }[name]
+        for mode in (torch.no_grad, torch.enable_grad):
+            with mode(), pytest.raises(RuntimeError, match="has no forward-mode derivative"):
+                call()
+        with torch.inference_mode():  # (no tangents there)
+            call()
+
+
 @pytest.mark.parametrize("mode", [torch.no_grad, torch.enable_grad, torch.inference_mode])
 @pytest.mark.parametrize("dtype", [BF, L.FP8])
 def test_appending_counts_as_a_change_of_the_cache(dtype, mode):
