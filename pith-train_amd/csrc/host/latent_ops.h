@@ -167,16 +167,11 @@ Two latent_attention(const Tensor& q_latent, const Tensor& q_pe, const Tensor& l
   return python_body<Two>("latent_attention", q_latent, q_pe, latent, k_pe, scale, table, lengths, cu_q, softmax_scale, tree);
 }
 
-// No gradients: a call that would have to record one, or to carry a forward-mode tangent on, is refused rather than cut off from the graph. (While
-// forward mode is off, as in inference mode, there are no tangents.)
+// No gradients: a call that would have to record one, or to carry a forward-mode tangent on, is refused rather than cut off from the graph.
 bool records(const Tensor& t) { return t.requires_grad(); }
 bool records(const OptTensor& t) { return t.has_value() && t->requires_grad(); }
 bool records(double) { return false; }
 bool records(int64_t) { return false; }
-bool tangent(const Tensor& t) { return t._fw_grad(0).defined(); }
-bool tangent(const OptTensor& t) { return t.has_value() && tangent(*t); }
-bool tangent(double) { return false; }
-bool tangent(int64_t) { return false; }
 template <auto BODY>
 struct ServingOp;
 template <typename R, typename... Args, R (*BODY)(Args...)>

@@ -824,7 +824,17 @@ Three mla_assemble_bwd(const Tensor& dqo, const Tensor& dko, const Tensor& dvo, 
 template <typename Sig>
 auto op_handle(const char* name) { return c10::Dispatcher::singleton().findSchemaOrThrow(name, "").typed<Sig>(); }
 
+// No operator has a forward-mode derivative: a tangent is refused, not left out. (While forward mode is off, as in inference mode, there are none.)
+bool tangent(const Tensor& t) { return t.defined() && t._fw_grad(0).defined(); }
+bool tangent(const OptTensor& t) { return t.has_value() && tangent(*t); }
+bool tangent(double) { return false; }
+bool tangent(int64_t) { return false; }
+bool tangent(bool) { return false; }
+template <typename T>
+void no_tangent(const T& x) { TORCH_CHECK(!tangent(x), "pithtrain_amd operators have no forward-mode derivative"); }
+
 bool any_requires_grad(std::initializer_list<const Tensor*> ts) {
+  for (const Tensor* t : ts) no_tangent(*t);
   if (!at::GradMode::is_enabled()) return false;
   for (const Tensor* t : ts)
     if (t->defined() && t->requires_grad()) return true;
@@ -1062,6 +1072,7 @@ struct BackwardOp<BODY> {
     static const auto op = op_handle<std::tuple<Tensors...>(Args...)>(NAME);
     bool recorded = false;
     variable_list inputs;
+    (no_tangent(args), ...);
     if (at::GradMode::is_enabled()) {
       (collect(inputs, args), ...);
       for (const Tensor& t : inputs) recorded |= t.requires_grad();
