@@ -24,6 +24,7 @@ import os
 from typing import NamedTuple, Optional, Tuple
 
 import torch
+from torch.autograd import forward_ad
 
 from pithtrain_amd import _C
 from pithtrain_amd._ext import define_op
@@ -98,6 +99,16 @@ def _check_positions(position_ids: torch.Tensor, positions: int) -> None:
         assert 0 <= lo and hi < positions, f"position_ids span [{lo}, {hi}], the rotary tables hold {positions} positions"
 
 
+def _no_gradients(what: str, *tensors: Optional[torch.Tensor]) -> None:
+    """The ops' refusal, for calls that write into tensors of the caller's and so go past them."""
+    recorded = torch.is_grad_enabled()
+    for t in tensors:
+        if t is not None and recorded and t.requires_grad:
+            raise RuntimeError(f"{what} has no backward: call it under torch.no_grad(), or detach what requires a gradient")
+        if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+            raise RuntimeError(f"{what} has no forward-mode derivative")
+
+
 def _launch(name: str, args, like: torch.Tensor) -> None:
     with torch.cuda.device(like.device):
         _C.check(getattr(_C.lib(), name)(_C.byref(args), _C.current_stream(like)))
@@ -156,6 +167,7 @@ def _table_args(page_table: torch.Tensor, b: int) -> Tuple[int, int, int]:
 def latent_cache_gather_into(cache: LatentCache, page_table: torch.Tensor, cu_rows: torch.Tensor, latent_out: torch.Tensor, k_pe_out: torch.Tensor) -> None:
     """latent_cache_gather into tensors of the caller's, [rows, 512] and [rows, 64] bf16 with rows of their own stride; those from cu_rows[b] on keep
     what they hold."""
+    _no_gradients("latent_cache_gather_into", *cache, latent_out, k_pe_out)
     _C.require_device(latent_out, k_pe_out, page_table, cu_rows)
     rows = latent_out.shape[0]
     for name, t, d in (("latent_out", latent_out, LATENT), ("k_pe_out", k_pe_out, ROPE)):
@@ -236,6 +248,7 @@ def latent_attention_into(
     softmax_scale: float, tree_mask: Optional[torch.Tensor], o: torch.Tensor, lse: torch.Tensor,
 ) -> None:  # fmt: skip
     """latent_attention into tensors of the caller's: o [T, h, 512] bf16 and lse [h, T] fp32. Tokens from cu_q[b] on keep what they hold."""
+    _no_gradients("latent_attention_into", q_latent, q_pe, *cache, o, lse)
     _C.require_device(q_latent, q_pe, page_table, lengths, cu_q, o, lse)
     assert q_latent.dtype == torch.bfloat16 and q_latent.dim() == 3 and q_latent.shape[2] == LATENT, f"q_latent must be a bfloat16 [tokens, heads, {LATENT}] tensor, got {q_latent.dtype} {list(q_latent.shape)}"
     t, h, _ = q_latent.shape

@@ -250,6 +250,36 @@ def test_arguments_that_require_a_gradient_are_refused():
         L.absorb_value(x, w)
 
 
+def _into_calls():
+    """Calls into tensors of the caller's, with every tensor that could record a gradient."""
+    z, i32 = _zeros, torch.int32
+    gather = [z(4, 16, 512), z(4, 16, 64), z(5, 512), z(5, 64)]
+    gather8 = [z(4, 16, 512, d=L.FP8), z(4, 16, 64), z(4, 16, d=torch.float32), z(5, 512), z(5, 64)]
+    attention = [z(3, 2, 512), z(3, 2, 64), z(4, 16, 512), z(4, 16, 64), z(3, 2, 512), z(2, 3, d=torch.float32)]
+    return {
+        "gather": (gather, lambda c, p, o, op: L.latent_cache_gather_into(L.LatentCache(c, p), z(2, 2, d=i32), z(3, d=i32), o, op)),
+        "gather_e4m3": (gather8, lambda c, p, s, o, op: L.latent_cache_gather_into(L.LatentCache(c, p, s), z(2, 2, d=i32), z(3, d=i32), o, op)),
+        "attention": (attention, lambda q, qp, c, p, o, lse: L.latent_attention_into(q, qp, L.LatentCache(c, p), z(2, 2, d=i32), z(2, d=i32), z(3, d=i32), 0.1, None, o, lse)),
+    }
+
+
+@pytest.mark.parametrize("name", _into_calls())
+def test_calls_into_given_tensors_refuse_gradients(name):
+    tensors, call = _into_calls()[name]
+    for i, t in enumerate(tensors):
+        if t.dtype == L.FP8:
+            continue
+        one = [x.clone().requires_grad_() if k == i else x for k, x in enumerate(tensors)]
+        with pytest.raises(RuntimeError, match="has no backward"):
+            call(*one)
+        for mode in (torch.no_grad, torch.inference_mode):
+            with mode(), pytest.raises(RuntimeError, match="need tensors on a GPU"):
+                call(*one)
+        with torch.autograd.forward_ad.dual_level(), torch.no_grad(), pytest.raises(RuntimeError, match="has no forward-mode derivative"):
+            one[i] = torch.autograd.forward_ad.make_dual(t, t)
+            call(*one)
+
+
 @pytest.mark.parametrize("name", _calls("cpu"))
 def test_tangents_are_refused(name):
     """Forward-mode derivatives would be left out of the result in silence."""
