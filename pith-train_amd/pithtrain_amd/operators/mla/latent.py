@@ -367,9 +367,11 @@ def latent_decode(
     softmax_scale: float, eps: float = 1e-6, tree_mask: Optional[torch.Tensor] = None,
 ) -> torch.Tensor:  # fmt: skip
     """The layer between its projections for new tokens, o [T, h, 128]: their rows go into the cache, then q [T, h, 192] attends to the cached rows
-    of its sequences (lengths count the new rows). Five launches, or six for very many rows; arguments as in the functions above."""
+    of its sequences (lengths count the new rows). Five launches, or six for very many rows; arguments as in the functions above. Rows of o from
+    cu_q[b] on hold nothing. What is refused for q, kv_a, a weight, the tables, the cache or a gradient has written nothing; page_table, lengths, cu_q and
+    tree_mask are looked at when the new rows are in the cache (the same call with the right ones writes them again)."""
+    q_latent, q_pe = absorb_query(q, kv_b_weight, cos, sin, position_ids)  # first: what it refuses must leave the cache as it was
     latent_cache_append(kv_a, norm_weight, cos, sin, position_ids, slots, cache, eps)
-    q_latent, q_pe = absorb_query(q, kv_b_weight, cos, sin, position_ids)
     o_latent, _ = latent_attention(q_latent, q_pe, cache, page_table, lengths, cu_q, softmax_scale, tree_mask)
     return absorb_value(o_latent, kv_b_weight)
 

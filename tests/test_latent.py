@@ -319,6 +319,27 @@ def test_appending_counts_as_a_change_of_the_cache(dtype, mode):
         y.sum().backward()
 
 
+@pytest.mark.parametrize("name", ["q", "kv_a", "norm_weight", "kv_b_weight", "cos", "latent", "k_pe"])
+def test_a_decoding_step_that_is_refused_for_a_gradient_writes_nothing(name):
+    z, i32, i64 = (lambda *s, d=BF: _zeros(*s, d=d, dev="meta")), torch.int32, torch.int64
+    t = dict(q=z(2, 2, 192), kv_a=z(2, 576), norm_weight=z(512), kv_b_weight=z(512, 512), cos=z(8, 64), sin=z(8, 64), position_ids=z(2, d=i64), slots=z(2, d=i64),
+             latent=z(4, 16, 512), k_pe=z(4, 16, 64), page_table=z(2, 2, d=i32), lengths=z(2, d=i32), cu_q=z(3, d=i32))  # fmt: skip
+
+    def call():
+        cache = L.LatentCache(t["latent"], t["k_pe"])
+        args = [t[n] for n in ("q", "kv_a", "norm_weight", "kv_b_weight", "cos", "sin", "position_ids", "slots")]
+        return MLA(2, 192, 128).decode(*args, cache, *(t[n] for n in ("page_table", "lengths", "cu_q")))
+
+    assert call().shape == (2, 2, 128) and t["latent"]._version > 0  # (the count says who wrote)
+    t[name].requires_grad_()
+    before = t["latent"]._version, t["k_pe"]._version
+    with pytest.raises(RuntimeError, match="has no backward"):
+        call()
+    assert (t["latent"]._version, t["k_pe"]._version) == before
+    with torch.no_grad():
+        call()
+
+
 def test_a_cache_made_in_inference_mode_can_be_written_outside_it():
     with torch.inference_mode():
         cache = L.LatentCache.empty(4, 16, device="meta")
