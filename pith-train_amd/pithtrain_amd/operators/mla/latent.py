@@ -88,13 +88,13 @@ def _tables(cos: torch.Tensor, sin: torch.Tensor) -> int:
     return cos.shape[0]
 
 
-def _checking() -> bool:
+def _checking(index: torch.Tensor) -> bool:
     """Whether index tensors are looked at on the host, at the price of a device synchronisation (never while a graph is captured)."""
-    return os.environ.get("PITHTRAIN_AMD_CHECK_POSITIONS") == "1" and not torch.cuda.is_current_stream_capturing()
+    return os.environ.get("PITHTRAIN_AMD_CHECK_POSITIONS") == "1" and not (index.is_cuda and torch.cuda.is_current_stream_capturing())
 
 
 def _check_positions(position_ids: torch.Tensor, positions: int) -> None:
-    if _checking() and position_ids.numel():
+    if _checking(position_ids) and position_ids.numel():
         lo, hi = int(position_ids.min()), int(position_ids.max())
         assert 0 <= lo and hi < positions, f"position_ids span [{lo}, {hi}], the rotary tables hold {positions} positions"
 
@@ -144,7 +144,7 @@ def _append_body(kv_a, weight, cos, sin, position_ids, slots, latent, k_pe, scal
         position_ids=_index(position_ids, torch.int64, (t,), "position_ids"), slots=_index(slots, torch.int64, (t,), "slots"),
         T=t, P=positions, kv_a_rs=kv_a.stride(0) if t > 1 else LATENT + ROPE, eps=float(eps), weight_dtype=_C.dtype_code(weight), cache=cache,
     )  # fmt: skip
-    if _checking() and t:
+    if _checking(slots) and t:
         _check_positions(position_ids, positions)
         used = slots[slots >= 0]
         rows = latent.shape[0] * latent.shape[1]
@@ -272,7 +272,7 @@ def latent_attention_into(
     if tree_mask is not None:
         _C.require_device(q_latent, tree_mask)
         args.tree_mask = _index(tree_mask, torch.int64, (t,), "tree_mask")
-        if _checking() and b:
+        if _checking(cu_q) and b:
             assert int((cu_q[1:] - cu_q[:-1]).max()) <= MAX_DRAFTS, f"a tree has more than {MAX_DRAFTS} tokens"
     with torch.cuda.device(q_latent.device):
         need = _C.lib().pith_latent_attn_workspace_bytes(_C.byref(args))
@@ -349,15 +349,18 @@ def latent_attention(
 
 def tree_mask_of(parents: torch.Tensor) -> torch.Tensor:
     """Words for latent_attention from parents [..., n] (n at most 64): draft j of a tree hangs on draft parents[j] of the same tree, or on the
-    sequence itself where that is negative, and sees its ancestors and itself. Every parent comes before its children. int64 [..., n]."""
+    sequence itself where that is negative (or n or more: no draft of this tree), and sees its ancestors and itself. Every parent comes
+    before its children. int64 [..., n]. PITHTRAIN_AMD_CHECK_POSITIONS=1 raises for parents beyond the tree, at the price of a device synchronisation."""
     n = parents.shape[-1]
     assert n <= MAX_DRAFTS, f"a tree has at most {MAX_DRAFTS} tokens, got {n}"
+    if _checking(parents) and parents.numel():
+        assert int(parents.max()) < n, f"a parent is draft {int(parents.max())}, the tree has {n} drafts"
     own = torch.ones((), dtype=torch.int64, device=parents.device) << torch.arange(n, device=parents.device)
     words = own.expand(parents.shape).clone()
-    at = parents.long()
+    at = parents = torch.where(parents < n, parents.long(), -1)
     for _ in range(n):  # one step up the tree for all drafts at once
         words |= torch.where(at >= 0, own[at.clamp(0, max(n - 1, 0))] if n else own, 0)
-        at = torch.where(at >= 0, parents.long().gather(-1, at.clamp(min=0)), at)
+        at = torch.where(at >= 0, parents.gather(-1, at.clamp(min=0)), at)
     return words
 
 

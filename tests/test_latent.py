@@ -83,6 +83,18 @@ def test_tree_words_from_parents():
         L.tree_mask_of(torch.arange(-1, 64))
 
 
+@pytest.mark.parametrize("far", [3, 64, 2**31, 2**62])
+def test_a_parent_that_is_no_draft_of_the_tree_is_none(far, monkeypatch):
+    """On a GPU an index behind the last draft would end the process, not raise."""
+    parents = torch.tensor([[-1, 0, 1], [far, 0, far], [-far, -1, far]])
+    monkeypatch.delenv("PITHTRAIN_AMD_CHECK_POSITIONS", raising=False)
+    assert L.tree_mask_of(parents).tolist() == [[1, 3, 7], [1, 3, 4], [1, 2, 4]]
+    monkeypatch.setenv("PITHTRAIN_AMD_CHECK_POSITIONS", "1")
+    with pytest.raises(AssertionError, match="the tree has 3 drafts"):
+        L.tree_mask_of(parents)
+    assert L.tree_mask_of(parents[:1]).tolist() == [[1, 3, 7]]
+
+
 # ---------------------------------------------------------------------------------------------
 # The C interface
 

@@ -197,6 +197,21 @@ def test_a_chain_of_drafts_is_the_causal_call(gpu):
         assert torch.equal(x, y)
 
 
+def test_words_of_trees_on_the_device(gpu, monkeypatch):
+    """The same words as on the host, also for parents that are no drafts of their tree."""
+    monkeypatch.delenv("PITHTRAIN_AMD_CHECK_POSITIONS", raising=False)
+    g = torch.Generator().manual_seed(18)
+    for n in (1, 3, 64):
+        parents = torch.stack([torch.tensor([int(torch.randint(-1, max(i, 1), (1,), generator=g)) if i else -1 for i in range(n)]) for _ in range(5)])
+        parents[2, ::3] = 2**40
+        parents[3, ::2] = n
+        words = L.tree_mask_of(parents)
+        assert torch.equal(L.tree_mask_of(parents.to(gpu)).cpu(), words)
+    monkeypatch.setenv("PITHTRAIN_AMD_CHECK_POSITIONS", "1")
+    with pytest.raises(AssertionError, match="the tree has 64 drafts"):
+        L.tree_mask_of(parents.to(gpu))
+
+
 @pytest.mark.parametrize("tree", [None, "tree"])
 @pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
 def test_a_row_that_a_token_does_not_see_cannot_reach_it(gpu, bad, tree):
