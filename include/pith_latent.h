@@ -29,7 +29,8 @@ enum { PITH_FP8_E4M3 = 2 }; /* beside PITH_BF16 and PITH_F32 */
 /* The cache: `pages` pages of page_size rows (a power of two from 16 to 65536; fewer than 2^31 rows in all). Row r of page p holds
  *   latent + p*latent_ps + r*512   bf16, or e4m3 with scale + p*scale_ps + r (fp32): the feature is value * scale of its row
  *   k_pe   + p*k_pe_ps   + r*64    bf16
- * Page strides in elements; pointers and page strides keep 16-byte alignment (scale: 4 bytes). Slot s is row s % page_size of page s / page_size. */
+ * Page strides in elements (not used where there is one page); pointers and page strides keep 16-byte alignment (scale: 4 bytes). Slot s is row
+ * s % page_size of page s / page_size. */
 typedef struct {
   void* latent;
   void* k_pe;

@@ -38,9 +38,10 @@ inline int check_cache(const pith_latent_cache& c, const char* who) {
     return fail(PITH_ERR_BAD_SHAPE, "%s: page size %lld is not a power of two from 16 to 65536", who, (long long)c.page_size);
   if (c.pages < 1 || c.pages > ((int64_t)1 << 31) / c.page_size - 1)
     return fail(PITH_ERR_BAD_SHAPE, "%s: %lld pages of %lld rows: at least one, and fewer than 2^31 rows", who, (long long)c.pages, (long long)c.page_size);
-  if (c.latent_ps < c.page_size * kLatent || c.k_pe_ps < c.page_size * kRope || (fp8 && c.scale_ps < c.page_size))
+  const bool strides = c.pages > 1;  // those of a single page are never used
+  if (strides && (c.latent_ps < c.page_size * kLatent || c.k_pe_ps < c.page_size * kRope || (fp8 && c.scale_ps < c.page_size)))
     return fail(PITH_ERR_BAD_SHAPE, "%s: a page stride is shorter than a page", who);
-  if (!aligned16(c.latent) || !aligned16(c.k_pe) || c.latent_ps % (fp8 ? 16 : 8) || c.k_pe_ps % 8 || (fp8 && (uintptr_t)c.scale % 4))
+  if (!aligned16(c.latent) || !aligned16(c.k_pe) || (strides && (c.latent_ps % (fp8 ? 16 : 8) || c.k_pe_ps % 8)) || (fp8 && (uintptr_t)c.scale % 4))
     return fail(PITH_ERR_MISALIGNED, "%s: the cache breaks the 16-byte alignment", who);
   return PITH_OK;
 }

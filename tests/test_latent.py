@@ -207,6 +207,16 @@ def test_empty_calls_launch_nothing(name):
         assert fn(ctypes.byref(make(**kw)), None) == _C.PITH_OK
 
 
+@pytest.mark.parametrize("fp8", [False, True])
+def test_the_stride_of_a_single_page_is_not_used(fp8):
+    """A tensor whose first dimension has one element may carry any stride there."""
+    odd = dict(pages=1, latent_ps=515, k_pe_ps=3, **(dict(FP8, scale_ps=1) if fp8 else {}))
+    for name, (make, _) in CALLS.items():
+        if make is not _absorb:
+            args = make(cache=_cache(**odd), **({"rows": 0} if make is _gather else {"T": 0}))
+            assert getattr(_C.lib(), name)(ctypes.byref(args), None) == _C.PITH_OK, _C.lib().pith_last_error()
+
+
 def test_workspace_grows_with_nothing_but_the_device_and_the_row_blocks():
     need = lambda **kw: _C.lib().pith_latent_attn_workspace_bytes(ctypes.byref(_attn(**kw)))  # noqa: E731
     assert need(T=0) == need(B=0) == 0 and need() > 0

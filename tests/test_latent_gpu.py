@@ -404,6 +404,22 @@ def test_strided_queries_caches_and_tables(gpu, fp8):
         assert torch.equal(x, y)
 
 
+@pytest.mark.parametrize("fp8", [False, True], ids=["bf16", "fp8"])
+def test_a_cache_of_a_single_page_with_a_stride_of_its_own(gpu, fp8):
+    g, w, _, cos, sin = _layer(1, 52, gpu)
+    kv_a, idx = torch.randn(40, 576, generator=g).to(BF).to(gpu), torch.arange(40, device=gpu)
+    table, cu = torch.zeros(1, 1, dtype=I32, device=gpu), torch.tensor([0, 40], dtype=I32, device=gpu)
+    q_latent, q_pe = torch.randn(1, 4, 512, generator=g).to(BF).to(gpu), torch.randn(1, 4, 64, generator=g).to(BF).to(gpu)
+    want = None
+    for single in (lambda t: t, lambda t: t.as_strided(t.shape, (t.stride(1), *t.stride()[1:]))):
+        cache = L.LatentCache(*(None if t is None else single(t) for t in L.LatentCache.empty(1, 64, L.FP8 if fp8 else BF, gpu)))
+        L.latent_cache_append(kv_a, w, cos, sin, idx, idx, cache)
+        got = (*L.latent_cache_gather(cache, table, cu, 40), *L.latent_attention(q_latent, q_pe, cache, table, cu[1:], cu[:2] // 40, SCALE))
+        want = want or got
+        assert all(torch.equal(x, y) for x, y in zip(got, want))
+    assert cache.latent.stride(0) == 512 and torch.isfinite(want[0].float()).all()
+
+
 @pytest.mark.parametrize("offset", [1, 4])
 def test_contiguous_rows_off_their_alignment(gpu, offset):
     """Every input that may begin anywhere, as a contiguous slice of a flat buffer that is 2 or 8 bytes off: the aligned call's bits."""
