@@ -6,6 +6,7 @@ import math
 import os
 import re
 import subprocess
+import sys
 
 import pytest
 import torch
@@ -129,6 +130,21 @@ def test_struct_layouts_match_the_header(tmp_path):
         assert int(got[cname]) == ctypes.sizeof(st) == STRUCT_SIZES[_C.PITH_LATENT_VERSION][cname], cname
         for f, _ in st._fields_:
             assert int(got[f"{cname}.{f}"]) == getattr(st, f).offset, f"{cname}.{f}"
+
+
+@pytest.mark.parametrize("symbol, version", [("pith_latent_version", 100), ("pith_latent_version", 99), ("pith_version", 1)])
+def test_the_native_path_is_loaded_with_its_own_version_only(tmp_path, symbol, version):
+    """A library of another version lays arguments out differently. One symbol of it is put in front of the built library's."""
+    src, shim = tmp_path / "shim.c", tmp_path / "shim.so"
+    src.write_text(f"int {symbol}(void) {{ return {version}; }}\n")
+    subprocess.run(["gcc", "-shared", "-fPIC", str(src), "-o", str(shim)], check=True)
+    code = f"import ctypes; ctypes.CDLL({str(shim)!r}, ctypes.RTLD_GLOBAL); from pithtrain_amd import _ext"
+    env = {**os.environ, "PYTHONPATH": os.path.join(ROOT, "pith-train_amd")}
+    run = subprocess.run([sys.executable, "-c", code], env=env, capture_output=True, text=True)
+    if version == _C.PITH_LATENT_VERSION:
+        assert run.returncode == 0, run.stderr
+    else:
+        assert run.returncode == 1 and "build both again" in run.stderr, run.stderr
 
 
 def _cache(**kw):
