@@ -134,6 +134,9 @@ typedef struct {
 } pith_latent_attn_args;
 
 int64_t pith_latent_attn_workspace_bytes(const pith_latent_attn_args* args);
+/* Query rows to a workgroup of the kernel that such a call takes, 16 or 64; 0 for a call that launches nothing or is rejected for its sizes. A row's
+ * keys are cut, and its sums ordered, by that and by the lengths of all sequences of the call. */
+int pith_latent_attn_rows(const pith_latent_attn_args* args);
 int pith_latent_attn(const pith_latent_attn_args* args, pith_stream_t stream);
 
 #ifdef __cplusplus

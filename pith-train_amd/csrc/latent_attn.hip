@@ -324,6 +324,11 @@ extern "C" int64_t pith_latent_attn_workspace_bytes(const pith_latent_attn_args*
   return plan_of(a).bytes;
 }
 
+extern "C" int pith_latent_attn_rows(const pith_latent_attn_args* a) {
+  if (check_attn(a, "pith_latent_attn_rows") != PITH_OK || a->T == 0 || a->B == 0) return 0;
+  return plan_of(a).rows;
+}
+
 extern "C" int pith_latent_attn(const pith_latent_attn_args* a, pith_stream_t stream) {
   const char* who = "pith_latent_attn";
   if (const int rc = check_attn(a, who)) return rc;

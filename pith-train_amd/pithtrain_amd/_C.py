@@ -212,6 +212,7 @@ LATENT_SYMBOLS = {
     "pith_latent_absorb_query": (c_int, [POINTER(LatentAbsorbArgs), c_void_p]),
     "pith_latent_absorb_value": (c_int, [POINTER(LatentAbsorbArgs), c_void_p]),
     "pith_latent_attn_workspace_bytes": (c_int64, [POINTER(LatentAttnArgs)]),
+    "pith_latent_attn_rows": (c_int, [POINTER(LatentAttnArgs)]),
     "pith_latent_attn": (c_int, [POINTER(LatentAttnArgs), c_void_p]),
 }
 

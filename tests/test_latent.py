@@ -241,6 +241,16 @@ def test_workspace_grows_with_nothing_but_the_device_and_the_row_blocks():
     assert need(H=0) == 0  # what pith_latent_attn rejects
 
 
+def test_rows_of_a_workgroup_go_by_the_rows_of_a_sequence_and_the_work_list():
+    rows = lambda **kw: _C.lib().pith_latent_attn_rows(ctypes.byref(_attn(**kw)))  # noqa: E731
+    wide = dict(table_width=4096, table_rs=4096)
+    assert rows(T=0) == rows(B=0) == rows(H=0) == 0  # nothing to launch, or what pith_latent_attn rejects
+    assert rows(T=2, H=16, lse_hs=2, **wide) == 16  # sixteen rows a sequence
+    assert rows(T=3, H=16, lse_hs=3, **wide) == 64
+    assert rows(T=2, H=17, lse_hs=2, **wide) == 64
+    assert rows(T=64, H=128, lse_hs=64) == 64 and rows(T=3, H=16, lse_hs=3) == 16  # and a work list of some length
+
+
 # ---------------------------------------------------------------------------------------------
 # The Python entry points
 

@@ -307,6 +307,86 @@ def test_blocks_of_64_rows_are_not_reached_by_rows_of_e4m3_that_they_do_not_see(
         test_a_single_draft_that_does_not_see_itself_is_not_reached_by_its_row(gpu, fp8, 40)
 
 
+# The tests below say which kernel they are about and hold that the call takes it.
+def _takes(b, rows):
+    c = _C.LatentCacheArgs(latent=256, k_pe=256, pages=b.latent.shape[0], page_size=b.page, latent_ps=b.page * 512, k_pe_ps=b.page * 64, dtype=_C.PITH_BF16)
+    args = _C.LatentAttnArgs(cache=c, T=b.q_latent.shape[0], B=len(b.counts), H=b.h, table_width=b.table.shape[1], table_rs=b.table.shape[1])
+    assert _C.lib().pith_latent_attn_rows(_C.byref(args)) == rows
+
+
+WIDTHS = {16: 0, 64: 2048}  # of page tables, by the rows of the kernel that they make calls of more than 16 rows a sequence take
+
+
+@pytest.mark.parametrize("fp8", [False, True], ids=["bf16", "fp8"])
+@pytest.mark.parametrize("name", LENGTH_SETS)
+@pytest.mark.parametrize("rows, h", [(64, 37), (64, 128), (16, 16)])
+def test_either_kernel_matches_the_oracle(gpu, monkeypatch, name, rows, h, fp8):
+    monkeypatch.setattr(sys.modules[__name__], "MIN_WIDTH", WIDTHS[rows])
+    counts, lengths = LENGTH_SETS[name]
+    b = Batch(gpu, counts, lengths, h, page=16 if name in ("tiny", "prompt") else 64, fp8=fp8, seed=len(name) + h)
+    _takes(b, rows)
+    b.check(*b.attention(), name)
+
+
+@pytest.mark.parametrize("fp8", [False, True], ids=["bf16", "fp8"])
+@pytest.mark.parametrize("rows", [16, 64])
+def test_token_offsets_that_go_back_in_either_kernel(gpu, monkeypatch, rows, fp8):
+    """They are taken as their maximum so far: no token belongs to two sequences. More sequences than a wavefront scans at once."""
+    monkeypatch.setattr(sys.modules[__name__], "MIN_WIDTH", WIDTHS[rows])
+    n, h = 70, {16: 16, 64: 150}[rows]
+    b = Batch(gpu, [3, 0] + [0] * (n - 3) + [5], [40] * n, h, seed=16, fp8=fp8)
+    _takes(b, rows)
+    want = b.attention()
+    b.check(*want)
+    b.cu_q[2:-1] = torch.tensor([0, 3, 1, -7], dtype=I32, device=gpu).repeat(n)[: n - 2]
+    for x, y in zip(b.attention(), want):
+        assert torch.equal(x, y)
+
+
+@pytest.mark.parametrize("fp8", [False, True], ids=["bf16", "fp8"])
+@pytest.mark.parametrize("rows", [16, 64])
+def test_nonsense_in_the_index_tensors_stays_in_memory_in_either_kernel(gpu, monkeypatch, rows, fp8):
+    """Pages, lengths and token offsets out of range: clamped, whatever comes of it."""
+    monkeypatch.setattr(sys.modules[__name__], "MIN_WIDTH", WIDTHS[rows])
+    b = Batch(gpu, [1, 2], [100, 130], {16: 8, 64: 40}[rows], seed=11, fp8=fp8)
+    _takes(b, rows)
+    if fp8:
+        b.latent.view(torch.uint8).fill_(0x38)  # 1.0
+        b.scale.fill_(1.0)
+    else:
+        b.latent.nan_to_num_(0.0)
+    b.k_pe.nan_to_num_(0.0)
+    table, lens, cu = b.table.clone(), b.lens.clone(), b.cu_q.clone()
+    b.table[:] = torch.tensor([-(2**31), -1, 2**31 - 1], dtype=I32, device=gpu)[torch.arange(b.table.shape[1], device=gpu) % 3]
+    assert torch.isfinite(b.attention()[0].float()).all()
+    for far in ([2**31 - 1, 2**31 - 1], [-5, -(2**31)]):
+        b.lens[:] = torch.tensor(far, dtype=I32, device=gpu)
+        o, lse = b.attention()
+        assert torch.isfinite(o.float()).all()
+    assert (o == 0).all() and (lse == -math.inf).all()
+    b.lens[:] = 50
+    for offsets in ([0, 2**31 - 1, 5], [-7, 3, 1], [3, 2, 1], [-(2**31), 2**31 - 1, -(2**31)]):
+        b.cu_q[:] = torch.tensor(offsets, dtype=I32, device=gpu)
+        b.attention()
+    torch.cuda.synchronize()
+    b.table.copy_(table), b.lens.copy_(lens), b.cu_q.copy_(cu)
+    b.check(*b.attention())
+
+
+@pytest.mark.parametrize("tree", ["tree", "holes"])
+@pytest.mark.parametrize("rows", [16, 64])
+def test_tokens_behind_the_last_sequence_in_either_kernel(gpu, monkeypatch, rows, tree):
+    """A padded batch: the rows of tokens that belong to no sequence are left as they were, the others as in a call without them."""
+    monkeypatch.setattr(sys.modules[__name__], "MIN_WIDTH", WIDTHS[rows])
+    h = {16: 4, 64: 40}[rows]
+    b = Batch(gpu, [2, 1], [40, 300], h, seed=10, extra_tokens=5, tree=tree)
+    _takes(b, rows)
+    o, lse = torch.full((8, h, 512), 7.0, dtype=BF, device=gpu), torch.full((h, 8), 7.0, device=gpu)
+    L.latent_attention_into(b.q_latent, b.q_pe, b.cache, b.table, b.lens, b.cu_q, SCALE, b.words, o, lse)
+    assert (o[3:] == 7).all() and (lse[:, 3:] == 7).all()
+    b.check(o[:3], lse[:, :3])
+
+
 def test_large_scores_in_blocks_of_64_rows_do_not_overflow(gpu, monkeypatch):
     monkeypatch.setattr(sys.modules[__name__], "MIN_WIDTH", 2048)
     test_large_scores_do_not_overflow(gpu)
