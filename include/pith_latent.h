@@ -66,8 +66,9 @@ int pith_latent_append(const pith_latent_append_args* args, pith_stream_t stream
 
 /* ------------------------------------------------------------------------------------------
  * Cached rows of B sequences, one behind the other, as bf16 (value * scale, rounded once): what the expanded form of a prompt behind a cached
- * prefix reads. Sequence b's rows 0 .. cu_rows[b+1]-cu_rows[b]-1 lie in the pages page_table[b, :] (int32, row stride table_rs, table_width
- * entries) and go to output rows cu_rows[b] ..; cu_rows [B+1] int32 ascending from 0. Output rows from cu_rows[B] up to `rows` are left alone. */
+ * prefix reads (kv_b_proj of them gives keys in two parts and values for pith_attn_fwd without a mask). Sequence b's rows 0 ..
+ * cu_rows[b+1]-cu_rows[b]-1 lie in the pages page_table[b, :] (int32, row stride table_rs, table_width entries) and go to output rows cu_rows[b] ..;
+ * cu_rows [B+1] int32 ascending from 0. Output rows from cu_rows[B] up to `rows` are left alone. */
 typedef struct {
   pith_latent_cache cache;
   const int32_t* page_table;

@@ -12,7 +12,7 @@ kv_b_proj.weight of a head,
     absorb_query          q -> (W_uk^T q_nope, rotated q_pe)
     latent_attention      causal attention of the newest tokens of every sequence to its cached rows, or of a tree of drafted tokens
     absorb_value          its result -> W_uv of it, the input of o_proj
-    latent_cache_gather   cached rows back as bf16, for the expanded form of a prompt behind a cached prefix
+    latent_cache_gather   cached rows back as bf16, for the expanded form of a prompt behind a cached prefix (see there)
     latent_decode         the first four in a row: what stands between the layer's projections (MLA.decode calls it)
 
  T : new tokens of all sequences, one behind the other, b : sequences, h : heads.
@@ -319,7 +319,11 @@ def latent_cache_append(
 def latent_cache_gather(cache: LatentCache, page_table: torch.Tensor, cu_rows: torch.Tensor, rows: int) -> Tuple[torch.Tensor, torch.Tensor]:
     """(latent [rows, 512], k_pe [rows, 64]) bf16: the first cu_rows[i + 1] - cu_rows[i] cached rows of every sequence i, one sequence behind the
     other. page_table [b, n] int32: the pages of each; cu_rows [b + 1] int32 ascending from 0, on the device; rows: how many to make room for, at
-    least cu_rows[b]. Rows from cu_rows[b] on are not written."""
+    least cu_rows[b]. Rows from cu_rows[b] on are not written.
+
+    With kv_b_proj the rows become keys in two parts and values, for the expanded form of a prompt behind a cached prefix: _mla_fwd(q, k_nope, v, scale,
+    causal=False, k_pe=k_pe) of the rotated queries over the prefix (k_pe is rotated already; mla_assemble_qkv would do it again), _mla_fwd(..., causal=True) of
+    the prompt over itself, and _online_softmax_combine_log2 of the two."""
     return _gather_op(cache.latent, cache.k_pe, cache.scale, page_table, cu_rows, rows)
 
 

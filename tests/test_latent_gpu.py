@@ -727,6 +727,58 @@ def test_prompt_then_steps_agree_with_the_expanded_layer(gpu, fp8):
         assert torch.equal(o, L.absorb_value(L.latent_attention(ql, qp, cache, table, lens, cu, layer.softmax_scale)[0], kv_b))
 
 
+@pytest.mark.parametrize("fp8", [False, True], ids=["bf16", "fp8"])
+@pytest.mark.parametrize("prefix,new", [(1, 1), (77, 130), (300, 33), (1000, 257)])
+def test_a_prompt_behind_a_cached_prefix_in_expanded_form(gpu, prefix, new, fp8):
+    """Gathered rows as keys in two parts (nothing is rotated again) and values, without a mask; the prompt against itself, causal; the two joined by
+    their LSE. Against the layer in 64 bits, from the rows that the cache holds.
+
+    Per element: keys, values, weights, the part and the rotated parts are rounded to bf16. With k = |q| . |W| |c| + |q_pe| . |p| the largest score of
+    absolute values of a row, in nats, a score is off by at most d = 3 u k (the query's rotation and the key's, which is rounded once here and once in the
+    cache) + 2^-13 k (sums of 512 and 192 fp32 products): 2 d of the mass, as weight and denominator; the value's and the weight's rounding u each, the part's u of |o|, of both parts."""
+    from pithtrain_amd.operators.mla.hip import _mla_fwd
+    from pithtrain_amd.operators.mla_assemble import mla_assemble_qkv
+    from pithtrain_amd.operators.ring_attention.mla import _online_softmax_combine_log2
+
+    h, page = 4, 16
+    g, w, kv_b, _, _ = _layer(h, 60 + new, gpu)
+    cos, sin = _tables(prefix + new, gpu)
+    total = prefix + new
+    cache = L.LatentCache.empty(-(-total // page) + 1, page, L.FP8 if fp8 else BF, gpu)
+    table = torch.randperm(cache.latent.shape[0], generator=g)[: -(-total // page)][None].to(I32).to(gpu)
+    pos = torch.arange(total, device=gpu)
+    kv_a = torch.randn(total, 576, generator=g).to(BF).to(gpu)
+    L.latent_cache_append(kv_a, w, cos, sin, pos, table[0, pos // page].long() * page + pos % page, cache)
+    q = (0.5 * torch.randn(1, new, h, 192, generator=g)).to(BF).to(gpu)
+
+    # as a program does it
+    offsets = torch.tensor([0, prefix], dtype=I32, device=gpu)
+    c, pe = L.latent_cache_gather(cache, table, offsets, prefix)
+    kv = (c @ kv_b.T).view(1, prefix, h, 256)
+    mine, mine_pe = L.latent_cache_gather(cache, table, torch.tensor([0, total], dtype=I32, device=gpu), total)
+    own_kv = (mine[prefix:] @ kv_b.T).view(1, new, h, 256)
+    q_rot, k_own, v_own = mla_assemble_qkv(q, own_kv, kv_a[None, prefix:, None, 512:], cos, sin, pos[None, prefix:])
+    before = _mla_fwd(q_rot, kv[..., :128].contiguous(), kv[..., 128:].contiguous(), SCALE, causal=False, k_pe=pe[None])
+    own = _mla_fwd(q_rot, k_own, v_own, SCALE, causal=True)
+    o, lse = _online_softmax_combine_log2(*before, *own)
+
+    rows, rot = (t.double().cpu() for t in (mine, mine_pe))
+    qc, wt = q[0].double().cpu(), kv_b.double().cpu().view(h, 256, 512)
+    qr = O.rotate(q[0, :, :, 128:].cpu(), cos.cpu(), sin.cpu(), pos[prefix:].cpu())
+    seen = O.sees(new, total)
+    for i in range(h):
+        keys, values = rows @ wt[i, :128].T, rows @ wt[i, 128:].T
+        keys_mass, values_mass = rows.abs() @ wt[i, :128].abs().T, rows.abs() @ wt[i, 128:].abs().T
+        s = ((qc[:, i, :128] @ keys.T + qr[:, i] @ rot.T) * SCALE).masked_fill(~seen, -math.inf)
+        weights = s.softmax(-1)
+        want, want_lse = weights @ values, torch.logsumexp(s, -1) / math.log(2)
+        k = ((qc[:, i, :128].abs() @ (keys.abs() + 2.0**-7 * keys_mass).T + qr[:, i].abs() @ rot.abs().T) * SCALE).masked_fill(~seen, 0).amax(-1)
+        d = (3 * U + 2.0**-13) * k
+        mass = weights @ (values.abs() + 2.0**-13 * values_mass)
+        _within(o[0, :, i], want, (3 * U + 2.0**-10 + 2 * d)[:, None] * mass, f"o of head {i}")
+        _within(lse[0, i], want_lse, d / math.log(2) + 2.0**-14, f"lse of head {i}")
+
+
 def test_results_do_not_depend_on_the_run(gpu):
     b = Batch(gpu, [1] * 9, [3000 + 37 * i for i in range(9)], 16, seed=30)
     first = b.attention()
