@@ -113,7 +113,8 @@ int pith_latent_absorb_value(const pith_latent_absorb_args* args, pith_stream_t 
  * cu_q count as their maximum so far, so that a token belongs to one sequence.
  * q_latent [T,H,512], q_pe [T,H,64], o [T,H,512] bf16 with token and head strides (multiples of 8); lse [H,T] fp32 (head stride lse_hs).
  * lengths [B], cu_q [B+1], page_table [B, table_width] int32; tree_mask [T] int64 or NULL. All of them are read by the kernels only: a call that
- * was captured into a graph can be replayed after their contents, and those of the cache, have changed. They must not change while it runs.
+ * was captured into a graph can be replayed after their contents, and those of the cache, have changed. They must not change while it runs, and o
+ * and lse must not overlap what it reads.
  * workspace: pith_latent_attn_workspace_bytes of the same arguments, 256-byte aligned, used by the call's kernels only. Calls that may overlap in
  * time need one each. */
 typedef struct {

@@ -8,8 +8,10 @@
 // workgroups, ranges can therefore be a little longer and each lie in one row block: every row block is taken for as many tiles as fill whole ranges, LEAST
 // tiles or more, the ranges as short as the workgroups allow. The row blocks of a sequence are then cut alike, and as an XCD's workgroups take ranges that
 // follow one another, they go through the same tiles at the same time, which its cache fetches about once. Blocks of 64 rows (several a sequence) gain by
-// that up to a quarter of their time, so ranges may be a quarter longer: a call for 128 heads took 80 us with ranges cut anywhere and takes 72, one for trees of
-// up to 48 drafts 192 and 166 (with all tiles in the caches, 67 and 146).
+// that up to a quarter of their time, so their ranges may be a quarter longer beside the START tiles: a call for 128 heads took 80 us with ranges cut anywhere and
+// takes 72, one for trees of up to 48 drafts 192 and 166 (with all tiles in the caches, 67 and 146).
+// So how a row's keys are cut follows from the lengths of all sequences of the call, and with that the references, and the order of its sums: the same row in
+// another batch may differ in its last bits. Nothing else of one row reaches another: its reference is its own, and so are its infinities and NaN.
 // A workgroup whose range covers a row block wholly writes its rows; parts of a row block leave (reference, sum, unnormalised result) in fp32 in the
 // workspace, and a second kernel joins them in the order of the keys (results do not depend on scheduling).
 #pragma once

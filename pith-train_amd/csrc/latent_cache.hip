@@ -1,8 +1,8 @@
 // The latent cache's rows: written as new tokens come (RMS norm of the latent part, rotation of the rotary part, quantisation), and read back.
 //
 // Both move memory and little else. A token is one wavefront's work: its 512 latent features are 16 bytes a lane, so a row goes in and out by
-// whole 1-KB instructions and its sums stay in registers. 8192 tokens into a bf16 cache 6.5 us (21 MB, 3.3 TB/s: two rounds of loads that wait for one another),
-// 32 tokens 3.6 us (an empty kernel 2.5); 75000 rows of 16 sequences out of an e4m3 cache 31.6 us (156 MB, 4.9 TB/s, the rate of a large copy), 1021 rows 4.6 us.
+// whole 1-KB instructions and its sums stay in registers. 8192 tokens into a bf16 cache 6.5 us (21 MB, 3.3 TB/s: four rounds of loads that wait for one another,
+// the slot, the row and the weights behind the branch on it, then, behind the latent row's store, the position and its row of the tables), 32 tokens 3.6 us (an empty kernel 2.5); 75000 rows of 16 sequences out of an e4m3 cache 31.6 us (156 MB, 4.9 TB/s, the rate of a large copy), 1021 rows 4.6 us.
 #include "latent_common.h"
 
 namespace pith {
@@ -35,7 +35,8 @@ struct AppendParams {
 
 // n = c * rsqrt(mean(c^2) + eps) * weight in fp32; bf16 rows are rounded once, e4m3 rows once behind the division by their scale (to nearest even;
 // the largest feature becomes +-448 exactly). The scale is the fp32 quotient, not a power of two: it costs nothing where it is applied (a factor of
-// the whole row, to the score and to the softmax weight) and keeps up to a bit of precision.
+// the whole row, to the score and to the softmax weight) and keeps up to a bit of precision. (The order of the sum of squares and rsqrtf leave the last bit
+// of a feature open in fp32, so one that lies next to the middle of two e4m3 values may go to either.)
 template <bool FP8, bool W_F32>
 __global__ __launch_bounds__(kThreads) void latent_append_kernel(AppendParams p) {
   const int lane = threadIdx.x & 63;

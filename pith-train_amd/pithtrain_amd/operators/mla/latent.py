@@ -37,7 +37,7 @@ FP8 = torch.float8_e4m3fn
 class LatentCache(NamedTuple):
     """Pages of cached rows. latent [pages, page_size, 512] bf16 or float8_e4m3fn, k_pe [pages, page_size, 64] bf16, scale [pages, page_size] fp32
     (e4m3 only: a feature is value * scale of its row). page_size is a power of two from 16 to 65536; rows of a page are contiguous, pages may be
-    further apart (the layers of a model can share one allocation). Slot s is row s % page_size of page s // page_size."""
+    further apart (the layers of a model can share one allocation); pages begin at multiples of 16 bytes. Slot s is row s % page_size of page s // page_size."""
 
     latent: torch.Tensor
     k_pe: torch.Tensor
@@ -165,8 +165,8 @@ def _table_args(page_table: torch.Tensor, b: int) -> Tuple[int, int, int]:
 
 
 def latent_cache_gather_into(cache: LatentCache, page_table: torch.Tensor, cu_rows: torch.Tensor, latent_out: torch.Tensor, k_pe_out: torch.Tensor) -> None:
-    """latent_cache_gather into tensors of the caller's, [rows, 512] and [rows, 64] bf16 with rows of their own stride; those from cu_rows[b] on keep
-    what they hold."""
+    """latent_cache_gather into tensors of the caller's, [rows, 512] and [rows, 64] bf16 with rows of their own stride that begin at multiples of 16
+    bytes; those from cu_rows[b] on keep what they hold."""
     _no_gradients("latent_cache_gather_into", *cache, latent_out, k_pe_out)
     _C.require_device(latent_out, k_pe_out, page_table, cu_rows)
     rows = latent_out.shape[0]
@@ -247,7 +247,8 @@ def latent_attention_into(
     q_latent: torch.Tensor, q_pe: torch.Tensor, cache: LatentCache, page_table: torch.Tensor, lengths: torch.Tensor, cu_q: torch.Tensor,
     softmax_scale: float, tree_mask: Optional[torch.Tensor], o: torch.Tensor, lse: torch.Tensor,
 ) -> None:  # fmt: skip
-    """latent_attention into tensors of the caller's: o [T, h, 512] bf16 and lse [h, T] fp32. Tokens from cu_q[b] on keep what they hold."""
+    """latent_attention into tensors of the caller's: o [T, h, 512] bf16, whose rows begin at multiples of 16 bytes, and lse [h, T] fp32; neither overlaps
+    what the call reads. Tokens from cu_q[b] on keep what they hold."""
     _no_gradients("latent_attention_into", q_latent, q_pe, *cache, o, lse)
     _C.require_device(q_latent, q_pe, page_table, lengths, cu_q, o, lse)
     assert q_latent.dtype == torch.bfloat16 and q_latent.dim() == 3 and q_latent.shape[2] == LATENT, f"q_latent must be a bfloat16 [tokens, heads, {LATENT}] tensor, got {q_latent.dtype} {list(q_latent.shape)}"
@@ -347,7 +348,7 @@ def latent_attention(
     Tokens cu_q[i] .. cu_q[i + 1] - 1 are the n newest of sequence i, whose lengths[i] cached rows (theirs included: append them first) lie in the
     pages page_table[i]. Token k of them sees the rows up to lengths[i] - n + k; with tree_mask ([T] int64) all rows in front of the n newest, and of
     those row j where bit j of the token's word is set (tree_mask_of makes such words; n is at most 64). A token that sees no row gets 0 and an lse
-    of -inf. Tokens from cu_q[b] on are not written. page_table [b, pages], lengths [b] and cu_q [b + 1] are int32, on the device."""
+    of -inf. Tokens from cu_q[b] on are not written. The same call gives the same bits; in a batch of other sequences a token's last bits may differ. page_table [b, pages], lengths [b] and cu_q [b + 1] are int32, on the device."""
     return _attention_op(q_latent, q_pe, cache.latent, cache.k_pe, cache.scale, page_table, lengths, cu_q, softmax_scale, tree_mask)
 
 

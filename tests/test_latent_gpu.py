@@ -387,6 +387,26 @@ def test_tokens_behind_the_last_sequence_in_either_kernel(gpu, monkeypatch, rows
     b.check(o[:3], lse[:, :3])
 
 
+@pytest.mark.parametrize("fp8", [False, True], ids=["bf16", "fp8"])
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("rows", [16, 64])
+def test_a_query_that_is_not_finite_spoils_its_own_row_only(gpu, monkeypatch, rows, bad, fp8):
+    """The same bits for all others of the batch, those of the same row block among them; joined from several parts, too."""
+    monkeypatch.setattr(sys.modules[__name__], "MIN_WIDTH", WIDTHS[rows])
+    h = {16: 5, 64: 24}[rows]
+    b = Batch(gpu, [3, 1, 2], [700, 5000, 64], h, page=16, seed=19, fp8=fp8)
+    _takes(b, rows)
+    want_o, want_lse = b.attention()
+    b.check(want_o, want_lse)
+    spoilt = torch.zeros(6, h, dtype=torch.bool)
+    for token, head in ((1, 2), (3, 0), (5, h - 1)):
+        b.q_latent[token, head, 7] = bad
+        spoilt[token, head] = True
+    o, lse = b.attention()
+    assert torch.equal(o[~spoilt], want_o[~spoilt]) and torch.equal(lse.T[~spoilt], want_lse.T[~spoilt])
+    assert torch.isnan(o[spoilt].float()).all()
+
+
 def test_large_scores_in_blocks_of_64_rows_do_not_overflow(gpu, monkeypatch):
     monkeypatch.setattr(sys.modules[__name__], "MIN_WIDTH", 2048)
     test_large_scores_do_not_overflow(gpu)
