@@ -387,6 +387,38 @@ def test_tokens_behind_the_last_sequence_in_either_kernel(gpu, monkeypatch, rows
     b.check(o[:3], lse[:, :3])
 
 
+# Ranges that hold several row blocks, of one sequence and of several: a prompt against itself, a batch of many single tokens.
+@pytest.mark.parametrize("fp8", [False, True], ids=["bf16", "fp8"])
+@pytest.mark.parametrize("rows, counts, lengths, h", [(64, [601, 3], [700, 40], 64), (16, [1] * 1100, [1 + 37 * i % 90 for i in range(1100)], 16)], ids=["prompt", "single tokens"])
+def test_more_row_blocks_than_workgroups_in_either_kernel(gpu, monkeypatch, rows, counts, lengths, h, fp8):
+    monkeypatch.setattr(sys.modules[__name__], "MIN_WIDTH", WIDTHS[rows])
+    b = Batch(gpu, counts, lengths, h, page=16, seed=20, fp8=fp8)
+    _takes(b, rows)
+    b.check(*b.attention())
+
+
+def test_empty_calls_return_empty_results(gpu):
+    """No tokens, no sequences, no rows: nothing is written."""
+    b = Batch(gpu, [0, 0], [40, 0], 4, seed=21)
+    z = lambda *s, d=BF: torch.zeros(*s, dtype=d, device=gpu)  # noqa: E731
+    cos, sin = _tables(8, gpu)
+    none, start = z(0, d=I64), z(1, d=I32)
+
+    def calls():
+        L.latent_cache_append(z(0, 576), z(512), cos, sin, none, none, b.cache)
+        return [
+            b.attention()[0], b.attention()[1], L.latent_attention(z(3, 4, 512), z(3, 4, 64), b.cache, b.table[:0], b.lens[:0], start, SCALE)[0],
+            *L.latent_cache_gather(b.cache, b.table[:0], start, 5), *L.latent_cache_gather(b.cache, b.table, z(3, d=I32), 0),
+            *L.absorb_query(z(0, 4, 192), z(1024, 512), cos, sin, none), L.absorb_value(z(0, 4, 512), z(1024, 512)),
+            MLA(4, 192, 128).decode(z(0, 4, 192), z(0, 576), z(512), z(1024, 512), cos, sin, none, none, b.cache, b.table, b.lens, b.cu_q),
+        ]  # fmt: skip
+
+    want = [(0, 4, 512), (4, 0), (3, 4, 512), (5, 512), (5, 64), (0, 512), (0, 64), (0, 4, 512), (0, 4, 64), (0, 4, 128), (0, 4, 128)]
+    before = [t.clone() for t in b.cache[:2]]
+    assert [tuple(t.shape) for t in calls()] == want
+    assert all(torch.equal(x.view(torch.uint8), y.view(torch.uint8)) for x, y in zip(b.cache, before))
+
+
 @pytest.mark.parametrize("fp8", [False, True], ids=["bf16", "fp8"])
 @pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
 @pytest.mark.parametrize("rows", [16, 64])
