@@ -10,8 +10,8 @@
 // one another and read each key fragment four times: 128 heads 81 us against 74, trees of up to 48 drafts 246 against 217.)
 // Trees of up to 48 drafts over 16 sequences of up to 16384 rows, 16 heads (147 GF): 162 us a call; in a kernel trace, median (least), 196 (175) and 11.8 for the
 // join. 128 heads over 32 sequences of up to 8192 rows (46 GF, 201 MB): 73 us a call, 64.6 (61.1) and 10.3. From e4m3 172 and 67 us a call. A scoring wave is busy
-// for 1700 of a tile's 1850 cycles (half in products, half in softmax), an adding one for 1500: the chain of a scoring wave bounds a tile. (Sixteen waves of half
-// the size, a higher priority for the scoring ones, and 4, 6 or 8 fragments read ahead all took the same time within 1 %.)
+// for 1700 of a tile's 1850 cycles (half in products, half in softmax), an adding one for 1500, so a scoring wave's chain is the nearest bound; sixteen waves of
+// half the size, a higher priority for the scoring ones, and 4, 6 or 8 fragments read ahead all took the same time within 1 %, and why is open.
 // All 64 rows of a block are multiplied and weighed, and written as a part, whether the sequence brings them or not: two tokens of 16 heads pay for four.
 // Weights are formed against a reference of each row that all waves know from earlier tiles; only a score beyond its slack (kSlack) makes them meet, two
 // barriers more, to move it.

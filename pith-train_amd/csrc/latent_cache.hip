@@ -2,7 +2,8 @@
 //
 // Both move memory and little else. A token is one wavefront's work: its 512 latent features are 16 bytes a lane, so a row goes in and out by
 // whole 1-KB instructions and its sums stay in registers. 8192 tokens into a bf16 cache 6.5 us (21 MB, 3.3 TB/s: four rounds of loads that wait for one another,
-// the slot, the row and the weights behind the branch on it, then, behind the latent row's store, the position and its row of the tables), 32 tokens 3.6 us (an empty kernel 2.5); 75000 rows of 16 sequences out of an e4m3 cache 31.6 us (156 MB, 4.9 TB/s, the rate of a large copy), 1021 rows 4.6 us.
+// the slot, the row and the weights behind the branch on it, then, behind the latent row's store, the position and its row of the tables), 32 tokens
+// 3.6 us (an empty kernel 2.5); 75000 rows of 16 sequences out of an e4m3 cache 31.6 us (156 MB, 4.9 TB/s, the rate of a large copy), 1021 rows 4.6 us.
 #include "latent_common.h"
 
 namespace pith {

@@ -37,7 +37,8 @@ FP8 = torch.float8_e4m3fn
 class LatentCache(NamedTuple):
     """Pages of cached rows. latent [pages, page_size, 512] bf16 or float8_e4m3fn, k_pe [pages, page_size, 64] bf16, scale [pages, page_size] fp32
     (e4m3 only: a feature is value * scale of its row). page_size is a power of two from 16 to 65536; rows of a page are contiguous, pages may be
-    further apart (the layers of a model can share one allocation); pages begin at multiples of 16 bytes. Slot s is row s % page_size of page s // page_size."""
+    further apart (the layers of a model can share one allocation) and begin at multiples of 16 bytes. Slot s is row s % page_size of page
+    s // page_size."""
 
     latent: torch.Tensor
     k_pe: torch.Tensor
@@ -348,7 +349,8 @@ def latent_attention(
     Tokens cu_q[i] .. cu_q[i + 1] - 1 are the n newest of sequence i, whose lengths[i] cached rows (theirs included: append them first) lie in the
     pages page_table[i]. Token k of them sees the rows up to lengths[i] - n + k; with tree_mask ([T] int64) all rows in front of the n newest, and of
     those row j where bit j of the token's word is set (tree_mask_of makes such words; n is at most 64). A token that sees no row gets 0 and an lse
-    of -inf. Tokens from cu_q[b] on are not written. The same call gives the same bits; in a batch of other sequences a token's last bits may differ. page_table [b, pages], lengths [b] and cu_q [b + 1] are int32, on the device."""
+    of -inf. Tokens from cu_q[b] on are not written. The same call gives the same bits; in a batch of other sequences a token's last bits may differ.
+    page_table [b, pages], lengths [b] and cu_q [b + 1] are int32, on the device."""
     return _attention_op(q_latent, q_pe, cache.latent, cache.k_pe, cache.scale, page_table, lengths, cu_q, softmax_scale, tree_mask)
 
 
