@@ -969,6 +969,29 @@ def test_compiled_operators_match_eager(gpu):
             assert torch.equal(x, y)
 
 
+@pytest.mark.parametrize("fp8", [False, True], ids=["bf16", "fp8"])
+def test_a_compiled_decoding_step_writes_the_cache(gpu, fp8):
+    """The same result and the same rows in the cache as the eager step's, whose tensors the compiled one changes in place."""
+    g, w, kv_b, cos, sin = _layer(4, 35, gpu)
+    q, kv_a = torch.randn(3, 4, 192, generator=g).to(BF).to(gpu), torch.randn(3, 576, generator=g).to(BF).to(gpu)
+    idx, table = torch.arange(3, device=gpu), torch.zeros(1, 1, dtype=I32, device=gpu)
+    lens, cu = torch.tensor([3], dtype=I32, device=gpu), torch.tensor([0, 3], dtype=I32, device=gpu)
+    layer = MLA(4, 192, 128)
+
+    def step(*cache):
+        return layer.decode(q, kv_a, w, kv_b, cos, sin, idx, idx, L.LatentCache(*cache), table, lens, cu)
+
+    caches = [[t for t in L.LatentCache.empty(1, 16, L.FP8 if fp8 else BF, gpu) if t is not None] for _ in range(2)]
+    for t in caches[0] + caches[1]:
+        t.view(torch.uint8).zero_()
+    with torch.no_grad():
+        want = step(*caches[0])
+        got = torch.compile(step, backend="aot_eager", fullgraph=True)(*caches[1])
+    assert torch.equal(got, want)
+    for x, y in zip(*caches):
+        assert torch.equal(x.view(torch.uint8), y.view(torch.uint8)) and y.view(torch.uint8).any()
+
+
 # ---------------------------------------------------------------------------------------------
 # Refusals
 
