@@ -1,0 +1,269 @@
+// The key-value cache's rows: written as new tokens come (RMS norm and rotation of q and k, quantisation), and what the selection of pages wants to know of
+// them, the least and largest value of every key feature of a page.
+//
+// Both move memory and little else. A row of a head is 16 bytes a lane: a group of dim / 8 lanes holds it in registers from the load to the store, its sums are a
+// few steps between lanes, and the rotation's partner (half a row away) comes from the lane half a group away. Query, key and value rows are rows of
+// one launch.
+#include "kv_common.h"
+
+namespace pith {
+namespace {
+
+constexpr int kThreads = 256;
+
+struct KVAppendParams {
+  const __bf16 *q, *k, *v;
+  const void *q_weight, *k_weight;
+  const __bf16 *cos, *sin;
+  const int64_t *pos, *slots;
+  __bf16* q_out;
+  int64_t P, rows;  // positions, slots
+  int64_t q_ts, q_hs, k_ts, k_hs, v_ts, v_hs, q_out_ts, q_out_hs;
+  int total, per_token, H;
+  float eps;
+  KVCache cache;
+};
+
+template <int LANES>
+__device__ __forceinline__ float group_sum(float x) {
+#pragma unroll
+  for (int m = 1; m < LANES; m <<= 1) x += __shfl_xor(x, m);
+  return x;
+}
+template <int LANES>
+__device__ __forceinline__ float group_max(float x) {
+#pragma unroll
+  for (int m = 1; m < LANES; m <<= 1) x = fmaxf(x, __shfl_xor(x, m));
+  return x;
+}
+
+__device__ __forceinline__ void unpack8(u32x4 x, float (&v)[8]) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) v[2 * e] = bf16lo_to_f32(x[e]), v[2 * e + 1] = bf16hi_to_f32(x[e]);
+}
+
+// Weights: 0 none, 1 bf16, 2 fp32. The norm, the rotation and the division by the scale are fp32, rounded once (to nearest even; e4m3: the largest feature
+// becomes +-448 exactly). The scale is the fp32 quotient, not a power of two, as in the latent cache.
+template <int D, bool FP8, int WEIGHT>
+__global__ __launch_bounds__(kThreads) void kv_append_kernel(KVAppendParams p) {
+  constexpr int kLanes = D / 8;
+  const int row = (blockIdx.x * kThreads + threadIdx.x) / kLanes, sub = threadIdx.x % kLanes;
+  if (row >= p.total) return;  // (whole groups of lanes)
+  const int t = row / p.per_token, r = row - t * p.per_token;
+  const int heads = p.cache.heads;
+  const int what = r < p.H ? 0 : r < p.H + heads ? 1 : 2;  // q, k, v
+  const int head = what == 0 ? r : what == 1 ? r - p.H : r - p.H - heads;
+  const int64_t slot = p.slots[t];
+  const bool kept = slot >= 0 && slot < p.rows;
+  if (what != 0 && !kept) return;
+  const __bf16* const src = what == 0 ? p.q + t * p.q_ts + head * p.q_hs : what == 1 ? p.k + t * p.k_ts + head * p.k_hs : p.v + t * p.v_ts + head * p.v_hs;
+  float x[8];
+  unpack8(*reinterpret_cast<const u32x4*>(src + 8 * sub), x);
+  if (what != 2) {
+    const int64_t at = clamped_position(p.pos[t], p.P) * D + 8 * sub;
+    float c[8], s[8];
+    unpack8(*reinterpret_cast<const u32x4*>(p.cos + at), c);
+    unpack8(*reinterpret_cast<const u32x4*>(p.sin + at), s);
+    if constexpr (WEIGHT != 0) {
+      const void* const weight = what == 0 ? p.q_weight : p.k_weight;
+      float w[8];
+      if constexpr (WEIGHT == 2) {
+        const f32x4* const from = reinterpret_cast<const f32x4*>(weight) + 2 * sub;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) w[e] = from[e >> 2][e & 3];
+      } else {
+        unpack8(reinterpret_cast<const u32x4*>(weight)[sub], w);
+      }
+      float sum = 0.f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) sum += x[e] * x[e];
+      const float inv = rsqrtf(group_sum<kLanes>(sum) * (1.f / D) + p.eps);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] = x[e] * inv * w[e];
+    }
+    const bool upper = sub >= kLanes / 2;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float other = __shfl_xor(x[e], kLanes / 2);
+      x[e] = x[e] * c[e] + (upper ? other : -other) * s[e];
+    }
+  }
+  const auto packed = [&]() __attribute__((always_inline)) {
+    u32x4 out;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) out[e] = pack_bf16x2(x[2 * e], x[2 * e + 1]);
+    return out;
+  };
+  if (what == 0) {
+    *reinterpret_cast<u32x4*>(p.q_out + t * p.q_out_ts + head * p.q_out_hs + 8 * sub) = packed();
+    return;
+  }
+  const int64_t page = slot >> p.cache.page_shift, in_page = ((int64_t)head << p.cache.page_shift) + (slot & ((1 << p.cache.page_shift) - 1));
+  char* const dst = what == 1 ? p.cache.k + page * p.cache.k_ps : p.cache.v + page * p.cache.v_ps;
+  if constexpr (FP8) {
+    float top = 0.f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(x[e]));
+    const float scale = group_max<kLanes>(top) / kFp8Max;
+    float y[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float z = scale > 0.f ? x[e] / scale : x[e];  // (a row of zeros stays one; NaN stays NaN)
+      y[e] = z > kFp8Max ? kFp8Max : (z < -kFp8Max ? -kFp8Max : z);
+    }
+    u32x2 out;
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      int word = __builtin_amdgcn_cvt_pk_fp8_f32(y[4 * e], y[4 * e + 1], 0, false);
+      word = __builtin_amdgcn_cvt_pk_fp8_f32(y[4 * e + 2], y[4 * e + 3], word, true);
+      out[e] = (uint32_t)word;
+    }
+    *reinterpret_cast<u32x2*>(dst + in_page * D + 8 * sub) = out;
+    if (sub == 0) {
+      if (what == 1) p.cache.k_scale[page * p.cache.k_scale_ps + in_page] = scale;
+      else p.cache.v_scale[page * p.cache.v_scale_ps + in_page] = scale;
+    }
+  } else {
+    *reinterpret_cast<u32x4*>(dst + in_page * (2 * D) + 16 * sub) = packed();
+  }
+}
+
+struct KVBoundsParams {
+  KVCache cache;
+  __bf16* bounds;
+  const int32_t *table, *lengths, *cu_q;
+  int64_t table_rs, bounds_ps;
+  int T, table_width;
+};
+
+// NaN stays, as in a comparison-free definition: the least and largest of rows with a NaN are NaN.
+__device__ __forceinline__ float least(float a, float b) { return b < a || b != b ? b : a; }
+__device__ __forceinline__ float largest(float a, float b) { return b > a || b != b ? b : a; }
+
+// blockIdx.x: sequence, blockIdx.y: key-value head, blockIdx.z: every how many-th of the pages that its new tokens filled. A group of lanes takes every
+// 256 / kLanes-th row; what the groups found meets in LDS.
+template <int D, bool FP8>
+__global__ __launch_bounds__(kThreads) void kv_bounds_kernel(KVBoundsParams p) {
+  constexpr int kLanes = D / 8, kGroups = kThreads / kLanes;
+  __shared__ float found[2][kGroups][D];
+  const int sub = threadIdx.x % kLanes, group = threadIdx.x / kLanes;
+  const int b = blockIdx.x, head = blockIdx.y;
+  const int page_size = 1 << p.cache.page_shift;
+  const int length = min(max(p.lengths[b], 0), p.table_width << p.cache.page_shift);
+  const int n = p.cu_q ? min(max(p.cu_q[b + 1] - p.cu_q[b], 0), p.T) : 1;
+  for (int i = (max(length - n, 0) >> p.cache.page_shift) + blockIdx.z; i < length >> p.cache.page_shift; i += gridDim.z) {
+    const int64_t page = safe_page(p.table[b * p.table_rs + i], p.cache.pages);
+    float lo[8], hi[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) lo[e] = INFINITY, hi[e] = -INFINITY;
+    const char* const rows = p.cache.k + page * p.cache.k_ps + (int64_t)head * page_size * (FP8 ? D : 2 * D);
+    for (int r = group; r < page_size; r += kGroups) {
+      float x[8];
+      if constexpr (FP8) {
+        const u32x2 raw = *reinterpret_cast<const u32x2*>(rows + (int64_t)r * D + 8 * sub);
+        const float scale = p.cache.k_scale[page * p.cache.k_scale_ps + (int64_t)head * page_size + r];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const bf16x2 two = (e & 1) ? fp8x2_to_bf16<true>(raw[e >> 1]) : fp8x2_to_bf16<false>(raw[e >> 1]);
+          x[2 * e] = (float)two[0] * scale, x[2 * e + 1] = (float)two[1] * scale;
+        }
+      } else {
+        unpack8(*reinterpret_cast<const u32x4*>(rows + (int64_t)r * (2 * D) + 16 * sub), x);
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) lo[e] = least(lo[e], x[e]), hi[e] = largest(hi[e], x[e]);
+    }
+    __syncthreads();  // the page before has been read
+#pragma unroll
+    for (int e = 0; e < 8; ++e) found[0][group][8 * sub + e] = lo[e], found[1][group][8 * sub + e] = hi[e];
+    __syncthreads();
+    if (threadIdx.x < 2 * D) {
+      const int which = threadIdx.x / D, d = threadIdx.x % D;
+      float x = found[which][0][d];
+      for (int g = 1; g < kGroups; ++g) x = which == 0 ? least(x, found[0][g][d]) : largest(x, found[1][g][d]);
+      p.bounds[page * p.bounds_ps + (int64_t)head * (2 * D) + threadIdx.x] = (__bf16)x;
+    }
+  }
+}
+
+}  // namespace
+}  // namespace pith
+
+using namespace pith;
+
+extern "C" int pith_kv_append(const pith_kv_append_args* a, pith_stream_t stream) {
+  const char* who = "pith_kv_append";
+  if (!a) return fail(PITH_ERR_NULL_POINTER, "%s: args is NULL", who);
+  if (const int rc = check_cache(a->cache, who)) return rc;
+  const int64_t dim = a->cache.dim, heads = a->cache.heads;
+  if (a->T < 0 || a->T > 0x7fffffff || a->P < 1 || a->H < 1 || a->H > 1024)
+    return fail(PITH_ERR_BAD_SHAPE, "%s: T = %lld tokens, %lld query heads (1 to 1024), tables of %lld positions", who, (long long)a->T, (long long)a->H, (long long)a->P);
+  if (a->T == 0) return PITH_OK;
+  if (a->T * (a->H + 2 * heads) > 0x7fffffff - 64) return fail(PITH_ERR_UNSUPPORTED, "%s: 2^31 rows or more in a call", who);
+  if (!a->q || !a->k || !a->v || !a->q_out || !a->cos || !a->sin || !a->position_ids || !a->slots || (a->q_weight == nullptr) != (a->k_weight == nullptr))
+    return fail(PITH_ERR_NULL_POINTER, "%s: a required pointer is NULL (the weights are given together or not at all)", who);
+  if (a->q_weight && a->weight_dtype != PITH_BF16 && a->weight_dtype != PITH_F32) return fail(PITH_ERR_BAD_DTYPE, "%s: weight_dtype %d", who, a->weight_dtype);
+  if ((a->T > 1 && (a->q_ts < dim || a->k_ts < dim || a->v_ts < dim || a->q_out_ts < dim)) || (a->H > 1 && (a->q_hs < dim || a->q_out_hs < dim)) ||
+      (heads > 1 && (a->k_hs < dim || a->v_hs < dim)))
+    return fail(PITH_ERR_BAD_SHAPE, "%s: a stride is shorter than a row", who);
+  if (!aligned16(a->q) || !aligned16(a->k) || !aligned16(a->v) || !aligned16(a->q_out) || !aligned16(a->cos) || !aligned16(a->sin) || !aligned16(a->q_weight) ||
+      !aligned16(a->k_weight) || (a->q_ts | a->q_hs | a->k_ts | a->k_hs | a->v_ts | a->v_hs | a->q_out_ts | a->q_out_hs) % 8 || (uintptr_t)a->position_ids % 8 ||
+      (uintptr_t)a->slots % 8)
+    return fail(PITH_ERR_MISALIGNED, "%s: q, k, v, q_out, weights and tables need 16-byte alignment and strides of multiples of 8", who);
+  KVAppendParams p = {};
+  p.q = (const __bf16*)a->q; p.k = (const __bf16*)a->k; p.v = (const __bf16*)a->v; p.q_out = (__bf16*)a->q_out;
+  p.q_weight = a->q_weight; p.k_weight = a->k_weight; p.cos = (const __bf16*)a->cos; p.sin = (const __bf16*)a->sin;
+  p.pos = a->position_ids; p.slots = a->slots; p.P = a->P; p.rows = a->cache.pages * a->cache.page_size;
+  p.q_ts = a->q_ts; p.q_hs = a->q_hs; p.k_ts = a->k_ts; p.k_hs = a->k_hs; p.v_ts = a->v_ts; p.v_hs = a->v_hs; p.q_out_ts = a->q_out_ts; p.q_out_hs = a->q_out_hs;
+  p.per_token = (int)(a->H + 2 * heads); p.total = (int)(a->T * p.per_token); p.H = (int)a->H; p.eps = a->eps;
+  p.cache = to_device(a->cache);
+  const int per_block = kThreads / (int)(dim / 8);
+  const unsigned grid = (unsigned)(((int64_t)p.total + per_block - 1) / per_block);
+  hipStream_t s = (hipStream_t)stream;
+  begin_launch();
+  const bool fp8 = a->cache.dtype == PITH_FP8_E4M3;
+  const int weight = !a->q_weight ? 0 : a->weight_dtype == PITH_BF16 ? 1 : 2;
+  const auto launch = [&](auto d, auto f) {
+    constexpr int D = decltype(d)::value;
+    constexpr bool F = decltype(f)::value;
+    if (weight == 0) kv_append_kernel<D, F, 0><<<grid, kThreads, 0, s>>>(p);
+    else if (weight == 1) kv_append_kernel<D, F, 1><<<grid, kThreads, 0, s>>>(p);
+    else kv_append_kernel<D, F, 2><<<grid, kThreads, 0, s>>>(p);
+  };
+  using std::integral_constant;
+  if (dim == 128 && fp8) launch(integral_constant<int, 128>(), integral_constant<bool, true>());
+  else if (dim == 128) launch(integral_constant<int, 128>(), integral_constant<bool, false>());
+  else if (fp8) launch(integral_constant<int, 64>(), integral_constant<bool, true>());
+  else launch(integral_constant<int, 64>(), integral_constant<bool, false>());
+  return check_launch(who);
+}
+
+extern "C" int pith_kv_bounds(const pith_kv_bounds_args* a, pith_stream_t stream) {
+  const char* who = "pith_kv_bounds";
+  if (!a) return fail(PITH_ERR_NULL_POINTER, "%s: args is NULL", who);
+  if (const int rc = check_cache(a->cache, who)) return rc;
+  const pith_kv_cache& c = a->cache;
+  if (const int rc = check_table(a->T, a->B, c.heads, a->table_width, c.page_size, !a->cu_q, who)) return rc;
+  if (a->T == 0 || a->B == 0) return PITH_OK;
+  if (a->table_width == 0) return fail(PITH_ERR_BAD_SHAPE, "%s: an empty page table holds no rows", who);
+  if (!a->bounds || !a->page_table || !a->lengths) return fail(PITH_ERR_NULL_POINTER, "%s: a required pointer is NULL", who);
+  if ((a->B > 1 && a->table_rs < a->table_width) || (c.pages > 1 && a->bounds_ps < c.heads * 2 * c.dim))
+    return fail(PITH_ERR_BAD_SHAPE, "%s: a stride is shorter than what it steps over", who);
+  if (!aligned16(a->bounds) || (c.pages > 1 && a->bounds_ps % 8) || (uintptr_t)a->page_table % 4 || (uintptr_t)a->lengths % 4 || (uintptr_t)a->cu_q % 4)
+    return fail(PITH_ERR_MISALIGNED, "%s: bounds need 16-byte alignment and a page stride of a multiple of 8", who);
+  KVBoundsParams p = {};
+  p.cache = to_device(c);
+  p.bounds = (__bf16*)a->bounds; p.table = a->page_table; p.lengths = a->lengths; p.cu_q = a->cu_q;
+  p.table_rs = a->B > 1 ? a->table_rs : 0; p.bounds_ps = c.pages > 1 ? a->bounds_ps : 0;
+  p.T = (int)a->T; p.table_width = (int)a->table_width;
+  const int64_t most = a->T / c.page_size + 1;  // pages that the tokens of one sequence can fill
+  const dim3 grid((unsigned)a->B, (unsigned)c.heads, (unsigned)(most < 64 ? most : 64));
+  hipStream_t s = (hipStream_t)stream;
+  begin_launch();
+  const bool fp8 = c.dtype == PITH_FP8_E4M3;
+  if (c.dim == 128 && fp8) kv_bounds_kernel<128, true><<<grid, kThreads, 0, s>>>(p);
+  else if (c.dim == 128) kv_bounds_kernel<128, false><<<grid, kThreads, 0, s>>>(p);
+  else if (fp8) kv_bounds_kernel<64, true><<<grid, kThreads, 0, s>>>(p);
+  else kv_bounds_kernel<64, false><<<grid, kThreads, 0, s>>>(p);
+  return check_launch(who);
+}

@@ -1,4 +1,4 @@
-"""ctypes binding of libpith_hip.so (declarations in include/pith_hip.h and include/pith_latent.h).
+"""ctypes binding of libpith_hip.so (declarations in include/pith_hip.h, include/pith_latent.h and include/pith_kv.h).
 
 There is no fallback: if the library has not been built, or a call returns an error code, an
 exception is raised. PyTorch is used only for device memory and streams; every tensor argument
@@ -15,6 +15,7 @@ LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "lib", "libp
 
 PITH_VERSION = 202  # of include/pith_hip.h, whose structs are declared below
 PITH_LATENT_VERSION = 100  # of include/pith_latent.h
+PITH_KV_VERSION = 100  # of include/pith_kv.h
 
 PITH_BF16, PITH_F32, PITH_FP8_E4M3 = 0, 1, 2
 PITH_BASE_2, PITH_BASE_E = 0, 1
@@ -171,6 +172,57 @@ class LatentAttnArgs(Structure):
     ]  # fmt: skip
 
 
+class KVCacheArgs(Structure):
+    _fields_ = [
+        ("k", c_void_p), ("v", c_void_p), ("k_scale", c_void_p), ("v_scale", c_void_p),
+        ("pages", c_int64), ("page_size", c_int64), ("heads", c_int64), ("dim", c_int64),
+        ("k_ps", c_int64), ("v_ps", c_int64), ("k_scale_ps", c_int64), ("v_scale_ps", c_int64), ("dtype", c_int32), ("reserved0", c_int32),
+    ]  # fmt: skip
+
+
+class PlanStepArgs(Structure):
+    _fields_ = [
+        ("counts", c_void_p), ("lengths", c_void_p), ("page_table", c_void_p), ("free_pages", c_void_p), ("free_count", c_void_p),
+        ("cu_q", c_void_p), ("position_ids", c_void_p), ("slots", c_void_p), ("granted", c_void_p), ("lengths_out", c_void_p), ("free_count_out", c_void_p),
+        ("workspace", c_void_p), ("workspace_bytes", c_int64),
+        ("B", c_int64), ("T", c_int64), ("table_rs", c_int64), ("table_width", c_int64), ("pool_size", c_int64), ("page_size", c_int64),
+    ]  # fmt: skip
+
+
+class KVAppendArgs(Structure):
+    _fields_ = [
+        ("q", c_void_p), ("k", c_void_p), ("v", c_void_p), ("q_weight", c_void_p), ("k_weight", c_void_p), ("cos", c_void_p), ("sin", c_void_p),
+        ("position_ids", c_void_p), ("slots", c_void_p), ("q_out", c_void_p), ("T", c_int64), ("P", c_int64), ("H", c_int64),
+        ("q_ts", c_int64), ("q_hs", c_int64), ("k_ts", c_int64), ("k_hs", c_int64), ("v_ts", c_int64), ("v_hs", c_int64),
+        ("q_out_ts", c_int64), ("q_out_hs", c_int64), ("eps", c_float), ("weight_dtype", c_int32), ("cache", KVCacheArgs),
+    ]  # fmt: skip
+
+
+class KVAttnArgs(Structure):
+    _fields_ = [
+        ("q", c_void_p), ("cache", KVCacheArgs), ("page_table", c_void_p), ("lengths", c_void_p), ("cu_q", c_void_p), ("tree_mask", c_void_p),
+        ("o", c_void_p), ("lse", c_void_p), ("workspace", c_void_p), ("workspace_bytes", c_int64),
+        ("T", c_int64), ("B", c_int64), ("H", c_int64), ("table_rs", c_int64), ("table_hs", c_int64), ("table_width", c_int64),
+        ("q_ts", c_int64), ("q_hs", c_int64), ("o_ts", c_int64), ("o_hs", c_int64), ("lse_hs", c_int64), ("scale", c_float), ("head_tables", c_int32),
+    ]  # fmt: skip
+
+
+class KVBoundsArgs(Structure):
+    _fields_ = [
+        ("cache", KVCacheArgs), ("bounds", c_void_p), ("page_table", c_void_p), ("lengths", c_void_p), ("cu_q", c_void_p),
+        ("T", c_int64), ("B", c_int64), ("table_rs", c_int64), ("table_width", c_int64), ("bounds_ps", c_int64),
+    ]  # fmt: skip
+
+
+class KVSelectArgs(Structure):
+    _fields_ = [
+        ("q", c_void_p), ("bounds", c_void_p), ("page_table", c_void_p), ("lengths", c_void_p), ("cu_q", c_void_p),
+        ("table_out", c_void_p), ("lengths_out", c_void_p), ("workspace", c_void_p), ("workspace_bytes", c_int64),
+        ("T", c_int64), ("B", c_int64), ("H", c_int64), ("heads", c_int64), ("dim", c_int64), ("pages", c_int64), ("page_size", c_int64), ("keep", c_int64),
+        ("q_ts", c_int64), ("q_hs", c_int64), ("table_rs", c_int64), ("table_width", c_int64), ("bounds_ps", c_int64),
+    ]  # fmt: skip
+
+
 # name -> (restype, argtypes); must list every symbol declared in include/pith_hip.h
 SYMBOLS = {
     "pith_version": (c_int, []),
@@ -216,6 +268,19 @@ LATENT_SYMBOLS = {
     "pith_latent_attn": (c_int, [POINTER(LatentAttnArgs), c_void_p]),
 }
 
+# the same for include/pith_kv.h
+KV_SYMBOLS = {
+    "pith_kv_version": (c_int, []),
+    "pith_plan_step_workspace_bytes": (c_int64, [POINTER(PlanStepArgs)]),
+    "pith_plan_step": (c_int, [POINTER(PlanStepArgs), c_void_p]),
+    "pith_kv_append": (c_int, [POINTER(KVAppendArgs), c_void_p]),
+    "pith_kv_attn_workspace_bytes": (c_int64, [POINTER(KVAttnArgs)]),
+    "pith_kv_attn": (c_int, [POINTER(KVAttnArgs), c_void_p]),
+    "pith_kv_bounds": (c_int, [POINTER(KVBoundsArgs), c_void_p]),
+    "pith_kv_select_workspace_bytes": (c_int64, [POINTER(KVSelectArgs)]),
+    "pith_kv_select": (c_int, [POINTER(KVSelectArgs), c_void_p]),
+}
+
 _lib = None
 
 
@@ -229,7 +294,7 @@ def lib() -> ctypes.CDLL:
                 "(there is no non-HIP fallback for these operators)"
             )
         handle = ctypes.CDLL(LIB_PATH)
-        for name, (restype, argtypes) in {**SYMBOLS, **LATENT_SYMBOLS}.items():
+        for name, (restype, argtypes) in {**SYMBOLS, **LATENT_SYMBOLS, **KV_SYMBOLS}.items():
             fn = getattr(handle, name)
             fn.restype = restype
             fn.argtypes = argtypes
@@ -237,6 +302,8 @@ def lib() -> ctypes.CDLL:
             raise ImportError(f"{LIB_PATH} has interface version {handle.pith_version()}, this package needs {PITH_VERSION}: build it again")
         if handle.pith_latent_version() != PITH_LATENT_VERSION:
             raise ImportError(f"{LIB_PATH} has latent interface version {handle.pith_latent_version()}, this package needs {PITH_LATENT_VERSION}: build it again")
+        if handle.pith_kv_version() != PITH_KV_VERSION:
+            raise ImportError(f"{LIB_PATH} has key-value cache interface version {handle.pith_kv_version()}, this package needs {PITH_KV_VERSION}: build it again")
         _lib = handle
     return _lib
 
@@ -302,5 +369,6 @@ def bhs_strides(t: torch.Tensor, what: str):
 __all__ = [
     "lib", "check", "PithError", "CombineArgs", "AttnFwdArgs", "KeyChunk", "AttnDeltaArgs", "AttnBwdArgs", "AttnBwdPlan", "NormRopeArgs", "MlaAssembleArgs", "DeviceInfo", "SYMBOLS",
     "LatentCacheArgs", "LatentAppendArgs", "LatentGatherArgs", "LatentAbsorbArgs", "LatentAttnArgs", "LATENT_SYMBOLS",
+    "KVCacheArgs", "PlanStepArgs", "KVAppendArgs", "KVAttnArgs", "KVBoundsArgs", "KVSelectArgs", "KV_SYMBOLS",
     "dtype_code", "current_stream", "require_device", "bshd_batch_stride", "bshd_head_range_strides", "bhs_strides", "byref",
 ]  # fmt: skip

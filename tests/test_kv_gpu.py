@@ -1,0 +1,776 @@
+"""The key-value cache's operators and the planning of a step on the GPU against the fp64 oracle, through the public entry points.
+
+Bounds are elementwise and come from the arithmetic, u = 2^-8 being bf16's half step relative to the value (torch.finfo(bfloat16).eps / 2):
+
+  a result rounded once from fp32         u |want|; norm and rotation on top 2^-19 of the sum of the absolute values of what the rotation adds (the mean of up to
+                                          128 squares, rsqrt, three products and a sum, each off by a few 2^-24)
+  e4m3 rows                               2^-4 |want| of the value, but half of its finest step, 2^-10, times the row's scale at least; scales 2^-18
+  attention                               the weights P (times the row's scale) are rounded to bf16: u sum P |v|. A score's sum of d products is off by at
+                                          most e = (d + 8) 2^-24 (sum of their absolute values, in bits), its exp2, the subtraction of the maximum and the
+                                          rescaling by 2^-16 in all: weight and denominator 2 (e ln 2 + 2^-16) sum P |v|. And u |want| for the result.
+  lse                                     e + 2^-17 bits (|lse| < 64: its own step is 2^-18)
+  plans, bounds of pages and selections   equal
+"""
+
+import math
+
+import pytest
+import torch
+
+from oracle import kv_oracle as O
+from oracle import prologue_oracle as P
+from pithtrain_amd.operators import paging
+from pithtrain_amd.operators.gqa import kv_cache as K
+from pithtrain_amd.operators.mla import latent as L
+
+pytestmark = pytest.mark.gpu
+BF = torch.bfloat16
+U = 2.0**-8
+I32, I64 = torch.int32, torch.int64
+
+
+def _within(got, want, bound, what):
+    got, want, bound = got.double().cpu(), want.double().cpu(), bound.double().cpu()
+    assert got.shape == want.shape, (what, got.shape, want.shape)
+    assert torch.equal(torch.isfinite(got), torch.isfinite(want)), f"{what}: finite and non-finite values elsewhere than expected"
+    fine = torch.isfinite(want)
+    assert torch.equal(got[~fine], want[~fine]), f"{what}: other infinities"
+    over = ((got - want).abs() - bound)[fine]
+    assert over.numel() == 0 or over.max() <= 0, f"{what}: off by {((got - want).abs() / bound.clamp_min(1e-300))[fine].max():.3f} times the bound"
+
+
+# ---------------------------------------------------------------------------------------------
+# Attention
+
+
+class Batch:
+    """Sequences in a cache. counts: new tokens of each, lengths: cached rows of each. Everything that no sequence owns (rows behind the last one of a
+    page, pages of nobody, table entries that are not needed) holds NaN or nonsense."""
+
+    def __init__(self, dev, counts, lengths, heads=(8, 2, 128), page=64, fp8=False, tree=None, seed=0, extra_tokens=0, q_std=1.0, width=0):
+        g = torch.Generator().manual_seed(seed)
+        mk = lambda *s: torch.randn(*s, generator=g)  # noqa: E731
+        self.h, self.hkv, self.d = heads
+        self.counts, self.lengths, self.dev, self.page, self.scale = counts, lengths, dev, page, self.d**-0.5
+        t = sum(counts) + extra_tokens
+        need = [-(-n // page) for n in lengths]
+        pages, width = sum(need) + 3, max(max(need), 1, width) + 1
+        order = torch.randperm(pages, generator=g)
+        table = torch.randint(-5, 2 * pages, (len(counts), width), generator=g).to(I32)  # entries behind a sequence's pages are never followed
+        at = 0
+        for i, n in enumerate(need):
+            table[i, :n] = order[at : at + n]
+            at += n
+        self.table = table.to(dev)
+        self.kv = []
+        self.scales = []
+        for _ in range(2):
+            x = torch.full((pages, page, self.hkv, self.d), math.nan)
+            for i, n in enumerate(lengths):
+                j = torch.arange(n)
+                x[table[i, j // page].long(), j % page] = mk(n, self.hkv, self.d) * (0.5 + torch.rand(self.hkv, self.d, generator=g))
+            x = x.transpose(1, 2).contiguous()
+            scale = None
+            if fp8:
+                scale = x.abs().amax(-1) / 448
+                x = (x / scale[..., None]).clamp(-448, 448).to(L.FP8)
+                scale = scale.to(dev)
+            self.kv.append((x if fp8 else x.to(BF)).to(dev))
+            self.scales.append(scale)
+        self.q = (q_std * mk(t, self.h, self.d)).to(BF).to(dev)
+        self.cu_q = torch.tensor([0] + torch.tensor(counts).cumsum(0).tolist(), dtype=I32, device=dev)
+        self.lens = torch.tensor(lengths, dtype=I32, device=dev)
+        self.words = None
+        if tree is not None:
+            rows = [L.tree_mask_of(torch.tensor([int(torch.randint(max(-1, i - 6), i, (1,), generator=g)) for i in range(n)], dtype=I64)) if n else torch.empty(0, dtype=I64) for n in counts]
+            self.words = torch.cat(rows + [torch.zeros(extra_tokens, dtype=I64)])
+            if tree == "holes":  # words that leave rows out, and nothing at all for some
+                self.words &= torch.randint(-(1 << 62), 1 << 62, self.words.shape, generator=g)
+                self.words[::3] = 0
+            self.words = self.words.to(dev)
+
+    @property
+    def cache(self):
+        return K.KVCache(*self.kv, *self.scales)
+
+    def rows(self, table, length):
+        """Keys and values of the first rows of a table's pages at the values they hold, [hkv, length, d]."""
+        j = torch.arange(length, device=self.dev)
+        p, r = table[j // self.page].long(), j % self.page
+        out = []
+        for x, scale in zip(self.kv, self.scales):
+            y = x.to(torch.float32)[p, :, r].double() * (1.0 if scale is None else scale[p, :, r].double()[..., None])
+            out.append(y.transpose(0, 1).cpu())
+        return out
+
+    def attention(self, words="own"):
+        return K.kv_attention(self.q, self.cache, self.table, self.lens, self.cu_q, self.scale, self.words if words == "own" else words)
+
+    def close(self, o, lse, q, k, v, seen, what, slack=0.0):
+        want, want_lse, mass, spread = O.attention(q.cpu(), k, v, seen, self.scale)
+        e = (self.d + 8) * 2.0**-24 * spread + slack * want_lse.T.abs().nan_to_num(posinf=0.0)
+        _within(o, want, U * want.abs() + (U + 2 * (e[..., None] * math.log(2) + 2.0**-16)) * mass, f"{what}: o")
+        _within(lse, want_lse, e.T + 2.0**-17, f"{what}: lse")
+
+    def check(self, o, lse, what="", slack=0.0):
+        o, lse, first = o.cpu(), lse.cpu(), 0
+        for i, (n, length) in enumerate(zip(self.counts, self.lengths)):
+            sl = slice(first, first + n)
+            first += n
+            if n == 0:
+                continue
+            seen = O.sees(n, length, None if self.words is None else self.words[sl].tolist())
+            self.close(o[sl], lse[:, sl], self.q[sl], *self.rows(self.table[i], length), seen, f"{what} sequence {i}", slack)
+
+
+LENGTH_SETS = {
+    "one_row": ([1], [1]),
+    "tiny": ([1, 1, 1, 1, 1], [1, 15, 16, 17, 31]),
+    "tile_ends": ([1] * 9, [32, 33, 63, 64, 65, 96, 127, 128, 129]),
+    "ordinary": ([1, 1, 1], [517, 1, 1301]),
+    "none": ([1, 0, 1, 0], [0, 70, 40, 0]),
+    "few_tokens": ([2, 3, 1, 5], [2, 64, 700, 37]),
+    "prompt": ([70, 33], [70, 129]),
+    "contradiction": ([4, 3], [2, 0]),  # more new tokens than rows: the first of them see nothing
+}
+HEADS = [(32, 4, 128), (8, 2, 64), (5, 1, 128), (3, 3, 64), (40, 2, 128), (16, 1, 64), (70, 1, 128)]
+BOTH = pytest.mark.parametrize("fp8", [False, True], ids=["bf16", "fp8"])
+
+
+@BOTH
+@pytest.mark.parametrize("heads", HEADS[:4], ids=str)
+@pytest.mark.parametrize("name", LENGTH_SETS)
+def test_attention_matches_the_oracle(gpu, name, heads, fp8):
+    counts, lengths = LENGTH_SETS[name]
+    b = Batch(gpu, counts, lengths, heads, page=16 if name in ("tiny", "prompt") else 64, fp8=fp8, seed=len(name))
+    b.check(*b.attention(), name)
+
+
+@BOTH
+@pytest.mark.parametrize("heads", HEADS, ids=str)
+def test_attention_of_other_head_counts(gpu, heads, fp8):
+    b = Batch(gpu, [1, 2, 9], [333, 90, 200], heads, page=32, fp8=fp8, seed=heads[0])
+    b.check(*b.attention())
+
+
+@BOTH
+@pytest.mark.parametrize("page", [16, 32, 128, 1024])
+def test_attention_page_sizes(gpu, page, fp8):
+    b = Batch(gpu, [1, 3], [page + 5, 2 * page], page=page, fp8=fp8, seed=page)
+    b.check(*b.attention())
+
+
+@BOTH
+@pytest.mark.parametrize("heads", [(8, 1, 128), (4, 2, 64)], ids=str)
+def test_attention_of_one_long_sequence_is_joined_from_many_parts(gpu, fp8, heads):
+    b = Batch(gpu, [1, 1], [20011, 3], heads, fp8=fp8, seed=3, q_std=2.0)
+    b.check(*b.attention())
+
+
+def test_attention_of_more_sequences_than_a_wavefront_scans_at_once(gpu):
+    g = torch.Generator().manual_seed(4)
+    counts = torch.randint(0, 3, (150,), generator=g).tolist()
+    lengths = [max(n, int(x)) for n, x in zip(counts, torch.randint(0, 400, (150,), generator=g))]
+    b = Batch(gpu, counts, lengths, (4, 2, 64), page=16, seed=5)
+    b.check(*b.attention())
+
+
+def test_attention_of_more_row_blocks_than_workgroups(gpu):
+    b = Batch(gpu, [1] * 300, [7 + i % 200 for i in range(300)], (8, 4, 64), page=16, seed=6)
+    b.check(*b.attention())
+
+
+def test_large_scores_do_not_overflow(gpu):
+    b = Batch(gpu, [1, 2], [300, 65], seed=6, q_std=200.0)
+    o, lse = b.attention()
+    assert torch.isfinite(o.float()).all() and lse.abs().max() > 500
+    b.check(o, lse, slack=2.0**-22)  # lse is in the hundreds here: its bound grows with it (a few more roundings of 2^-24 |lse|)
+
+
+@BOTH
+@pytest.mark.parametrize("kind", ["tree", "holes"])
+@pytest.mark.parametrize("counts,lengths,heads", [([1], [1], (8, 2, 128)), ([8, 8], [517, 8], (16, 2, 64)), ([64, 1, 33], [64, 300, 1000], (3, 1, 128)), ([7, 0, 12], [40, 5, 12], (8, 1, 64)), ([64], [63], (2, 2, 128))])
+def test_tree_attention_matches_the_oracle(gpu, counts, lengths, heads, kind, fp8):
+    b = Batch(gpu, counts, lengths, heads, page=16, fp8=fp8, tree=kind, seed=sum(counts) + heads[0])
+    o, lse = b.attention()
+    b.check(o, lse, kind)
+    if kind == "holes" and lengths == [1]:
+        assert (o == 0).all() and (lse == -math.inf).all()
+
+
+def test_a_chain_of_drafts_is_the_causal_call(gpu):
+    b = Batch(gpu, [5, 9], [200, 60], seed=8)
+    words = torch.cat([L.tree_mask_of(torch.arange(-1, n - 1)) for n in b.counts]).to(gpu)
+    for x, y in zip(b.attention(), b.attention(words)):
+        assert torch.equal(x, y)
+
+
+@BOTH
+@pytest.mark.parametrize("tree", [None, "tree"])
+@pytest.mark.parametrize("where", ["key", "value", "scale"])
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("heads", [(8, 2, 128), (6, 1, 64), (24, 2, 128)], ids=str)
+def test_a_row_that_a_token_does_not_see_cannot_reach_it(gpu, bad, where, tree, fp8, heads):
+    """The newest row of a sequence holds infinities or NaN: tokens that do not see it are computed as ever, and those that do know of it."""
+    if where == "scale" and not fp8:
+        pytest.skip("bf16 rows have no scale")
+    b = Batch(gpu, [6, 6], [70, 6], heads, page=16, seed=9, tree=tree, fp8=fp8)
+    want_o, want_lse = b.attention()
+    blind = torch.ones(12, dtype=torch.bool)
+    for i in range(2):
+        j = b.lengths[i] - 1
+        page, row = b.table[i, j // 16].long(), j % 16
+        for which in {"key": [0], "value": [1], "scale": [0, 1]}[where]:
+            if where == "scale":
+                b.scales[which][page, :, row] = bad
+            elif fp8:
+                b.kv[which].view(torch.uint8)[page, :, row, 20:] = 0x7F
+            else:
+                b.kv[which][page, :, row, 20:] = bad
+        blind[6 * i + 5] = False
+        if tree:
+            blind[6 * i : 6 * i + 6] = (b.words[6 * i : 6 * i + 6].cpu() >> 5) & 1 == 0
+    assert 2 <= blind.sum() < 12
+    o, lse = b.attention()
+    assert torch.equal(o[blind], want_o[blind]) and torch.equal(lse[:, blind], want_lse[:, blind])
+    if where == "value":
+        assert torch.equal(lse, want_lse) and torch.equal(o[..., :20], want_o[..., :20])
+        got = o[~blind][..., 20:].float()
+        assert (torch.isnan(got) if math.isnan(bad) or fp8 else got == bad).all()
+    else:
+        assert torch.isnan(o[~blind].float()).any()
+
+
+@BOTH
+def test_a_single_draft_that_does_not_see_itself_is_not_reached_by_its_row(gpu, fp8):
+    b = Batch(gpu, [1, 1], [90, 1], page=16, fp8=fp8, tree="tree", seed=14)
+    b.words.zero_()
+    want = b.attention()
+    b.check(*want)
+    for i in range(2):
+        j = b.lengths[i] - 1
+        for x in b.kv:
+            x[b.table[i, j // 16].long(), :, j % 16] = math.nan
+    assert all(torch.equal(x, y) for x, y in zip(b.attention(), want))
+
+
+def test_tokens_behind_the_last_sequence_keep_what_they_hold(gpu):
+    b = Batch(gpu, [2, 1], [40, 70], extra_tokens=3, seed=10)
+    o, lse = torch.full_like(b.q, 7.0), torch.full((b.h, 6), 8.0, device=gpu)
+    K.kv_attention_into(b.q, b.cache, b.table, b.lens, b.cu_q, b.scale, None, o, lse)
+    b.check(o[:3], lse[:, :3])
+    assert (o[3:] == 7).all() and (lse[:, 3:] == 8).all()
+
+
+@BOTH
+def test_strides(gpu, fp8):
+    """Queries and results as slices, a cache whose layers share an allocation, a page table as a column range, results of heads apart."""
+    b = Batch(gpu, [2, 1], [40, 170], seed=11, fp8=fp8, page=32)
+    want = b.attention()
+    wide = torch.zeros(3, b.h + 3, 2 * b.d, dtype=BF, device=gpu)
+    wide[:, 1:-2, b.d :] = b.q
+    layers = []
+    for x in b.kv + ([] if b.scales[0] is None else b.scales):
+        both = torch.zeros((x.shape[0], 2) + tuple(x.shape[1:]), dtype=x.dtype, device=gpu)
+        both[:, 1].copy_(x)
+        layers.append(both[:, 1])
+    table = torch.full((2, b.table.shape[1] + 5), -3, dtype=I32, device=gpu)
+    table[:, 2:-3] = b.table
+    o, lse = torch.zeros(3, 2 * b.h, b.d, dtype=BF, device=gpu), torch.zeros(b.h, 9, device=gpu)
+    K.kv_attention_into(wide[:, 1:-2, b.d :], K.KVCache(*layers), table[:, 2:-3], b.lens, b.cu_q, b.scale, None, o[:, ::2], lse[:, 4:7])
+    assert torch.equal(o[:, ::2], want[0]) and torch.equal(lse[:, 4:7], want[1]) and (o[:, 1::2] == 0).all() and (lse[:, :4] == 0).all()
+    got = K.kv_attention(wide[:, 1:-2, b.d :], K.KVCache(*layers), table[:, 2:-3], b.lens, b.cu_q, b.scale)
+    assert all(torch.equal(x, y) for x, y in zip(got, want))
+    odd = torch.zeros(3, b.h, b.d + 1, dtype=BF, device=gpu)  # rows off the alignment: copied
+    odd[..., 1:] = b.q
+    got = K.kv_attention(odd[..., 1:], b.cache, b.table, b.lens, b.cu_q, b.scale)
+    assert all(torch.equal(x, y) for x, y in zip(got, want))
+
+
+@BOTH
+@pytest.mark.parametrize("heads", [(8, 2, 128), (6, 3, 64), (20, 1, 128)], ids=str)
+def test_attention_with_a_table_of_every_head(gpu, fp8, heads):
+    """Every token and head attends to rows of its own choice, with and without token offsets."""
+    b = Batch(gpu, [1, 1, 1], [200, 90, 333], heads, page=16, fp8=fp8, seed=12)
+    g = torch.Generator().manual_seed(13)
+    t, hkv = 3, b.hkv
+    table, lengths = torch.full((t, hkv, 7), -1, dtype=I32), torch.zeros(t, hkv, dtype=I32)
+    for i in range(t):
+        for j in range(hkv):
+            n = int(torch.randint(0, 8, (1,), generator=g)) if i else 7
+            pages = torch.randint(0, b.lengths[i] // 16, (n,), generator=g)  # whole pages, one more than once perhaps
+            table[i, j, :n] = b.table[i].cpu()[pages]
+            lengths[i, j] = max(n * 16 - int(torch.randint(0, 16, (1,), generator=g)), 0)
+    assert (lengths == 0).any() or hkv == 1
+    for cu_q in (None, torch.arange(t + 1, dtype=I32, device=gpu)):
+        o, lse = (x.cpu() for x in K.kv_attention(b.q, b.cache, table.to(gpu), lengths.to(gpu), cu_q, b.scale))
+        for i in range(t):
+            for j in range(hkv):
+                n, mine = int(lengths[i, j]), slice(j * (b.h // hkv), (j + 1) * (b.h // hkv))
+                k, v = b.rows(table[i, j].to(gpu).clamp(min=0), n)
+                b.close(o[i : i + 1, mine], lse[mine, i : i + 1], b.q[i : i + 1, mine], k[j : j + 1], v[j : j + 1], O.sees(1, n), f"token {i} head {j}")
+
+
+def test_bad_tables_lengths_and_offsets_stay_in_memory(gpu):
+    """Nonsense in what the kernels index by: wrong rows, but every token of a sequence is written, and nothing else."""
+    b = Batch(gpu, [2, 1, 1], [40, 70, 300], extra_tokens=2, seed=10, page=16)
+    for table, lens, cu_q in [
+        (torch.full_like(b.table, 2**31 - 1), b.lens, b.cu_q),
+        (torch.full_like(b.table, -(2**31)), b.lens, b.cu_q),
+        (b.table, torch.tensor([2**31 - 1, -5, -(2**31)], dtype=I32, device=gpu), b.cu_q),
+        (b.table, b.lens, torch.tensor([-7, 3, 2, 2**31 - 1], dtype=I32, device=gpu)),
+        (b.table, b.lens, torch.tensor([9, 9, 9, 9], dtype=I32, device=gpu)),
+    ]:
+        o, lse = torch.full_like(b.q, 7.0), torch.full((b.h, 6), 8.0, device=gpu)
+        K.kv_attention_into(b.q, b.cache, table, lens, cu_q, b.scale, None, o, lse)
+        K.kv_select_pages(b.q, torch.zeros(b.kv[0].shape[0], b.hkv, 2, b.d, dtype=BF, device=gpu), table, lens, cu_q, 16, 3)
+        K.kv_page_bounds(b.cache, b.cache.empty_bounds(), table, lens, cu_q, 6)
+        torch.cuda.synchronize()
+    assert (o == 7).all() and (lse == 8).all()  # offsets behind the tokens: nobody's
+
+
+# ---------------------------------------------------------------------------------------------
+# Append
+
+
+def _tables(d, n=50):
+    cos, sin = P.cos_sin_table(torch.arange(n).unsqueeze(0), d, dtype=BF)
+    return cos[0], sin[0]
+
+
+@BOTH
+@pytest.mark.parametrize("weight", [BF, torch.float32, None], ids=str)
+@pytest.mark.parametrize("heads", [(32, 4, 128), (5, 1, 64), (3, 3, 128)], ids=str)
+@pytest.mark.parametrize("t", [1, 13, 130])
+def test_append_matches_the_oracle(gpu, t, heads, weight, fp8):
+    h, hkv, d = heads
+    g = torch.Generator().manual_seed(t + h)
+    mk = lambda *s: torch.randn(*s, generator=g)  # noqa: E731
+    qkv = (2 * mk(t, h + 2 * hkv, d) * (0.2 + torch.rand(t, 1, 1, generator=g))).to(BF)
+    qkv[t // 2, h + hkv :] = 0  # a row of zeros
+    q, k, v = qkv.split((h, hkv, hkv), 1)
+    w = [None, None] if weight is None else [(1 + 0.3 * mk(d)).to(weight) for _ in range(2)]
+    cos, sin = _tables(d)
+    page = 16
+    pages = -(-t // page) + 2
+    pos, slots = torch.randint(0, 50, (t,), generator=g), torch.randperm(pages * page, generator=g)[:t]
+    if t > 1:
+        slots[3], slots[7] = -1, pages * page  # padding
+    cache = K.KVCache.empty(pages, hkv, d, page, L.FP8 if fp8 else BF, gpu)
+    for x in cache:
+        if x is not None:
+            x.view(torch.uint8).fill_(0x11)
+    before = [None if x is None else x.clone() for x in cache]
+    on = lambda x: None if x is None else x.to(gpu)  # noqa: E731
+    out = K.kv_cache_append(*qkv.to(gpu).split((h, hkv, hkv), 1), on(w[0]), on(w[1]), on(cos), on(sin), on(pos), on(slots), cache, 1e-6)
+    want, mass = O.norm_rope(q, w[0], cos, sin, pos, 1e-6)
+    _within(out, want, U * want.abs() + 2.0**-19 * mass, "q")
+    kept = (slots >= 0) & (slots < pages * page)
+    p, r = slots[kept] // page, slots[kept] % page
+    for i, (x, what) in enumerate(((O.norm_rope(k, w[1], cos, sin, pos, 1e-6), "k"), ((v.double(), v.double().abs()), "v"))):
+        want, mass = x[0][kept], x[1][kept]
+        got = cache[i].cpu().to(torch.float32)[p, :, r].double()
+        if fp8:
+            scale = cache[2 + i].cpu()[p, :, r].double()
+            top = want.abs().amax(-1) / 448
+            _within(scale, top, 2.0**-18 * (top + mass.amax(-1) / 448), what + " scale")
+            got = got * scale[..., None]
+            _within(got, want, 2.0**-4 * want.abs() + 2.0**-10 * scale[..., None] + 2.0**-18 * mass, what)
+        else:
+            _within(got, want, U * want.abs() + 2.0**-19 * mass, what)
+    untouched = torch.ones(pages * page, dtype=torch.bool)
+    untouched[slots[kept]] = False
+    for x, y in zip(cache, before):
+        if x is not None:
+            x, y = (z.view(torch.uint8).cpu().transpose(1, 2).reshape(pages * page, -1) if z.dim() == 4 else z.view(I32).cpu().transpose(1, 2).reshape(pages * page, -1) for z in (x, y))
+            assert torch.equal(x[untouched], y[untouched]), "rows of nobody were written"
+
+
+def test_append_is_the_training_prologue(gpu):
+    """The same bits as qk_norm_rope, which the layer was trained with."""
+    from pithtrain_amd.operators.norm_rope import qk_norm_rope
+
+    g = torch.Generator().manual_seed(20)
+    t, h, hkv, d = 37, 32, 4, 128
+    q, k, v = (torch.randn(t, n, d, generator=g).to(BF).to(gpu) for n in (h, hkv, hkv))
+    w = [(1 + 0.2 * torch.randn(d, generator=g)).to(BF).to(gpu) for _ in range(2)]
+    cos, sin = (x.to(gpu) for x in _tables(d))
+    with torch.no_grad():
+        want_q, want_k = qk_norm_rope(q[None], k[None], *w, cos[None, :t], sin[None, :t], 1e-6)
+    cache = K.KVCache.empty(2, hkv, d, 64, device=gpu)
+    at = torch.arange(t, device=gpu)
+    got = K.kv_cache_append(q, k, v, *w, cos, sin, at, at, cache, 1e-6)
+    step = 2.0**-7  # the sums of squares may be added in another order: at most a step of bf16 apart
+    _within(got, want_q[0], step * want_q[0].abs(), "q")
+    _within(cache.k[0, :, :t].transpose(0, 1), want_k[0], step * want_k[0].abs(), "k")
+    assert torch.equal(cache.v[0, :, :t].transpose(0, 1), v)
+
+
+def test_append_in_place_and_copied(gpu):
+    """Rows off the alignment and tables that are not contiguous are copied."""
+    g = torch.Generator().manual_seed(21)
+    t, h, hkv, d = 6, 4, 2, 64
+    q, k, v = (torch.randn(t, n, d, generator=g).to(BF).to(gpu) for n in (h, hkv, hkv))
+    cos, sin = (x.to(gpu) for x in _tables(d))
+    at = torch.arange(t, device=gpu)
+    caches = [K.KVCache.empty(1, hkv, d, 16, device=gpu) for _ in range(2)]
+    want = K.kv_cache_append(q, k, v, None, None, cos, sin, at, at, caches[0])
+    odd = [torch.zeros(t, x.shape[1], d + 1, dtype=BF, device=gpu) for x in (q, k, v)]
+    for x, y in zip(odd, (q, k, v)):
+        x[..., 1:] = y
+    wide = [torch.cat((x, x), 1)[:, :d] for x in (cos, sin)]
+    got = K.kv_cache_append(*(x[..., 1:] for x in odd), None, None, *wide, at, at, caches[1])
+    assert torch.equal(got, want) and all(torch.equal(x[:, :, :t], y[:, :, :t]) for x, y in zip(caches[0][:2], caches[1][:2]))
+
+
+def test_checked_positions_and_slots(gpu, monkeypatch):
+    monkeypatch.setenv("PITHTRAIN_AMD_CHECK_POSITIONS", "1")
+    z = lambda *s: torch.zeros(*s, dtype=BF, device=gpu)  # noqa: E731
+    cos, sin = (x.to(gpu) for x in _tables(64))
+    cache = K.KVCache.empty(2, 1, 64, 16, device=gpu)
+    call = lambda pos, slots: K.kv_cache_append(z(2, 1, 64), z(2, 1, 64), z(2, 1, 64), None, None, cos, sin, torch.tensor(pos, device=gpu), torch.tensor(slots, device=gpu), cache)  # noqa: E731
+    call([0, 49], [-1, 31])
+    with pytest.raises(AssertionError, match="positions"):
+        call([0, 50], [0, 1])
+    with pytest.raises(AssertionError, match="the cache holds 32 rows"):
+        call([0, 1], [0, 32])
+    with pytest.raises(AssertionError, match="same slot"):
+        call([0, 1], [5, 5])
+
+
+# ---------------------------------------------------------------------------------------------
+# Bounds and selection
+
+
+@BOTH
+@pytest.mark.parametrize("heads", [(8, 2, 128), (3, 3, 64)], ids=str)
+@pytest.mark.parametrize("page", [16, 64, 256])
+def test_bounds_of_the_pages_that_a_step_fills(gpu, page, heads, fp8):
+    counts, lengths = [1, 1, 1, 3 * page, 5, 0, 2 * page + 1], [page, page + 1, 3 * page, 3 * page, 2 * page + 2, 2 * page, 4 * page]
+    b = Batch(gpu, counts, lengths, heads, page=page, fp8=fp8, seed=page)
+    bounds = torch.full_like(b.cache.empty_bounds(), 3.0)
+    K.kv_page_bounds(b.cache, bounds, b.table, b.lens, b.cu_q, sum(counts))
+    filled = torch.zeros(len(bounds), dtype=torch.bool)
+    for i, (n, length) in enumerate(zip(counts, lengths)):
+        for j in range((length - n) // page, length // page):
+            if (j + 1) * page > length - n:
+                p = int(b.table[i, j])
+                filled[p] = True
+                k = b.kv[0][p].float() if b.scales[0] is None else b.kv[0][p].float() * b.scales[0][p][..., None]
+                assert torch.equal(bounds[p].cpu(), torch.stack((k.amin(1), k.amax(1)), 1).to(BF).cpu()), (i, j)
+    assert 5 <= filled.sum() < len(bounds) and (bounds[~filled.to(gpu)] == 3).all()
+    if not fp8:
+        p = int(b.table[0, 0])
+        b.kv[0][p, 0, 3, 5], b.kv[0][p, 0, 4, 6] = math.nan, math.inf
+        K.kv_page_bounds(b.cache, bounds, b.table, b.lens, b.cu_q, sum(counts))
+        assert torch.isnan(bounds[p, 0, :, 5]).all() and bounds[p, 0, 1, 6] == math.inf and torch.isfinite(bounds[p, 0, 0, 6])
+
+
+def _selection(gpu, lengths, heads, keep, counts=None, page=16, seed=0, bounds=None, extra=0):
+    counts = counts or [1] * len(lengths)
+    b = Batch(gpu, counts, [1] * len(lengths), heads, page=page, seed=seed, extra_tokens=extra)
+    g = torch.Generator().manual_seed(seed + 1)
+    width, (h, hkv, d) = max(-(-n // page) for n in lengths) + 2, heads
+    pages = len(lengths) * width
+    table = torch.randperm(pages, generator=g).to(I32).view(len(lengths), width)
+    if bounds is None:
+        x = torch.randn(pages, hkv, 2, d, generator=g)
+        bounds = torch.stack((x.amin(2), x.amax(2)), 2).to(BF)
+    lens = torch.tensor(lengths, dtype=I32, device=gpu)
+    cu_q = None if all(n == 1 for n in counts) and not extra else b.cu_q
+    chosen, rows = K.kv_select_pages(b.q, bounds.to(gpu), table.to(gpu), lens, cu_q, page, keep)
+    chosen, rows, t = chosen.cpu(), rows.cpu(), 0
+    for i, (n, length) in enumerate(zip(counts, lengths)):
+        for k in range(n):
+            visible = max(length - n + k + 1, 0)
+            want = O.select(b.q[t].cpu(), bounds[table[i].long()], visible, page, keep)
+            for j in range(hkv):
+                assert chosen[t, j].tolist() == table[i][want[j]].tolist() + [-1] * (keep - len(want[j])), (t, j)
+                assert int(rows[t, j]) == visible - (-(-visible // page) - len(want[j])) * page
+            t += 1
+    assert (chosen[t:] == -1).all() and (rows[t:] == 0).all()
+
+
+@pytest.mark.parametrize("keep", [1, 2, 5, 64, 300])
+@pytest.mark.parametrize("heads", [(8, 2, 128), (3, 3, 64), (32, 2, 64), (5, 1, 128)], ids=str)
+def test_selected_pages_are_the_oracles(gpu, heads, keep):
+    _selection(gpu, [1, 16, 17, 16 * 66, 16 * 200 + 3, 0], heads, keep, seed=keep)
+
+
+def test_selection_for_drafts_and_padding(gpu):
+    _selection(gpu, [300, 33, 4, 600], (4, 2, 64), 4, counts=[3, 20, 6, 1], seed=5, extra=3)
+
+
+def test_selection_from_more_pages_than_stay_in_lds(gpu):
+    _selection(gpu, [16 * 9001 + 5, 16 * 8193], (2, 1, 64), 77, seed=6)
+
+
+def test_equal_scores_go_to_the_pages_that_come_first(gpu):
+    g = torch.Generator().manual_seed(7)
+    bounds = torch.randint(0, 2, (102, 2, 2, 64), generator=g).to(BF)  # few different scores
+    bounds[:, 1] = 0.5
+    _selection(gpu, [16 * 100], (4, 2, 64), 30, seed=8, bounds=bounds)
+
+
+def test_scores_that_are_no_numbers(gpu):
+    g = torch.Generator().manual_seed(9)
+    x = torch.randn(102, 1, 2, 64, generator=g)
+    bounds = torch.stack((x.amin(2), x.amax(2)), 2).to(BF)
+    bounds[::7, 0, :, 3] = math.nan
+    bounds[1::7, 0, 1, 3] = math.inf
+    bounds[2::7, 0, 0, 4] = -math.inf
+    _selection(gpu, [16 * 100 - 1], (3, 1, 64), 60, seed=10, bounds=bounds)
+
+
+def test_sparse_attention_of_all_pages_is_the_dense_call(gpu):
+    b = Batch(gpu, [1, 1, 2], [200, 90, 333], page=16, seed=15)
+    bounds = b.cache.empty_bounds().zero_()
+    selected = K.kv_select_pages(b.q, bounds, b.table, b.lens, b.cu_q, 16, 30)
+    b.check(*K.kv_attention(b.q, b.cache, *selected, None, b.scale))
+
+
+# ---------------------------------------------------------------------------------------------
+# Planning
+
+
+def _plan_case(gpu, counts, lengths, page, tokens, spare, width, seed=0, into=False):
+    g = torch.Generator().manual_seed(seed)
+    held = [-(-n // page) for n in lengths]
+    pages = sum(held) + spare
+    order = torch.randperm(pages, generator=g).tolist()
+    table, at = [], 0
+    for n in held:
+        table.append(order[at : at + n] + [-9] * (width - n))
+        at += n
+    free = order[at:] + [-1] * sum(held)
+    want = O.plan(counts, lengths, table, free, spare, page, tokens)
+    i32 = lambda x: torch.tensor(x, dtype=I32, device=gpu)  # noqa: E731
+    wide = torch.full((len(counts), width + 3), -4, dtype=I32, device=gpu)
+    wide[:, 1 : 1 + width] = torch.tensor(table, dtype=I32).view(len(counts), width)
+    tab, pool = wide[:, 1 : 1 + width], paging.PagePool(i32(free), i32([spare]))
+    c, n = i32(counts), i32(lengths)
+    if into:
+        mk = lambda k, d=I32: torch.full((k,), 77, dtype=d, device=gpu)  # noqa: E731
+        plan = paging.StepPlan(mk(len(counts) + 1), n, mk(tokens, I64), mk(tokens, I64), mk(len(counts)), pool.count)
+        paging.plan_step_into(c, n, tab, pool, page, plan)
+    else:
+        plan = paging.plan_step(c, n, tab, pool, page, tokens)
+        assert n.tolist() == lengths and pool.count.tolist() == [spare]
+    for name, got in {**plan._asdict(), "page_table": tab, "free": pool.free}.items():
+        assert got.tolist() == want[name], name
+    assert (wide[:, 0] == -4).all() and (wide[:, 1 + width :] == -4).all()
+    return want
+
+
+@pytest.mark.parametrize("into", [False, True])
+@pytest.mark.parametrize("b", [1, 5, 64, 300, 1500])
+@pytest.mark.parametrize("scarce", [False, True])
+def test_plans_are_the_oracles(gpu, b, scarce, into):
+    g = torch.Generator().manual_seed(b)
+    rand = lambda lo, hi, n=1: torch.randint(lo, hi, (n,), generator=g).tolist()  # noqa: E731
+    for page, most in ((16, 40), (64, 3)):
+        lengths, counts = rand(0, 150, b), rand(-1, most, b)
+        need = sum(-(-(n + max(c, 0)) // page) + (-n // page) for n, c in zip(lengths, counts))
+        tokens = sum(max(c, 0) for c in counts) + 5
+        want = _plan_case(gpu, counts, lengths, page, tokens, need // 3 if scarce else need + 2, 200 // page + 2, seed=b, into=into)
+        assert scarce or all(x == max(c, 0) for x, c in zip(want["granted"], counts))
+
+
+def test_plans_of_long_prompts(gpu):
+    """Tokens in a launch of their own; a table that is too narrow; fewer tokens than the counts say; nothing at all."""
+    _plan_case(gpu, [9000, 0, 3000, 7], [5, 70, 16, 64], 16, 12007, 800, 700, seed=1)
+    _plan_case(gpu, [9000, 0, 3000, 7], [5, 70, 16, 64], 16, 12007, 560, 700, seed=1, into=True)
+    want = _plan_case(gpu, [40, 17, 3], [5, 0, 16], 16, 60, 50, 2, seed=2)
+    assert want["granted"] == [0, 17, 3]
+    _plan_case(gpu, [20, 30, 4], [1, 2, 3], 16, 33, 50, 8, seed=3)
+    _plan_case(gpu, [0, 0], [3, 0], 16, 0, 1, 1)
+    _plan_case(gpu, [-1, -1, 33], [32, 31, 0], 16, 33, 0, 3)
+    plan = paging.plan_step(*(torch.empty(0, dtype=I32, device=gpu) for _ in range(2)), torch.empty(0, 4, dtype=I32, device=gpu), paging.PagePool.full(3, gpu), 16, 2)
+    assert plan.cu_q.tolist() == [0] and plan.slots.tolist() == [-1, -1] and plan.free_count.tolist() == [3]
+
+
+def test_nonsense_in_a_plan_stays_in_memory(gpu):
+    i32 = lambda x: torch.tensor(x, dtype=I32, device=gpu)  # noqa: E731
+    big = 2**31 - 1
+    for count in (-5, big):
+        for lengths, counts in (([big, -big, 3], [1, 2, 3]), ([big, big, big], [-1, -7, big]), ([5, 5, 5], [big, big, big])):
+            table, free = torch.full((3, 4), big, dtype=I32, device=gpu), torch.full((6,), -big, dtype=I32, device=gpu)
+            plan = paging.plan_step(i32(counts), i32(lengths), table, paging.PagePool(free, i32([count])), 16, 9)
+            assert 0 <= int(plan.free_count) <= 6 and int(plan.cu_q[-1]) <= 9
+            paging.plan_step(i32(counts), i32(lengths), table, paging.PagePool(free, i32([count])), 16, 20000)
+    torch.cuda.synchronize()
+
+
+# ---------------------------------------------------------------------------------------------
+# Together
+
+
+def _answer(gpu, fp8, keep, captured=False):
+    """Requests come, are answered and end, planned on the device; every token's result against dense attention to the rows that the caches hold."""
+    h, hkv, d, page, pages, b, width = 8, 2, 128, 16, 40, 3, 12
+    g = torch.Generator().manual_seed(30)
+    cache = K.KVCache.empty(pages, hkv, d, page, L.FP8 if fp8 else BF, gpu)
+    for x in cache:
+        if x is not None:
+            x.view(torch.uint8).fill_(0x7F)  # NaN
+    bounds = cache.empty_bounds().fill_(math.nan)
+    pool = paging.PagePool.full(pages, gpu)
+    table, lengths = torch.full((b, width), -1, dtype=I32, device=gpu), torch.zeros(b, dtype=I32, device=gpu)
+    cos, sin = (x.to(gpu) for x in _tables(d, 300))
+    w = [(1 + 0.2 * torch.randn(d, generator=g)).to(BF).to(gpu) for _ in range(2)]
+    history = [torch.empty(0, 0)] * b
+    scale = d**-0.5
+    steps = [[70, 33, 0], [1, 1, 20], [1, 1, 1], [1, -1, 1], [1, 90, 1], [3, 1, 1]] + [[1, 1, 1]] * 18
+    tokens = 110
+    mk = lambda n, t=I32: torch.zeros(n, dtype=t, device=gpu)  # noqa: E731
+    plan = paging.StepPlan(mk(b + 1), lengths, mk(tokens, I64), mk(tokens, I64), mk(b), pool.count)
+    counts = mk(b)
+    qkv = torch.zeros(tokens, h + 2 * hkv, d, dtype=BF, device=gpu)
+
+    def step():
+        paging.plan_step_into(counts, lengths, table, pool, page, plan)
+        return K.kv_decode(*qkv.split((h, hkv, hkv), 1), *w, cos, sin, plan.position_ids, plan.slots, cache, table, lengths, plan.cu_q, scale, bounds=bounds, keep=keep)
+
+    graph, out = None, None
+    used = 0
+    for n, new in enumerate(steps):
+        counts.copy_(torch.tensor(new, dtype=I32))
+        qkv.copy_(torch.randn(tokens, h + 2 * hkv, d, generator=g).to(BF))
+        if not captured:
+            out = step()
+        elif graph is None:
+            graph = torch.cuda.CUDAGraph()
+            side = torch.cuda.Stream()
+            side.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.graph(graph, stream=side):
+                out = step()
+            graph.replay()
+        else:
+            graph.replay()
+        torch.cuda.synchronize()
+        used += 1
+        want_lengths = [0 if c < 0 else history[i].shape[1] + c if history[i].numel() else c for i, c in enumerate(new)]
+        assert lengths.tolist() == want_lengths and plan.granted.tolist() == [max(c, 0) for c in new]
+        q = O.norm_rope(qkv[:, :h].cpu(), w[0].cpu(), cos.cpu(), sin.cpu(), plan.position_ids.cpu(), 1e-6)[0]
+        first = 0
+        for i, c in enumerate(new):
+            length = want_lengths[i]
+            rows = []
+            j = torch.arange(length, device=gpu)
+            p, r = table[i, j // page].long(), j % page
+            for x, s in ((cache.k, cache.k_scale), (cache.v, cache.v_scale)):
+                y = x.to(torch.float32)[p, :, r].double()
+                rows.append((y if s is None else y * s[p, :, r].double()[..., None]).transpose(0, 1).cpu())
+            if history[i].numel() and c >= 0:
+                assert torch.equal(rows[0][:, : history[i].shape[1]], history[i]), "rows of earlier steps have changed"
+            history[i] = rows[0] if length else torch.empty(0, 0)
+            for k in range(max(c, 0)):
+                seen = O.sees(c, length)[k : k + 1].expand(1, length).clone()
+                visible = length - c + k + 1
+                if keep is not None:
+                    of_pages = torch.stack([torch.stack((rows[0][:, m * page : (m + 1) * page].amin(1), rows[0][:, m * page : (m + 1) * page].amax(1)), 1) for m in range(-(-visible // page))])
+                    # (queries are those of the oracle, not the rounded ones: pages whose scores lie closer together than that may go either way)
+                    kept = O.select(q[first + k].to(BF), of_pages.to(BF), visible, page, keep)
+                for head in range(hkv):
+                    mine, mask = slice(head * (h // hkv), (head + 1) * (h // hkv)), seen.clone()
+                    if keep is not None:
+                        mask &= torch.tensor([m // page in kept[head] for m in range(length)])
+                    want, _, mass, spread = O.attention(q[first + k : first + k + 1, mine], rows[0][head : head + 1], rows[1][head : head + 1], mask, scale)
+                    # q is rounded to bf16 on the way: its score is off by u sum |q k| more
+                    e = ((d + 8) * 2.0**-24 + U) * spread
+                    _within(out[first + k : first + k + 1, mine], want, U * want.abs() + (U + 2 * (e[..., None] * math.log(2) + 2.0**-16)) * mass, f"step {n} request {i} token {k} head {head}")
+            first += max(c, 0)
+    return used
+
+
+@BOTH
+def test_requests_that_come_and_go(gpu, fp8):
+    assert _answer(gpu, fp8, None) == 24
+
+
+def test_requests_that_come_and_go_over_all_their_pages(gpu):
+    assert _answer(gpu, False, 12) == 24
+
+
+def test_a_captured_step_follows_its_requests(gpu):
+    assert _answer(gpu, False, None, captured=True) == 24
+
+
+def test_the_latent_cache_takes_the_same_plan(gpu):
+    """Slots, positions and lengths of a plan in the MLA layer's step: the rows go where the tables say."""
+    g = torch.Generator().manual_seed(31)
+    page, b = 16, 2
+    cache = L.LatentCache.empty(9, page, device=gpu)
+    pool, table = paging.PagePool.full(9, gpu), torch.full((b, 5), -1, dtype=I32, device=gpu)
+    lengths = torch.zeros(b, dtype=I32, device=gpu)
+    cos, sin = (x.to(gpu) for x in _tables(64, 100))
+    w = torch.ones(512, dtype=BF, device=gpu)
+    rows = [torch.empty(0, 512)] * b
+    for counts in ([20, 3], [1, 1], [-1, 1], [30, 15]):
+        c = torch.tensor(counts, dtype=I32, device=gpu)
+        n = sum(max(x, 0) for x in counts)
+        plan = paging.plan_step(c, lengths, table, pool, page, n + 1)
+        lengths, pool = plan.lengths, paging.PagePool(pool.free, plan.free_count)
+        kv_a = torch.randn(n + 1, 576, generator=g).to(BF).to(gpu)
+        L.latent_cache_append(kv_a, w, cos, sin, plan.position_ids, plan.slots, cache)
+        first = 0
+        normed = torch.nn.functional.rms_norm(kv_a[:, :512].double().cpu(), (512,), eps=1e-6)
+        for i, x in enumerate(counts):
+            rows[i] = torch.empty(0, 512) if x < 0 else torch.cat((rows[i], normed[first : first + x]))
+            first += max(x, 0)
+        cu_rows = torch.cat((torch.zeros(1, dtype=I32, device=gpu), lengths.cumsum(0).to(I32)))
+        got, _ = L.latent_cache_gather(cache, table, cu_rows, int(cu_rows[-1]))
+        want = torch.cat(rows)
+        _within(got, want, U * want.abs() + 2.0**-19 * want.abs(), f"{counts}")
+
+
+def test_on_another_stream(gpu):
+    b = Batch(gpu, [1, 1], [3000, 700], seed=16)
+    want = b.attention()
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        got = [b.attention() for _ in range(5)]
+        plan = paging.plan_step(torch.ones(2, dtype=I32, device=gpu), b.lens, b.table.clone(), paging.PagePool.full(3, gpu), 64, 2)
+    s.synchronize()
+    assert all(torch.equal(x, y) for one in got for x, y in zip(one, want)) and plan.cu_q.tolist() == [0, 1, 2]
+
+
+def test_a_captured_call_follows_lengths_and_tables(gpu):
+    b = Batch(gpu, [1, 2, 1], [40, 300, 1000], seed=17, page=16)
+    want = b.attention()  # (the first call of a kind is not in the graph)
+    graph = torch.cuda.CUDAGraph()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.graph(graph, stream=side):
+        got = b.attention()
+    for lengths in ([40, 300, 1000], [1, 2, 999], [33, 290, 16], [40, 300, 1000]):
+        b.lens.copy_(torch.tensor(lengths, dtype=I32))
+        graph.replay()
+        torch.cuda.synchronize()
+        b.lengths = lengths
+        b.check(*got, str(lengths))
+        assert all(torch.equal(x, y) for x, y in zip(got, b.attention()))
+    assert all(torch.equal(x, y) for x, y in zip(got, want))
+
+
+def test_what_an_operator_writes_counts_as_changed(gpu):
+    b = Batch(gpu, [1], [64], (4, 2, 64), seed=18)
+    bounds, cos = b.cache.empty_bounds(), torch.ones(80, 64, dtype=BF, device=gpu)
+    one = torch.zeros(1, dtype=I64, device=gpu)
+    versions = [x._version for x in (b.kv[0], b.kv[1], bounds, b.table)]
+    K.kv_cache_append(b.q, b.q[:, :2], b.q[:, :2], None, None, cos, cos, one, one, b.cache)
+    K.kv_page_bounds(b.cache, bounds, b.table, b.lens, b.cu_q, 1)
+    paging.plan_step(torch.ones(1, dtype=I32, device=gpu), b.lens, b.table, paging.PagePool.full(3, gpu), 64, 1)
+    assert all(x._version > v for x, v in zip((b.kv[0], b.kv[1], bounds, b.table), versions))
+
+
+def test_empty_calls(gpu):
+    b = Batch(gpu, [1], [64], (4, 2, 64), seed=19)
+    none = lambda *s, d=BF: torch.empty(*s, dtype=d, device=gpu)  # noqa: E731
+    o, lse = K.kv_attention(b.q[:0], b.cache, b.table, b.lens, torch.zeros(2, dtype=I32, device=gpu), b.scale)
+    assert o.shape == (0, 4, 64) and lse.shape == (4, 0)
+    K.kv_attention(b.q[:0], b.cache, b.table[:0], b.lens[:0], None, b.scale)
+    assert K.kv_cache_append(b.q[:0], b.q[:0, :2], b.q[:0, :2], None, None, none(4, 64), none(4, 64), none(0, d=I64), none(0, d=I64), b.cache).shape == (0, 4, 64)
+    selected = K.kv_select_pages(b.q, b.cache.empty_bounds(), b.table[:0], b.lens[:0], torch.zeros(1, dtype=I32, device=gpu), 64, 3)
+    assert (selected.page_table == -1).all() and (selected.lengths == 0).all()
