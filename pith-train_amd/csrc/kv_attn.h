@@ -1,0 +1,724 @@
+// Attention of new tokens to the rows of a key-value cache: the work list, the kernel, and what its join needs.
+//
+//   S = kappa Q K^T,  O = softmax(S) V        for the query heads that share a key-value head
+//
+// Work list. The query rows of a sequence and key-value head (row = token * group + head of the group, n tokens: n * group rows) are cut into row blocks of
+// M = 16, 32 or 64 rows, each of which goes through all of the sequence's keys in steps of 128; the steps of all row blocks, one behind the other, are dealt
+// to the workgroups in equal ranges. Lengths are read on the device, so nothing depends on the host knowing them: a captured call follows its sequences as
+// they grow, and one long sequence among short ones is spread over as many workgroups as its share of the steps. Where there are fewer row blocks than
+// workgroups, ranges may be a little longer and each lie in one row block (to begin one costs queries, a first tile and a part). An XCD's workgroups take
+// ranges that follow one another, so that row blocks of one head find each other's keys in its cache.
+// Where page tables are so short that no row block is worth cutting, every workgroup takes one, whole, and there is nothing to join.
+// A workgroup whose range covers a row block wholly writes its rows; parts leave (reference, sum, unnormalised result) in fp32 in the workspace, and a second
+// kernel joins them in the order of the keys (results do not depend on scheduling). So how a row's keys are cut, its references and the order of its sums
+// follow from the lengths of all sequences of the call; nothing else of one row reaches another.
+//
+// The kernel. Memory bounds it: a key row and a value row of 512 bytes (bf16, 128 features) stand against 4 * 128 flop for each of the group's rows. So
+// the four wavefronts of a workgroup (one a SIMD: 512 registers each) walk alone, each through every fourth tile of 32 keys, with no barrier until the
+// segment ends: a wave brings its tiles global -> LDS by direct loads into a ring of its own (32 KB of keys and values in flight a wave, 128 KB a compute
+// unit) and waits with counted waits for its own requests only, for the keys while the values are still under way. Products are 16x16x32 with the query
+// row as the result's column, so a lane owns one row, and the scores of a lane are its part of operand B of the second product as they stand: key 4 g + v
+// of either half tile is contracted at place 8 g + v or 8 g + 4 + v, and the values are read (transposed, from LDS) in that order. No weight moves between lanes.
+// The waves' results of a segment are joined through LDS.
+// A fragment that was read serves all 16-row groups of the block: 64 rows cost a tile's reads once. With M = 64 the products are 1024 of a tile's cycles, and
+// the tile still comes more slowly than that from memory.
+// The weights go into the second product as bf16, which is what the matrix cores take beside a cache of bf16 (or e4m3, widened exactly): half a step, 2^-8, of
+// each, while their sum is of the unrounded ones. With e4m3 a weight is rounded once, when its row's scale is in it.
+#pragma once
+
+#include "cache_attn.h"
+#include "kv_common.h"
+
+namespace pith {
+
+constexpr int kKVThreads = 256, kKVWaves = 4;
+constexpr int kTileKeys = 32, kStepKeys = kKVWaves * kTileKeys;
+
+// What the join needs of a row block: first of its rows within the sequence and head, first token and head of that, its rows, and the slots of its parts, the
+// first and, of the workgroups behind that one, the last (equal: nothing to join).
+struct KVJoin {
+  int row0, tok0, head, rows, first, last;
+};
+
+struct KVAttnParams {
+  const __bf16* q;
+  KVCache cache;
+  const int32_t *table, *lengths, *cu_q;
+  const int64_t* tree;
+  __bf16* o;
+  float* lse;
+  int64_t table_rs, table_hs, q_ts, q_hs, o_ts, o_hs, lse_hs;
+  int T, B, H, group, table_width;
+  int head_tables;  // key-value heads with tables of their own, or 1: tables of all
+  int max_len;      // table_width * page_size
+  float kappa;      // scale * log2(e)
+  int whole;        // steps of the longest row block where none is cut, else 0
+  // workspace (not used where none is cut)
+  int* items;        // number of row blocks of this call
+  KVJoin* joins;     // [row blocks]
+  float2* stats;     // [slots][M] reference (in bits) and sum
+  float* parts;      // [slots][M][D]; slot 2 i: workgroup i's part that begins with its range, 2 i + 1: one that begins later
+  int max_items;     // capacity of joins
+};
+
+// A sequence, or a sequence's key-value head where these have tables of their own.
+struct KVWork {
+  int tok0, n, len;   // first token, new tokens, cached rows
+  int blocks, steps;  // row blocks of all its heads, steps of each
+};
+
+template <int M>
+__device__ __forceinline__ KVWork kv_work(const KVAttnParams& p, int c0, int c1, int length) {
+  KVWork s;
+  s.tok0 = c0;
+  s.n = c1 - c0;
+  s.len = min(max(length, 0), p.max_len);
+  s.blocks = (s.n * p.group + M - 1) / M * (p.cache.heads / p.head_tables);
+  s.steps = max((s.len + kStepKeys - 1) / kStepKeys, 1);  // rows without keys get their zeros from an empty step
+  return s;
+}
+// Token offsets are taken as their maximum so far, so that whatever they hold no token belongs to two sequences, and the work list is no longer than the
+// host has made sure of.
+__device__ __forceinline__ int kv_offset(const KVAttnParams& p, int b) { return p.cu_q ? min(max(p.cu_q[b], 0), p.T) : b; }
+
+// Sums and maxima over the workgroup. `turn` says which half of `shared` is used: one barrier a call is enough if it alternates.
+struct BlockScan {
+  int (*shared)[kKVWaves];  // [2]
+  int turn;
+  __device__ __forceinline__ int sum(int x, int& total) {  // inclusive
+    const int mine = wave_scan(x), wave = threadIdx.x >> 6;
+    if ((threadIdx.x & 63) == 63) shared[turn][wave] = mine;
+    __syncthreads();
+    int before = 0;
+    total = 0;
+#pragma unroll
+    for (int w = 0; w < kKVWaves; ++w) {
+      const int s = shared[turn][w];
+      before += w < wave ? s : 0;
+      total += s;
+    }
+    turn ^= 1;
+    return before + mine;
+  }
+  __device__ __forceinline__ int most_before(int x, int& all) {  // maxima of values from 0 on, of the threads in front
+    const int mine = wave_scan_max(x), wave = threadIdx.x >> 6;
+    if ((threadIdx.x & 63) == 63) shared[turn][wave] = mine;
+    __syncthreads();
+    int before = (threadIdx.x & 63) == 0 ? 0 : __builtin_amdgcn_update_dpp(0, mine, 0x138, 0xf, 0xf, false);  // from the lane below
+    all = 0;
+#pragma unroll
+    for (int w = 0; w < kKVWaves; ++w) {
+      const int s = shared[turn][w];
+      before = w < wave ? max(before, s) : before;
+      all = max(all, s);
+    }
+    turn ^= 1;
+    return before;
+  }
+};
+
+// Where a range begins.
+struct KVStart {
+  KVWork s;
+  int seq, item, block, step, found;  // sequence, row blocks in front of it, row block and step in it
+};
+
+// A workgroup's way through its range of the work list, segment by segment (steps of one row block); all of it is uniform.
+template <int M>
+struct KVWalk {
+  static constexpr int kEach = 4;                      // sequences of a thread
+  static constexpr int kAtOnce = kEach * kKVThreads;   // of a workgroup
+  static constexpr int kStart = 2, kLeast = 1;
+  int range, per, begin, at, end;  // this workgroup's range, its length, begin, place, end
+  int seq, item, block, step;
+  bool single;  // one segment a range
+  KVWork s;
+
+  __device__ __forceinline__ int taken(int steps) const { return single && per > 1 ? (steps + per - 1) / per * per : steps; }  // steps that a row block is taken for
+
+  // Sequences s0 + kEach * thread .. of all.
+  __device__ __forceinline__ void load(const KVAttnParams& p, int s0, BlockScan& scan, int& behind, KVWork (&x)[kEach]) const {
+    const int count = p.B * p.head_tables, i0 = s0 + kEach * threadIdx.x;
+    int c0[kEach], c1[kEach], length[kEach];
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) {
+      const bool some = i0 + e < count;
+      const int b = some ? (p.head_tables == 1 ? i0 + e : (i0 + e) / p.head_tables) : 0;
+      c0[e] = some ? kv_offset(p, b) : 0;
+      c1[e] = some ? kv_offset(p, b + 1) : 0;
+      length[e] = some ? p.lengths[i0 + e] : 0;
+    }
+    if (p.cu_q) {
+      int upto = 0, all;
+#pragma unroll
+      for (int e = 0; e < kEach; ++e) upto = max(upto, c0[e]);
+      upto = max(scan.most_before(upto, all), behind);
+      behind = max(behind, all);
+#pragma unroll
+      for (int e = 0; e < kEach; ++e) {
+        upto = max(upto, c0[e]);
+        c0[e] = upto;
+        c1[e] = max(c1[e], upto);
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) x[e] = kv_work<M>(p, c0[e], i0 + e < count ? c1[e] : c0[e], length[e]);
+  }
+
+  // False: nothing to do.
+  __device__ __forceinline__ bool start(const KVAttnParams& p, int (*shared)[kKVWaves], KVStart* found) {
+    BlockScan scan = {shared, 0};
+    const int count = p.B * p.head_tables, groups = gridDim.x;
+    KVWork x[kEach];
+    int behind = 0, total = 0, blocks_total = 0, sum;
+    single = false;
+    per = p.whole;
+    if (threadIdx.x == 0) found->found = 0;
+    const auto work = [&]() __attribute__((always_inline)) {
+      int w = 0;
+#pragma unroll
+      for (int e = 0; e < kEach; ++e) w += x[e].blocks * taken(x[e].steps);
+      return w;
+    };
+    const auto blocks = [&]() __attribute__((always_inline)) {
+      int k = 0;
+#pragma unroll
+      for (int e = 0; e < kEach; ++e) k += x[e].blocks;
+      return k;
+    };
+    if (p.whole) {
+      single = true;
+      load(p, 0, scan, behind, x);
+    } else {
+      for (int s0 = 0; s0 < count; s0 += kAtOnce) {
+        load(p, s0, scan, behind, x);
+        scan.sum(work(), sum);
+        total += sum;
+        scan.sum(blocks(), sum);
+        blocks_total += sum;
+      }
+      // (named as global memory: with a store to anywhere behind it, all waits for LDS in the kernel would be waits for everything)
+      if (blockIdx.x == 0 && threadIdx.x == 0) *(__attribute__((address_space(1))) int*)(uintptr_t)p.items = min(blocks_total, p.max_items);
+      per = total <= groups ? 1 : __builtin_amdgcn_readfirstlane((total + groups - 1) / groups);  // (divisions leave the scalar registers)
+      if (blocks_total < groups && count <= kAtOnce && total < 1 << 30) {  // (more sequences are not looked up twice)
+        const int most = per + kStart;
+        int longer = max(per, kLeast);
+        for (int ranges; longer <= most; longer = max(longer + 1, __builtin_amdgcn_readfirstlane((int)(longer * ((float)ranges / groups))))) {
+          int k = 0;
+#pragma unroll
+          for (int e = 0; e < kEach; ++e) k += x[e].blocks * (longer > 1 ? (x[e].steps + longer - 1) / longer : x[e].steps);
+          scan.sum(k, ranges);
+          ranges = __builtin_amdgcn_readfirstlane(ranges);
+          if (ranges <= groups) {
+            per = longer;
+            single = true;
+            break;
+          }
+        }
+      }
+    }
+    range = (blockIdx.x & 7) * (groups >> 3) + (blockIdx.x >> 3);  // an XCD's workgroups (every eighth) take ranges that follow one another
+    begin = at = range * per;
+    end = at + per;  // (the host has bounded total + gridDim.x)
+    int before = 0, blocks_before = 0;  // in front of these sequences
+    behind = 0;
+    for (int s0 = 0; s0 < count; s0 += kAtOnce) {
+      if (count > kAtOnce) load(p, s0, scan, behind, x);
+      int w = work(), k = blocks(), sum_w, sum_k;
+      int upto = scan.sum(w, sum_w) + before;
+      int item0 = scan.sum(k, sum_k) + blocks_before - k;
+      if (upto > at && upto - w <= at) {  // one thread of all
+        int first = upto - w;
+#pragma unroll
+        for (int e = 0; e < kEach; ++e) {
+          const int each = taken(x[e].steps), mine = x[e].blocks * each;
+          if (first <= at && at < first + mine) {
+            const int block = (at - first) / each;
+            *found = KVStart{x[e], s0 + kEach * (int)threadIdx.x + e, item0, block, at - first - block * each, 1};
+          }
+          first += mine;
+          item0 += x[e].blocks;
+        }
+      }
+      before += sum_w;
+      blocks_before += sum_k;
+      if (before > at) break;  // (uniform)
+    }
+    __syncthreads();
+    const auto uniform = [](int v) { return __builtin_amdgcn_readfirstlane(v); };
+    if (!uniform(found->found)) return false;
+    s.tok0 = uniform(found->s.tok0), s.n = uniform(found->s.n), s.len = uniform(found->s.len), s.blocks = uniform(found->s.blocks), s.steps = uniform(found->s.steps);
+    seq = uniform(found->seq), item = uniform(found->item), block = uniform(found->block), step = uniform(found->step);
+    if (!single) end = min(end, total);
+    return true;
+  }
+  __device__ __forceinline__ int n_steps() const { return min(s.steps - step, end - at); }
+  __device__ __forceinline__ int blocks_of_head(const KVAttnParams& p) const { return p.head_tables == 1 ? s.blocks / p.cache.heads : s.blocks; }
+  __device__ __forceinline__ bool whole() const { return n_steps() == s.steps; }
+  __device__ __forceinline__ int slot() const { return 2 * range + (at == begin ? 0 : 1); }
+  // Who ends a row block says how it was cut.
+  __device__ __forceinline__ void leave_join(const KVAttnParams& p, int row0, int head, int rows) const {
+    if (p.whole || step + n_steps() != s.steps || threadIdx.x != 0 || item + block >= p.max_items) return;
+    int first = 0, last = 0;
+    if (!whole()) {
+      const int from = at - step;  // of the row block in the work list
+      const int id = from / per;
+      first = 2 * id + (from == id * per ? 0 : 1);
+      last = 2 * range;
+    }
+    p.joins[item + block] = KVJoin{row0, s.tok0, head, rows, first, last};
+  }
+  // On to the next segment. False: the range is done.
+  __device__ __forceinline__ bool next(const KVAttnParams& p) {
+    at += n_steps();
+    if (single || at >= end) return false;
+    step = 0;
+    if (++block == s.blocks) {
+      block = 0;
+      item += s.blocks;
+      do {
+        ++seq;
+        const int b = p.head_tables == 1 ? seq : seq / p.head_tables;
+        const bool same = p.head_tables > 1 && seq % p.head_tables != 0;  // another head of the same tokens
+        const int c0 = same ? s.tok0 : s.tok0 + s.n;
+        s = kv_work<M>(p, c0, same ? c0 + s.n : max(kv_offset(p, b + 1), c0), p.lengths[seq]);
+      } while (s.blocks == 0);
+    }
+    return true;
+  }
+};
+
+// ---------------------------------------------------------------------------------------------
+// Tiles
+
+// 32 rows of keys or of values, packed: rows of 256, 128 or 64 bytes lie 1, 2 or 4 to an LDS line of 256. Piece (16 bytes) q of row r lies at q ^ swizzle(r) of
+// its row. LDS serves 256 bytes a cycle, and a wavefront's 16-byte reads as lanes 0-3 12-15 20-27, then 4-11 16-19 28-31, and the upper half alike, 8-byte
+// reads by halves. The fragment reads of keys (lane c + 16 g: row c, piece q + g) then have rows {0-3, 12-15} at piece q and {4-11} at q + 1, and the
+// transposed reads of values rows 0-7 (bf16; two pieces each) or 0-7 and 16-23 (e4m3; one piece each): no two on one bank in either.
+template <int ROW>
+__device__ __forceinline__ constexpr int kv_swizzle(int r) {
+  return ROW == 256 ? 2 * (r & 7) : ROW == 128 ? 2 * ((r >> 1) & 3) | ((r >> 4) & 1) : 2 * ((r >> 2) & 1) | ((r >> 4) & 1);
+}
+
+template <int D, bool FP8>
+struct KVTile {
+  static constexpr int kRow = FP8 ? D : 2 * D;                // bytes
+  static constexpr int kBytes = kTileKeys * kRow;             // of keys, and of values
+  static constexpr int kLoads = kBytes / 1024;                // instructions of a wave, for either
+  static constexpr int kScaleLoads = FP8 ? 1 : 0;             // 32 scales of keys and 32 of values
+  static constexpr int kScaleBytes = FP8 ? 256 : 0;
+  static constexpr int kSlot = 2 * kBytes + kScaleBytes;
+  static constexpr int kSlots = FP8 || D == 64 ? 4 : 2;       // tiles of a wave in flight
+  static constexpr int kRing = kSlots * kSlot;
+  static constexpr int kAll = kScaleLoads + 2 * kLoads;       // requests of a tile
+
+  // Place in the source, within 16 rows, of what lane `lane` brings in instruction 0; that of instruction n is ^ (source_xor(n)) and 1024 n behind.
+  static __device__ __forceinline__ int source(int lane) {
+    constexpr int kPieces = kRow / 16, kRows = 256 / kRow;  // of a row, of a line
+    const int row = kRows * (lane >> 4) + (lane & 15) / kPieces, piece = (lane & 15) % kPieces;
+    return row * kRow + ((piece ^ kv_swizzle<kRow>(row)) << 4);
+  }
+  static __device__ __forceinline__ constexpr int source_xor(int n) { return kRow == 256 ? 128 * (n & 1) : kRow == 128 ? 16 * (n >> 1) : 16 * n; }
+  // Place in a tile of piece q of row r (< 32).
+  static __device__ __forceinline__ int place(int r, int q) { return r * kRow + ((q ^ kv_swizzle<kRow>(r)) << 4); }
+};
+
+// A wave's requests for the 32 rows from key on (a multiple of 32): two times sixteen rows, each of one page. Rows behind the sequence's last one come as the
+// page holds them, or the last sixteen again: nobody sees them, and clean_values takes out what is not finite.
+template <int D, bool FP8>
+struct KVLoads {
+  using T = KVTile<D, FP8>;
+  int64_t page[2];
+  int in_page[2];
+  __device__ __forceinline__ KVLoads(const KVAttnParams& p, const int (&page_)[2], int key, int last, int head) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      page[h] = safe_page(__builtin_amdgcn_readfirstlane(page_[h]), p.cache.pages);
+      in_page[h] = (head << p.cache.page_shift) + (min(key + 16 * h, last) & ((1 << p.cache.page_shift) - 16));
+    }
+  }
+  __device__ __forceinline__ void rows(const char* base, int64_t page_bytes, char* dst, int source) const {
+#pragma unroll
+    for (int n = 0; n < T::kLoads; ++n) {
+      constexpr int kPerHalf = T::kLoads / 2;
+      const int h = n / kPerHalf, i = n % kPerHalf;
+      const char* const from = base + page[h] * page_bytes + (int64_t)in_page[h] * T::kRow;
+      const int at = source ^ T::source_xor(n);
+      if (i == 0) load_lds16(from, at, dst + n * 1024);
+      else if (i == 1) load_lds16_next<1024>(from, at);
+      else if (i == 2) load_lds16_next<2 * 1024>(from, at);
+      else load_lds16_next<3 * 1024>(from, at);
+    }
+  }
+  __device__ __forceinline__ void keys(const KVAttnParams& p, char* slot, int source, int lane) const {
+    if constexpr (FP8) {  // scales: lanes 0-31 of the keys, 32-63 of the values
+      const int h = (lane >> 4) & 1;
+      const float* const from = lane < 32 ? p.cache.k_scale + (h ? page[1] * p.cache.k_scale_ps + in_page[1] : page[0] * p.cache.k_scale_ps + in_page[0])
+                                          : p.cache.v_scale + (h ? page[1] * p.cache.v_scale_ps + in_page[1] : page[0] * p.cache.v_scale_ps + in_page[0]);
+      load_lds4(from + (lane & 15), slot + 2 * T::kBytes);
+    }
+    rows(p.cache.k, p.cache.k_ps, slot, source);
+  }
+  __device__ __forceinline__ void values(const KVAttnParams& p, char* slot, int source) const { rows(p.cache.v, p.cache.v_ps, slot + T::kBytes, source); }
+};
+
+// Until all but the last `later` tiles' requests and EXTRA more are there.
+template <int D, bool FP8, int EXTRA>
+__device__ __forceinline__ void wait_tiles(int later) {
+  constexpr int kAll = KVTile<D, FP8>::kAll;
+  if (later >= 3) wait_loads<KVTile<D, FP8>::kSlots == 4 ? 3 * kAll + EXTRA : 0>();
+  else if (later == 2) wait_loads<KVTile<D, FP8>::kSlots == 4 ? 2 * kAll + EXTRA : 0>();
+  else if (later == 1) wait_loads<kAll + EXTRA>();
+  else wait_loads<EXTRA>();
+}
+
+// Operand A over 32 keys, features 16 n ..; `first`: lds_address of the values + the lane's place. Element 4 h + v: key 16 h + 4 g + v.
+template <int D, bool FP8>
+__device__ __forceinline__ int kv_value_place(int c, int g) {
+  if constexpr (FP8) {
+    const int r = (c >> 3) * 16 + 4 * g + ((c >> 1) & 3);  // eight columns of a row a lane; rows 4-7 of a read are those of the upper half
+    return KVTile<D, FP8>::place(r, 0) + 8 * (c & 1);
+  } else {
+    return KVTile<D, FP8>::place(4 * g + (c >> 2), (c >> 1) & 1) + 8 * (c & 1);  // four columns of a row a lane
+  }
+}
+template <int D, bool FP8>
+__device__ __forceinline__ bf16x8 kv_value_fragment(uint32_t first, int n) {
+  if constexpr (FP8) {
+    typedef __attribute__((ext_vector_type(2))) int i32x2;
+    typedef __attribute__((address_space(3))) i32x2 lds_i32x2;
+    const i32x2 raw = __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_i32x2*)(uintptr_t)(first ^ (16 * n)));
+    return widen((uint32_t)raw[0], (uint32_t)raw[1]);
+  } else {
+    typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+    constexpr int kUpper = KVTile<D, FP8>::kRow == 128 ? 16 : 0;  // the swizzle of row 16 + r differs in that
+    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(uintptr_t)(first ^ (32 * n)));
+    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(uintptr_t)((first ^ (32 * n) ^ kUpper) + 16 * KVTile<D, FP8>::kRow));
+    typedef __attribute__((ext_vector_type(8))) short s16x8;
+    return __builtin_bit_cast(bf16x8, s16x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]});
+  }
+}
+
+// Key of element e of a lane's eight, within the tile.
+__device__ __forceinline__ int key_of(int g, int e) { return 16 * (e >> 2) + 4 * g + (e & 3); }
+
+// Which of a lane's eight keys from key0 on a row of token tok sees: bit e. In the last tiles of a sequence only, so what a token sees is looked up anew there.
+__device__ __forceinline__ uint32_t seen_keys(const KVAttnParams& p, const KVWork& s, int tok, int key0, int g) {
+  uint32_t lo = 0, hi = 0;
+  if (p.tree) {
+    const uint64_t word = (uint64_t)p.tree[s.tok0 + tok];
+    lo = (uint32_t)word;
+    hi = (uint32_t)(word >> 32);
+  }
+  const int ctx = s.len - s.n;  // rows in front of the new ones (below zero only where the lengths contradict each other)
+  uint32_t seen = 0;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const int key = key0 + key_of(g, e), draft = key - ctx;
+    const uint32_t bits = draft < 32 ? lo : hi;
+    const int by_word = (draft < 0) | ((draft < 64) & (int)((bits >> (draft & 31)) & 1u));
+    const int ok = (p.tree ? by_word : (int)(draft <= tok)) & (int)(key < s.len);
+    seen |= (uint32_t)ok << e;
+  }
+  return seen;
+}
+
+__device__ __forceinline__ bool finite_pair(uint32_t x) { return (x & 0x7f80u) != 0x7f80u && (x & 0x7f800000u) != 0x7f800000u; }
+
+// Values that are not finite, in a tile that some rows see in part only: a row's weight of a key it does not see is 0, and must stay so against whatever the
+// key's value holds. Rows that do see such a value get it here, by a plain sum; then it is 0 in LDS. Rare, and as slow as it likes to be.
+// weight[r]: of the lane's eight keys, seen[r]: bits of them.
+template <int D, bool FP8, int R>
+__device__ __forceinline__ void clean_values(char* values, int lane, const bf16x8 (&weight)[R], const uint32_t (&seen)[R], f32x4 (&acc)[R][D / 16]) {
+  using T = KVTile<D, FP8>;
+  const auto bad_word = [](uint32_t x) {
+    if constexpr (FP8) return (x & 0x7fu) == 0x7fu || (x & 0x7f00u) == 0x7f00u || (x & 0x7f0000u) == 0x7f0000u || (x & 0x7f000000u) == 0x7f000000u;
+    else return !finite_pair(x);
+  };
+  bool bad = false;
+#pragma unroll
+  for (int i = 0; i < T::kBytes / 1024; ++i) {
+    const u32x4 x = *reinterpret_cast<const u32x4*>(values + 16 * lane + 1024 * i);
+    bad = bad || bad_word(x[0]) || bad_word(x[1]) || bad_word(x[2]) || bad_word(x[3]);
+  }
+  if (!__any(bad)) return;
+  const int c = lane & 15, g = lane >> 4;
+#pragma unroll 1
+  for (int j = 0; j < kTileKeys; ++j) {
+    const int owner = c + 16 * ((j >> 2) & 3), e = 4 * (j >> 4) + (j & 3);  // lane and element that hold key j of this lane's row
+    float w[R];
+    bool sees[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      float mine = 0.f;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) mine = k == e ? (float)weight[r][k] : mine;
+      w[r] = __shfl(mine, owner);
+      sees[r] = (__shfl((int)seen[r], owner) >> e) & 1;
+    }
+#pragma unroll
+    for (int n = 0; n < D / 16; ++n) {  // features 16 n + 4 g + v
+#pragma unroll
+      for (int v = 0; v < 4; ++v) {
+        const int d = 16 * n + 4 * g + v;
+        float x;
+        if constexpr (FP8) {
+          const uint32_t byte = *reinterpret_cast<const uint8_t*>(values + T::place(j, d >> 4) + (d & 15));
+          x = (byte & 0x7f) == 0x7f ? NAN : 0.f;
+        } else {
+          const uint32_t half = *reinterpret_cast<const uint16_t*>(values + T::place(j, d >> 3) + 2 * (d & 7));
+          x = (half & 0x7f80u) == 0x7f80u ? bf16_bits_to_f32(half) : 0.f;
+        }
+        const bool not_finite = x != 0.f;
+#pragma unroll
+        for (int r = 0; r < R; ++r) acc[r][n][v] = not_finite && sees[r] ? acc[r][n][v] + w[r] * x : acc[r][n][v];
+      }
+    }
+  }
+#pragma unroll 1
+  for (int i = 0; i < T::kBytes / 1024; ++i) {
+    u32x4* const at = reinterpret_cast<u32x4*>(values + 16 * lane + 1024 * i);
+    u32x4 x = *at;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      if constexpr (FP8) {
+#pragma unroll
+        for (int b = 0; b < 32; b += 8)
+          if (((x[k] >> b) & 0x7fu) == 0x7fu) x[k] &= ~(0xffu << b);
+      } else {
+        if ((x[k] & 0x7f80u) == 0x7f80u) x[k] &= 0xffff0000u;
+        if ((x[k] & 0x7f800000u) == 0x7f800000u) x[k] &= 0xffffu;
+      }
+    }
+    *at = x;
+  }
+}
+
+// ---------------------------------------------------------------------------------------------
+
+template <int D, bool FP8, int R>
+__global__ __launch_bounds__(kKVThreads, 1) void kv_attn_kernel(KVAttnParams p) {
+  using T = KVTile<D, FP8>;
+  using Loads = KVLoads<D, FP8>;
+  constexpr int M = 16 * R, kSteps = D / 32;  // of the score's contraction
+  constexpr int kRegion = T::kRing > M * D * 4 ? T::kRing : M * D * 4;  // of a wave: its tiles, then its results
+  __shared__ __attribute__((aligned(1024))) char lds[kKVWaves * kRegion];
+  __shared__ float2 wave_stats[kKVWaves][M];
+  __shared__ int scan[2][kKVWaves];
+  __shared__ KVStart found;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int c = lane & 15, g = lane >> 4;
+  KVWalk<M> walk;
+  if (!walk.start(p, scan, &found)) return;
+  char* const ring = lds + wave * kRegion;
+  const int source = T::source(lane);
+  const int key_at = T::place(c, g);  // of keys 0-15; 16-31 differ by this:
+  constexpr int kUpperKey = 16 * T::kRow, kUpperXor = T::kRow == 256 ? 0 : 16;
+  const int value_at = T::kBytes + kv_value_place<D, FP8>(c, g);
+
+  do {
+    const KVWork& s = walk.s;
+    const int per_head = walk.blocks_of_head(p);
+    const int head = p.head_tables == 1 ? __builtin_amdgcn_readfirstlane(walk.block / per_head) : walk.seq % p.head_tables;
+    const int row0 = (p.head_tables == 1 ? walk.block - head * per_head : walk.block) * M;  // within the sequence and head
+    const int rows = min(s.n * p.group - row0, M);
+    const ScalarTable table = (ScalarTable)(uintptr_t)(p.table + (p.head_tables == 1 ? walk.seq : walk.seq / p.head_tables) * p.table_rs + head * p.table_hs);
+    const int last = max(s.len - 1, 0);
+    const int tile0 = walk.step * kKVWaves + wave;  // this wave's first
+    const int tiles = min((s.len + kTileKeys - 1) / kTileKeys, (walk.step + walk.n_steps()) * kKVWaves);
+    const int n_tiles = tiles > tile0 ? (tiles - tile0 + kKVWaves - 1) / kKVWaves : 0;
+
+    bf16x8 q[R][kSteps];
+    int tok[R];
+    f32x4 acc[R][D / 16];
+    float m[R], l[R];  // reference and sum (this lane's keys) of a row
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const int row = row0 + min(16 * r + c, rows - 1);
+      tok[r] = row / p.group;
+      const __bf16* const from = p.q + (int64_t)(s.tok0 + tok[r]) * p.q_ts + (int64_t)(head * p.group + row - tok[r] * p.group) * p.q_hs;
+#pragma unroll
+      for (int i = 0; i < kSteps; ++i)  // e4m3 keys are read 16 features at a time: steps 2 i, 2 i + 1 contract features 64 i + 16 g + {0..7, 8..15}
+        q[r][i] = *reinterpret_cast<const bf16x8*>(from + (FP8 ? 64 * (i >> 1) + 16 * g + 8 * (i & 1) : 32 * i + 8 * g));
+#pragma unroll
+      for (int n = 0; n < D / 16; ++n) acc[r][n] = f32x4{};
+      m[r] = -INFINITY;
+      l[r] = 0.f;
+    }
+
+    const auto key_of_tile = [&](int i) { return (tile0 + i * kKVWaves) * kTileKeys; };
+    int pages[2];
+    const auto look_up = [&](int i) __attribute__((always_inline)) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) pages[h] = table[min(key_of_tile(i) + 16 * h, last) >> p.cache.page_shift];
+    };
+#pragma unroll 1
+    for (int i = 0; i < min(T::kSlots, n_tiles); ++i) {
+      look_up(i);
+      const Loads loads(p, pages, key_of_tile(i), last, head);
+      loads.keys(p, ring + i * T::kSlot, source, lane);
+      loads.values(p, ring + i * T::kSlot, source);
+    }
+    look_up(T::kSlots);
+    int slot_at = 0;
+#pragma unroll 1
+    for (int i = 0; i < n_tiles; ++i) {
+      char* const slot = ring + slot_at;
+      const int key0 = key_of_tile(i);
+      const int later = min(T::kSlots - 1, n_tiles - 1 - i);
+      const bool more = i + T::kSlots < n_tiles;
+      wait_tiles<D, FP8, T::kLoads>(later);  // the keys
+      f32x4 score[R][2];
+      float k_scale[8], v_scale[8];
+      {
+        const uint32_t first = lds_address(slot) + key_at;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const uint32_t row = h == 0 ? first : (first ^ kUpperXor) + kUpperKey;
+#pragma unroll
+          for (int r = 0; r < R; ++r) score[r][h] = f32x4{};
+#pragma unroll
+          for (int j = 0; j < (FP8 ? kSteps / 2 : kSteps); ++j) {
+            if constexpr (FP8) {
+              const u32x4 raw = *lds_at<u32x4>(row ^ (64 * j));
+              const bf16x8 k0 = widen(raw[0], raw[1]), k1 = widen(raw[2], raw[3]);
+#pragma unroll
+              for (int r = 0; r < R; ++r) score[r][h] = mfma16(k1, q[r][2 * j + 1], mfma16(k0, q[r][2 * j], score[r][h]));
+            } else {
+              const bf16x8 k = *lds_at<bf16x8>(row ^ (64 * j));
+#pragma unroll
+              for (int r = 0; r < R; ++r) score[r][h] = mfma16(k, q[r][j], score[r][h]);
+            }
+          }
+          if constexpr (FP8) {
+            const f32x4 a = *reinterpret_cast<const f32x4*>(slot + 2 * T::kBytes + 4 * (16 * h + 4 * g));
+            const f32x4 b = *reinterpret_cast<const f32x4*>(slot + 2 * T::kBytes + 128 + 4 * (16 * h + 4 * g));
+#pragma unroll
+            for (int v = 0; v < 4; ++v) k_scale[4 * h + v] = a[v] * p.kappa, v_scale[4 * h + v] = b[v];
+          }
+        }
+      }
+      const bool partial = key0 + kTileKeys > s.len - s.n + (p.tree ? 0 : 1);  // some row may not see all of it
+      bf16x8 weight[R];
+      uint32_t seen[R];
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        float y[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) y[e] = score[r][e >> 2][e & 3] * (FP8 ? k_scale[e] : p.kappa);
+        if (partial) {
+          seen[r] = seen_keys(p, s, tok[r], key0, g);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) y[e] = (seen[r] >> e) & 1 ? y[e] : -INFINITY;
+        }
+        float top = y[0];
+#pragma unroll
+        for (int e = 1; e < 8; ++e) top = fmaxf(top, y[e]);
+        if (__any(top > m[r] + kSlack)) {
+          const float moved_to = moved(m[r], quad_max(top));
+          const float alpha = moved_to == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m[r] - moved_to);
+          l[r] *= alpha;
+#pragma unroll
+          for (int n = 0; n < D / 16; ++n) scale_in_place(acc[r][n], alpha);
+          m[r] = moved_to;
+        }
+        const float ref = m[r] == -INFINITY ? 0.f : m[r];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          y[e] = __builtin_amdgcn_exp2f(y[e] - ref);
+          l[r] += y[e];
+        }
+        if constexpr (FP8) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) y[e] = scaled(y[e], v_scale[e]);
+        }
+        weight[r] = to_bf16x8(y[0], y[1], y[2], y[3], y[4], y[5], y[6], y[7]);
+      }
+      const Loads loads(p, pages, key_of_tile(i + T::kSlots), last, head);
+      if (more) {  // (the keys have been read: their products have been used)
+        loads.keys(p, slot, source, lane);
+        look_up(i + T::kSlots + 1);
+        wait_loads<(T::kSlots - 1) * T::kAll + T::kScaleLoads + T::kLoads>();
+      } else {
+        wait_tiles<D, FP8, 0>(later);  // the values
+      }
+      if (partial) clean_values<D, FP8, R>(slot + T::kBytes, lane, weight, seen, acc);
+      const uint32_t values = lds_address(slot) + value_at;
+#pragma unroll
+      for (int n = 0; n < D / 16; ++n) {
+        const bf16x8 v = kv_value_fragment<D, FP8>(values, n);
+#pragma unroll
+        for (int r = 0; r < R; ++r) acc[r][n] = mfma16(v, weight[r], acc[r][n]);
+      }
+      if (more) {
+        __builtin_amdgcn_s_waitcnt(0xC07F);  // the values have been read
+        asm volatile("" ::: "memory");
+        loads.values(p, slot, source);
+      }
+      slot_at = slot_at + T::kSlot == T::kRing ? 0 : slot_at + T::kSlot;
+    }
+
+    // The waves' results of the segment, joined through LDS: a wave's rows lie in its own region, piece (four features) q of row r at q ^ (r % 16).
+    constexpr int kRowPieces = D / 4;
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      l[r] = quad_sum(l[r]);
+      if (g == 0) wave_stats[wave][16 * r + c] = make_float2(m[r], l[r]);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      float top = -INFINITY;
+#pragma unroll
+      for (int w = 0; w < kKVWaves; ++w) top = fmaxf(top, wave_stats[w][16 * r + c].x);
+      const float f = __builtin_amdgcn_exp2f(m[r] - (top == -INFINITY ? 0.f : top));
+#pragma unroll
+      for (int n = 0; n < D / 16; ++n) *reinterpret_cast<f32x4*>(ring + ((16 * r + c) * kRowPieces + ((4 * n + g) ^ c)) * 16) = acc[r][n] * f;
+    }
+    __syncthreads();
+    const bool whole = walk.whole();
+    const int64_t slot = walk.slot();
+    for (int i = threadIdx.x; i < rows * kRowPieces; i += kKVThreads) {
+      const int row = i / kRowPieces, piece = i % kRowPieces;
+      float top = -INFINITY, sum = 0.f;
+      float2 st[kKVWaves];
+#pragma unroll
+      for (int w = 0; w < kKVWaves; ++w) st[w] = wave_stats[w][row], top = fmaxf(top, st[w].x);
+      const float ref = top == -INFINITY ? 0.f : top;
+      f32x4 x = {};
+#pragma unroll
+      for (int w = 0; w < kKVWaves; ++w) {
+        x += *reinterpret_cast<const f32x4*>(lds + w * kRegion + (row * kRowPieces + (piece ^ (row & 15))) * 16);
+        sum += st[w].y * __builtin_amdgcn_exp2f(st[w].x - ref);  // (a wave that saw nothing: 0; one that saw NaN only: NaN)
+      }
+      if (whole) {
+        const int tok = (row0 + row) / p.group, h = head * p.group + row0 + row - tok * p.group;
+        const int64_t t = s.tok0 + tok;
+        const f32x4 o = sum == 0.f ? f32x4{} : x * (1.f / sum);
+        *reinterpret_cast<u32x2*>(p.o + t * p.o_ts + h * p.o_hs + 4 * piece) = u32x2{pack_bf16x2(o[0], o[1]), pack_bf16x2(o[2], o[3])};
+        if (piece == 0) p.lse[h * p.lse_hs + t] = sum == 0.f ? -INFINITY : ref + __builtin_amdgcn_logf(sum);
+      } else {
+        *reinterpret_cast<f32x4*>(p.parts + (slot * M + row) * D + 4 * piece) = x;
+        if (piece == 0) p.stats[slot * M + row] = make_float2(top, sum);
+      }
+    }
+    walk.leave_join(p, row0, head, rows);
+    __syncthreads();  // the rings are free
+  } while (walk.next(p));
+}
+
+template <int D>
+void launch_kv_attn(const KVAttnParams& p, bool fp8, int row_groups, int workgroups, hipStream_t s) {
+  const auto launch = [&](auto f) {
+    constexpr bool F = decltype(f)::value;
+    if (row_groups == 1) kv_attn_kernel<D, F, 1><<<workgroups, kKVThreads, 0, s>>>(p);
+    else if (row_groups == 2) kv_attn_kernel<D, F, 2><<<workgroups, kKVThreads, 0, s>>>(p);
+    else kv_attn_kernel<D, F, 4><<<workgroups, kKVThreads, 0, s>>>(p);
+  };
+  if (fp8) launch(std::true_type());
+  else launch(std::false_type());
+}
+void launch_kv_attn_d128(const KVAttnParams& p, bool fp8, int row_groups, int workgroups, hipStream_t s);  // kv_attn.hip
+void launch_kv_attn_d64(const KVAttnParams& p, bool fp8, int row_groups, int workgroups, hipStream_t s);   // kv_attn_d64.hip
+
+}  // namespace pith

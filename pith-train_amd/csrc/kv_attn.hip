@@ -1,69 +1,125 @@
-// Attention of new tokens to the rows of a key-value cache (include/pith_kv.h).
-#include "kv_common.h"
+// Attention of new tokens to the rows of a key-value cache: heads of 128 features, the join, the plan of a call (see kv_attn.h; heads of 64: kv_attn_d64.hip).
+#include "kv_attn.h"
+
+#include <algorithm>
+#include <type_traits>
 
 namespace pith {
+
+void launch_kv_attn_d128(const KVAttnParams& p, bool fp8, int row_groups, int workgroups, hipStream_t s) { launch_kv_attn<128>(p, fp8, row_groups, workgroups, s); }
+
 namespace {
 
-struct KVAttnParams {
-  const __bf16* q;
-  KVCache cache;
-  const int32_t *table, *lengths, *cu_q;
-  const int64_t* tree;
-  __bf16* o;
-  float* lse;
-  int64_t table_rs, table_hs, q_ts, q_hs, o_ts, o_hs, lse_hs;
-  int T, B, H, group, table_width, head_tables;
-  float kappa;  // scale * log2(e)
-};
+constexpr int kJoinThreads = 512, kJoinRows = 4;
+constexpr int kMaxGroups = 512;  // workgroups of the attention kernel, at most, where row blocks are cut: kMaxGroups + 1 parts of one
 
-// A wave for every token and query head, a key after the other.
-template <int D, bool FP8>
-__global__ __launch_bounds__(64) void kv_attn_kernel(KVAttnParams p) {
-  const int lane = threadIdx.x, t = blockIdx.x, h = blockIdx.y, head = h / p.group;
-  int seq = t, first = t, n = 1;
-  if (p.cu_q) {  // offsets count as their maximum so far
-    int most = min(max(p.cu_q[0], 0), p.T);
-    for (seq = 0; seq < p.B; ++seq) {
-      first = most;
-      most = max(most, min(max(p.cu_q[seq + 1], 0), p.T));
-      if (t >= first && t < most) break;
+// Joins the parts of a row block: o = sum_i w_i O_i / sum_i w_i l_i, w_i = 2^(m_i - max m). blockIdx.x: row block, blockIdx.y: four rows of it. A wave forms
+// the weights of a row; then groups of threads, a piece of four features each, take every so many-th part and meet in LDS.
+template <int D>
+__global__ __launch_bounds__(kJoinThreads) void kv_join_kernel(KVAttnParams p, int m) {
+  constexpr int kPieces = D / 4, kEach = kJoinRows * kPieces, kGroups = kJoinThreads / kEach;
+  __shared__ f32x4 sums[kJoinThreads];
+  __shared__ float weights[kJoinRows][kMaxGroups + 1];
+  __shared__ float inverse[kJoinRows];  // of the rows' sums (0: nothing seen)
+  const int row0 = kJoinRows * blockIdx.y;
+  const int items = *p.items;
+  const KVJoin join = p.joins[blockIdx.x];  // (beyond `items` it is whatever the workspace held)
+  if ((int)blockIdx.x >= items || join.first == join.last || row0 >= join.rows) return;
+  const int n = min(join.last / 2 - join.first / 2 + 1, kMaxGroups + 1);  // parts: the first slot, then the even ones up to the last
+  const auto slot = [&](int i) { return (int64_t)(i == 0 ? join.first : 2 * (join.first / 2 + i)); };
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int group = threadIdx.x / kEach, row = threadIdx.x % kEach / kPieces, piece = threadIdx.x % kPieces;
+  const auto part = [&](int i) { return *reinterpret_cast<const f32x4*>(p.parts + (slot(i) * m + row0 + row) * D + 4 * piece); };
+  f32x4 x[4];  // the first ones are on their way while the weights are formed (those behind the last one: that one, not used)
+#pragma unroll
+  for (int k = 0; k < 4; ++k) x[k] = part(min(group + k * kGroups, n - 1));
+  const auto place = [&](int r, int& h, int64_t& t) {  // of a row of the row block
+    const int at = join.row0 + r, tok = at / p.group;
+    h = join.head * p.group + at - tok * p.group;
+    t = join.tok0 + tok;
+  };
+  if (wave < kJoinRows) {
+    const auto stat = [&](int i) { return p.stats[slot(i) * m + row0 + wave]; };
+    float top = -INFINITY, sum = 0.f;
+    for (int i = lane; i < n; i += 64) top = fmaxf(top, stat(i).x);
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) top = fmaxf(top, __shfl_xor(top, d));
+    const float ref = top == -INFINITY ? 0.f : top;
+    for (int i = lane; i < n; i += 64) {
+      const float2 s = stat(i);
+      const float w = __builtin_amdgcn_exp2f(s.x - ref);
+      weights[wave][i] = w;
+      sum += w * s.y;
     }
-    if (seq == p.B) return;
-    n = most - first;
-  }
-  const int length = min(max(p.lengths[p.head_tables ? seq * p.cache.heads + head : seq], 0), p.table_width << p.cache.page_shift);
-  const int32_t* const table = p.table + seq * p.table_rs + head * p.table_hs;
-  const uint64_t word = p.tree ? (uint64_t)p.tree[t] : 0;
-  constexpr int E = D / 64;
-  float q[E], o[E] = {}, m = -INFINITY, l = 0.f;
-  for (int e = 0; e < E; ++e) q[e] = (float)p.q[t * p.q_ts + h * p.q_hs + E * lane + e];
-  for (int j = 0; j < length; ++j) {
-    const int draft = j - (length - n);
-    const bool seen = p.tree ? draft < 0 || (draft < 64 && ((word >> (draft & 63)) & 1)) : draft <= t - first;
-    if (!seen) continue;
-    const int64_t page = safe_page(table[j >> p.cache.page_shift], p.cache.pages);
-    const int64_t row = ((int64_t)head << p.cache.page_shift) + (j & ((1 << p.cache.page_shift) - 1));
-    float k[E], v[E];
-    for (int e = 0; e < E; ++e) {
-      if constexpr (FP8) {
-        k[e] = (float)fp8x2_to_bf16<false>((uint8_t)p.cache.k[page * p.cache.k_ps + row * D + E * lane + e])[0] * p.cache.k_scale[page * p.cache.k_scale_ps + row];
-        v[e] = (float)fp8x2_to_bf16<false>((uint8_t)p.cache.v[page * p.cache.v_ps + row * D + E * lane + e])[0] * p.cache.v_scale[page * p.cache.v_scale_ps + row];
-      } else {
-        k[e] = (float)reinterpret_cast<const __bf16*>(p.cache.k + page * p.cache.k_ps)[row * D + E * lane + e];
-        v[e] = (float)reinterpret_cast<const __bf16*>(p.cache.v + page * p.cache.v_ps)[row * D + E * lane + e];
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) sum += __shfl_xor(sum, d);
+    if (lane == 0) {
+      inverse[wave] = sum == 0.f ? 0.f : 1.f / sum;
+      if (row0 + wave < join.rows) {
+        int h;
+        int64_t t;
+        place(row0 + wave, h, t);
+        p.lse[h * p.lse_hs + t] = sum == 0.f ? -INFINITY : ref + __builtin_amdgcn_logf(sum);
       }
     }
-    float s = 0.f;
-    for (int e = 0; e < E; ++e) s += q[e] * k[e];
-    for (int d = 1; d < 64; d <<= 1) s += __shfl_xor(s, d);
-    s *= p.kappa;
-    const float top = fmaxf(m, s), ref = top == -INFINITY ? 0.f : top, alpha = __builtin_amdgcn_exp2f(m - ref), w = __builtin_amdgcn_exp2f(s - ref);
-    l = l * alpha + w;
-    for (int e = 0; e < E; ++e) o[e] = o[e] * alpha + w * v[e];
-    m = top;
   }
-  for (int e = 0; e < E; ++e) p.o[t * p.o_ts + h * p.o_hs + E * lane + e] = (__bf16)(l == 0.f ? 0.f : o[e] / l);
-  if (lane == 0) p.lse[h * p.lse_hs + t] = l == 0.f ? -INFINITY : m + __builtin_amdgcn_logf(l);
+  __syncthreads();
+  f32x4 o = {};
+#pragma unroll
+  for (int k = 0; k < 4; ++k)
+    if (group + k * kGroups < n) o += x[k] * weights[row][group + k * kGroups];
+  int i = group + 4 * kGroups;
+  for (; i + 3 * kGroups < n; i += 4 * kGroups) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) x[k] = part(i + k * kGroups);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) o += x[k] * weights[row][i + k * kGroups];
+  }
+  for (; i < n; i += kGroups) o += part(i) * weights[row][i];
+  sums[threadIdx.x] = o;
+  __syncthreads();
+  if (group > 0 || row0 + row >= join.rows) return;
+#pragma unroll
+  for (int k = 1; k < kGroups; ++k) o += sums[k * kEach + threadIdx.x];
+  o = inverse[row] == 0.f ? f32x4{} : o * inverse[row];
+  int h;
+  int64_t t;
+  place(row0 + row, h, t);
+  *reinterpret_cast<u32x2*>(p.o + t * p.o_ts + h * p.o_hs + 4 * piece) = u32x2{pack_bf16x2(o[0], o[1]), pack_bf16x2(o[2], o[3])};
+}
+
+struct KVPlan {
+  int row_groups;  // of 16 query rows, to a row block
+  int workgroups;  // a multiple of 8
+  int whole;       // steps of the longest row block where none is cut, else 0
+  int64_t max_items;
+  int64_t joins_at, stats_at, parts_at, bytes;  // workspace
+};
+
+constexpr int64_t kWholeSteps = 4;
+
+KVPlan plan_of(const pith_kv_attn_args* a) {
+  KVPlan pl = {};
+  const int64_t rows = a->T * (a->H / a->cache.heads);  // of a key-value head
+  pl.row_groups = rows <= 16 * a->B ? 1 : rows <= 32 * a->B ? 2 : 4;
+  const int64_t m = 16 * pl.row_groups;
+  pl.max_items = ((rows + m - 1) / m + std::min(a->B, a->T)) * a->cache.heads;
+  const int64_t steps = (a->table_width * a->cache.page_size + kStepKeys - 1) / kStepKeys;
+  if (steps <= kWholeSteps) {
+    pl.whole = (int)steps;
+    pl.workgroups = (int)((pl.max_items + 7) & ~(int64_t)7);
+    pl.bytes = 256;
+    return pl;
+  }
+  const int units = compute_units_or_default() & ~7;
+  pl.workgroups = units < 8 ? 8 : units > kMaxGroups ? kMaxGroups : units;
+  const auto up = [](int64_t x) { return (x + 255) & ~(int64_t)255; };
+  const int64_t slot_rows = 2 * pl.workgroups * m;
+  pl.joins_at = 256;
+  pl.stats_at = pl.joins_at + up(pl.max_items * (int64_t)sizeof(KVJoin));
+  pl.parts_at = pl.stats_at + up(slot_rows * (int64_t)sizeof(float2));
+  pl.bytes = pl.parts_at + slot_rows * a->cache.dim * 4;
+  return pl;
 }
 
 int check_attn(const pith_kv_attn_args* a, const char* who) {
@@ -72,6 +128,10 @@ int check_attn(const pith_kv_attn_args* a, const char* who) {
   if (const int rc = check_table(a->T, a->B, a->cache.heads, a->table_width, a->cache.page_size, !a->cu_q, who)) return rc;
   if (a->H < 1 || a->H > 1024 || a->H % a->cache.heads)
     return fail(PITH_ERR_BAD_SHAPE, "%s: %lld query heads (at most 1024) of %lld key-value heads", who, (long long)a->H, (long long)a->cache.heads);
+  // counted in 32 bits on the device: row blocks, and the steps of the whole work list
+  const int64_t items = ((a->T * (a->H / a->cache.heads) + 15) / 16 + a->B) * a->cache.heads;
+  if (items > 1 << 24 || a->B * a->cache.heads > 1 << 24 || items * (a->table_width * a->cache.page_size / kStepKeys + 1) > 0x7fffffff - (1 << 25))
+    return fail(PITH_ERR_UNSUPPORTED, "%s: too many row blocks for page tables of that width: call it with fewer tokens at a time", who);
   if (a->head_tables && a->tree_mask) return fail(PITH_ERR_UNSUPPORTED, "%s: tables of the heads go with causal attention", who);
   return PITH_OK;
 }
@@ -83,7 +143,7 @@ using namespace pith;
 
 extern "C" int64_t pith_kv_attn_workspace_bytes(const pith_kv_attn_args* a) {
   if (check_attn(a, "pith_kv_attn_workspace_bytes") != PITH_OK || a->T == 0 || a->B == 0) return 0;
-  return 256;
+  return plan_of(a).bytes;
 }
 
 extern "C" int pith_kv_attn(const pith_kv_attn_args* a, pith_stream_t stream) {
@@ -100,22 +160,33 @@ extern "C" int pith_kv_attn(const pith_kv_attn_args* a, pith_stream_t stream) {
   if (!aligned16(a->q) || !aligned16(a->o) || (a->q_ts | a->q_hs | a->o_ts | a->o_hs) % 8 || (uintptr_t)a->workspace % 256 || (uintptr_t)a->page_table % 4 ||
       (uintptr_t)a->lengths % 4 || (uintptr_t)a->cu_q % 4 || (uintptr_t)a->lse % 4 || (uintptr_t)a->tree_mask % 8)
     return fail(PITH_ERR_MISALIGNED, "%s: queries and results need 16-byte alignment and strides of multiples of 8, the workspace 256-byte alignment", who);
-  const int64_t need = pith_kv_attn_workspace_bytes(a);
-  if (a->workspace_bytes < need) return fail(PITH_ERR_BAD_SHAPE, "%s: the workspace has %lld bytes, %lld are needed", who, (long long)a->workspace_bytes, (long long)need);
+  const KVPlan pl = plan_of(a);
+  if (a->workspace_bytes < pl.bytes) return fail(PITH_ERR_BAD_SHAPE, "%s: the workspace has %lld bytes, %lld are needed", who, (long long)a->workspace_bytes, (long long)pl.bytes);
   KVAttnParams p = {};
   p.q = (const __bf16*)a->q; p.cache = to_device(a->cache); p.table = a->page_table; p.lengths = a->lengths; p.cu_q = a->cu_q; p.tree = a->tree_mask;
   p.o = (__bf16*)a->o; p.lse = a->lse;
   p.table_rs = a->B > 1 ? a->table_rs : 0; p.table_hs = a->head_tables && heads > 1 ? a->table_hs : 0;
   p.q_ts = a->q_ts; p.q_hs = a->q_hs; p.o_ts = a->o_ts; p.o_hs = a->o_hs; p.lse_hs = a->lse_hs;
-  p.T = (int)a->T; p.B = (int)a->B; p.H = (int)a->H; p.group = (int)(a->H / heads); p.table_width = (int)a->table_width; p.head_tables = a->head_tables != 0;
+  p.T = (int)a->T; p.B = (int)a->B; p.H = (int)a->H; p.group = (int)(a->H / heads); p.table_width = (int)a->table_width;
+  p.head_tables = a->head_tables ? (int)heads : 1;
+  p.max_len = (int)(a->table_width * a->cache.page_size);
   p.kappa = a->scale * 1.4426950408889634f;
+  p.whole = pl.whole;
+  char* const ws = (char*)a->workspace;
+  p.items = (int*)ws;
+  p.joins = (KVJoin*)(ws + pl.joins_at);
+  p.stats = (float2*)(ws + pl.stats_at);
+  p.parts = (float*)(ws + pl.parts_at);
+  p.max_items = (int)pl.max_items;
   hipStream_t s = (hipStream_t)stream;
-  const dim3 grid((unsigned)a->T, (unsigned)a->H);
-  begin_launch();
   const bool fp8 = a->cache.dtype == PITH_FP8_E4M3;
-  if (dim == 128 && fp8) kv_attn_kernel<128, true><<<grid, 64, 0, s>>>(p);
-  else if (dim == 128) kv_attn_kernel<128, false><<<grid, 64, 0, s>>>(p);
-  else if (fp8) kv_attn_kernel<64, true><<<grid, 64, 0, s>>>(p);
-  else kv_attn_kernel<64, false><<<grid, 64, 0, s>>>(p);
+  begin_launch();
+  if (dim == 128) launch_kv_attn_d128(p, fp8, pl.row_groups, pl.workgroups, s);
+  else launch_kv_attn_d64(p, fp8, pl.row_groups, pl.workgroups, s);
+  if (!pl.whole) {
+    const dim3 grid((unsigned)pl.max_items, (unsigned)(16 * pl.row_groups / kJoinRows));
+    if (dim == 128) kv_join_kernel<128><<<grid, kJoinThreads, 0, s>>>(p, 16 * pl.row_groups);
+    else kv_join_kernel<64><<<grid, kJoinThreads, 0, s>>>(p, 16 * pl.row_groups);
+  }
   return check_launch(who);
 }
