@@ -117,7 +117,7 @@ int pith_kv_append(const pith_kv_append_args* args, pith_stream_t stream);
  * cu_q count as their maximum so far, so that a token belongs to one sequence.
  * head_tables = 0: page_table [B, table_width] (row stride table_rs) and lengths [B] are those of all heads. head_tables = 1: page_table
  * [B, heads, table_width] (strides table_rs, table_hs) and lengths [B, heads]: every key-value head has rows of its own, as pith_kv_select leaves them
- * (causal only: no tree_mask).
+ * (one token a sequence: no cu_q, no tree_mask).
  * q [T,H,dim], o [T,H,dim] bf16 with token and head strides (multiples of 8); lse [H,T] fp32 (head stride lse_hs). H is a multiple of cache.heads.
  * cu_q [B+1], lengths and tables int32; tree_mask [T] int64 or NULL.
  * workspace: pith_kv_attn_workspace_bytes of the same arguments, 256-byte aligned, used by the call's kernels only. Calls that may overlap in time need one

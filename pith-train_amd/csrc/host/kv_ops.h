@@ -117,11 +117,10 @@ Two kv_attention(const Tensor& q, const Tensor& k, const Tensor& v, const OptTen
     bool ok = kv_cache_args(a.cache, q, k, v, k_scale, v_scale) && rows_of(q, q, 3, a.cache.dim) && (!tree || is_index(*tree, q, at::kLong, {a.T}));
     if (ok && lengths.dim() == 2) {  // tables of the heads
       a.B = lengths.size(0);
-      ok = !tree && is_index(lengths, q, at::kInt, {a.B, a.cache.heads}) && on(table, q) && table.scalar_type() == at::kInt && table.dim() == 3 && table.size(0) == a.B &&
-           table.size(1) == a.cache.heads && (table.size(2) == 1 || table.stride(2) == 1) && (cu_q ? is_index(*cu_q, q, at::kInt, {a.B + 1}) : a.T == a.B);
+      ok = !tree && !cu_q && is_index(lengths, q, at::kInt, {a.B, a.cache.heads}) && on(table, q) && table.scalar_type() == at::kInt && table.dim() == 3 && table.size(0) == a.B &&
+           table.size(1) == a.cache.heads && (table.size(2) == 1 || table.stride(2) == 1) && a.T == a.B;
       if (ok) {
         a.page_table = table.data_ptr<int32_t>(); a.lengths = lengths.data_ptr<int32_t>();
-        a.cu_q = cu_q ? cu_q->data_ptr<int32_t>() : nullptr;
         a.table_width = table.size(2);
         a.table_hs = a.cache.heads > 1 ? table.stride(1) : a.table_width;
         a.table_rs = a.B > 1 ? table.stride(0) : a.table_width * a.cache.heads;

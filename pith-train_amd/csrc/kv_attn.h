@@ -8,7 +8,9 @@
 // they grow, and one long sequence among short ones is spread over as many workgroups as its share of the steps. Where there are fewer row blocks than
 // workgroups, ranges may be a little longer and each lie in one row block (to begin one costs queries, a first tile and a part). An XCD's workgroups take
 // ranges that follow one another, so that row blocks of one head find each other's keys in its cache.
-// Where page tables are so short that no row block is worth cutting, every workgroup takes one, whole, and there is nothing to join.
+// Two kinds of calls need no such list. Where page tables are so short that no row block is worth cutting, every workgroup takes one, whole, and there is
+// nothing to join. And tables of the heads (selected pages) are nearly full for whoever has a long context, so their row blocks are cut into the same
+// number of parts each, as many as there are workgroups for.
 // A workgroup whose range covers a row block wholly writes its rows; parts leave (reference, sum, unnormalised result) in fp32 in the workspace, and a second
 // kernel joins them in the order of the keys (results do not depend on scheduling). So how a row's keys are cut, its references and the order of its sums
 // follow from the lengths of all sequences of the call; nothing else of one row reaches another.
@@ -34,10 +36,10 @@ namespace pith {
 constexpr int kKVThreads = 256, kKVWaves = 4;
 constexpr int kTileKeys = 32, kStepKeys = kKVWaves * kTileKeys;
 
-// What the join needs of a row block: first of its rows within the sequence and head, first token and head of that, its rows, and the slots of its parts, the
-// first and, of the workgroups behind that one, the last (equal: nothing to join).
+// What the join needs of a row block: first of its rows within the sequence and head, first token and head of that, its rows, and its parts: the slot of the
+// first, that of the second, and the slots from one to the next (parts = 1: nothing to join).
 struct KVJoin {
-  int row0, tok0, head, rows, first, last;
+  int row0, tok0, head, rows, first, second, stride, parts;
 };
 
 struct KVAttnParams {
@@ -53,11 +55,12 @@ struct KVAttnParams {
   int max_len;      // table_width * page_size
   float kappa;      // scale * log2(e)
   int whole;        // steps of the longest row block where none is cut, else 0
+  int parts;        // of every row block, where all are cut alike, else 0
   // workspace (not used where none is cut)
   int* items;        // number of row blocks of this call
   KVJoin* joins;     // [row blocks]
   float2* stats;     // [slots][M] reference (in bits) and sum
-  float* parts;      // [slots][M][D]; slot 2 i: workgroup i's part that begins with its range, 2 i + 1: one that begins later
+  float* results;    // [slots][M][D] of parts; slot 2 i: of workgroup i's that begins with its range, 2 i + 1: one that begins later (cut alike: slot i)
   int max_items;     // capacity of joins
 };
 
@@ -73,7 +76,7 @@ __device__ __forceinline__ KVWork kv_work(const KVAttnParams& p, int c0, int c1,
   s.tok0 = c0;
   s.n = c1 - c0;
   s.len = min(max(length, 0), p.max_len);
-  s.blocks = (s.n * p.group + M - 1) / M * (p.cache.heads / p.head_tables);
+  s.blocks = (s.n * p.group + M - 1) / M * (p.head_tables > 1 ? 1 : p.cache.heads);
   s.steps = max((s.len + kStepKeys - 1) / kStepKeys, 1);  // rows without keys get their zeros from an empty step
   return s;
 }
@@ -81,192 +84,138 @@ __device__ __forceinline__ KVWork kv_work(const KVAttnParams& p, int c0, int c1,
 // host has made sure of.
 __device__ __forceinline__ int kv_offset(const KVAttnParams& p, int b) { return p.cu_q ? min(max(p.cu_q[b], 0), p.T) : b; }
 
-// Sums and maxima over the workgroup. `turn` says which half of `shared` is used: one barrier a call is enough if it alternates.
-struct BlockScan {
-  int (*shared)[kKVWaves];  // [2]
-  int turn;
-  __device__ __forceinline__ int sum(int x, int& total) {  // inclusive
-    const int mine = wave_scan(x), wave = threadIdx.x >> 6;
-    if ((threadIdx.x & 63) == 63) shared[turn][wave] = mine;
-    __syncthreads();
-    int before = 0;
-    total = 0;
-#pragma unroll
-    for (int w = 0; w < kKVWaves; ++w) {
-      const int s = shared[turn][w];
-      before += w < wave ? s : 0;
-      total += s;
-    }
-    turn ^= 1;
-    return before + mine;
-  }
-  __device__ __forceinline__ int most_before(int x, int& all) {  // maxima of values from 0 on, of the threads in front
-    const int mine = wave_scan_max(x), wave = threadIdx.x >> 6;
-    if ((threadIdx.x & 63) == 63) shared[turn][wave] = mine;
-    __syncthreads();
-    int before = (threadIdx.x & 63) == 0 ? 0 : __builtin_amdgcn_update_dpp(0, mine, 0x138, 0xf, 0xf, false);  // from the lane below
-    all = 0;
-#pragma unroll
-    for (int w = 0; w < kKVWaves; ++w) {
-      const int s = shared[turn][w];
-      before = w < wave ? max(before, s) : before;
-      all = max(all, s);
-    }
-    turn ^= 1;
-    return before;
-  }
-};
-
-// Where a range begins.
-struct KVStart {
-  KVWork s;
-  int seq, item, block, step, found;  // sequence, row blocks in front of it, row block and step in it
-};
-
-// A workgroup's way through its range of the work list, segment by segment (steps of one row block); all of it is uniform.
+// A workgroup's way through its range of the work list, segment by segment (steps of one row block). Every wave walks for itself; all of it is wave-uniform.
 template <int M>
 struct KVWalk {
-  static constexpr int kEach = 4;                      // sequences of a thread
-  static constexpr int kAtOnce = kEach * kKVThreads;   // of a workgroup
   static constexpr int kStart = 2, kLeast = 1;
   int range, per, begin, at, end;  // this workgroup's range, its length, begin, place, end
-  int seq, item, block, step;
-  bool single;  // one segment a range
+  int seq, item, block, step;      // sequence, row blocks in front of it, row block, first step of the segment
+  bool single;                     // one segment a range
   KVWork s;
 
   __device__ __forceinline__ int taken(int steps) const { return single && per > 1 ? (steps + per - 1) / per * per : steps; }  // steps that a row block is taken for
 
-  // Sequences s0 + kEach * thread .. of all.
-  __device__ __forceinline__ void load(const KVAttnParams& p, int s0, BlockScan& scan, int& behind, KVWork (&x)[kEach]) const {
-    const int count = p.B * p.head_tables, i0 = s0 + kEach * threadIdx.x;
-    int c0[kEach], c1[kEach], length[kEach];
-#pragma unroll
-    for (int e = 0; e < kEach; ++e) {
-      const bool some = i0 + e < count;
-      const int b = some ? (p.head_tables == 1 ? i0 + e : (i0 + e) / p.head_tables) : 0;
-      c0[e] = some ? kv_offset(p, b) : 0;
-      c1[e] = some ? kv_offset(p, b + 1) : 0;
-      length[e] = some ? p.lengths[i0 + e] : 0;
-    }
-    if (p.cu_q) {
-      int upto = 0, all;
-#pragma unroll
-      for (int e = 0; e < kEach; ++e) upto = max(upto, c0[e]);
-      upto = max(scan.most_before(upto, all), behind);
-      behind = max(behind, all);
-#pragma unroll
-      for (int e = 0; e < kEach; ++e) {
-        upto = max(upto, c0[e]);
-        c0[e] = upto;
-        c1[e] = max(c1[e], upto);
-      }
-    }
-#pragma unroll
-    for (int e = 0; e < kEach; ++e) x[e] = kv_work<M>(p, c0[e], i0 + e < count ? c1[e] : c0[e], length[e]);
-  }
-
   // False: nothing to do.
-  __device__ __forceinline__ bool start(const KVAttnParams& p, int (*shared)[kKVWaves], KVStart* found) {
-    BlockScan scan = {shared, 0};
-    const int count = p.B * p.head_tables, groups = gridDim.x;
-    KVWork x[kEach];
-    int behind = 0, total = 0, blocks_total = 0, sum;
-    single = false;
-    per = p.whole;
-    if (threadIdx.x == 0) found->found = 0;
-    const auto work = [&]() __attribute__((always_inline)) {
-      int w = 0;
-#pragma unroll
-      for (int e = 0; e < kEach; ++e) w += x[e].blocks * taken(x[e].steps);
-      return w;
-    };
-    const auto blocks = [&]() __attribute__((always_inline)) {
-      int k = 0;
-#pragma unroll
-      for (int e = 0; e < kEach; ++e) k += x[e].blocks;
-      return k;
-    };
-    if (p.whole) {
+  __device__ __forceinline__ bool start(const KVAttnParams& p, int lane) {
+    const int groups = gridDim.x;
+    range = (blockIdx.x & 7) * (groups >> 3) + (blockIdx.x >> 3);  // an XCD's workgroups (every eighth) take ranges that follow one another
+    const auto uniform = [](int v) __attribute__((always_inline)) { return __builtin_amdgcn_readfirstlane(v); };
+    if (!p.cu_q && (p.whole || p.parts)) {  // one token a sequence: all have the same number of row blocks
+      const int parts = p.parts ? p.parts : 1, each = (p.group + M - 1) / M * (p.head_tables > 1 ? 1 : p.cache.heads);
+      const int all = uniform(range / parts), part = range - all * parts;
+      seq = uniform(all / each);
+      if (seq >= p.B * p.head_tables) return false;
+      block = all - seq * each;
+      item = seq * each;
+      const int b = uniform(p.head_tables > 1 ? seq / p.head_tables : seq);
+      s = kv_work<M>(p, b, b + 1, uniform(p.lengths[seq]));
+      per = uniform((s.steps + parts - 1) / parts);
+      step = begin = at = part * per;  // (beyond the row block's last step: a part without keys)
+      end = at + per;
       single = true;
-      load(p, 0, scan, behind, x);
+      if (p.parts && blockIdx.x == 0 && threadIdx.x == 0) *(__attribute__((address_space(1))) int*)(uintptr_t)p.items = min(p.B * p.head_tables * each, p.max_items);
+      return true;
+    }
+    KVWork x = {};
+    int w = 0, k = 0, sw = 0, sk = 0, total = 0, blocks_total = 0;
+    int behind = 0;  // the sequences that were loaded: their last offset
+    const auto load = [&](int b0) __attribute__((always_inline)) {  // 64 sequences
+      if (b0 == 0) behind = kv_offset(p, 0);
+      const bool some = b0 + lane < p.B;
+      const int length = some ? p.lengths[b0 + lane] : 0;
+      const int c1 = max(wave_scan_max(some ? kv_offset(p, b0 + lane + 1) : 0), behind);  // (lanes without one: no tokens)
+      x = kv_work<M>(p, __builtin_amdgcn_update_dpp(behind, c1, 0x138, 0xf, 0xf, false), c1, length);  // from the lane below
+      behind = __builtin_amdgcn_readlane(c1, 63);
+    };
+    const auto sums = [&]() __attribute__((always_inline)) {
+      k = x.blocks;
+      w = k * taken(x.steps);
+      sw = wave_scan(w);
+      sk = wave_scan(k);
+    };
+    single = p.whole != 0;
+    per = p.whole;
+    if (p.whole) {
+      load(0);
+      sums();
     } else {
-      for (int s0 = 0; s0 < count; s0 += kAtOnce) {
-        load(p, s0, scan, behind, x);
-        scan.sum(work(), sum);
-        total += sum;
-        scan.sum(blocks(), sum);
-        blocks_total += sum;
+#pragma unroll 1
+      for (int b0 = 0; b0 < p.B; b0 += 64) {
+        load(b0);
+        sums();
+        total += __builtin_amdgcn_readlane(sw, 63);
+        blocks_total += __builtin_amdgcn_readlane(sk, 63);
       }
       // (named as global memory: with a store to anywhere behind it, all waits for LDS in the kernel would be waits for everything)
       if (blockIdx.x == 0 && threadIdx.x == 0) *(__attribute__((address_space(1))) int*)(uintptr_t)p.items = min(blocks_total, p.max_items);
-      per = total <= groups ? 1 : __builtin_amdgcn_readfirstlane((total + groups - 1) / groups);  // (divisions leave the scalar registers)
-      if (blocks_total < groups && count <= kAtOnce && total < 1 << 30) {  // (more sequences are not looked up twice)
+      per = total <= groups ? 1 : uniform((total + groups - 1) / groups);  // (divisions leave the scalar registers)
+      if (blocks_total < groups && p.B <= 64 && total < 1 << 30) {  // (more sequences are not looked up twice)
         const int most = per + kStart;
         int longer = max(per, kLeast);
-        for (int ranges; longer <= most; longer = max(longer + 1, __builtin_amdgcn_readfirstlane((int)(longer * ((float)ranges / groups))))) {
-          int k = 0;
-#pragma unroll
-          for (int e = 0; e < kEach; ++e) k += x[e].blocks * (longer > 1 ? (x[e].steps + longer - 1) / longer : x[e].steps);
-          scan.sum(k, ranges);
-          ranges = __builtin_amdgcn_readfirstlane(ranges);
+#pragma unroll 1
+        for (int ranges; longer <= most; longer = max(longer + 1, uniform((int)(longer * ((float)ranges / groups))))) {
+          ranges = __builtin_amdgcn_readlane(wave_scan(k * (longer > 1 ? (x.steps + longer - 1) / longer : x.steps)), 63);
           if (ranges <= groups) {
             per = longer;
             single = true;
+            if (per > 1) sums();
             break;
           }
         }
       }
     }
-    range = (blockIdx.x & 7) * (groups >> 3) + (blockIdx.x >> 3);  // an XCD's workgroups (every eighth) take ranges that follow one another
     begin = at = range * per;
     end = at + per;  // (the host has bounded total + gridDim.x)
-    int before = 0, blocks_before = 0;  // in front of these sequences
-    behind = 0;
-    for (int s0 = 0; s0 < count; s0 += kAtOnce) {
-      if (count > kAtOnce) load(p, s0, scan, behind, x);
-      int w = work(), k = blocks(), sum_w, sum_k;
-      int upto = scan.sum(w, sum_w) + before;
-      int item0 = scan.sum(k, sum_k) + blocks_before - k;
-      if (upto > at && upto - w <= at) {  // one thread of all
-        int first = upto - w;
-#pragma unroll
-        for (int e = 0; e < kEach; ++e) {
-          const int each = taken(x[e].steps), mine = x[e].blocks * each;
-          if (first <= at && at < first + mine) {
-            const int block = (at - first) / each;
-            *found = KVStart{x[e], s0 + kEach * (int)threadIdx.x + e, item0, block, at - first - block * each, 1};
-          }
-          first += mine;
-          item0 += x[e].blocks;
-        }
+    int before = 0;  // steps in front of the sequence
+    item = 0;
+#pragma unroll 1
+    for (int b0 = 0; b0 < p.B; b0 += 64) {
+      if (p.B > 64) {
+        load(b0);
+        sums();
       }
-      before += sum_w;
-      blocks_before += sum_k;
-      if (before > at) break;  // (uniform)
+      const uint64_t beyond = __ballot(before + sw > at);
+      if (beyond != 0) {
+        const int i = __builtin_ctzll(beyond);
+        seq = b0 + i;
+        before += __builtin_amdgcn_readlane(sw - w, i);
+        item += __builtin_amdgcn_readlane(sk - k, i);
+        s.tok0 = __builtin_amdgcn_readlane(x.tok0, i);
+        s.n = __builtin_amdgcn_readlane(x.n, i);
+        s.len = __builtin_amdgcn_readlane(x.len, i);
+        s.blocks = __builtin_amdgcn_readlane(x.blocks, i);
+        s.steps = __builtin_amdgcn_readlane(x.steps, i);
+        const int each = uniform(taken(s.steps));
+        block = uniform((at - before) / each);
+        step = at - before - block * each;
+        if (!single) end = min(end, total);
+        return true;
+      }
+      before += __builtin_amdgcn_readlane(sw, 63);
+      item += __builtin_amdgcn_readlane(sk, 63);
     }
-    __syncthreads();
-    const auto uniform = [](int v) { return __builtin_amdgcn_readfirstlane(v); };
-    if (!uniform(found->found)) return false;
-    s.tok0 = uniform(found->s.tok0), s.n = uniform(found->s.n), s.len = uniform(found->s.len), s.blocks = uniform(found->s.blocks), s.steps = uniform(found->s.steps);
-    seq = uniform(found->seq), item = uniform(found->item), block = uniform(found->block), step = uniform(found->step);
-    if (!single) end = min(end, total);
-    return true;
+    return false;
   }
-  __device__ __forceinline__ int n_steps() const { return min(s.steps - step, end - at); }
-  __device__ __forceinline__ int blocks_of_head(const KVAttnParams& p) const { return p.head_tables == 1 ? s.blocks / p.cache.heads : s.blocks; }
-  __device__ __forceinline__ bool whole() const { return n_steps() == s.steps; }
-  __device__ __forceinline__ int slot() const { return 2 * range + (at == begin ? 0 : 1); }
+  __device__ __forceinline__ int n_steps() const { return min(s.steps - step, end - at); }  // (a part without keys: 0 or less)
+  __device__ __forceinline__ bool whole(const KVAttnParams& p) const { return p.parts ? p.parts == 1 : n_steps() == s.steps; }
+  __device__ __forceinline__ int slot(const KVAttnParams& p) const { return p.parts ? range : 2 * range + (at == begin ? 0 : 1); }
   // Who ends a row block says how it was cut.
   __device__ __forceinline__ void leave_join(const KVAttnParams& p, int row0, int head, int rows) const {
-    if (p.whole || step + n_steps() != s.steps || threadIdx.x != 0 || item + block >= p.max_items) return;
-    int first = 0, last = 0;
-    if (!whole()) {
-      const int from = at - step;  // of the row block in the work list
-      const int id = from / per;
-      first = 2 * id + (from == id * per ? 0 : 1);
-      last = 2 * range;
+    if (p.whole || threadIdx.x != 0 || item + block >= p.max_items) return;
+    KVJoin join = {row0, s.tok0, head, rows, 0, 0, 0, 1};
+    if (p.parts) {
+      if (step != 0) return;
+      join.first = range, join.second = range + 1, join.stride = 1, join.parts = p.parts;
+    } else {
+      if (step + n_steps() != s.steps) return;
+      if (!whole(p)) {
+        const int from = at - step;  // of the row block in the work list
+        const int id = from / per;
+        join.first = 2 * id + (from == id * per ? 0 : 1);
+        join.second = 2 * id + 2, join.stride = 2, join.parts = range - id + 1;
+      }
     }
-    p.joins[item + block] = KVJoin{row0, s.tok0, head, rows, first, last};
+    p.joins[item + block] = join;
   }
   // On to the next segment. False: the range is done.
   __device__ __forceinline__ bool next(const KVAttnParams& p) {
@@ -278,10 +227,8 @@ struct KVWalk {
       item += s.blocks;
       do {
         ++seq;
-        const int b = p.head_tables == 1 ? seq : seq / p.head_tables;
-        const bool same = p.head_tables > 1 && seq % p.head_tables != 0;  // another head of the same tokens
-        const int c0 = same ? s.tok0 : s.tok0 + s.n;
-        s = kv_work<M>(p, c0, same ? c0 + s.n : max(kv_offset(p, b + 1), c0), p.lengths[seq]);
+        const int c0 = s.tok0 + s.n;
+        s = kv_work<M>(p, c0, max(kv_offset(p, seq + 1), c0), p.lengths[seq]);
       } while (s.blocks == 0);
     }
     return true;
@@ -423,56 +370,49 @@ __device__ __forceinline__ uint32_t seen_keys(const KVAttnParams& p, const KVWor
   return seen;
 }
 
-__device__ __forceinline__ bool finite_pair(uint32_t x) { return (x & 0x7f80u) != 0x7f80u && (x & 0x7f800000u) != 0x7f800000u; }
-
 // Values that are not finite, in a tile that some rows see in part only: a row's weight of a key it does not see is 0, and must stay so against whatever the
-// key's value holds. Rows that do see such a value get it here, by a plain sum; then it is 0 in LDS. Rare, and as slow as it likes to be.
-// weight[r]: of the lane's eight keys, seen[r]: bits of them.
+// key's value holds. What such a value makes of a row that does see it is an infinity or NaN whatever the rest: `up` and `down` note, for each of the lane's
+// features (bit 4 n + v), whether one above and one below all numbers was seen (NaN is both). Then it is 0 in LDS. Rare, and as slow as it likes to be.
 template <int D, bool FP8, int R>
-__device__ __forceinline__ void clean_values(char* values, int lane, const bf16x8 (&weight)[R], const uint32_t (&seen)[R], f32x4 (&acc)[R][D / 16]) {
+__device__ __forceinline__ void clean_values(char* values, int lane, const uint32_t (&seen)[R], uint32_t (&up)[R], uint32_t (&down)[R]) {
   using T = KVTile<D, FP8>;
-  const auto bad_word = [](uint32_t x) {
-    if constexpr (FP8) return (x & 0x7fu) == 0x7fu || (x & 0x7f00u) == 0x7f00u || (x & 0x7f0000u) == 0x7f0000u || (x & 0x7f000000u) == 0x7f000000u;
-    else return !finite_pair(x);
+  const auto finite = [](u32x4 x) __attribute__((always_inline)) {
+    bool ok = true;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      if constexpr (FP8) ok = ok && ((x[k] & 0x7fu) != 0x7fu) & ((x[k] & 0x7f00u) != 0x7f00u) & ((x[k] & 0x7f0000u) != 0x7f0000u) & ((x[k] & 0x7f000000u) != 0x7f000000u);
+      else ok = ok && ((x[k] & 0x7f80u) != 0x7f80u) & ((x[k] & 0x7f800000u) != 0x7f800000u);
+    }
+    return ok;
   };
   bool bad = false;
 #pragma unroll
-  for (int i = 0; i < T::kBytes / 1024; ++i) {
-    const u32x4 x = *reinterpret_cast<const u32x4*>(values + 16 * lane + 1024 * i);
-    bad = bad || bad_word(x[0]) || bad_word(x[1]) || bad_word(x[2]) || bad_word(x[3]);
-  }
+  for (int i = 0; i < T::kBytes / 1024; ++i) bad = bad || !finite(*reinterpret_cast<const u32x4*>(values + 16 * lane + 1024 * i));
   if (!__any(bad)) return;
   const int c = lane & 15, g = lane >> 4;
 #pragma unroll 1
   for (int j = 0; j < kTileKeys; ++j) {
     const int owner = c + 16 * ((j >> 2) & 3), e = 4 * (j >> 4) + (j & 3);  // lane and element that hold key j of this lane's row
-    float w[R];
-    bool sees[R];
-#pragma unroll
-    for (int r = 0; r < R; ++r) {
-      float mine = 0.f;
-#pragma unroll
-      for (int k = 0; k < 8; ++k) mine = k == e ? (float)weight[r][k] : mine;
-      w[r] = __shfl(mine, owner);
-      sees[r] = (__shfl((int)seen[r], owner) >> e) & 1;
+    uint32_t above = 0, below = 0;  // of the key's values
+#pragma unroll 1
+    for (int i = 0; i < D / 4; ++i) {
+      const int d = 16 * (i >> 2) + 4 * g + (i & 3);
+      bool inf, nan, negative;
+      if constexpr (FP8) {  // (e4m3 has no infinities)
+        const uint32_t x = *reinterpret_cast<const uint8_t*>(values + T::place(j, d >> 4) + (d & 15));
+        inf = false, nan = (x & 0x7f) == 0x7f, negative = false;
+      } else {
+        const uint32_t x = *reinterpret_cast<const uint16_t*>(values + T::place(j, d >> 3) + 2 * (d & 7));
+        inf = (x & 0x7fffu) == 0x7f80u, nan = (x & 0x7fffu) > 0x7f80u, negative = (x & 0x8000u) != 0;
+      }
+      above |= (uint32_t)(nan || (inf && !negative)) << i;
+      below |= (uint32_t)(nan || (inf && negative)) << i;
     }
 #pragma unroll
-    for (int n = 0; n < D / 16; ++n) {  // features 16 n + 4 g + v
-#pragma unroll
-      for (int v = 0; v < 4; ++v) {
-        const int d = 16 * n + 4 * g + v;
-        float x;
-        if constexpr (FP8) {
-          const uint32_t byte = *reinterpret_cast<const uint8_t*>(values + T::place(j, d >> 4) + (d & 15));
-          x = (byte & 0x7f) == 0x7f ? NAN : 0.f;
-        } else {
-          const uint32_t half = *reinterpret_cast<const uint16_t*>(values + T::place(j, d >> 3) + 2 * (d & 7));
-          x = (half & 0x7f80u) == 0x7f80u ? bf16_bits_to_f32(half) : 0.f;
-        }
-        const bool not_finite = x != 0.f;
-#pragma unroll
-        for (int r = 0; r < R; ++r) acc[r][n][v] = not_finite && sees[r] ? acc[r][n][v] + w[r] * x : acc[r][n][v];
-      }
+    for (int r = 0; r < R; ++r) {
+      const bool sees = (__shfl((int)seen[r], owner) >> e) & 1;
+      up[r] |= sees ? above : 0;
+      down[r] |= sees ? below : 0;
     }
   }
 #pragma unroll 1
@@ -504,12 +444,10 @@ __global__ __launch_bounds__(kKVThreads, 1) void kv_attn_kernel(KVAttnParams p) 
   constexpr int kRegion = T::kRing > M * D * 4 ? T::kRing : M * D * 4;  // of a wave: its tiles, then its results
   __shared__ __attribute__((aligned(1024))) char lds[kKVWaves * kRegion];
   __shared__ float2 wave_stats[kKVWaves][M];
-  __shared__ int scan[2][kKVWaves];
-  __shared__ KVStart found;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int c = lane & 15, g = lane >> 4;
   KVWalk<M> walk;
-  if (!walk.start(p, scan, &found)) return;
+  if (!walk.start(p, lane)) return;
   char* const ring = lds + wave * kRegion;
   const int source = T::source(lane);
   const int key_at = T::place(c, g);  // of keys 0-15; 16-31 differ by this:
@@ -518,11 +456,21 @@ __global__ __launch_bounds__(kKVThreads, 1) void kv_attn_kernel(KVAttnParams p) 
 
   do {
     const KVWork& s = walk.s;
-    const int per_head = walk.blocks_of_head(p);
-    const int head = p.head_tables == 1 ? __builtin_amdgcn_readfirstlane(walk.block / per_head) : walk.seq % p.head_tables;
-    const int row0 = (p.head_tables == 1 ? walk.block - head * per_head : walk.block) * M;  // within the sequence and head
+    int head, row0;  // row0: within the sequence and head
+    const int32_t* entries;
+    if (p.head_tables > 1) {
+      const int b = __builtin_amdgcn_readfirstlane(walk.seq / p.head_tables);
+      head = walk.seq - b * p.head_tables;
+      row0 = walk.block * M;
+      entries = p.table + b * p.table_rs + head * p.table_hs;
+    } else {
+      const int per_head = (s.n * p.group + M - 1) / M;
+      head = __builtin_amdgcn_readfirstlane(walk.block / per_head);
+      row0 = (walk.block - head * per_head) * M;
+      entries = p.table + walk.seq * p.table_rs;
+    }
     const int rows = min(s.n * p.group - row0, M);
-    const ScalarTable table = (ScalarTable)(uintptr_t)(p.table + (p.head_tables == 1 ? walk.seq : walk.seq / p.head_tables) * p.table_rs + head * p.table_hs);
+    const ScalarTable table = (ScalarTable)(uintptr_t)entries;
     const int last = max(s.len - 1, 0);
     const int tile0 = walk.step * kKVWaves + wave;  // this wave's first
     const int tiles = min((s.len + kTileKeys - 1) / kTileKeys, (walk.step + walk.n_steps()) * kKVWaves);
@@ -532,6 +480,7 @@ __global__ __launch_bounds__(kKVThreads, 1) void kv_attn_kernel(KVAttnParams p) 
     int tok[R];
     f32x4 acc[R][D / 16];
     float m[R], l[R];  // reference and sum (this lane's keys) of a row
+    uint32_t up[R], down[R];  // see clean_values
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       const int row = row0 + min(16 * r + c, rows - 1);
@@ -544,6 +493,7 @@ __global__ __launch_bounds__(kKVThreads, 1) void kv_attn_kernel(KVAttnParams p) 
       for (int n = 0; n < D / 16; ++n) acc[r][n] = f32x4{};
       m[r] = -INFINITY;
       l[r] = 0.f;
+      up[r] = down[r] = 0;
     }
 
     const auto key_of_tile = [&](int i) { return (tile0 + i * kKVWaves) * kTileKeys; };
@@ -642,7 +592,7 @@ __global__ __launch_bounds__(kKVThreads, 1) void kv_attn_kernel(KVAttnParams p) 
       } else {
         wait_tiles<D, FP8, 0>(later);  // the values
       }
-      if (partial) clean_values<D, FP8, R>(slot + T::kBytes, lane, weight, seen, acc);
+      if (partial) clean_values<D, FP8, R>(slot + T::kBytes, lane, seen, up, down);
       const uint32_t values = lds_address(slot) + value_at;
 #pragma unroll
       for (int n = 0; n < D / 16; ++n) {
@@ -674,10 +624,16 @@ __global__ __launch_bounds__(kKVThreads, 1) void kv_attn_kernel(KVAttnParams p) 
       const float f = __builtin_amdgcn_exp2f(m[r] - (top == -INFINITY ? 0.f : top));
 #pragma unroll
       for (int n = 0; n < D / 16; ++n) *reinterpret_cast<f32x4*>(ring + ((16 * r + c) * kRowPieces + ((4 * n + g) ^ c)) * 16) = acc[r][n] * f;
+      if (__any((up[r] | down[r]) != 0))
+#pragma unroll 1
+        for (int i = 0; i < D / 4; ++i)
+          if (((up[r] | down[r]) >> i) & 1)
+            *reinterpret_cast<float*>(ring + ((16 * r + c) * kRowPieces + ((4 * (i >> 2) + g) ^ c)) * 16 + 4 * (i & 3)) =
+                !((down[r] >> i) & 1) ? INFINITY : (up[r] >> i) & 1 ? NAN : -INFINITY;
     }
     __syncthreads();
-    const bool whole = walk.whole();
-    const int64_t slot = walk.slot();
+    const bool whole = walk.whole(p);
+    const int64_t slot = walk.slot(p);
     for (int i = threadIdx.x; i < rows * kRowPieces; i += kKVThreads) {
       const int row = i / kRowPieces, piece = i % kRowPieces;
       float top = -INFINITY, sum = 0.f;
@@ -698,7 +654,7 @@ __global__ __launch_bounds__(kKVThreads, 1) void kv_attn_kernel(KVAttnParams p) 
         *reinterpret_cast<u32x2*>(p.o + t * p.o_ts + h * p.o_hs + 4 * piece) = u32x2{pack_bf16x2(o[0], o[1]), pack_bf16x2(o[2], o[3])};
         if (piece == 0) p.lse[h * p.lse_hs + t] = sum == 0.f ? -INFINITY : ref + __builtin_amdgcn_logf(sum);
       } else {
-        *reinterpret_cast<f32x4*>(p.parts + (slot * M + row) * D + 4 * piece) = x;
+        *reinterpret_cast<f32x4*>(p.results + (slot * M + row) * D + 4 * piece) = x;
         if (piece == 0) p.stats[slot * M + row] = make_float2(top, sum);
       }
     }

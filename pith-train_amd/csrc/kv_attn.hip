@@ -24,12 +24,12 @@ __global__ __launch_bounds__(kJoinThreads) void kv_join_kernel(KVAttnParams p, i
   const int row0 = kJoinRows * blockIdx.y;
   const int items = *p.items;
   const KVJoin join = p.joins[blockIdx.x];  // (beyond `items` it is whatever the workspace held)
-  if ((int)blockIdx.x >= items || join.first == join.last || row0 >= join.rows) return;
-  const int n = min(join.last / 2 - join.first / 2 + 1, kMaxGroups + 1);  // parts: the first slot, then the even ones up to the last
-  const auto slot = [&](int i) { return (int64_t)(i == 0 ? join.first : 2 * (join.first / 2 + i)); };
+  if ((int)blockIdx.x >= items || join.parts == 1 || row0 >= join.rows) return;
+  const int n = min(join.parts, kMaxGroups + 1);
+  const auto slot = [&](int i) { return (int64_t)(i == 0 ? join.first : join.second + (i - 1) * join.stride); };
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int group = threadIdx.x / kEach, row = threadIdx.x % kEach / kPieces, piece = threadIdx.x % kPieces;
-  const auto part = [&](int i) { return *reinterpret_cast<const f32x4*>(p.parts + (slot(i) * m + row0 + row) * D + 4 * piece); };
+  const auto part = [&](int i) { return *reinterpret_cast<const f32x4*>(p.results + (slot(i) * m + row0 + row) * D + 4 * piece); };
   f32x4 x[4];  // the first ones are on their way while the weights are formed (those behind the last one: that one, not used)
 #pragma unroll
   for (int k = 0; k < 4; ++k) x[k] = part(min(group + k * kGroups, n - 1));
@@ -92,8 +92,9 @@ struct KVPlan {
   int row_groups;  // of 16 query rows, to a row block
   int workgroups;  // a multiple of 8
   int whole;       // steps of the longest row block where none is cut, else 0
+  int parts;       // of every row block, where all are cut alike, else 0
   int64_t max_items;
-  int64_t joins_at, stats_at, parts_at, bytes;  // workspace
+  int64_t joins_at, stats_at, results_at, bytes;  // workspace
 };
 
 constexpr int64_t kWholeSteps = 4;
@@ -113,12 +114,17 @@ KVPlan plan_of(const pith_kv_attn_args* a) {
   }
   const int units = compute_units_or_default() & ~7;
   pl.workgroups = units < 8 ? 8 : units > kMaxGroups ? kMaxGroups : units;
+  if (a->head_tables) {
+    pl.max_items = (a->H / a->cache.heads + m - 1) / m * a->cache.heads * a->B;
+    pl.parts = (int)std::min(std::max<int64_t>(pl.workgroups / pl.max_items, 1), steps);
+    pl.workgroups = (int)((pl.max_items * pl.parts + 7) & ~(int64_t)7);
+  }
   const auto up = [](int64_t x) { return (x + 255) & ~(int64_t)255; };
-  const int64_t slot_rows = 2 * pl.workgroups * m;
+  const int64_t slot_rows = (pl.parts ? 1 : 2) * (int64_t)pl.workgroups * m;
   pl.joins_at = 256;
   pl.stats_at = pl.joins_at + up(pl.max_items * (int64_t)sizeof(KVJoin));
-  pl.parts_at = pl.stats_at + up(slot_rows * (int64_t)sizeof(float2));
-  pl.bytes = pl.parts_at + slot_rows * a->cache.dim * 4;
+  pl.results_at = pl.stats_at + up(slot_rows * (int64_t)sizeof(float2));
+  pl.bytes = pl.results_at + slot_rows * a->cache.dim * 4;
   return pl;
 }
 
@@ -132,7 +138,7 @@ int check_attn(const pith_kv_attn_args* a, const char* who) {
   const int64_t items = ((a->T * (a->H / a->cache.heads) + 15) / 16 + a->B) * a->cache.heads;
   if (items > 1 << 24 || a->B * a->cache.heads > 1 << 24 || items * (a->table_width * a->cache.page_size / kStepKeys + 1) > 0x7fffffff - (1 << 25))
     return fail(PITH_ERR_UNSUPPORTED, "%s: too many row blocks for page tables of that width: call it with fewer tokens at a time", who);
-  if (a->head_tables && a->tree_mask) return fail(PITH_ERR_UNSUPPORTED, "%s: tables of the heads go with causal attention", who);
+  if (a->head_tables && (a->tree_mask || a->cu_q)) return fail(PITH_ERR_UNSUPPORTED, "%s: tables of the heads go with one token a sequence: no cu_q, no tree_mask", who);
   return PITH_OK;
 }
 
@@ -171,19 +177,19 @@ extern "C" int pith_kv_attn(const pith_kv_attn_args* a, pith_stream_t stream) {
   p.head_tables = a->head_tables ? (int)heads : 1;
   p.max_len = (int)(a->table_width * a->cache.page_size);
   p.kappa = a->scale * 1.4426950408889634f;
-  p.whole = pl.whole;
+  p.whole = pl.whole; p.parts = pl.parts;
   char* const ws = (char*)a->workspace;
   p.items = (int*)ws;
   p.joins = (KVJoin*)(ws + pl.joins_at);
   p.stats = (float2*)(ws + pl.stats_at);
-  p.parts = (float*)(ws + pl.parts_at);
+  p.results = (float*)(ws + pl.results_at);
   p.max_items = (int)pl.max_items;
   hipStream_t s = (hipStream_t)stream;
   const bool fp8 = a->cache.dtype == PITH_FP8_E4M3;
   begin_launch();
   if (dim == 128) launch_kv_attn_d128(p, fp8, pl.row_groups, pl.workgroups, s);
   else launch_kv_attn_d64(p, fp8, pl.row_groups, pl.workgroups, s);
-  if (!pl.whole) {
+  if (!pl.whole && pl.parts != 1) {
     const dim3 grid((unsigned)pl.max_items, (unsigned)(16 * pl.row_groups / kJoinRows));
     if (dim == 128) kv_join_kernel<128><<<grid, kJoinThreads, 0, s>>>(p, 16 * pl.row_groups);
     else kv_join_kernel<64><<<grid, kJoinThreads, 0, s>>>(p, 16 * pl.row_groups);

@@ -115,6 +115,7 @@ def _sequences(args, like, page_table, lengths, cu_q, t, head_tables=None) -> No
         args.table_hs = page_table.stride(1) if head_tables > 1 else width
         args.table_rs = page_table.stride(0) if b > 1 else width * head_tables
         args.head_tables = 1
+        assert cu_q is None, "page tables of the heads go with one token a sequence: no cu_q"
     else:
         assert lengths.dim() == 1, "lengths must be one-dimensional, or [b, heads] with a page table of every head"
         b = lengths.shape[0]
@@ -309,7 +310,7 @@ def kv_attention(
     no row gets 0 and an lse of -inf. Tokens from cu_q[b] on are not written. The same call gives the same bits; in a batch of other sequences a token's last
     bits may differ. page_table [b, pages], lengths [b] and cu_q [b + 1] are int32, on the device.
 
-    With page_table [b, hkv, pages] and lengths [b, hkv] every key-value head has rows of its own (kv_select_pages; causal only)."""
+    With page_table [b, hkv, pages] and lengths [b, hkv] every key-value head has rows of its own (kv_select_pages; one token a sequence, no cu_q)."""
     return _attention_op(q, cache.k, cache.v, cache.k_scale, cache.v_scale, page_table, lengths, cu_q, softmax_scale, tree_mask)
 
 

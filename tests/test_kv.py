@@ -189,7 +189,8 @@ CALLS = {
     "pith_kv_attn": (_attn, TABLES + [
         (dict(q=None), NULL), (dict(workspace=None), NULL), (dict(lse=None), NULL), (dict(H=0), SHAPE), (dict(H=3), SHAPE), (dict(H=1026), SHAPE), (dict(q_hs=120), SHAPE), (dict(o_ts=120), SHAPE),
         (dict(lse_hs=3), SHAPE), (dict(workspace_bytes=64), SHAPE), (dict(q=264), ALIGN), (dict(q_hs=132), ALIGN), (dict(o_ts=516), ALIGN), (dict(workspace=384), ALIGN),
-        (dict(tree_mask=260), ALIGN), (dict(head_tables=1, table_hs=4, table_rs=8, tree_mask=256), UNSUPPORTED), (dict(head_tables=1, table_hs=3, table_rs=8), SHAPE)]),
+        (dict(tree_mask=260), ALIGN), (dict(head_tables=1, table_hs=4, table_rs=8, T=2, cu_q=None, tree_mask=256), UNSUPPORTED), (dict(head_tables=1, table_hs=4, table_rs=8), UNSUPPORTED),
+        (dict(head_tables=1, table_hs=3, table_rs=8, T=2, cu_q=None), SHAPE)]),
     "pith_kv_bounds": (_bounds, TABLES + [(dict(bounds=None), NULL), (dict(bounds_ps=504), SHAPE), (dict(bounds_ps=516), ALIGN), (dict(bounds=264), ALIGN)]),
     "pith_kv_select": (_select, TABLES + [
         (dict(q=None), NULL), (dict(bounds=None), NULL), (dict(table_out=None), NULL), (dict(workspace=None), NULL), (dict(H=3), SHAPE), (dict(heads=0), SHAPE), (dict(dim=32), UNSUPPORTED),

@@ -290,7 +290,7 @@ def test_strides(gpu, fp8):
 @BOTH
 @pytest.mark.parametrize("heads", [(8, 2, 128), (6, 3, 64), (20, 1, 128)], ids=str)
 def test_attention_with_a_table_of_every_head(gpu, fp8, heads):
-    """Every token and head attends to rows of its own choice, with and without token offsets."""
+    """Every token and head attends to rows of its own choice."""
     b = Batch(gpu, [1, 1, 1], [200, 90, 333], heads, page=16, fp8=fp8, seed=12)
     g = torch.Generator().manual_seed(13)
     t, hkv = 3, b.hkv
@@ -302,13 +302,17 @@ def test_attention_with_a_table_of_every_head(gpu, fp8, heads):
             table[i, j, :n] = b.table[i].cpu()[pages]
             lengths[i, j] = max(n * 16 - int(torch.randint(0, 16, (1,), generator=g)), 0)
     assert (lengths == 0).any() or hkv == 1
-    for cu_q in (None, torch.arange(t + 1, dtype=I32, device=gpu)):
-        o, lse = (x.cpu() for x in K.kv_attention(b.q, b.cache, table.to(gpu), lengths.to(gpu), cu_q, b.scale))
+    for width in (7, 60):  # whole, and cut into parts some of which are empty
+        wide = torch.full((t, hkv, width), -1, dtype=I32)
+        wide[..., :7] = table
+        o, lse = (x.cpu() for x in K.kv_attention(b.q, b.cache, wide.to(gpu), lengths.to(gpu), None, b.scale))
         for i in range(t):
             for j in range(hkv):
                 n, mine = int(lengths[i, j]), slice(j * (b.h // hkv), (j + 1) * (b.h // hkv))
                 k, v = b.rows(table[i, j].to(gpu).clamp(min=0), n)
                 b.close(o[i : i + 1, mine], lse[mine, i : i + 1], b.q[i : i + 1, mine], k[j : j + 1], v[j : j + 1], O.sees(1, n), f"token {i} head {j}")
+    with pytest.raises(AssertionError, match="no cu_q"):
+        K.kv_attention(b.q, b.cache, table.to(gpu), lengths.to(gpu), b.cu_q, b.scale)
 
 
 def test_bad_tables_lengths_and_offsets_stay_in_memory(gpu):
