@@ -33,6 +33,30 @@ __device__ __forceinline__ int wave_scan_max(int x) {
   return max_dpp<0x143, 0xc>(x);
 }
 
+// A value of another lane of the row of 16.
+template <int CTRL>
+__device__ __forceinline__ float lane_dpp(float x) {
+  return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), CTRL, 0xf, 0xf, true));
+}
+constexpr int kDppXor1 = 0xB1, kDppXor2 = 0x4E, kDppHalfMirror = 0x141, kDppMirror = 0x140, kDppRotate8 = 0x128, kDppQuadMirror = 0x1B;
+// Over groups of 8 or 16 lanes; all of a group have the result. (Behind the first two steps lanes of a quad agree, so a mirrored half or row is as good as an
+// exchanged one.)
+template <int LANES, typename F>
+__device__ __forceinline__ float group_reduce(float x, const F& f) {
+  static_assert(LANES == 8 || LANES == 16, "rows of 64 or 128 features");
+  x = f(x, lane_dpp<kDppXor1>(x));
+  x = f(x, lane_dpp<kDppXor2>(x));
+  x = f(x, lane_dpp<kDppHalfMirror>(x));
+  if constexpr (LANES == 16) x = f(x, lane_dpp<kDppMirror>(x));
+  return x;
+}
+// Of the lane half a group away.
+template <int LANES>
+__device__ __forceinline__ float other_half(float x) {
+  if constexpr (LANES == 16) return lane_dpp<kDppRotate8>(x);
+  else return lane_dpp<kDppQuadMirror>(lane_dpp<kDppHalfMirror>(x));
+}
+
 // max / sum over the four lanes c, c + 16, c + 32, c + 48 that share a query row
 __device__ __forceinline__ float quad_max(float x) {
   const int i = __float_as_int(x);

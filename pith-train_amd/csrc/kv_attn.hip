@@ -97,7 +97,7 @@ struct KVPlan {
   int64_t joins_at, stats_at, results_at, bytes;  // workspace
 };
 
-constexpr int64_t kWholeSteps = 4;
+constexpr int64_t kWholeSteps = 8;
 
 KVPlan plan_of(const pith_kv_attn_args* a) {
   KVPlan pl = {};

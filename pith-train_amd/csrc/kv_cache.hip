@@ -4,12 +4,14 @@
 // Both move memory and little else. A row of a head is 16 bytes a lane: a group of dim / 8 lanes holds it in registers from the load to the store, its sums are a
 // few steps between lanes, and the rotation's partner (half a row away) comes from the lane half a group away. Query, key and value rows are rows of
 // one launch.
+#include "cache_attn.h"
 #include "kv_common.h"
 
 namespace pith {
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int64_t kManyTokens = 2048;  // from which on a wave takes a whole token
 
 struct KVAppendParams {
   const __bf16 *q, *k, *v;
@@ -18,113 +20,131 @@ struct KVAppendParams {
   const int64_t *pos, *slots;
   __bf16* q_out;
   int64_t P, rows;  // positions, slots
-  int64_t q_ts, q_hs, k_ts, k_hs, v_ts, v_hs, q_out_ts, q_out_hs;
-  int total, per_token, H;
+  int64_t q_ts, k_ts, v_ts, q_out_ts;
+  int q_hs, k_hs, v_hs, q_out_hs;
+  int T, H, per_wave;  // per_wave: pieces of a token's work for one wave
   float eps;
   KVCache cache;
 };
-
-template <int LANES>
-__device__ __forceinline__ float group_sum(float x) {
-#pragma unroll
-  for (int m = 1; m < LANES; m <<= 1) x += __shfl_xor(x, m);
-  return x;
-}
-template <int LANES>
-__device__ __forceinline__ float group_max(float x) {
-#pragma unroll
-  for (int m = 1; m < LANES; m <<= 1) x = fmaxf(x, __shfl_xor(x, m));
-  return x;
-}
 
 __device__ __forceinline__ void unpack8(u32x4 x, float (&v)[8]) {
 #pragma unroll
   for (int e = 0; e < 4; ++e) v[2 * e] = bf16lo_to_f32(x[e]), v[2 * e + 1] = bf16hi_to_f32(x[e]);
 }
 
+// A wave takes a token, whose position and slot are then scalars, and of it `per_wave` pieces of 64 / (D / 8) heads each, those of q, then of k, then of v (the
+// next one is on its way while one is computed): all of them where there are many tokens, so that the tables' rows and the weights come once, or one
+// where there are few, and latency counts. 8192 tokens of 32 + 4 + 4 heads: see launch_append.
 // Weights: 0 none, 1 bf16, 2 fp32. The norm, the rotation and the division by the scale are fp32, rounded once (to nearest even; e4m3: the largest feature
 // becomes +-448 exactly). The scale is the fp32 quotient, not a power of two, as in the latent cache.
 template <int D, bool FP8, int WEIGHT>
 __global__ __launch_bounds__(kThreads) void kv_append_kernel(KVAppendParams p) {
-  constexpr int kLanes = D / 8;
-  const int row = (blockIdx.x * kThreads + threadIdx.x) / kLanes, sub = threadIdx.x % kLanes;
-  if (row >= p.total) return;  // (whole groups of lanes)
-  const int t = row / p.per_token, r = row - t * p.per_token;
-  const int heads = p.cache.heads;
-  const int what = r < p.H ? 0 : r < p.H + heads ? 1 : 2;  // q, k, v
-  const int head = what == 0 ? r : what == 1 ? r - p.H : r - p.H - heads;
+  constexpr int kLanes = D / 8, kHeads = 64 / kLanes;
+  const int lane = threadIdx.x & 63, sub = lane % kLanes, group = lane / kLanes;
+  const int heads = p.cache.heads, q_pieces = (p.H + kHeads - 1) / kHeads, kv_pieces = (heads + kHeads - 1) / kHeads, pieces = q_pieces + 2 * kv_pieces;
+  const int wave = blockIdx.x * (kThreads / 64) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = (pieces + p.per_wave - 1) / p.per_wave;
+  const int t = __builtin_amdgcn_readfirstlane(wave / waves);
+  if (t >= p.T) return;
+  const int first = (wave - t * waves) * p.per_wave, last = min(first + p.per_wave, pieces) - 1;
   const int64_t slot = p.slots[t];
   const bool kept = slot >= 0 && slot < p.rows;
-  if (what != 0 && !kept) return;
-  const __bf16* const src = what == 0 ? p.q + t * p.q_ts + head * p.q_hs : what == 1 ? p.k + t * p.k_ts + head * p.k_hs : p.v + t * p.v_ts + head * p.v_hs;
-  float x[8];
-  unpack8(*reinterpret_cast<const u32x4*>(src + 8 * sub), x);
-  if (what != 2) {
-    const int64_t at = clamped_position(p.pos[t], p.P) * D + 8 * sub;
-    float c[8], s[8];
-    unpack8(*reinterpret_cast<const u32x4*>(p.cos + at), c);
-    unpack8(*reinterpret_cast<const u32x4*>(p.sin + at), s);
-    if constexpr (WEIGHT != 0) {
-      const void* const weight = what == 0 ? p.q_weight : p.k_weight;
-      float w[8];
-      if constexpr (WEIGHT == 2) {
-        const f32x4* const from = reinterpret_cast<const f32x4*>(weight) + 2 * sub;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) w[e] = from[e >> 2][e & 3];
-      } else {
-        unpack8(reinterpret_cast<const u32x4*>(weight)[sub], w);
-      }
-      float sum = 0.f;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) sum += x[e] * x[e];
-      const float inv = rsqrtf(group_sum<kLanes>(sum) * (1.f / D) + p.eps);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] = x[e] * inv * w[e];
-    }
-    const bool upper = sub >= kLanes / 2;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float other = __shfl_xor(x[e], kLanes / 2);
-      x[e] = x[e] * c[e] + (upper ? other : -other) * s[e];
-    }
-  }
-  const auto packed = [&]() __attribute__((always_inline)) {
-    u32x4 out;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) out[e] = pack_bf16x2(x[2 * e], x[2 * e + 1]);
-    return out;
+  const int64_t at = clamped_position(p.pos[t], p.P) * D + 8 * sub;
+
+  // What piece i is about: 0 q, 1 k, 2 v; its first head.
+  const auto what_of = [&](int i, int& head0) __attribute__((always_inline)) {
+    const int what = i < q_pieces ? 0 : i < q_pieces + kv_pieces ? 1 : 2;
+    head0 = (i - (what == 0 ? 0 : what == 1 ? q_pieces : q_pieces + kv_pieces)) * kHeads;
+    return what;
   };
-  if (what == 0) {
-    *reinterpret_cast<u32x4*>(p.q_out + t * p.q_out_ts + head * p.q_out_hs + 8 * sub) = packed();
-    return;
-  }
-  const int64_t page = slot >> p.cache.page_shift, in_page = ((int64_t)head << p.cache.page_shift) + (slot & ((1 << p.cache.page_shift) - 1));
-  char* const dst = what == 1 ? p.cache.k + page * p.cache.k_ps : p.cache.v + page * p.cache.v_ps;
-  if constexpr (FP8) {
-    float top = 0.f;
+  const auto load = [&](int i) __attribute__((always_inline)) {
+    int head0;
+    const int what = what_of(i, head0);
+    const __bf16* const base = what == 0 ? p.q + t * p.q_ts : what == 1 ? p.k + t * p.k_ts : p.v + t * p.v_ts;
+    const int hs = what == 0 ? p.q_hs : what == 1 ? p.k_hs : p.v_hs, head = min(head0 + group, (what == 0 ? p.H : heads) - 1);
+    return *reinterpret_cast<const u32x4*>(base + (head * hs + 8 * sub));
+  };
+  u32x4 next = load(first);
+  float c[8], s[8], qw[8], kw[8];
+  unpack8(*reinterpret_cast<const u32x4*>(p.cos + at), c);
+  unpack8(*reinterpret_cast<const u32x4*>(p.sin + at), s);
+  const auto weights = [&](const void* from, float (&w)[8]) __attribute__((always_inline)) {
+    if constexpr (WEIGHT == 2) {
+      const f32x4* const x = reinterpret_cast<const f32x4*>(from) + 2 * sub;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(x[e]));
-    const float scale = group_max<kLanes>(top) / kFp8Max;
-    float y[8];
+      for (int e = 0; e < 8; ++e) w[e] = x[e >> 2][e & 3];
+    } else if constexpr (WEIGHT == 1) {
+      unpack8(reinterpret_cast<const u32x4*>(from)[sub], w);
+    }
+  };
+  weights(p.q_weight, qw);
+  weights(p.k_weight, kw);
+  const float sign = sub >= kLanes / 2 ? 1.f : -1.f;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float z = scale > 0.f ? x[e] / scale : x[e];  // (a row of zeros stays one; NaN stays NaN)
-      y[e] = z > kFp8Max ? kFp8Max : (z < -kFp8Max ? -kFp8Max : z);
-    }
-    u32x2 out;
+  for (int e = 0; e < 8; ++e) s[e] *= sign;
+
+#pragma unroll 1
+  for (int i = first; i <= last; ++i) {
+    float x[8];
+    unpack8(next, x);
+    next = load(min(i + 1, last));
+    int head0;
+    const int what = what_of(i, head0), head = head0 + group;
+    if (what != 0 && !kept) break;  // (k and v are the last)
+    if (what != 2) {
+      if constexpr (WEIGHT != 0) {
+        float sum = 0.f;
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      int word = __builtin_amdgcn_cvt_pk_fp8_f32(y[4 * e], y[4 * e + 1], 0, false);
-      word = __builtin_amdgcn_cvt_pk_fp8_f32(y[4 * e + 2], y[4 * e + 3], word, true);
-      out[e] = (uint32_t)word;
+        for (int e = 0; e < 8; ++e) sum += x[e] * x[e];
+        const float inv = rsqrtf(group_reduce<kLanes>(sum, [](float a, float b) { return a + b; }) * (1.f / D) + p.eps);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = x[e] * inv * (what == 0 ? qw[e] : kw[e]);
+      }
+      float y[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) y[e] = x[e] * c[e] + other_half<kLanes>(x[e]) * s[e];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] = y[e];
     }
-    *reinterpret_cast<u32x2*>(dst + in_page * D + 8 * sub) = out;
-    if (sub == 0) {
-      if (what == 1) p.cache.k_scale[page * p.cache.k_scale_ps + in_page] = scale;
-      else p.cache.v_scale[page * p.cache.v_scale_ps + in_page] = scale;
+    const auto packed = [&]() __attribute__((always_inline)) {
+      u32x4 out;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) out[e] = pack_bf16x2(x[2 * e], x[2 * e + 1]);
+      return out;
+    };
+    if (what == 0) {
+      if (head < p.H) *reinterpret_cast<u32x4*>(p.q_out + t * p.q_out_ts + (head * p.q_out_hs + 8 * sub)) = packed();
+      continue;
     }
-  } else {
-    *reinterpret_cast<u32x4*>(dst + in_page * (2 * D) + 16 * sub) = packed();
+    const int64_t page = slot >> p.cache.page_shift, in_page = ((int64_t)head << p.cache.page_shift) + (slot & ((1 << p.cache.page_shift) - 1));
+    char* const dst = what == 1 ? p.cache.k + page * p.cache.k_ps : p.cache.v + page * p.cache.v_ps;
+    if constexpr (FP8) {
+      float top = 0.f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(x[e]));
+      const float scale = group_reduce<kLanes>(top, [](float a, float b) { return fmaxf(a, b); }) / kFp8Max;
+      float y[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float z = scale > 0.f ? x[e] / scale : x[e];  // (a row of zeros stays one; NaN stays NaN)
+        y[e] = z > kFp8Max ? kFp8Max : (z < -kFp8Max ? -kFp8Max : z);
+      }
+      u32x2 out;
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        int word = __builtin_amdgcn_cvt_pk_fp8_f32(y[4 * e], y[4 * e + 1], 0, false);
+        word = __builtin_amdgcn_cvt_pk_fp8_f32(y[4 * e + 2], y[4 * e + 3], word, true);
+        out[e] = (uint32_t)word;
+      }
+      if (head < heads) {
+        *reinterpret_cast<u32x2*>(dst + in_page * D + 8 * sub) = out;
+        if (sub == 0) {
+          if (what == 1) p.cache.k_scale[page * p.cache.k_scale_ps + in_page] = scale;
+          else p.cache.v_scale[page * p.cache.v_scale_ps + in_page] = scale;
+        }
+      }
+    } else {
+      if (head < heads) *reinterpret_cast<u32x4*>(dst + in_page * (2 * D) + 16 * sub) = packed();
+    }
   }
 }
 
@@ -136,9 +156,9 @@ struct KVBoundsParams {
   int T, table_width;
 };
 
-// NaN stays, as in a comparison-free definition: the least and largest of rows with a NaN are NaN.
-__device__ __forceinline__ float least(float a, float b) { return b < a || b != b ? b : a; }
-__device__ __forceinline__ float largest(float a, float b) { return b > a || b != b ? b : a; }
+// The least and largest of rows with a NaN are NaN.
+__device__ __forceinline__ float least(float a, float b) { return __builtin_elementwise_minimum(a, b); }
+__device__ __forceinline__ float largest(float a, float b) { return __builtin_elementwise_maximum(a, b); }
 
 // blockIdx.x: sequence, blockIdx.y: key-value head, blockIdx.z: every how many-th of the pages that its new tokens filled. A group of lanes takes every
 // 256 / kLanes-th row; what the groups found meets in LDS.
@@ -157,21 +177,36 @@ __global__ __launch_bounds__(kThreads) void kv_bounds_kernel(KVBoundsParams p) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) lo[e] = INFINITY, hi[e] = -INFINITY;
     const char* const rows = p.cache.k + page * p.cache.k_ps + (int64_t)head * page_size * (FP8 ? D : 2 * D);
-    for (int r = group; r < page_size; r += kGroups) {
-      float x[8];
-      if constexpr (FP8) {
-        const u32x2 raw = *reinterpret_cast<const u32x2*>(rows + (int64_t)r * D + 8 * sub);
-        const float scale = p.cache.k_scale[page * p.cache.k_scale_ps + (int64_t)head * page_size + r];
+    constexpr int kAtOnce = 4;  // rows in flight (those behind the page's last: that one again)
+    for (int r0 = group; r0 < page_size; r0 += kAtOnce * kGroups) {
+      u32x4 raw[kAtOnce];
+      float scale[kAtOnce];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const bf16x2 two = (e & 1) ? fp8x2_to_bf16<true>(raw[e >> 1]) : fp8x2_to_bf16<false>(raw[e >> 1]);
-          x[2 * e] = (float)two[0] * scale, x[2 * e + 1] = (float)two[1] * scale;
+      for (int k = 0; k < kAtOnce; ++k) {
+        const int r = min(r0 + k * kGroups, page_size - 1);
+        if constexpr (FP8) {
+          const u32x2 x = *reinterpret_cast<const u32x2*>(rows + (int64_t)r * D + 8 * sub);
+          raw[k][0] = x[0], raw[k][1] = x[1];
+          scale[k] = p.cache.k_scale[page * p.cache.k_scale_ps + (int64_t)head * page_size + r];
+        } else {
+          raw[k] = *reinterpret_cast<const u32x4*>(rows + (int64_t)r * (2 * D) + 16 * sub);
         }
-      } else {
-        unpack8(*reinterpret_cast<const u32x4*>(rows + (int64_t)r * (2 * D) + 16 * sub), x);
       }
 #pragma unroll
-      for (int e = 0; e < 8; ++e) lo[e] = least(lo[e], x[e]), hi[e] = largest(hi[e], x[e]);
+      for (int k = 0; k < kAtOnce; ++k) {
+        float x[8];
+        if constexpr (FP8) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const bf16x2 two = (e & 1) ? fp8x2_to_bf16<true>(raw[k][e >> 1]) : fp8x2_to_bf16<false>(raw[k][e >> 1]);
+            x[2 * e] = (float)two[0] * scale[k], x[2 * e + 1] = (float)two[1] * scale[k];
+          }
+        } else {
+          unpack8(raw[k], x);
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) lo[e] = least(lo[e], x[e]), hi[e] = largest(hi[e], x[e]);
+      }
     }
     __syncthreads();  // the page before has been read
 #pragma unroll
@@ -200,6 +235,9 @@ extern "C" int pith_kv_append(const pith_kv_append_args* a, pith_stream_t stream
     return fail(PITH_ERR_BAD_SHAPE, "%s: T = %lld tokens, %lld query heads (1 to 1024), tables of %lld positions", who, (long long)a->T, (long long)a->H, (long long)a->P);
   if (a->T == 0) return PITH_OK;
   if (a->T * (a->H + 2 * heads) > 0x7fffffff - 64) return fail(PITH_ERR_UNSUPPORTED, "%s: 2^31 rows or more in a call", who);
+  const int64_t far = 0x3fffffff;  // offsets within a token are counted in 32 bits
+  if (a->H * a->q_hs > far || a->H * a->q_out_hs > far || heads * a->k_hs > far || heads * a->v_hs > far)
+    return fail(PITH_ERR_UNSUPPORTED, "%s: heads of a token that lie 2^30 elements apart", who);
   if (!a->q || !a->k || !a->v || !a->q_out || !a->cos || !a->sin || !a->position_ids || !a->slots || (a->q_weight == nullptr) != (a->k_weight == nullptr))
     return fail(PITH_ERR_NULL_POINTER, "%s: a required pointer is NULL (the weights are given together or not at all)", who);
   if (a->q_weight && a->weight_dtype != PITH_BF16 && a->weight_dtype != PITH_F32) return fail(PITH_ERR_BAD_DTYPE, "%s: weight_dtype %d", who, a->weight_dtype);
@@ -214,11 +252,14 @@ extern "C" int pith_kv_append(const pith_kv_append_args* a, pith_stream_t stream
   p.q = (const __bf16*)a->q; p.k = (const __bf16*)a->k; p.v = (const __bf16*)a->v; p.q_out = (__bf16*)a->q_out;
   p.q_weight = a->q_weight; p.k_weight = a->k_weight; p.cos = (const __bf16*)a->cos; p.sin = (const __bf16*)a->sin;
   p.pos = a->position_ids; p.slots = a->slots; p.P = a->P; p.rows = a->cache.pages * a->cache.page_size;
-  p.q_ts = a->q_ts; p.q_hs = a->q_hs; p.k_ts = a->k_ts; p.k_hs = a->k_hs; p.v_ts = a->v_ts; p.v_hs = a->v_hs; p.q_out_ts = a->q_out_ts; p.q_out_hs = a->q_out_hs;
-  p.per_token = (int)(a->H + 2 * heads); p.total = (int)(a->T * p.per_token); p.H = (int)a->H; p.eps = a->eps;
+  p.q_ts = a->q_ts; p.k_ts = a->k_ts; p.v_ts = a->v_ts; p.q_out_ts = a->q_out_ts;
+  p.q_hs = (int)a->q_hs; p.k_hs = (int)a->k_hs; p.v_hs = (int)a->v_hs; p.q_out_hs = (int)a->q_out_hs;
+  p.T = (int)a->T; p.H = (int)a->H; p.eps = a->eps;
   p.cache = to_device(a->cache);
-  const int per_block = kThreads / (int)(dim / 8);
-  const unsigned grid = (unsigned)(((int64_t)p.total + per_block - 1) / per_block);
+  const int64_t per_piece = 512 / dim, pieces = (a->H + per_piece - 1) / per_piece + 2 * ((heads + per_piece - 1) / per_piece);
+  p.per_wave = a->T >= kManyTokens ? (int)pieces : 1;
+  const int64_t waves = a->T * ((pieces + p.per_wave - 1) / p.per_wave);
+  const unsigned grid = (unsigned)((waves + kThreads / 64 - 1) / (kThreads / 64));
   hipStream_t s = (hipStream_t)stream;
   begin_launch();
   const bool fp8 = a->cache.dtype == PITH_FP8_E4M3;

@@ -3,8 +3,9 @@
 // Everything is prefix sums over the requests: offsets are sums of the counts; pages that ended requests return go behind the pool's at sums of what they
 // held; pages that are taken come off its top at sums of what is needed. A request is served if what is needed up to it and it included does not exceed the
 // pool, or it needs nothing: sums only grow, so the served ones that need pages are a beginning of the list, and the order decides, not the schedule.
-// One workgroup does that; few tokens are its work too, many go to a second launch. All of it is latency: a step of 32 requests moves 1 KB.
-#include "latent_common.h"
+// One workgroup does that; few tokens are its work too, many go to a second launch. All of it is latency: a step of 32 requests moves 1 KB. Up to 64
+// requests are a lane each and need no barrier for their sums: 32 tokens FIGURE.
+#include "cache_attn.h"
 #include "pith_kv.h"
 
 namespace pith {
@@ -177,6 +178,83 @@ __global__ __launch_bounds__(256) void place_kernel(PlanParams p) {
   if (t < p.T) place_token(p, t, *p.top, [&](int i) { return (int64_t)p.cu_q[i]; }, [&](int i) { return p.requests[i]; });
 }
 
+// The same for up to 64 requests, a lane each: every wave forms all sums by itself, and looks a token's request up among its lanes. (LDS and barriers only
+// where pages come back.)
+__global__ __launch_bounds__(kThreads) void plan_few_kernel(PlanParams p) {
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
+  const int page = 1 << p.page_shift;
+  const bool some = lane < p.B;
+  const int most = (int)(p.table_width << p.page_shift), tokens = (int)p.T;
+  const int count = some ? p.counts[lane] : 0;
+  const int length = some ? min(max(p.lengths[lane], 0), most) : 0;
+  const int64_t had = min(max((int64_t)p.free_count[0], (int64_t)0), p.pool);
+  const auto pages_of = [&](int rows) { return (int)(((unsigned)rows + page - 1) >> p.page_shift); };
+  const int held = pages_of(length);
+
+  int64_t back = 0;
+  __syncthreads();  // every wave has read what the first will write
+  if (__any(count < 0)) {
+    int64_t upto = count < 0 ? held : 0;
+    const int64_t mine = upto;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const int64_t y = __shfl_up(upto, d);
+      if (lane >= d) upto += y;
+    }
+    back = __shfl(upto, 63);
+    for (int r = wave; r < p.B; r += waves) {
+      const int n = (int)__shfl(mine, r);
+      const int64_t base = had + __shfl(upto - mine, r);
+      for (int k = lane; k < n; k += 64)
+        if (base + k < p.pool) p.free_pages[base + k] = p.table[r * p.table_rs + k];
+    }
+    __syncthreads();  // what was laid on the pool is there
+  }
+  const int64_t top = min(had + back, p.pool);
+
+  const int wanted = min(max(count, 0), tokens);  // (their sum is at most 64 * 8192)
+  const int upto = wave_scan(wanted), first = min(upto - wanted, tokens), last = min(upto, tokens), rows = last - first;
+  const bool fits = count >= 0 && rows <= most - length;
+  const int need = fits ? pages_of(length + rows) - held : 0;
+  const int needed = wave_scan(need), taken = needed - need;
+  const bool served = fits && (need == 0 || needed <= top);
+  if (wave == 0) {
+    if (some) {
+      p.granted[lane] = served ? rows : 0;
+      p.lengths_out[lane] = count < 0 ? 0 : length + (served ? rows : 0);
+      p.cu_q[lane + 1] = last;
+    }
+    const int all = wave_scan_max(served && need > 0 ? needed : 0);
+    if (lane == 63) {
+      p.cu_q[0] = 0;
+      p.free_count_out[0] = (int32_t)(top - all);
+    }
+  }
+  const int end = __builtin_amdgcn_readlane(last, 63);
+  for (int t0 = wave * 64; t0 < tokens; t0 += 64 * waves) {
+    const int t = t0 + lane;
+    int r = 0;  // requests that end at or before t
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1)
+      if (__shfl(last, r + d - 1) <= t) r += d;
+    r = min(r, 63);
+    const int position = __shfl(length, r) + t - __shfl(first, r), index = position >> p.page_shift, in_page = position & (page - 1);
+    const int beyond = index - __shfl(held, r);
+    const int64_t at = top - 1 - __shfl(taken, r) - beyond;
+    int64_t slot = -1;
+    if (__shfl((int)served, r) && t < end) {
+      int32_t* const entry = p.table + r * p.table_rs + index;
+      const int32_t number = beyond < 0 ? *entry : p.free_pages[at];
+      if (beyond >= 0 && in_page == 0) *entry = number;
+      slot = ((int64_t)number << p.page_shift) + in_page;
+    }
+    if (t < tokens) {
+      p.positions[t] = t < end ? position : 0;
+      p.slots[t] = slot;
+    }
+  }
+}
+
 constexpr int64_t kTokensInOne = 8192;
 bool in_one(const pith_plan_step_args* a) { return a->B <= kInOne && a->T <= kTokensInOne; }
 
@@ -224,7 +302,10 @@ extern "C" int pith_plan_step(const pith_plan_step_args* a, pith_stream_t stream
   p.B = (int)a->B; p.page_shift = __builtin_ctzll((unsigned long long)a->page_size);
   hipStream_t s = (hipStream_t)stream;
   begin_launch();
-  if (one) {
+  if (one && a->B <= 64) {
+    const int64_t threads = (a->T + 63) & ~(int64_t)63;
+    plan_few_kernel<<<1, (unsigned)(threads < 64 ? 64 : threads > kThreads ? kThreads : threads), 0, s>>>(p);
+  } else if (one) {
     plan_kernel<true><<<1, kThreads, 0, s>>>(p);
   } else {
     p.top = (int64_t*)a->workspace;

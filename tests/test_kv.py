@@ -184,7 +184,7 @@ CALLS = {
         (dict(counts=258), ALIGN), (dict(workspace=264), ALIGN)]),
     "pith_kv_append": (_append, [
         (dict(q=None), NULL), (dict(v=None), NULL), (dict(q_out=None), NULL), (dict(slots=None), NULL), (dict(q_weight=None), NULL), (dict(T=-1), SHAPE), (dict(P=0), SHAPE), (dict(H=0), SHAPE),
-        (dict(H=1025), SHAPE), (dict(T=0x7fffffff), UNSUPPORTED), (dict(q_ts=120), SHAPE), (dict(k_hs=64), SHAPE), (dict(v_ts=64), SHAPE), (dict(q_out_hs=120), SHAPE), (dict(q_ts=516), ALIGN),
+        (dict(H=1025), SHAPE), (dict(T=0x7fffffff), UNSUPPORTED), (dict(q_hs=1 << 29), UNSUPPORTED), (dict(q_ts=120), SHAPE), (dict(k_hs=64), SHAPE), (dict(v_ts=64), SHAPE), (dict(q_out_hs=120), SHAPE), (dict(q_ts=516), ALIGN),
         (dict(v_hs=132), ALIGN), (dict(k=264), ALIGN), (dict(cos=264), ALIGN), (dict(k_weight=264), ALIGN), (dict(slots=260), ALIGN), (dict(weight_dtype=2), DTYPE)]),
     "pith_kv_attn": (_attn, TABLES + [
         (dict(q=None), NULL), (dict(workspace=None), NULL), (dict(lse=None), NULL), (dict(H=0), SHAPE), (dict(H=3), SHAPE), (dict(H=1026), SHAPE), (dict(q_hs=120), SHAPE), (dict(o_ts=120), SHAPE),
