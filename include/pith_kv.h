@@ -140,6 +140,9 @@ typedef struct {
 } pith_kv_attn_args;
 
 int64_t pith_kv_attn_workspace_bytes(const pith_kv_attn_args* args);
+/* Query rows to a row block of the kernel that such a call takes, 16, 32 or 64; 0 for a call that launches nothing or is rejected for its sizes. A row's
+ * keys are cut, and its sums ordered, by that and by the lengths of all sequences of the call. */
+int pith_kv_attn_rows(const pith_kv_attn_args* args);
 int pith_kv_attn(const pith_kv_attn_args* args, pith_stream_t stream);
 
 /* ------------------------------------------------------------------------------------------

@@ -31,6 +31,8 @@
 #include "cache_attn.h"
 #include "kv_common.h"
 
+#include <type_traits>
+
 namespace pith {
 
 constexpr int kKVThreads = 256, kKVWaves = 4;
@@ -309,6 +311,19 @@ struct KVLoads {
   __device__ __forceinline__ void values(const KVAttnParams& p, char* slot, int source) const { rows(p.cache.v, p.cache.v_ps, slot + T::kBytes, source); }
 };
 
+// Query rows row0 .. of a sequence and head into LDS, laid out like keys of bf16: 1 KB a request, every lane from an address of its own. (Loads of the compiler's
+// would make it wait for everything that is under way at their first use, in every turn of the loop.) Rows behind the block's last one are that one.
+template <int D, int R>
+__device__ __forceinline__ void stage_rows(const KVAttnParams& p, const KVWork& s, int head, int row0, int rows, char* area, int lane) {
+  using T = KVTile<D, false>;
+#pragma unroll
+  for (int n = 0; n < R * D / 32; ++n) {
+    const int row = (1024 * n + 16 * lane) / T::kRow, piece = (lane % (T::kRow / 16)) ^ (kv_swizzle<T::kRow>(row));
+    const int at = row0 + min(row, rows - 1), tok = at / p.group;
+    load_lds16_at(p.q + (int64_t)(s.tok0 + tok) * p.q_ts + (int64_t)(head * p.group + at - tok * p.group) * p.q_hs + 8 * piece, area + 1024 * n);
+  }
+}
+
 // Until all but the last `later` tiles' requests and EXTRA more are there.
 template <int D, bool FP8, int EXTRA>
 __device__ __forceinline__ void wait_tiles(int later) {
@@ -318,6 +333,7 @@ __device__ __forceinline__ void wait_tiles(int later) {
   else if (later == 1) wait_loads<kAll + EXTRA>();
   else wait_loads<EXTRA>();
 }
+
 
 // Operand A over 32 keys, features 16 n ..; `first`: lds_address of the values + the lane's place. Element 4 h + v: key 16 h + 4 g + v.
 template <int D, bool FP8>
@@ -351,21 +367,22 @@ __device__ __forceinline__ int key_of(int g, int e) { return 16 * (e >> 2) + 4 *
 
 // Which of a lane's eight keys from key0 on a row of token tok sees: bit e. In the last tiles of a sequence only, so what a token sees is looked up anew there.
 __device__ __forceinline__ uint32_t seen_keys(const KVAttnParams& p, const KVWork& s, int tok, int key0, int g) {
-  uint32_t lo = 0, hi = 0;
-  if (p.tree) {
-    const uint64_t word = (uint64_t)p.tree[s.tok0 + tok];
-    lo = (uint32_t)word;
-    hi = (uint32_t)(word >> 32);
-  }
   const int ctx = s.len - s.n;  // rows in front of the new ones (below zero only where the lengths contradict each other)
   uint32_t seen = 0;
+  if (p.tree) {
+    const uint64_t word = (uint64_t)p.tree[s.tok0 + tok];
+    const uint32_t lo = (uint32_t)word, hi = (uint32_t)(word >> 32);
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const int key = key0 + key_of(g, e), draft = key - ctx;
-    const uint32_t bits = draft < 32 ? lo : hi;
-    const int by_word = (draft < 0) | ((draft < 64) & (int)((bits >> (draft & 31)) & 1u));
-    const int ok = (p.tree ? by_word : (int)(draft <= tok)) & (int)(key < s.len);
-    seen |= (uint32_t)ok << e;
+    for (int e = 0; e < 8; ++e) {
+      const int key = key0 + key_of(g, e), draft = key - ctx;
+      const uint32_t bits = draft < 32 ? lo : hi;
+      const int ok = ((draft < 0) | ((draft < 64) & (int)((bits >> (draft & 31)) & 1u))) & (int)(key < s.len);
+      seen |= (uint32_t)ok << e;
+    }
+  } else {
+    const int end = min(ctx + tok + 1, s.len);  // keys that the row sees
+#pragma unroll
+    for (int e = 0; e < 8; ++e) seen |= (uint32_t)(key0 + key_of(g, e) < end) << e;
   }
   return seen;
 }
@@ -436,6 +453,8 @@ __device__ __forceinline__ void clean_values(char* values, int lane, const uint3
 
 // ---------------------------------------------------------------------------------------------
 
+// (At most 256 registers for up to 32 rows: with more at hand the compiler keeps the results in the accumulators' half of the file, and moves them out and
+// back for every rescaling that may come.)
 template <int D, bool FP8, int R>
 __global__ __launch_bounds__(kKVThreads, 1) void kv_attn_kernel(KVAttnParams p) {
   using T = KVTile<D, FP8>;
@@ -483,12 +502,7 @@ __global__ __launch_bounds__(kKVThreads, 1) void kv_attn_kernel(KVAttnParams p) 
     uint32_t up[R], down[R];  // see clean_values
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      const int row = row0 + min(16 * r + c, rows - 1);
-      tok[r] = row / p.group;
-      const __bf16* const from = p.q + (int64_t)(s.tok0 + tok[r]) * p.q_ts + (int64_t)(head * p.group + row - tok[r] * p.group) * p.q_hs;
-#pragma unroll
-      for (int i = 0; i < kSteps; ++i)  // e4m3 keys are read 16 features at a time: steps 2 i, 2 i + 1 contract features 64 i + 16 g + {0..7, 8..15}
-        q[r][i] = *reinterpret_cast<const bf16x8*>(from + (FP8 ? 64 * (i >> 1) + 16 * g + 8 * (i & 1) : 32 * i + 8 * g));
+      tok[r] = (row0 + min(16 * r + c, rows - 1)) / p.group;
 #pragma unroll
       for (int n = 0; n < D / 16; ++n) acc[r][n] = f32x4{};
       m[r] = -INFINITY;
@@ -502,14 +516,34 @@ __global__ __launch_bounds__(kKVThreads, 1) void kv_attn_kernel(KVAttnParams p) 
 #pragma unroll
       for (int h = 0; h < 2; ++h) pages[h] = table[min(key_of_tile(i) + 16 * h, last) >> p.cache.page_shift];
     };
-#pragma unroll 1
-    for (int i = 0; i < min(T::kSlots, n_tiles); ++i) {
+    const auto request = [&](int i) __attribute__((always_inline)) {  // one of the first tiles
       look_up(i);
       const Loads loads(p, pages, key_of_tile(i), last, head);
       loads.keys(p, ring + i * T::kSlot, source, lane);
       loads.values(p, ring + i * T::kSlot, source);
+    };
+    // The queries come through the last slots of the ring, behind the first tiles in the LDS and in front of them in the queue.
+    constexpr int kQuerySlots = (M * 2 * D + T::kSlot - 1) / T::kSlot, kFirst = T::kSlots - kQuerySlots;
+    static_assert(kFirst >= 1, "a tile beside the queries");
+    if (n_tiles > 0) {
+      char* const staged = ring + kFirst * T::kSlot;
+      stage_rows<D, R>(p, s, head, row0, rows, staged, lane);
+#pragma unroll 1
+      for (int i = 0; i < min(kFirst, n_tiles); ++i) request(i);
+      wait_tiles<D, FP8, 0>(min(kFirst, n_tiles));
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i) {  // e4m3 keys are read 16 features at a time: steps 2 i, 2 i + 1 contract features 64 i + 16 g + {0..7, 8..15}
+          const int piece = FP8 ? 8 * (i >> 1) + 2 * g + (i & 1) : 4 * i + g;
+          q[r][i] = *reinterpret_cast<const bf16x8*>(staged + KVTile<D, false>::place(16 * r + c, piece));
+        }
+      __builtin_amdgcn_s_waitcnt(0xC07F);  // the queries have been read
+      asm volatile("" ::: "memory");
+#pragma unroll 1
+      for (int i = kFirst; i < min(T::kSlots, n_tiles); ++i) request(i);
+      look_up(T::kSlots);
     }
-    look_up(T::kSlots);
     int slot_at = 0;
 #pragma unroll 1
     for (int i = 0; i < n_tiles; ++i) {
@@ -520,33 +554,45 @@ __global__ __launch_bounds__(kKVThreads, 1) void kv_attn_kernel(KVAttnParams p) 
       wait_tiles<D, FP8, T::kLoads>(later);  // the keys
       f32x4 score[R][2];
       float k_scale[8], v_scale[8];
-      {
+      {  // all fragments are asked for before the first product: an LDS read takes as long as several of them
+        constexpr int kReads = FP8 ? kSteps / 2 : kSteps;  // of a half tile
+        typename std::conditional<FP8, u32x4, bf16x8>::type raw[2][kReads];
         const uint32_t first = lds_address(slot) + key_at;
 #pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int j = 0; j < kReads; ++j) raw[h][j] = *lds_at<typename std::conditional<FP8, u32x4, bf16x8>::type>((h == 0 ? first ^ (64 * j) : (first ^ kUpperXor ^ (64 * j)) + kUpperKey));
+        f32x4 scales[4];
+        if constexpr (FP8)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            scales[h] = *reinterpret_cast<const f32x4*>(slot + 2 * T::kBytes + 4 * (16 * h + 4 * g));
+            scales[2 + h] = *reinterpret_cast<const f32x4*>(slot + 2 * T::kBytes + 128 + 4 * (16 * h + 4 * g));
+          }
+        if constexpr (R <= 2) __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const uint32_t row = h == 0 ? first : (first ^ kUpperXor) + kUpperKey;
 #pragma unroll
           for (int r = 0; r < R; ++r) score[r][h] = f32x4{};
 #pragma unroll
-          for (int j = 0; j < (FP8 ? kSteps / 2 : kSteps); ++j) {
+          for (int j = 0; j < kReads; ++j) {
             if constexpr (FP8) {
-              const u32x4 raw = *lds_at<u32x4>(row ^ (64 * j));
-              const bf16x8 k0 = widen(raw[0], raw[1]), k1 = widen(raw[2], raw[3]);
+              const bf16x8 k0 = widen(raw[h][j][0], raw[h][j][1]), k1 = widen(raw[h][j][2], raw[h][j][3]);
 #pragma unroll
-              for (int r = 0; r < R; ++r) score[r][h] = mfma16(k1, q[r][2 * j + 1], mfma16(k0, q[r][2 * j], score[r][h]));
+              for (int r = 0; r < R; ++r) score[r][h] = mfma16(k0, q[r][2 * j], score[r][h]);
+#pragma unroll
+              for (int r = 0; r < R; ++r) score[r][h] = mfma16(k1, q[r][2 * j + 1], score[r][h]);
             } else {
-              const bf16x8 k = *lds_at<bf16x8>(row ^ (64 * j));
 #pragma unroll
-              for (int r = 0; r < R; ++r) score[r][h] = mfma16(k, q[r][j], score[r][h]);
+              for (int r = 0; r < R; ++r) score[r][h] = mfma16(raw[h][j], q[r][j], score[r][h]);
             }
           }
-          if constexpr (FP8) {
-            const f32x4 a = *reinterpret_cast<const f32x4*>(slot + 2 * T::kBytes + 4 * (16 * h + 4 * g));
-            const f32x4 b = *reinterpret_cast<const f32x4*>(slot + 2 * T::kBytes + 128 + 4 * (16 * h + 4 * g));
-#pragma unroll
-            for (int v = 0; v < 4; ++v) k_scale[4 * h + v] = a[v] * p.kappa, v_scale[4 * h + v] = b[v];
-          }
         }
+        if constexpr (FP8)
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int v = 0; v < 4; ++v) k_scale[4 * h + v] = scales[h][v] * p.kappa, v_scale[4 * h + v] = scales[2 + h][v];
       }
       const bool partial = key0 + kTileKeys > s.len - s.n + (p.tree ? 0 : 1);  // some row may not see all of it
       bf16x8 weight[R];
@@ -583,6 +629,7 @@ __global__ __launch_bounds__(kKVThreads, 1) void kv_attn_kernel(KVAttnParams p) 
           for (int e = 0; e < 8; ++e) y[e] = scaled(y[e], v_scale[e]);
         }
         weight[r] = to_bf16x8(y[0], y[1], y[2], y[3], y[4], y[5], y[6], y[7]);
+        if constexpr (R > 2) __builtin_amdgcn_sched_barrier(0);
       }
       const Loads loads(p, pages, key_of_tile(i + T::kSlots), last, head);
       if (more) {  // (the keys have been read: their products have been used)
@@ -594,11 +641,17 @@ __global__ __launch_bounds__(kKVThreads, 1) void kv_attn_kernel(KVAttnParams p) 
       }
       if (partial) clean_values<D, FP8, R>(slot + T::kBytes, lane, seen, up, down);
       const uint32_t values = lds_address(slot) + value_at;
+      constexpr int kAhead = R <= 2 ? D / 16 : 4;  // fragments asked for at once (64 rows: as registers allow)
 #pragma unroll
-      for (int n = 0; n < D / 16; ++n) {
-        const bf16x8 v = kv_value_fragment<D, FP8>(values, n);
+      for (int n0 = 0; n0 < D / 16; n0 += kAhead) {
+        bf16x8 v[kAhead];
 #pragma unroll
-        for (int r = 0; r < R; ++r) acc[r][n] = mfma16(v, weight[r], acc[r][n]);
+        for (int n = 0; n < kAhead; ++n) v[n] = kv_value_fragment<D, FP8>(values, n0 + n);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int n = 0; n < kAhead; ++n)
+#pragma unroll
+          for (int r = 0; r < R; ++r) acc[r][n0 + n] = mfma16(v[n], weight[r], acc[r][n0 + n]);
       }
       if (more) {
         __builtin_amdgcn_s_waitcnt(0xC07F);  // the values have been read

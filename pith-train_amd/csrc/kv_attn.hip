@@ -97,25 +97,34 @@ struct KVPlan {
   int64_t joins_at, stats_at, results_at, bytes;  // workspace
 };
 
+// Steps (of 16 rows) up to which no row block is cut: below it the join's launch (4 us) costs more than what the cut gains. One sequence of 517 rows, 4 heads,
+// 9.5 us whole and 10.6 cut; 32 x 4 heads of 16 selected pages 18.8 and 18.6.
 constexpr int64_t kWholeSteps = 8;
 
 KVPlan plan_of(const pith_kv_attn_args* a) {
   KVPlan pl = {};
-  const int64_t rows = a->T * (a->H / a->cache.heads);  // of a key-value head
-  pl.row_groups = rows <= 16 * a->B ? 1 : rows <= 32 * a->B ? 2 : 4;
-  const int64_t m = 16 * pl.row_groups;
-  pl.max_items = ((rows + m - 1) / m + std::min(a->B, a->T)) * a->cache.heads;
+  const int units = compute_units_or_default() & ~7;
+  const int64_t group = a->H / a->cache.heads, rows = a->T * group;  // rows of a key-value head
   const int64_t steps = (a->table_width * a->cache.page_size + kStepKeys - 1) / kStepKeys;
-  if (steps <= kWholeSteps) {
+  const auto items = [&](int64_t m) { return ((rows + m - 1) / m + std::min(a->B, a->T)) * a->cache.heads; };
+  // Rows of a row block. Fewer bytes with more of them, but every workgroup begins and ends with 64 rows more slowly, and rows that are not there are computed
+  // all the same; so it goes by the rows of a sequence and by the steps that a workgroup has with blocks of 16 and full page tables. us at 16 / 32 / 64
+  // rows, bf16, heads of 32 / 4: 32 x 8192 rows, 2 tokens 74 / 76 / 82, 4 tokens 108 / 81 / 85, 8 tokens 198 / 117 / 93; 8 tokens: 16 x 8192 (80 steps)
+  // 106 / 65 / 52, 8 x 8192 (40) 63 / 32 / 34, 16 x 2048 (20) 30 / 25 / 29, 4 x 4096 (10) 19 / 20 / 24; 16 tokens, e4m3, 16 x 2048 (36) 53 / 47 / 41; 512
+  // tokens behind 8192 (257) 214 / 157 / 116.
+  const int64_t work = items(16) * steps / std::max(units, 8);
+  pl.row_groups = rows <= 16 * a->B || work <= 14 ? 1 : rows <= 32 * a->B || work <= 36 ? 2 : 4;
+  const int64_t m = 16 * pl.row_groups;
+  pl.max_items = items(m);
+  if (steps * pl.row_groups <= kWholeSteps) {
     pl.whole = (int)steps;
     pl.workgroups = (int)((pl.max_items + 7) & ~(int64_t)7);
     pl.bytes = 256;
     return pl;
   }
-  const int units = compute_units_or_default() & ~7;
   pl.workgroups = units < 8 ? 8 : units > kMaxGroups ? kMaxGroups : units;
   if (a->head_tables) {
-    pl.max_items = (a->H / a->cache.heads + m - 1) / m * a->cache.heads * a->B;
+    pl.max_items = (group + m - 1) / m * a->cache.heads * a->B;
     pl.parts = (int)std::min(std::max<int64_t>(pl.workgroups / pl.max_items, 1), steps);
     pl.workgroups = (int)((pl.max_items * pl.parts + 7) & ~(int64_t)7);
   }
@@ -150,6 +159,11 @@ using namespace pith;
 extern "C" int64_t pith_kv_attn_workspace_bytes(const pith_kv_attn_args* a) {
   if (check_attn(a, "pith_kv_attn_workspace_bytes") != PITH_OK || a->T == 0 || a->B == 0) return 0;
   return plan_of(a).bytes;
+}
+
+extern "C" int pith_kv_attn_rows(const pith_kv_attn_args* a) {
+  if (check_attn(a, "pith_kv_attn_rows") != PITH_OK || a->T == 0 || a->B == 0) return 0;
+  return 16 * plan_of(a).row_groups;
 }
 
 extern "C" int pith_kv_attn(const pith_kv_attn_args* a, pith_stream_t stream) {

@@ -275,6 +275,7 @@ KV_SYMBOLS = {
     "pith_plan_step": (c_int, [POINTER(PlanStepArgs), c_void_p]),
     "pith_kv_append": (c_int, [POINTER(KVAppendArgs), c_void_p]),
     "pith_kv_attn_workspace_bytes": (c_int64, [POINTER(KVAttnArgs)]),
+    "pith_kv_attn_rows": (c_int, [POINTER(KVAttnArgs)]),
     "pith_kv_attn": (c_int, [POINTER(KVAttnArgs), c_void_p]),
     "pith_kv_bounds": (c_int, [POINTER(KVBoundsArgs), c_void_p]),
     "pith_kv_select_workspace_bytes": (c_int64, [POINTER(KVSelectArgs)]),

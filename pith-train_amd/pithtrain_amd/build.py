@@ -42,7 +42,11 @@ HIPCC_FLAGS = [
 # them / after / with loops on 64 bytes: 2146 x 4 heads, 8 ranks, rank 3 358 / 368 / 356, 848 x 16, rank 0 221 / 225 / 220, 3 x 1856 x 4, rank 6
 # contiguous 401 / 410 / 401; 95 such shares 0.7 % faster, 205 of 128 and 192 features equal. Not the forward (all files aligned: 2884 x 8/2 of 128
 # without a mask 43.8 / 47.8).
-SOURCE_FLAGS = {"attn_bwd_chunks.hip": ["-falign-loops=64"]}
+# Attention to the key-value cache: with 512 registers a lane at hand the compiler would keep the results of matrix instructions in the accumulators' half of
+# the file, and move them out and back around every rescaling that may come; with 64 query rows it then spills inside the loop, whose reloads wait for every tile
+# under way. In the common half nothing spills (32 sequences of 8 tokens over up to 8192 rows, 64 query rows: FIGURE us).
+KV_ATTN_FLAGS = ["-mllvm", "-amdgpu-mfma-vgpr-form"]
+SOURCE_FLAGS = {"attn_bwd_chunks.hip": ["-falign-loops=64"], "kv_attn.hip": KV_ATTN_FLAGS, "kv_attn_d64.hip": KV_ATTN_FLAGS}
 
 
 def _hipcc() -> str:

@@ -233,8 +233,19 @@ def test_workspaces():
     assert plan() == 0 and plan(T=1 << 20) > 0 and plan(B=5000) >= 16 * 5000 and plan(page_size=8) == 0
     attn = lambda **kw: lib.pith_kv_attn_workspace_bytes(ctypes.byref(_attn(**kw)))  # noqa: E731
     assert attn(T=0) == attn(B=0) == attn(H=3) == 0 and attn() > 0
+    assert attn(table_width=4096, table_rs=4096) == attn(table_width=64, table_rs=64)  # whatever the lengths
     select = lambda **kw: lib.pith_kv_select_workspace_bytes(ctypes.byref(_select(**kw)))  # noqa: E731
     assert select() == 4 * 2 * 64 * 4 and select(T=0) == select(keep=0) == 0 and select(table_width=65) == 2 * select()
+
+
+def test_rows_of_a_row_block_go_by_the_rows_of_a_sequence_and_the_work_list():
+    rows = lambda **kw: _C.lib().pith_kv_attn_rows(ctypes.byref(_attn(**kw)))  # noqa: E731
+    assert rows(T=0) == rows(B=0) == rows(H=3) == 0  # nothing to launch, or what pith_kv_attn rejects
+    wide = dict(table_width=4096, table_rs=4096)
+    assert rows(T=16, lse_hs=16, **wide) == 16  # sixteen rows a sequence and key-value head
+    assert rows(T=17, lse_hs=17, **wide) == 32 and rows(T=32, lse_hs=32, **wide) == 32
+    assert rows(T=33, lse_hs=33, **wide) == 64
+    assert rows(T=64, lse_hs=64, table_width=16, table_rs=16) == 16  # and a work list of some length
 
 
 # ---------------------------------------------------------------------------------------------

@@ -19,6 +19,7 @@ import torch
 
 from oracle import kv_oracle as O
 from oracle import prologue_oracle as P
+from pithtrain_amd import _C
 from pithtrain_amd.operators import paging
 from pithtrain_amd.operators.gqa import kv_cache as K
 from pithtrain_amd.operators.mla import latent as L
@@ -43,18 +44,21 @@ def _within(got, want, bound, what):
 # Attention
 
 
+MIN_WIDTH = 0  # of page tables: blocks of more than 16 query rows are for those that are wide
+
+
 class Batch:
     """Sequences in a cache. counts: new tokens of each, lengths: cached rows of each. Everything that no sequence owns (rows behind the last one of a
     page, pages of nobody, table entries that are not needed) holds NaN or nonsense."""
 
-    def __init__(self, dev, counts, lengths, heads=(8, 2, 128), page=64, fp8=False, tree=None, seed=0, extra_tokens=0, q_std=1.0, width=0):
+    def __init__(self, dev, counts, lengths, heads=(8, 2, 128), page=64, fp8=False, tree=None, seed=0, extra_tokens=0, q_std=1.0):
         g = torch.Generator().manual_seed(seed)
         mk = lambda *s: torch.randn(*s, generator=g)  # noqa: E731
         self.h, self.hkv, self.d = heads
         self.counts, self.lengths, self.dev, self.page, self.scale = counts, lengths, dev, page, self.d**-0.5
         t = sum(counts) + extra_tokens
         need = [-(-n // page) for n in lengths]
-        pages, width = sum(need) + 3, max(max(need), 1, width) + 1
+        pages, width = sum(need) + 3, max(max(need), 1, MIN_WIDTH) + 1
         order = torch.randperm(pages, generator=g)
         table = torch.randint(-5, 2 * pages, (len(counts), width), generator=g).to(I32)  # entries behind a sequence's pages are never followed
         at = 0
@@ -196,6 +200,66 @@ def test_tree_attention_matches_the_oracle(gpu, counts, lengths, heads, kind, fp
     b.check(o, lse, kind)
     if kind == "holes" and lengths == [1]:
         assert (o == 0).all() and (lse == -math.inf).all()
+
+
+# Blocks of 32 and 64 rows: the same tests with page tables so wide that calls of more than 16 rows a sequence take them.
+def _rows_of(b):
+    c = _C.KVCacheArgs(k=256, v=256, pages=1, page_size=b.page, heads=b.hkv, dim=b.d, dtype=_C.PITH_BF16)
+    args = _C.KVAttnArgs(cache=c, cu_q=256, T=b.q.shape[0], B=len(b.counts), H=b.h, table_width=b.table.shape[1])
+    return _C.lib().pith_kv_attn_rows(_C.byref(args))
+
+
+def _wide(monkeypatch, rows):
+    """Page tables that make sure of it; returns what checks it."""
+    monkeypatch.setitem(globals(), "MIN_WIDTH", 1 << 16)
+
+    def taken(b):
+        assert _rows_of(b) == rows
+
+    return taken
+
+
+@BOTH
+@pytest.mark.parametrize("rows, heads", [(32, (16, 2, 128)), (64, (32, 2, 128)), (64, (32, 2, 64)), (32, (16, 2, 64)), (64, (74, 2, 128)), (64, (35, 1, 64))], ids=str)
+@pytest.mark.parametrize("name", ["none", "few_tokens", "prompt", "contradiction"])
+def test_blocks_of_more_rows_match_the_oracle(gpu, monkeypatch, name, rows, heads, fp8):
+    taken = _wide(monkeypatch, rows)
+    counts, lengths = LENGTH_SETS[name]
+    b = Batch(gpu, counts, lengths, heads, page=16 if name == "prompt" else 64, fp8=fp8, seed=len(name))
+    if name == "few_tokens":
+        taken(b)
+    b.check(*b.attention(), name)
+
+
+@BOTH
+@pytest.mark.parametrize("rows, heads, counts, lengths", [
+    (32, (4, 1, 128), [8, 4], [20011, 300]), (64, (8, 1, 64), [63], [9001]), (32, (16, 2, 128), [2, 0, 9] * 40, list(range(7, 127))), (64, (24, 2, 128), [3, 0, 9] * 40, list(range(9, 129))), (32, (3, 1, 64), [8] * 70, list(range(50, 120)))],
+    ids=["long", "longer", "many", "many_more", "odd"])  # fmt: skip
+def test_work_lists_of_blocks_of_more_rows(gpu, monkeypatch, rows, heads, counts, lengths, fp8):
+    taken = _wide(monkeypatch, rows)
+    b = Batch(gpu, counts, lengths, heads, page=16, fp8=fp8, seed=15, q_std=1.5)
+    taken(b)
+    b.check(*b.attention())
+
+
+@BOTH
+@pytest.mark.parametrize("kind", ["tree", "holes"])
+@pytest.mark.parametrize("rows, heads", [(32, (4, 2, 128)), (64, (6, 2, 64)), (64, (8, 1, 128))], ids=str)
+def test_trees_in_blocks_of_more_rows_match_the_oracle(gpu, monkeypatch, rows, heads, kind, fp8):
+    taken = _wide(monkeypatch, rows)
+    b = Batch(gpu, [12, 16, 9], [517, 16, 200], heads, page=16, fp8=fp8, tree=kind, seed=rows)
+    taken(b)
+    b.check(*b.attention(), kind)
+
+
+@BOTH
+@pytest.mark.parametrize("tree", [None, "tree"])
+@pytest.mark.parametrize("where", ["key", "value", "scale"])
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("heads", [(8, 2, 128), (14, 1, 64)], ids=str)
+def test_blocks_of_more_rows_are_not_reached_by_rows_that_they_do_not_see(gpu, monkeypatch, bad, where, tree, fp8, heads):
+    _wide(monkeypatch, 0)
+    test_a_row_that_a_token_does_not_see_cannot_reach_it(gpu, bad, where, tree, fp8, heads)
 
 
 def test_a_chain_of_drafts_is_the_causal_call(gpu):
