@@ -4,32 +4,50 @@
 //   score(page) = max over the heads of the group of sum_d max(q_d least_d, q_d largest_d)
 //
 // A choice must not depend on the order of a sum, or the same scores would choose differently elsewhere: products of two bf16 values are exact in fp32, and
-// their sum in fp64 loses nothing that a rounding to fp32 would show. Scores are kept as integers that sort like them, NaN above all.
+// their sum in fp64 loses nothing that a rounding to fp32 would show. But only the pages around the last one chosen need that. So scores are formed by matrix
+// instructions first, sum_d q+_d largest_d + q-_d least_d with q+ and q- the parts of q above and below zero, in fp32, beside the same sum of absolute values,
+// S: 2 D terms, each addition off by at most 2^-23 of S, so that a score is off by at most E = 2^-14 S (twice what the additions can lose; the largest S of all
+// pages). With v the score of the last one chosen by these, a page above v + 2 E is in (whoever may exceed it is above v, too), one below v - 2 E is out, and
+// the few between are summed in fp64, if they are more than there are places. v is found by histograms of 256 equal parts of the range that it lies in, two most
+// often, to within 2 E. Infinities and NaN have no bound of the error: a page with one is summed in fp64 at once. NaN counts above all.
+// A step of 32 tokens with 4 heads over up to 128 pages FIGURE; 8 tokens over up to 2048 pages FIGURE.
+#include "cache_attn.h"
 #include "kv_common.h"
+
+#include <type_traits>
 
 namespace pith {
 namespace {
 
-constexpr int kThreads = 256, kWaves = kThreads / 64;
-constexpr int kChunk = 64;  // pages of a workgroup that scores, one a lane
+constexpr int kThreads = 256;
+constexpr int kChunk = 128;  // pages of a workgroup that scores, sixteen a wave at a time
 
 struct KVSelectParams {
   const __bf16 *q, *bounds;
   const int32_t *table, *lengths, *cu_q;
   int32_t *table_out, *lengths_out;
-  uint32_t* keys;  // [T * heads][row]
+  uint2* pages_of;  // workspace, [T * heads][row]: score and S of each page, then the pages in question
   int64_t q_ts, q_hs, table_rs, bounds_ps, row;
   int T, B, heads, group, pages, page_shift, table_width, keep, chunks;
 };
 
-// Rows that token t sees, 0 for one that is nobody's.
-__device__ __forceinline__ int visible_rows(const KVSelectParams& p, int t, int seq) {
-  const int length = min(max(p.lengths[seq], 0), p.table_width << p.page_shift);
-  if (!p.cu_q) return length;
-  return t < p.cu_q[p.B] ? min(max(length - p.cu_q[seq + 1] + t + 1, 0), length) : 0;
-}
+// A token and key-value head.
+struct Item {
+  int t, head, seq, visible, pages;
+  const int32_t* table;
+};
 
-__device__ __forceinline__ float nan_max(float a, float b) { return b > a || b != b ? b : a; }
+__device__ __forceinline__ Item item_of(const KVSelectParams& p, int item, int lane) {
+  Item x;
+  x.t = item / p.heads;
+  x.head = item - x.t * p.heads;
+  x.seq = sequence_of(p.cu_q, p.B, x.t, lane);
+  const int length = min(max(p.lengths[x.seq], 0), p.table_width << p.page_shift);
+  x.visible = !p.cu_q ? length : x.t < p.cu_q[p.B] ? min(max(length - p.cu_q[x.seq + 1] + x.t + 1, 0), length) : 0;  // (a token that is nobody's: 0)
+  x.pages = (x.visible + (1 << p.page_shift) - 1) >> p.page_shift;
+  x.table = p.table + x.seq * p.table_rs;
+  return x;
+}
 
 __device__ __forceinline__ uint32_t sort_key(float x) {
   if (x != x) return 0xffffffffu;
@@ -37,135 +55,364 @@ __device__ __forceinline__ uint32_t sort_key(float x) {
   return u >> 31 ? ~u : u | 0x80000000u;
 }
 
-// Scores of 64 pages of a token and key-value head: a page a lane, out of LDS (rows of 4 D bytes, piece (16 bytes) k of row r at k ^ r % (D / 4), so that
-// the lanes' reads of one piece spread over the banks); a wave takes two heads of the group at a time.
-template <int D>
-__global__ __launch_bounds__(kThreads) void kv_score_kernel(KVSelectParams p) {
-  constexpr int kPieces = D / 4;  // of a page's bounds: D least, D largest
-  __shared__ __attribute__((aligned(16))) char rows[kChunk * kPieces * 16];
-  __shared__ float best[kWaves][kChunk];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int chunk = blockIdx.x % p.chunks, item = blockIdx.x / p.chunks;  // (token, head)
-  const int t = item / p.heads, head = item - t * p.heads;
-  const int seq = sequence_of(p.cu_q, p.B, t, lane);
-  const int visible = visible_rows(p, t, seq);
-  const int pages = (visible + (1 << p.page_shift) - 1) >> p.page_shift;
-  const int first = chunk * kChunk, n = min(pages - 1 - first, kChunk);  // (the token's own page is not scored)
-  if (pages <= p.keep || n <= 0) return;
-  const int32_t* const table = p.table + seq * p.table_rs + first;
+typedef __attribute__((ext_vector_type(8))) short s16x8;
+
+// Scores and S (infinity: not known) of TILES times sixteen pages, `first` .. and so on, of which `scored` exist: lane c + 16 g has those of page c (whatever g).
+// Operand A is sixteen heads, B sixteen pages, so a lane's results are four heads of one page.
+template <int D, int TILES>
+__device__ __forceinline__ void score_pages(const KVSelectParams& p, const Item& x, int first, int scored, int lane, float2 (&out)[TILES]) {
+  constexpr int kSteps = D / 32;
+  const int c = lane & 15, g = lane >> 4;
+  bf16x8 least[TILES][kSteps], largest[TILES][kSteps];
 #pragma unroll
-  for (int i = threadIdx.x; i < kChunk * kPieces; i += kThreads) {
-    const int r = i / kPieces, piece = i % kPieces;
-    const int64_t page = safe_page(table[min(r, n - 1)], p.pages);
-    *reinterpret_cast<u32x4*>(rows + r * (kPieces * 16) + ((piece ^ (r % kPieces)) << 4)) =
-        *reinterpret_cast<const u32x4*>(p.bounds + page * p.bounds_ps + (int64_t)head * (2 * D) + 8 * piece);
+  for (int i = 0; i < TILES; ++i) {
+    const int64_t page = safe_page(x.table[min(first + 16 * i + c, scored - 1)], p.pages);
+    const __bf16* const from = p.bounds + page * p.bounds_ps + (int64_t)x.head * (2 * D) + 8 * g;
+#pragma unroll
+    for (int k = 0; k < kSteps; ++k) {
+      least[i][k] = *reinterpret_cast<const bf16x8*>(from + 32 * k);
+      largest[i][k] = *reinterpret_cast<const bf16x8*>(from + D + 32 * k);
+    }
   }
-  __syncthreads();
-  float top = -INFINITY;
-  const char* const mine = rows + lane * (kPieces * 16);
-  for (int h = 2 * wave; h < p.group; h += 2 * kWaves) {
-    const __bf16* const q0 = p.q + t * p.q_ts + (int64_t)(head * p.group + h) * p.q_hs;
-    const __bf16* const q1 = p.q + t * p.q_ts + (int64_t)(head * p.group + min(h + 1, p.group - 1)) * p.q_hs;
-    double s0 = 0., s1 = 0.;
-#pragma unroll 2
-    for (int d = 0; d < D; d += 8) {
-      const u32x4 lo = *reinterpret_cast<const u32x4*>(mine + (((d / 8) ^ (lane % kPieces)) << 4));
-      const u32x4 hi = *reinterpret_cast<const u32x4*>(mine + (((d / 8 + D / 8) ^ (lane % kPieces)) << 4));
-      const u32x4 a = *reinterpret_cast<const u32x4*>(q0 + d), b = *reinterpret_cast<const u32x4*>(q1 + d);  // (wave-uniform)
+  // The split into q+ and q- asks for least <= largest; bounds of somebody else's making that are the other way round are exchanged. (As fp32 the upper of two
+  // features is compared with the lower one behind it: that says too often at most.)
+  int turned = 0;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const auto value = [&](const u32x4& x) { return e & 1 ? bf16hi_to_f32(x[e >> 1]) : bf16lo_to_f32(x[e >> 1]); };
-        const float x0 = value(a), x1 = value(b), least = value(lo), largest = value(hi);
-        s0 += (double)__builtin_elementwise_maximum(x0 * least, x0 * largest);  // (NaN stays)
-        s1 += (double)__builtin_elementwise_maximum(x1 * least, x1 * largest);
+  for (int i = 0; i < TILES; ++i)
+#pragma unroll
+    for (int k = 0; k < kSteps; ++k) {
+      const u32x4 a = __builtin_bit_cast(u32x4, least[i][k]), b = __builtin_bit_cast(u32x4, largest[i][k]);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) turned |= (int)(__uint_as_float(a[e]) > __uint_as_float(b[e])) | (int)(bf16lo_to_f32(a[e]) > bf16lo_to_f32(b[e]));
+    }
+  if (__any(turned)) {
+#pragma unroll
+    for (int i = 0; i < TILES; ++i)
+#pragma unroll
+      for (int k = 0; k < kSteps; ++k)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const __bf16 a = least[i][k][e], b = largest[i][k][e];
+          const bool other = (float)a > (float)b;
+          least[i][k][e] = other ? b : a, largest[i][k][e] = other ? a : b;
+        }
+  }
+#pragma unroll
+  for (int i = 0; i < TILES; ++i) out[i] = make_float2(-INFINITY, 0.f);
+#pragma unroll 1
+  for (int h0 = 0; h0 < p.group; h0 += 16) {
+    const __bf16* const from = p.q + x.t * p.q_ts + (int64_t)(x.head * p.group + min(h0 + c, p.group - 1)) * p.q_hs + 8 * g;
+    s16x8 q[kSteps];
+#pragma unroll
+    for (int k = 0; k < kSteps; ++k) q[k] = *reinterpret_cast<const s16x8*>(from + 32 * k);
+    f32x4 sum[TILES], mass[TILES];
+#pragma unroll
+    for (int i = 0; i < TILES; ++i) sum[i] = mass[i] = f32x4{};
+#pragma unroll
+    for (int k = 0; k < kSteps; ++k) {
+      const s16x8 below = q[k] >> 15;  // all bits where q is below zero
+      const auto bf = [](s16x8 v) __attribute__((always_inline)) { return __builtin_bit_cast(bf16x8, v); };
+      const auto magnitude = [&](bf16x8 v) __attribute__((always_inline)) { return bf(__builtin_bit_cast(s16x8, v) & (short)0x7fff); };
+      const bf16x8 up = bf(q[k] & ~below), down = bf(q[k] & below), down_size = magnitude(down);
+#pragma unroll
+      for (int i = 0; i < TILES; ++i) {
+        sum[i] = mfma16(up, largest[i][k], mfma16(down, least[i][k], sum[i]));
+        mass[i] = mfma16(up, magnitude(largest[i][k]), mfma16(down_size, magnitude(least[i][k]), mass[i]));
       }
     }
-    top = nan_max(nan_max(top, (float)s0), (float)s1);
-  }
-  best[wave][lane] = top;
-  __syncthreads();
-  if (wave == 0 && lane < n) {
 #pragma unroll
-    for (int w = 1; w < kWaves; ++w) top = nan_max(top, best[w][lane]);
-    p.keys[item * p.row + first + lane] = sort_key(top);
+    for (int i = 0; i < TILES; ++i)
+#pragma unroll
+      for (int v = 0; v < 4; ++v) {
+        out[i].x = fmaxf(out[i].x, sum[i][v]);
+        out[i].y = fmaxf(out[i].y, mass[i][v] < INFINITY ? mass[i][v] : INFINITY);
+      }
   }
+#pragma unroll
+  for (int i = 0; i < TILES; ++i) out[i] = make_float2(quad_max(out[i].x), quad_max(out[i].y));
 }
 
-// Inclusive sums over the workgroup.
-__device__ __forceinline__ int block_scan(int x, int* waves) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+// A page's score in fp64, by a whole wavefront: eight lanes a head, eight heads at a time.
+template <int D>
+__device__ __forceinline__ float exact_score(const KVSelectParams& p, const Item& x, int index, int lane) {
+  constexpr int E = D / 8;  // features of a lane
+  const int64_t page = safe_page(x.table[index], p.pages);
+  const __bf16* const from = p.bounds + page * p.bounds_ps + (int64_t)x.head * (2 * D) + E * (lane & 7);
+  bf16x8 least[E / 8], largest[E / 8];
 #pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const int y = __shfl_up(x, d);
-    if (lane >= d) x += y;
+  for (int e = 0; e < E / 8; ++e) {
+    least[e] = *reinterpret_cast<const bf16x8*>(from + 8 * e);
+    largest[e] = *reinterpret_cast<const bf16x8*>(from + D + 8 * e);
   }
-  __syncthreads();
-  if (lane == 63) waves[wave] = x;
-  __syncthreads();
-  for (int w = 0; w < wave; ++w) x += waves[w];
-  return x;
+  float best = -INFINITY;
+#pragma unroll 1
+  for (int h0 = 0; h0 < p.group; h0 += 8) {
+    const __bf16* const row = p.q + x.t * p.q_ts + (int64_t)(x.head * p.group + min(h0 + (lane >> 3), p.group - 1)) * p.q_hs + E * (lane & 7);
+    double sum = 0.;
+#pragma unroll
+    for (int e = 0; e < E / 8; ++e) {
+      const bf16x8 q = *reinterpret_cast<const bf16x8*>(row + 8 * e);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) sum += (double)__builtin_elementwise_maximum((float)q[k] * (float)least[e][k], (float)q[k] * (float)largest[e][k]);  // (NaN stays)
+    }
+#pragma unroll
+    for (int d = 1; d < 8; d <<= 1) sum += __shfl_xor(sum, d);
+    best = __builtin_elementwise_maximum(best, (float)sum);
+  }
+#pragma unroll
+  for (int d = 8; d < 64; d <<= 1) best = __builtin_elementwise_maximum(best, __shfl_xor(best, d));
+  return best;
 }
 
-constexpr int kInLds = 8192;  // scores that are kept in LDS
+template <int D>
+__global__ __launch_bounds__(kThreads) void kv_score_kernel(KVSelectParams p) {
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int chunk = blockIdx.x % p.chunks, item = blockIdx.x / p.chunks;
+  const Item x = item_of(p, item, lane);
+  const int scored = x.pages - 1, first = chunk * kChunk + 32 * wave;  // (the token's own page is not scored)
+  if (x.pages <= p.keep || first >= scored) return;
+  float2 found[2];
+  score_pages<D, 2>(p, x, first, scored, lane, found);
+  if (lane < 32) reinterpret_cast<float2*>(p.pages_of)[item * p.row + first + lane] = lane < 16 ? found[0] : found[1];  // (of those behind the last: not read)
+}
 
-// The keep - 1 largest of a token's and head's scores: their least one digit by digit (8 bits, from the top, a histogram each), then every thread counts those
-// above it and equal to it in a stretch of the sequence, and writes its own behind those of the stretches in front of it.
-__global__ __launch_bounds__(kThreads) void kv_pick_kernel(KVSelectParams p) {
-  __shared__ uint32_t kept[kInLds];
-  __shared__ int histogram[256];
-  __shared__ int waves[kWaves], digit, rest;
-  const int tid = threadIdx.x, lane = tid & 63;
-  const int item = blockIdx.x, t = item / p.heads;
-  const int seq = sequence_of(p.cu_q, p.B, t, lane);
-  const int visible = visible_rows(p, t, seq);
-  const int pages = (visible + (1 << p.page_shift) - 1) >> p.page_shift;
-  const int n = min(pages, p.keep);
-  const int32_t* const table = p.table + seq * p.table_rs;
-  int32_t* const out = p.table_out + (int64_t)item * p.keep;
-  if (tid == 0) p.lengths_out[item] = visible - ((pages - n) << p.page_shift);
-  for (int i = n + tid; i < p.keep; i += kThreads) out[i] = -1;
-  if (pages <= p.keep) {
-    for (int i = tid; i < n; i += kThreads) out[i] = table[i];
-    return;
-  }
-  if (tid == 0) out[n - 1] = table[pages - 1];
-  if (n == 1) return;
-  const uint32_t* const keys = p.keys + item * p.row;
-  const int scored = pages - 1;
-  const bool in_lds = scored <= kInLds;
-  if (in_lds)
-    for (int i = tid; i < scored; i += kThreads) kept[i] = keys[i];
-  const auto key = [&](int i) { return in_lds ? kept[i] : keys[i]; };
-  uint32_t least = 0;  // of the largest ones, as far as its digits are known
-  int want = n - 1;    // of those that begin with these digits
-  for (int shift = 24; shift >= 0; shift -= 8) {
-    histogram[tid] = 0;
+// Sums and maxima over a workgroup, one barrier each (the other half of what is shared is still being read from the call before).
+template <int THREADS, int E>
+struct Team {
+  static constexpr int kGroups = THREADS / 64, kListed = 128;
+  struct Shared {
+    int2 sums[2][kGroups];
+    __attribute__((aligned(16))) int histogram[2][256];
+    int chosen[E * kGroups];
+    int listed;
+    uint2 list[kListed];
+  };
+  Shared& shared;
+  int turn;
+  __device__ __forceinline__ explicit Team(Shared& s) : shared(s), turn(0) {}
+  __device__ __forceinline__ float2 most(float a, float b) {
+    const auto wave_max = [](float x) __attribute__((always_inline)) { return quad_max(group_reduce<16>(x, [](float y, float z) { return fmaxf(y, z); })); };
+    a = wave_max(a), b = wave_max(b);
+    if ((threadIdx.x & 63) == 63) shared.sums[turn][threadIdx.x >> 6] = make_int2(__float_as_int(a), __float_as_int(b));
     __syncthreads();
-    for (int i = tid; i < scored; i += kThreads) {
-      const uint32_t k = key(i);
-      if (shift == 24 || (k ^ least) >> (shift + 8) == 0) atomicAdd(&histogram[(k >> shift) & 255], 1);
+#pragma unroll
+    for (int w = 0; w < kGroups; ++w) {
+      const int2 s = shared.sums[turn][w];
+      a = fmaxf(a, __int_as_float(s.x)), b = fmaxf(b, __int_as_float(s.y));
+    }
+    turn ^= 1;
+    return make_float2(a, b);
+  }
+  __device__ __forceinline__ int2 sums(int x, int y) {
+    x = wave_scan(x), y = wave_scan(y);
+    if ((threadIdx.x & 63) == 63) shared.sums[turn][threadIdx.x >> 6] = make_int2(x, y);
+    __syncthreads();
+    int2 all = make_int2(0, 0);
+#pragma unroll
+    for (int w = 0; w < kGroups; ++w) all.x += shared.sums[turn][w].x, all.y += shared.sums[turn][w].y;
+    turn ^= 1;
+    return all;
+  }
+};
+
+// A score as the search for v sees it: infinities and what comes near them become large numbers, in the same order.
+__device__ __forceinline__ float in_range(float x) { return x != x ? 1e37f : fminf(fmaxf(x, -1e37f), 1e37f); }
+
+// Of the n pages of a token and head the `want` (fewer) with the largest scores: their numbers to out, in their order. score: in_range, of pages tid + THREADS e;
+// mass: the largest S of this thread's; memory: room for n. By a whole workgroup.
+template <int D, int THREADS, int E>
+__device__ __forceinline__ void choose(const KVSelectParams& p, const Item& x, Team<THREADS, E>& team, const float (&score)[E], float mass, int n, int want, uint2* memory, int32_t* out) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  auto& shared = team.shared;
+  const auto each = [&](const auto& f) __attribute__((always_inline)) {
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+      if (tid + THREADS * e < n) f(e, score[e]);
+  };
+  if (tid < 256) shared.histogram[0][tid] = 0;
+  if (tid == 0) shared.listed = 0;
+  float a = -INFINITY, b = -INFINITY;
+  each([&](int, float s) __attribute__((always_inline)) { a = fmaxf(a, s), b = fmaxf(b, -s); });
+  float2 r = team.most(a, b);
+  float high = r.x, low = -r.y;  // v lies between
+  const float off = 2.f * (team.most(mass, 0.f).x * 0x1p-14f + 0x1p-60f);  // 2 E (and terms that are below the normal range)
+  int left = want;  // v is the how many-th of those between them
+#pragma unroll 1
+  for (int turn = 0; high - low > off; turn ^= 1) {
+    const float scale = 255.f / (high - low);
+    const auto part_of = [&](float s) __attribute__((always_inline)) { return min((int)((s - low) * scale), 255); };  // (low: 0, high: another)
+    if (tid < 256) shared.histogram[turn ^ 1][tid] = 0;
+    each([&](int, float s) __attribute__((always_inline)) {
+      if (s >= low && s <= high) atomicAdd(&shared.histogram[turn][part_of(s)], 1);
+    });
+    __syncthreads();
+    // every wave looks the part up: four parts a lane, from the highest
+    const int4 h = *reinterpret_cast<const int4*>(&shared.histogram[turn][252 - 4 * lane]);
+    const int mine = h.x + h.y + h.z + h.w, upto = wave_scan(mine);
+    const int j = __builtin_ctzll(__ballot(upto >= left));
+    left -= __builtin_amdgcn_readlane(upto - mine, j);
+    const int hw = __builtin_amdgcn_readlane(h.w, j), hz = __builtin_amdgcn_readlane(h.z, j), hy = __builtin_amdgcn_readlane(h.y, j);
+    int part = 255 - 4 * j;
+    if (left > hw) {
+      left -= hw, --part;
+      if (left > hz) {
+        left -= hz, --part;
+        if (left > hy) left -= hy, --part;
+      }
+    }
+    a = b = -INFINITY;
+    each([&](int, float s) __attribute__((always_inline)) {
+      if (s >= low && s <= high && part_of(s) == part) a = fmaxf(a, s), b = fmaxf(b, -s);
+    });
+    r = team.most(a, b);
+    high = r.x, low = -r.y;
+  }
+
+  int in = 0, open = 0;
+  uint32_t is_in = 0, is_open = 0;  // bit e
+  each([&](int e, float s) __attribute__((always_inline)) {
+    const bool yes = s > high + off, no = s < low - off;
+    in += yes, open += !yes && !no;
+    is_in |= (uint32_t)yes << e, is_open |= (uint32_t)(!yes && !no) << e;
+  });
+  const int2 all = team.sums(in, open);
+  const int places = want - all.x;  // for those in question
+  if (all.y == places) {
+    is_in |= is_open;
+  } else {  // (uniform)
+    uint2* const list = all.y <= Team<THREADS, E>::kListed ? shared.list : memory;
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+      if ((is_open >> e) & 1) list[atomicAdd(&shared.listed, 1)].x = tid + THREADS * e;  // (in any order: what follows goes by the pages' numbers)
+    __syncthreads();
+#pragma unroll 1
+    for (int k = wave; k < all.y; k += THREADS / 64) {
+      const float exact = exact_score<D>(p, x, __builtin_amdgcn_readfirstlane(list[k].x), lane);
+      if (lane == 0) list[k].y = sort_key(exact);
     }
     __syncthreads();
-    const int mine = histogram[255 - tid], upto = block_scan(mine, waves);
-    if (upto >= want && upto - mine < want) digit = 255 - tid, rest = want - (upto - mine);
-    __syncthreads();
-    least |= (uint32_t)digit << shift;
-    want = rest;
+    // a page in question is in if fewer than `places` of the others are in front of it
+#pragma unroll 1
+    for (int e = 0; e < E; ++e) {
+      if (__any((is_open >> e) & 1)) {
+        const uint32_t i = tid + THREADS * e;
+        uint32_t key = 0;
+        for (int k = 0; k < all.y; ++k) key = list[k].x == i ? list[k].y : key;
+        int rank = 0;
+        for (int k = 0; k < all.y; ++k) {
+          const uint2 other = list[k];
+          rank += other.y > key || (other.y == key && other.x < i);
+        }
+        is_in |= (uint32_t)(((is_open >> e) & 1) && rank < places) << e;
+      }
+    }
   }
-  const int each = (scored + kThreads - 1) / kThreads, from = min(tid * each, scored), to = min(from + each, scored);
-  int above = 0, equal = 0;
-  for (int i = from; i < to; ++i) {
-    const uint32_t k = key(i);
-    above += k > least;
-    equal += k == least;
+  // their places: of the wave's pages for each e, then of all in front
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    const uint64_t mine = __ballot((is_in >> e) & 1);
+    if (lane == 0) shared.chosen[e * (THREADS / 64) + wave] = __popcll(mine);
   }
-  const int equals_before = block_scan(equal, waves) - equal;  // of equal ones the first `want` count
-  const int take = min(max(want - equals_before, 0), equal);
-  int at = block_scan(above + take, waves) - (above + take), equals = 0;
-  for (int i = from; i < to; ++i) {
-    const uint32_t k = key(i);
-    if (k > least || (k == least && equals++ < take)) out[at++] = table[i];
+  __syncthreads();
+  int before = 0;
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    int here = before;
+#pragma unroll
+    for (int w = 0; w < THREADS / 64; ++w) {
+      const int c = shared.chosen[e * (THREADS / 64) + w];
+      here += w < wave ? c : 0;
+      before += c;
+    }
+    const uint64_t mine = __ballot((is_in >> e) & 1);
+    if ((is_in >> e) & 1) out[here + __popcll(mine & ((1ull << lane) - 1))] = x.table[tid + THREADS * e];
   }
+}
+
+// A page whose S is not known gets its score in fp64 (`index`: of lane 0's page; by a whole wavefront).
+template <int D>
+__device__ __forceinline__ float settle_unknown(const KVSelectParams& p, const Item& x, int index, bool real, float2 found, int lane) {
+  float score = found.x;
+  uint64_t unknown = __ballot(real && !(found.y < INFINITY));
+  while (unknown != 0) {
+    const int j = __builtin_ctzll(unknown);
+    unknown &= unknown - 1;
+    const float exact = exact_score<D>(p, x, __builtin_amdgcn_readfirstlane(index + j), lane);
+    score = lane == j ? exact : score;
+  }
+  return in_range(score);
+}
+
+// What needs no scores: rows and places that stay empty, the token's own page, tokens that see no more pages than are kept. False: that was all.
+__device__ __forceinline__ bool begin_choice(const KVSelectParams& p, const Item& x, int item, int32_t* out) {
+  const int n = min(x.pages, p.keep);
+  if (threadIdx.x == 0) p.lengths_out[item] = x.visible - ((x.pages - n) << p.page_shift);
+  for (int i = n + threadIdx.x; i < p.keep; i += blockDim.x) out[i] = -1;
+  if (x.pages <= p.keep) {
+    for (int i = threadIdx.x; i < n; i += blockDim.x) out[i] = x.table[i];
+    return false;
+  }
+  if (threadIdx.x == 0) out[n - 1] = x.table[x.pages - 1];
+  return n > 1;
+}
+
+template <int D, int THREADS, int E>
+__global__ __launch_bounds__(THREADS) void kv_pick_kernel(KVSelectParams p) {
+  __shared__ typename Team<THREADS, E>::Shared shared;
+  const int item = blockIdx.x, lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const Item x = item_of(p, item, lane);
+  int32_t* const out = p.table_out + (int64_t)item * p.keep;
+  if (!begin_choice(p, x, item, out)) return;
+  uint2* const memory = p.pages_of + item * p.row;
+  const int n = x.pages - 1;
+  float score[E], s[E], mass = 0.f;
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    const float2 found = reinterpret_cast<const float2*>(memory)[min((int)threadIdx.x + THREADS * e, n - 1)];
+    score[e] = found.x, s[e] = found.y;
+  }
+  bool known = true;
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    known = known && s[e] < INFINITY;
+    mass = s[e] < INFINITY ? fmaxf(mass, s[e]) : mass;
+    score[e] = known ? in_range(score[e]) : score[e];
+  }
+  if (__any(!known)) {  // (rare)
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+      score[e] = settle_unknown<D>(p, x, 64 * wave + THREADS * e, (int)threadIdx.x + THREADS * e < n, make_float2(score[e], s[e]), lane);
+  }
+  Team<THREADS, E> team(shared);
+  choose<D, THREADS, E>(p, x, team, score, mass, n, p.keep - 1, memory, out);
+}
+
+// Scores and choice in one launch, for tables of up to kFewPages pages.
+constexpr int kFewPages = 256, kSomePages = 2048, kMostPages = 16384;
+template <int D>
+__global__ __launch_bounds__(kThreads) void kv_pick_few_kernel(KVSelectParams p) {
+  __shared__ typename Team<kThreads, 1>::Shared shared;
+  __shared__ float scores[kFewPages];
+  const int item = blockIdx.x, lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const Item x = item_of(p, item, lane);
+  int32_t* const out = p.table_out + (int64_t)item * p.keep;
+  if (!begin_choice(p, x, item, out)) return;
+  const int n = x.pages - 1;
+  float mass = 0.f;
+#pragma unroll 1
+  for (int first = 32 * wave; first < n; first += kChunk) {
+    float2 found[2];
+    score_pages<D, 2>(p, x, first, n, lane, found);
+    const float2 mine = lane < 16 ? found[0] : found[1];
+    const bool real = lane < 32 && first + lane < n;
+    const float s = settle_unknown<D>(p, x, first, real, mine, lane);
+    if (real) scores[first + lane] = s;
+    mass = real && mine.y < INFINITY ? fmaxf(mass, mine.y) : mass;
+  }
+  __syncthreads();
+  const float score[1] = {scores[threadIdx.x]};
+  Team<kThreads, 1> team(shared);
+  choose<D, kThreads, 1>(p, x, team, score, mass, n, p.keep - 1, p.pages_of + item * p.row, out);
 }
 
 int check_select(const pith_kv_select_args* a, const char* who) {
@@ -174,6 +421,7 @@ int check_select(const pith_kv_select_args* a, const char* who) {
   if (const int rc = check_table(a->T, a->B, a->heads, a->table_width, a->page_size, !a->cu_q, who)) return rc;
   if (a->H < 1 || a->H > 1024 || a->H % a->heads) return fail(PITH_ERR_BAD_SHAPE, "%s: %lld query heads (at most 1024) of %lld key-value heads", who, (long long)a->H, (long long)a->heads);
   if (a->keep < 1 || a->keep > 1 << 20) return fail(PITH_ERR_BAD_SHAPE, "%s: keep = %lld pages (1 to 2^20)", who, (long long)a->keep);
+  if (a->table_width > kMostPages) return fail(PITH_ERR_UNSUPPORTED, "%s: page tables of %lld pages, at most %d", who, (long long)a->table_width, kMostPages);
   if (a->T * a->heads > 0x7fffffff / ((a->table_width + kChunk - 1) / kChunk + 1) || a->T * a->heads > (int64_t)1 << 24)
     return fail(PITH_ERR_UNSUPPORTED, "%s: too many tokens for page tables of that width: call it with fewer at a time", who);
   return PITH_OK;
@@ -188,7 +436,7 @@ using namespace pith;
 
 extern "C" int64_t pith_kv_select_workspace_bytes(const pith_kv_select_args* a) {
   if (check_select(a, "pith_kv_select_workspace_bytes") != PITH_OK || a->B == 0) return 0;
-  return a->T * a->heads * chunks_of(a) * kChunk * 4;
+  return a->T * a->heads * chunks_of(a) * kChunk * (int64_t)sizeof(uint2);
 }
 
 extern "C" int pith_kv_select(const pith_kv_select_args* a, pith_stream_t stream) {
@@ -207,7 +455,7 @@ extern "C" int pith_kv_select(const pith_kv_select_args* a, pith_stream_t stream
   if (a->workspace_bytes < need) return fail(PITH_ERR_BAD_SHAPE, "%s: the workspace has %lld bytes, %lld are needed", who, (long long)a->workspace_bytes, (long long)need);
   KVSelectParams p = {};
   p.q = (const __bf16*)a->q; p.bounds = (const __bf16*)a->bounds; p.table = a->page_table; p.lengths = a->lengths; p.cu_q = a->cu_q;
-  p.table_out = a->table_out; p.lengths_out = a->lengths_out; p.keys = (uint32_t*)a->workspace;
+  p.table_out = a->table_out; p.lengths_out = a->lengths_out; p.pages_of = (uint2*)a->workspace;
   p.q_ts = a->q_ts; p.q_hs = a->q_hs; p.table_rs = a->B > 1 ? a->table_rs : 0; p.bounds_ps = a->pages > 1 ? a->bounds_ps : 0;
   p.chunks = (int)chunks_of(a); p.row = (int64_t)p.chunks * kChunk;
   p.T = (int)a->T; p.B = (int)a->B; p.heads = (int)a->heads; p.group = (int)(a->H / a->heads);
@@ -215,10 +463,17 @@ extern "C" int pith_kv_select(const pith_kv_select_args* a, pith_stream_t stream
   hipStream_t s = (hipStream_t)stream;
   begin_launch();
   const unsigned items = (unsigned)(a->T * a->heads);
-  if (a->keep > 1 && a->table_width > a->keep) {  // (else nothing is scored)
-    if (a->dim == 128) kv_score_kernel<128><<<items * (unsigned)p.chunks, kThreads, 0, s>>>(p);
-    else kv_score_kernel<64><<<items * (unsigned)p.chunks, kThreads, 0, s>>>(p);
-  }
-  kv_pick_kernel<<<items, kThreads, 0, s>>>(p);
+  const auto launch = [&](auto d) {
+    constexpr int D = decltype(d)::value;
+    if (a->table_width <= kFewPages) {
+      kv_pick_few_kernel<D><<<items, kThreads, 0, s>>>(p);
+      return;
+    }
+    if (a->keep > 1 && a->table_width > a->keep) kv_score_kernel<D><<<items * (unsigned)p.chunks, kThreads, 0, s>>>(p);  // (else nothing is scored)
+    if (a->table_width <= kSomePages) kv_pick_kernel<D, 512, kSomePages / 512><<<items, 512, 0, s>>>(p);
+    else kv_pick_kernel<D, 1024, kMostPages / 1024><<<items, 1024, 0, s>>>(p);
+  };
+  if (a->dim == 128) launch(std::integral_constant<int, 128>());
+  else launch(std::integral_constant<int, 64>());
   return check_launch(who);
 }

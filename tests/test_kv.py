@@ -235,7 +235,7 @@ def test_workspaces():
     assert attn(T=0) == attn(B=0) == attn(H=3) == 0 and attn() > 0
     assert attn(table_width=4096, table_rs=4096) == attn(table_width=64, table_rs=64)  # whatever the lengths
     select = lambda **kw: lib.pith_kv_select_workspace_bytes(ctypes.byref(_select(**kw)))  # noqa: E731
-    assert select() == 4 * 2 * 64 * 4 and select(T=0) == select(keep=0) == 0 and select(table_width=65) == 2 * select()
+    assert select() == 4 * 2 * 128 * 8 and select(T=0) == select(keep=0) == 0 and select(table_width=129) == 2 * select()
 
 
 def test_rows_of_a_row_block_go_by_the_rows_of_a_sequence_and_the_work_list():
