@@ -46,6 +46,14 @@ bool sequence_args(A& a, const Tensor& like, const Tensor& table, const Tensor& 
   return true;
 }
 
+// A part of `whole` as a tensor of its own: n elements from byte `at` on.
+Tensor part_of(const Tensor& whole, int64_t at, int64_t n, at::ScalarType type) {
+  Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(whole.storage()), whole.key_set(), c10::scalarTypeToTypeMeta(type));
+  t.unsafeGetTensorImpl()->set_storage_offset(at / (int64_t)c10::elementSize(type));
+  t.unsafeGetTensorImpl()->set_sizes_contiguous({n});
+  return t;
+}
+
 using Six = std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor>;
 
 Six plan_step(const Tensor& counts, const Tensor& lengths, const Tensor& table, const Tensor& free_pages, const Tensor& free_count, int64_t page_size, int64_t tokens) {
@@ -56,19 +64,19 @@ Six plan_step(const Tensor& counts, const Tensor& lengths, const Tensor& table, 
     const int32_t* entries = nullptr;
     if (is_index(counts, counts, at::kInt, {a.B}) && is_index(lengths, counts, at::kInt, {a.B}) && page_table_args(table, counts, a.B, &entries, &a.table_rs, &a.table_width) &&
         is_index(free_pages, counts, at::kInt, {a.pool_size}) && is_index(free_count, counts, at::kInt, {1})) {
-      Tensor cu_q = fresh(counts, {a.B + 1}, at::kInt), after = fresh(counts, {a.B}, at::kInt), positions = fresh(counts, {tokens}, at::kLong),
-             slots = fresh(counts, {tokens}, at::kLong), granted = fresh(counts, {a.B}, at::kInt), count = fresh(counts, {1}, at::kInt);
+      // one allocation for all results and the workspace: six of them would take longer than the kernel
+      a.workspace_bytes = pith_plan_step_workspace_bytes(&a);
+      const int64_t ints = a.workspace_bytes + 16 * tokens;
+      const Tensor whole = fresh(counts, {ints + 4 * (3 * a.B + 2)}, at::kByte);
+      const Tensor positions = part_of(whole, a.workspace_bytes, tokens, at::kLong), slots = part_of(whole, a.workspace_bytes + 8 * tokens, tokens, at::kLong),
+                   cu_q = part_of(whole, ints, a.B + 1, at::kInt), after = part_of(whole, ints + 4 * (a.B + 1), a.B, at::kInt),
+                   granted = part_of(whole, ints + 4 * (2 * a.B + 1), a.B, at::kInt), count = part_of(whole, ints + 4 * (3 * a.B + 1), 1, at::kInt);
+      a.workspace = whole.data_ptr();
       a.counts = counts.data_ptr<int32_t>(); a.lengths = lengths.data_ptr<int32_t>();
       a.page_table = table.data_ptr<int32_t>();
       a.free_pages = free_pages.data_ptr<int32_t>(); a.free_count = free_count.data_ptr<int32_t>();
       a.cu_q = cu_q.data_ptr<int32_t>(); a.position_ids = positions.data_ptr<int64_t>(); a.slots = slots.data_ptr<int64_t>();
       a.granted = granted.data_ptr<int32_t>(); a.lengths_out = after.data_ptr<int32_t>(); a.free_count_out = count.data_ptr<int32_t>();
-      a.workspace_bytes = pith_plan_step_workspace_bytes(&a);
-      Tensor ws;
-      if (a.workspace_bytes > 0) {
-        ws = fresh(counts, {a.workspace_bytes}, at::kByte);
-        a.workspace = ws.data_ptr();
-      }
       if (accepted(pith_plan_step(&a, stream_of(counts)))) return {cu_q, after, positions, slots, granted, count};
     }
   }

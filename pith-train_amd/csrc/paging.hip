@@ -212,7 +212,7 @@ __global__ __launch_bounds__(kThreads) void plan_few_kernel(PlanParams p) {
   }
   const int64_t top = min(had + back, p.pool);
 
-  const int wanted = min(max(count, 0), tokens);  // (their sum is at most 64 * 8192)
+  const int wanted = min(max(count, 0), tokens);  // (their sum is below 2^31: few tokens, or 2^24 at most)
   const int upto = wave_scan(wanted), first = min(upto - wanted, tokens), last = min(upto, tokens), rows = last - first;
   const bool fits = count >= 0 && rows <= most - length;
   const int need = fits ? pages_of(length + rows) - held : 0;
@@ -229,7 +229,12 @@ __global__ __launch_bounds__(kThreads) void plan_few_kernel(PlanParams p) {
       p.cu_q[0] = 0;
       p.free_count_out[0] = (int32_t)(top - all);
     }
+    if (p.requests) {  // (the tokens are for the next launch)
+      if (some) p.requests[lane] = Request{length, served, taken};
+      if (lane == 63) *p.top = top;
+    }
   }
+  if (p.requests) return;
   const int end = __builtin_amdgcn_readlane(last, 63);
   for (int t0 = wave * 64; t0 < tokens; t0 += 64 * waves) {
     const int t = t0 + lane;
@@ -278,7 +283,7 @@ extern "C" int pith_kv_version(void) { return PITH_KV_VERSION; }
 
 extern "C" int64_t pith_plan_step_workspace_bytes(const pith_plan_step_args* a) {
   if (check_plan(a, "pith_plan_step_workspace_bytes") != PITH_OK || in_one(a)) return 0;
-  return 16 + a->B * (int64_t)sizeof(Request);
+  return (16 + a->B * (int64_t)sizeof(Request) + 15) & ~(int64_t)15;
 }
 
 extern "C" int pith_plan_step(const pith_plan_step_args* a, pith_stream_t stream) {
@@ -310,7 +315,8 @@ extern "C" int pith_plan_step(const pith_plan_step_args* a, pith_stream_t stream
   } else {
     p.top = (int64_t*)a->workspace;
     p.requests = (Request*)((char*)a->workspace + 16);
-    plan_kernel<false><<<1, kThreads, 0, s>>>(p);
+    if (a->B <= 64 && a->T <= 1 << 24) plan_few_kernel<<<1, 256, 0, s>>>(p);
+    else plan_kernel<false><<<1, kThreads, 0, s>>>(p);
     if (a->T > 0) place_kernel<<<(unsigned)((a->T + 255) / 256), 256, 0, s>>>(p);
   }
   return check_launch(who);
