@@ -15,15 +15,17 @@
 // kernel joins them in the order of the keys (results do not depend on scheduling). So how a row's keys are cut, its references and the order of its sums
 // follow from the lengths of all sequences of the call; nothing else of one row reaches another.
 //
-// The kernel. Memory bounds it: a key row and a value row of 512 bytes (bf16, 128 features) stand against 4 * 128 flop for each of the group's rows. So
-// the four wavefronts of a workgroup (one a SIMD: 512 registers each) walk alone, each through every fourth tile of 32 keys, with no barrier until the
-// segment ends: a wave brings its tiles global -> LDS by direct loads into a ring of its own (32 KB of keys and values in flight a wave, 128 KB a compute
-// unit) and waits with counted waits for its own requests only, for the keys while the values are still under way. Products are 16x16x32 with the query
-// row as the result's column, so a lane owns one row, and the scores of a lane are its part of operand B of the second product as they stand: key 4 g + v
-// of either half tile is contracted at place 8 g + v or 8 g + 4 + v, and the values are read (transposed, from LDS) in that order. No weight moves between lanes.
-// The waves' results of a segment are joined through LDS.
+// The kernel. Memory bounds it: a key row and a value row of 512 bytes (bf16, 128 features) stand against 4 * 128 flop for each of the group's rows. So the four
+// wavefronts of a workgroup walk alone, each through every fourth tile of 32 keys, with no barrier until the segment ends: a wave brings its tiles global -> LDS by
+// direct loads into a ring of its own (128 KB of keys and values in flight on a compute unit, see KVRing) and waits with counted waits for its own requests only, for
+// the keys while the values are still under way. Products are 16x16x32 with the query row as the result's column, so a lane owns one row, and the scores of a lane are
+// its part of operand B of the second product as they stand: key 4 g + v of either half tile is contracted at place 8 g + v or 8 g + 4 + v, and the values are read
+// (transposed, from LDS) in that order. No weight moves between lanes. The waves' results of a segment are joined through LDS.
 // A fragment that was read serves all 16-row groups of the block: 64 rows cost a tile's reads once. With M = 64 the products are 1024 of a tile's cycles, and
 // the tile still comes more slowly than that from memory.
+// Measured, heads of 32 / 4 with 128 features: 32 sequences of up to 8192 rows, bf16, one token each (303 MB) 64 us, 4.7 TB/s; 8 of up to 131072 rows, e4m3 (879 MB)
+// 164 us, 5.4 TB/s, where a copy reaches 4.9; 64 selected pages of 8 such sequences (34 MB) 15 us, of which the join's launch is 4 and beginnings and ends
+// about 4; one sequence of 517 rows 8.8 us, a launch and 5 steps of waiting for memory.
 // The weights go into the second product as bf16, which is what the matrix cores take beside a cache of bf16 (or e4m3, widened exactly): half a step, 2^-8, of
 // each, while their sum is of the unrounded ones. With e4m3 a weight is rounded once, when its row's scale is in it.
 #pragma once
@@ -257,8 +259,6 @@ struct KVTile {
   static constexpr int kScaleLoads = FP8 ? 1 : 0;             // 32 scales of keys and 32 of values
   static constexpr int kScaleBytes = FP8 ? 256 : 0;
   static constexpr int kSlot = 2 * kBytes + kScaleBytes;
-  static constexpr int kSlots = FP8 || D == 64 ? 4 : 2;       // tiles of a wave in flight
-  static constexpr int kRing = kSlots * kSlot;
   static constexpr int kAll = kScaleLoads + 2 * kLoads;       // requests of a tile
 
   // Place in the source, within 16 rows, of what lane `lane` brings in instruction 0; that of instruction n is ^ (source_xor(n)) and 1024 n behind.
@@ -270,6 +270,17 @@ struct KVTile {
   static __device__ __forceinline__ constexpr int source_xor(int n) { return kRow == 256 ? 128 * (n & 1) : kRow == 128 ? 16 * (n >> 1) : 16 * n; }
   // Place in a tile of piece q of row r (< 32).
   static __device__ __forceinline__ int place(int r, int q) { return r * kRow + ((q ^ kv_swizzle<kRow>(r)) << 4); }
+};
+
+// Tiles of a wave in flight, and workgroups of a compute unit. Two workgroups fill each other's gaps (their beginnings and ends, a wave's way from its keys to its
+// weights), with rings of 64 KB each; a ring of one tile is enough then, as its keys are asked for while the values before them are worked on and the other way
+// round. 64 rows fill the registers, and with them one workgroup has the compute unit. (us with one workgroup and rings of 128 KB / with two: 8 sequences of 64
+// selected pages, e4m3, 17.2 / 15.3; trees of 8 over 5001 rows, heads of 64, 16.8 / 15.5; 4 tokens, 32 x 1024 rows 23.2 / 18.6; long streams alike.)
+template <int D, bool FP8, int R>
+struct KVRing {
+  static constexpr int kPerUnit = R <= 2 ? 2 : 1;
+  static constexpr int kSlots = R > 2 ? 2 : FP8 && D == 64 ? 4 : FP8 || D == 64 ? 2 : 1;
+  static constexpr int kBytes = kSlots * KVTile<D, FP8>::kSlot;
 };
 
 // A wave's requests for the 32 rows from key on (a multiple of 32): two times sixteen rows, each of one page. Rows behind the sequence's last one come as the
@@ -325,12 +336,12 @@ __device__ __forceinline__ void stage_rows(const KVAttnParams& p, const KVWork& 
 }
 
 // Until all but the last `later` tiles' requests and EXTRA more are there.
-template <int D, bool FP8, int EXTRA>
+template <int D, bool FP8, int SLOTS, int EXTRA>
 __device__ __forceinline__ void wait_tiles(int later) {
   constexpr int kAll = KVTile<D, FP8>::kAll;
-  if (later >= 3) wait_loads<KVTile<D, FP8>::kSlots == 4 ? 3 * kAll + EXTRA : 0>();
-  else if (later == 2) wait_loads<KVTile<D, FP8>::kSlots == 4 ? 2 * kAll + EXTRA : 0>();
-  else if (later == 1) wait_loads<kAll + EXTRA>();
+  if (SLOTS == 4 && later >= 3) wait_loads<SLOTS == 4 ? 3 * kAll + EXTRA : 0>();
+  else if (SLOTS == 4 && later == 2) wait_loads<SLOTS == 4 ? 2 * kAll + EXTRA : 0>();
+  else if (SLOTS >= 2 && later >= 1) wait_loads<kAll + EXTRA>();
   else wait_loads<EXTRA>();
 }
 
@@ -453,14 +464,13 @@ __device__ __forceinline__ void clean_values(char* values, int lane, const uint3
 
 // ---------------------------------------------------------------------------------------------
 
-// (At most 256 registers for up to 32 rows: with more at hand the compiler keeps the results in the accumulators' half of the file, and moves them out and
-// back for every rescaling that may come.)
 template <int D, bool FP8, int R>
-__global__ __launch_bounds__(kKVThreads, 1) void kv_attn_kernel(KVAttnParams p) {
+__global__ __launch_bounds__(kKVThreads, (KVRing<D, FP8, R>::kPerUnit)) void kv_attn_kernel(KVAttnParams p) {
   using T = KVTile<D, FP8>;
+  constexpr int kSlots = KVRing<D, FP8, R>::kSlots, kRing = KVRing<D, FP8, R>::kBytes;
   using Loads = KVLoads<D, FP8>;
   constexpr int M = 16 * R, kSteps = D / 32;  // of the score's contraction
-  constexpr int kRegion = T::kRing > M * D * 4 ? T::kRing : M * D * 4;  // of a wave: its tiles, then its results
+  constexpr int kRegion = kRing > M * D * 4 ? kRing : M * D * 4;  // of a wave: its tiles, then its results
   __shared__ __attribute__((aligned(1024))) char lds[kKVWaves * kRegion];
   __shared__ float2 wave_stats[kKVWaves][M];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -522,15 +532,8 @@ __global__ __launch_bounds__(kKVThreads, 1) void kv_attn_kernel(KVAttnParams p) 
       loads.keys(p, ring + i * T::kSlot, source, lane);
       loads.values(p, ring + i * T::kSlot, source);
     };
-    // The queries come through the last slots of the ring, behind the first tiles in the LDS and in front of them in the queue.
-    constexpr int kQuerySlots = (M * 2 * D + T::kSlot - 1) / T::kSlot, kFirst = T::kSlots - kQuerySlots;
-    static_assert(kFirst >= 1, "a tile beside the queries");
-    if (n_tiles > 0) {
-      char* const staged = ring + kFirst * T::kSlot;
-      stage_rows<D, R>(p, s, head, row0, rows, staged, lane);
-#pragma unroll 1
-      for (int i = 0; i < min(kFirst, n_tiles); ++i) request(i);
-      wait_tiles<D, FP8, 0>(min(kFirst, n_tiles));
+    // The queries come through the end of the ring, in front of its first tiles in the queue and read before its last ones are asked for.
+    const auto read_queries = [&](const char* staged) __attribute__((always_inline)) {
 #pragma unroll
       for (int r = 0; r < R; ++r)
 #pragma unroll
@@ -540,18 +543,39 @@ __global__ __launch_bounds__(kKVThreads, 1) void kv_attn_kernel(KVAttnParams p) 
         }
       __builtin_amdgcn_s_waitcnt(0xC07F);  // the queries have been read
       asm volatile("" ::: "memory");
+    };
+    if (n_tiles > 0) {
+      if constexpr (kSlots == 1) {  // the only tile's values wait for them
+        static_assert(M * 2 * D <= T::kBytes, "the queries lie where the values will");
+        stage_rows<D, R>(p, s, head, row0, rows, ring + T::kBytes, lane);
+        look_up(0);
+        const Loads loads(p, pages, key_of_tile(0), last, head);
+        loads.keys(p, ring, source, lane);
+        wait_loads<T::kScaleLoads + T::kLoads>();
+        read_queries(ring + T::kBytes);
+        loads.values(p, ring, source);
+      } else {
+        constexpr int kQuerySlots = (M * 2 * D + T::kSlot - 1) / T::kSlot, kFirst = kSlots - kQuerySlots;
+        static_assert(kFirst >= 1, "a tile beside the queries");
+        char* const staged = ring + kFirst * T::kSlot;
+        stage_rows<D, R>(p, s, head, row0, rows, staged, lane);
 #pragma unroll 1
-      for (int i = kFirst; i < min(T::kSlots, n_tiles); ++i) request(i);
-      look_up(T::kSlots);
+        for (int i = 0; i < min(kFirst, n_tiles); ++i) request(i);
+        wait_tiles<D, FP8, kSlots, 0>(min(kFirst, n_tiles));
+        read_queries(staged);
+#pragma unroll 1
+        for (int i = kFirst; i < min(kSlots, n_tiles); ++i) request(i);
+      }
+      look_up(kSlots);
     }
     int slot_at = 0;
 #pragma unroll 1
     for (int i = 0; i < n_tiles; ++i) {
       char* const slot = ring + slot_at;
       const int key0 = key_of_tile(i);
-      const int later = min(T::kSlots - 1, n_tiles - 1 - i);
-      const bool more = i + T::kSlots < n_tiles;
-      wait_tiles<D, FP8, T::kLoads>(later);  // the keys
+      const int later = min(kSlots - 1, n_tiles - 1 - i);
+      const bool more = i + kSlots < n_tiles;
+      wait_tiles<D, FP8, kSlots, T::kLoads>(later);  // the keys
       f32x4 score[R][2];
       float k_scale[8], v_scale[8];
       {  // all fragments are asked for before the first product: an LDS read takes as long as several of them
@@ -631,13 +655,13 @@ __global__ __launch_bounds__(kKVThreads, 1) void kv_attn_kernel(KVAttnParams p) 
         weight[r] = to_bf16x8(y[0], y[1], y[2], y[3], y[4], y[5], y[6], y[7]);
         if constexpr (R > 2) __builtin_amdgcn_sched_barrier(0);
       }
-      const Loads loads(p, pages, key_of_tile(i + T::kSlots), last, head);
+      const Loads loads(p, pages, key_of_tile(i + kSlots), last, head);
       if (more) {  // (the keys have been read: their products have been used)
         loads.keys(p, slot, source, lane);
-        look_up(i + T::kSlots + 1);
-        wait_loads<(T::kSlots - 1) * T::kAll + T::kScaleLoads + T::kLoads>();
+        look_up(i + kSlots + 1);
+        wait_loads<(kSlots - 1) * T::kAll + T::kScaleLoads + T::kLoads>();
       } else {
-        wait_tiles<D, FP8, 0>(later);  // the values
+        wait_tiles<D, FP8, kSlots, 0>(later);  // the values
       }
       if (partial) clean_values<D, FP8, R>(slot + T::kBytes, lane, seen, up, down);
       const uint32_t values = lds_address(slot) + value_at;
@@ -658,7 +682,7 @@ __global__ __launch_bounds__(kKVThreads, 1) void kv_attn_kernel(KVAttnParams p) 
         asm volatile("" ::: "memory");
         loads.values(p, slot, source);
       }
-      slot_at = slot_at + T::kSlot == T::kRing ? 0 : slot_at + T::kSlot;
+      slot_at = slot_at + T::kSlot == kRing ? 0 : slot_at + T::kSlot;
     }
 
     // The waves' results of the segment, joined through LDS: a wave's rows lie in its own region, piece (four features) q of row r at q ^ (r % 16).
@@ -718,11 +742,15 @@ __global__ __launch_bounds__(kKVThreads, 1) void kv_attn_kernel(KVAttnParams p) 
 
 template <int D>
 void launch_kv_attn(const KVAttnParams& p, bool fp8, int row_groups, int workgroups, hipStream_t s) {
+  if constexpr (D == 128)
+    if (row_groups == 4) {  // (bf16 only, see plan_of)
+      kv_attn_kernel<128, false, 4><<<workgroups, kKVThreads, 0, s>>>(p);
+      return;
+    }
   const auto launch = [&](auto f) {
     constexpr bool F = decltype(f)::value;
     if (row_groups == 1) kv_attn_kernel<D, F, 1><<<workgroups, kKVThreads, 0, s>>>(p);
-    else if (row_groups == 2) kv_attn_kernel<D, F, 2><<<workgroups, kKVThreads, 0, s>>>(p);
-    else kv_attn_kernel<D, F, 4><<<workgroups, kKVThreads, 0, s>>>(p);
+    else kv_attn_kernel<D, F, 2><<<workgroups, kKVThreads, 0, s>>>(p);
   };
   if (fp8) launch(std::true_type());
   else launch(std::false_type());

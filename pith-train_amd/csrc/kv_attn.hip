@@ -97,32 +97,35 @@ struct KVPlan {
   int64_t joins_at, stats_at, results_at, bytes;  // workspace
 };
 
-// Steps (of 16 rows) up to which no row block is cut: below it the join's launch (4 us) costs more than what the cut gains. One sequence of 517 rows, 4 heads,
-// 9.5 us whole and 10.6 cut; 32 x 4 heads of 16 selected pages 18.8 and 18.6.
-constexpr int64_t kWholeSteps = 8;
-
 KVPlan plan_of(const pith_kv_attn_args* a) {
   KVPlan pl = {};
-  const int units = compute_units_or_default() & ~7;
+  const int units = std::max(compute_units_or_default() & ~7, 8);
   const int64_t group = a->H / a->cache.heads, rows = a->T * group;  // rows of a key-value head
-  const int64_t steps = (a->table_width * a->cache.page_size + kStepKeys - 1) / kStepKeys;
-  const auto items = [&](int64_t m) { return ((rows + m - 1) / m + std::min(a->B, a->T)) * a->cache.heads; };
-  // Rows of a row block. Fewer bytes with more of them, but every workgroup begins and ends with 64 rows more slowly, and rows that are not there are computed
-  // all the same; so it goes by the rows of a sequence and by the steps that a workgroup has with blocks of 16 and full page tables. us at 16 / 32 / 64
-  // rows, bf16, heads of 32 / 4: 32 x 8192 rows, 2 tokens 74 / 76 / 82, 4 tokens 108 / 81 / 85, 8 tokens 198 / 117 / 93; 8 tokens: 16 x 8192 (80 steps)
-  // 106 / 65 / 52, 8 x 8192 (40) 63 / 32 / 34, 16 x 2048 (20) 30 / 25 / 29, 4 x 4096 (10) 19 / 20 / 24; 16 tokens, e4m3, 16 x 2048 (36) 53 / 47 / 41; 512
-  // tokens behind 8192 (257) 214 / 157 / 116.
-  const int64_t work = items(16) * steps / std::max(units, 8);
-  pl.row_groups = rows <= 16 * a->B || work <= 14 ? 1 : rows <= 32 * a->B || work <= 36 ? 2 : 4;
+  const int64_t steps = (a->table_width * a->cache.page_size + kStepKeys - 1) / kStepKeys, sequences = std::min(a->B, a->T);
+  const auto items = [&](int64_t m) { return ((rows + m - 1) / m + sequences) * a->cache.heads; };
+  // Rows of a row block. Fewer bytes and products with more of them, but every workgroup begins and ends with them more slowly, and rows that are not there are
+  // computed all the same: so 16 for sequences of no more, and while a compute unit has few steps with blocks of 16 and full page tables. us at 16 / 32 rows, heads
+  // of 32 / 4: 8 tokens, e4m3, 8 x 4096 rows (20 steps) 24 / 26, bf16, 16 x 2048 (20) 23 / 24, 8 x 8192 (40) 38 / 33, 16 x 8192 (80) 114 / 53; 16 tokens, e4m3, 16 x
+  // 2048 (36) 41 / 37; 2 tokens, 32 x 8192 75 / 76. And 64 for bf16 heads of 128 where that halves the row blocks and keys and values are more than the caches hold
+  // well: 8 tokens, 32 x 8192 (360 MB) 115 at 32 rows and 92 at 64, 16 tokens, 4 x 16384 45 / 39, but 512 tokens behind 8192 rows (17 MB) 107 / 117, 64 tokens, 4 x
+  // 8192 (67 MB) 65 / 69. (With e4m3 and with heads of 64 the 64 rows lost everywhere: 16 tokens, 16 x 8192 e4m3 77 / 80.)
+  const double work = (double)items(16) * steps / units, bytes = (double)sequences * steps * kStepKeys * a->cache.heads * 512;
+  const int64_t each = (rows + sequences - 1) / sequences;
+  const bool halved = 19 * ((each + 63) / 64) <= 10 * ((each + 31) / 32);
+  if (rows <= 16 * a->B || work <= 28) pl.row_groups = 1;
+  else pl.row_groups = a->cache.dtype == PITH_BF16 && a->cache.dim == 128 && halved && bytes >= (96 << 20) ? 4 : 2;
   const int64_t m = 16 * pl.row_groups;
+  const int per_unit = pl.row_groups <= 2 ? 2 : 1;  // workgroups (KVRing)
   pl.max_items = items(m);
-  if (steps * pl.row_groups <= kWholeSteps) {
+  // No row block is cut where that would gain less than the join's launch costs (4 us), as long as there are few enough of them to begin at once, one on a compute unit: one
+  // sequence of 517 rows, 4 heads, 8.8 us whole and 10.6 cut, 8 x 1024 rows, 8 tokens 12 / 17, 23 x 71 rows 10 / 13; but 64 x 900 rows (384 row blocks) 28 / 25, 86 x 2 14.6 / 13.1.
+  if (steps * pl.row_groups <= 8 && pl.max_items <= units) {
     pl.whole = (int)steps;
     pl.workgroups = (int)((pl.max_items + 7) & ~(int64_t)7);
     pl.bytes = 256;
     return pl;
   }
-  pl.workgroups = units < 8 ? 8 : units > kMaxGroups ? kMaxGroups : units;
+  pl.workgroups = std::min(per_unit * units, kMaxGroups);
   if (a->head_tables) {
     pl.max_items = (group + m - 1) / m * a->cache.heads * a->B;
     pl.parts = (int)std::min(std::max<int64_t>(pl.workgroups / pl.max_items, 1), steps);
