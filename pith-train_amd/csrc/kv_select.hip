@@ -10,10 +10,12 @@
 // pages). With v the score of the last one chosen by these, a page above v + 2 E is in (whoever may exceed it is above v, too), one below v - 2 E is out, and
 // the few between are summed in fp64, if they are more than there are places. v is found by histograms of 256 equal parts of the range that it lies in, two most
 // often, to within 2 E. Infinities and NaN have no bound of the error: a page with one is summed in fp64 at once. NaN counts above all.
-// A step of 32 tokens with 4 heads over up to 128 pages FIGURE; 8 tokens over up to 2048 pages FIGURE.
+// All of it is latency: 32 tokens with heads of 32 / 4 over up to 128 pages 12 us, one launch; 8 over up to 2048 pages 23 us, of which the scores are 9 (27 MB of bounds,
+// 3 TB/s) and the choice 10 (two histograms, one barrier a step, and the few pages in fp64).
 #include "cache_attn.h"
 #include "kv_common.h"
 
+#include <algorithm>
 #include <type_traits>
 
 namespace pith {
@@ -28,24 +30,31 @@ struct KVSelectParams {
   int32_t *table_out, *lengths_out;
   uint2* pages_of;  // workspace, [T * heads][row]: score and S of each page, then the pages in question
   int64_t q_ts, q_hs, table_rs, bounds_ps, row;
-  int T, B, heads, group, pages, page_shift, table_width, keep, chunks;
+  int T, B, heads, group, pages, page_shift, table_width, keep, chunks, tokens;
 };
 
 // A token and key-value head.
 struct Item {
-  int t, head, seq, visible, pages;
+  int t, head, seq, length, end, visible, pages;  // end: of the sequence's tokens
   const int32_t* table;
 };
+
+__device__ __forceinline__ int pages_of(const KVSelectParams& p, int rows) { return (rows + (1 << p.page_shift) - 1) >> p.page_shift; }
+
+__device__ __forceinline__ void see(const KVSelectParams& p, Item& x) {  // what token x.t sees of its sequence (a token that is nobody's: nothing)
+  x.visible = !p.cu_q ? x.length : x.t < x.end ? min(max(x.length - x.end + x.t + 1, 0), x.length) : 0;
+  x.pages = pages_of(p, x.visible);
+}
 
 __device__ __forceinline__ Item item_of(const KVSelectParams& p, int item, int lane) {
   Item x;
   x.t = item / p.heads;
   x.head = item - x.t * p.heads;
   x.seq = sequence_of(p.cu_q, p.B, x.t, lane);
-  const int length = min(max(p.lengths[x.seq], 0), p.table_width << p.page_shift);
-  x.visible = !p.cu_q ? length : x.t < p.cu_q[p.B] ? min(max(length - p.cu_q[x.seq + 1] + x.t + 1, 0), length) : 0;  // (a token that is nobody's: 0)
-  x.pages = (x.visible + (1 << p.page_shift) - 1) >> p.page_shift;
+  x.length = min(max(p.lengths[x.seq], 0), p.table_width << p.page_shift);
+  x.end = p.cu_q ? p.cu_q[x.seq + 1] : x.t + 1;
   x.table = p.table + x.seq * p.table_rs;
+  see(p, x);
   return x;
 }
 
@@ -57,80 +66,88 @@ __device__ __forceinline__ uint32_t sort_key(float x) {
 
 typedef __attribute__((ext_vector_type(8))) short s16x8;
 
-// Scores and S (infinity: not known) of TILES times sixteen pages, `first` .. and so on, of which `scored` exist: lane c + 16 g has those of page c (whatever g).
-// Operand A is sixteen heads, B sixteen pages, so a lane's results are four heads of one page.
+// The bounds of TILES times sixteen pages, `first` .. and so on, of which `held` exist: lane c + 16 g has eight features of page c, from 8 g on, of each 32.
 template <int D, int TILES>
-__device__ __forceinline__ void score_pages(const KVSelectParams& p, const Item& x, int first, int scored, int lane, float2 (&out)[TILES]) {
-  constexpr int kSteps = D / 32;
-  const int c = lane & 15, g = lane >> 4;
+struct PageBounds {
+  static constexpr int kSteps = D / 32;
   bf16x8 least[TILES][kSteps], largest[TILES][kSteps];
+
+  __device__ __forceinline__ void load(const KVSelectParams& p, const Item& x, int first, int held, int lane) {
+    const int c = lane & 15, g = lane >> 4;
 #pragma unroll
-  for (int i = 0; i < TILES; ++i) {
-    const int64_t page = safe_page(x.table[min(first + 16 * i + c, scored - 1)], p.pages);
-    const __bf16* const from = p.bounds + page * p.bounds_ps + (int64_t)x.head * (2 * D) + 8 * g;
+    for (int i = 0; i < TILES; ++i) {
+      const int64_t page = safe_page(x.table[min(first + 16 * i + c, held - 1)], p.pages);
+      const __bf16* const from = p.bounds + page * p.bounds_ps + (int64_t)x.head * (2 * D) + 8 * g;
 #pragma unroll
-    for (int k = 0; k < kSteps; ++k) {
-      least[i][k] = *reinterpret_cast<const bf16x8*>(from + 32 * k);
-      largest[i][k] = *reinterpret_cast<const bf16x8*>(from + D + 32 * k);
+      for (int k = 0; k < kSteps; ++k) {
+        least[i][k] = *reinterpret_cast<const bf16x8*>(from + 32 * k);
+        largest[i][k] = *reinterpret_cast<const bf16x8*>(from + D + 32 * k);
+      }
     }
-  }
-  // The split into q+ and q- asks for least <= largest; bounds of somebody else's making that are the other way round are exchanged. (As fp32 the upper of two
-  // features is compared with the lower one behind it: that says too often at most.)
-  int turned = 0;
-#pragma unroll
-  for (int i = 0; i < TILES; ++i)
-#pragma unroll
-    for (int k = 0; k < kSteps; ++k) {
-      const u32x4 a = __builtin_bit_cast(u32x4, least[i][k]), b = __builtin_bit_cast(u32x4, largest[i][k]);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) turned |= (int)(__uint_as_float(a[e]) > __uint_as_float(b[e])) | (int)(bf16lo_to_f32(a[e]) > bf16lo_to_f32(b[e]));
-    }
-  if (__any(turned)) {
+    // The split into q+ and q- asks for least <= largest; bounds of somebody else's making that are the other way round are exchanged. (As fp32 the upper of two
+    // features is compared with the lower one behind it: that says too often at most.)
+    int turned = 0;
 #pragma unroll
     for (int i = 0; i < TILES; ++i)
 #pragma unroll
-      for (int k = 0; k < kSteps; ++k)
+      for (int k = 0; k < kSteps; ++k) {
+        const u32x4 a = __builtin_bit_cast(u32x4, least[i][k]), b = __builtin_bit_cast(u32x4, largest[i][k]);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const __bf16 a = least[i][k][e], b = largest[i][k][e];
-          const bool other = (float)a > (float)b;
-          least[i][k][e] = other ? b : a, largest[i][k][e] = other ? a : b;
-        }
+        for (int e = 0; e < 4; ++e) turned |= (int)(__uint_as_float(a[e]) > __uint_as_float(b[e])) | (int)(bf16lo_to_f32(a[e]) > bf16lo_to_f32(b[e]));
+      }
+    if (__any(turned)) {
+#pragma unroll
+      for (int i = 0; i < TILES; ++i)
+#pragma unroll
+        for (int k = 0; k < kSteps; ++k)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const __bf16 a = least[i][k][e], b = largest[i][k][e];
+            const bool other = (float)a > (float)b;
+            least[i][k][e] = other ? b : a, largest[i][k][e] = other ? a : b;
+          }
+    }
   }
+
+  // Scores and S (infinity: not known) of the token's head: lane c + 16 g has those of page c (whatever g). Operand A is sixteen heads, B sixteen pages, so a
+  // lane's results are four heads of one page.
+  __device__ __forceinline__ void score(const KVSelectParams& p, const Item& x, int lane, float2 (&out)[TILES]) const {
+    const int c = lane & 15, g = lane >> 4;
 #pragma unroll
-  for (int i = 0; i < TILES; ++i) out[i] = make_float2(-INFINITY, 0.f);
+    for (int i = 0; i < TILES; ++i) out[i] = make_float2(-INFINITY, 0.f);
 #pragma unroll 1
-  for (int h0 = 0; h0 < p.group; h0 += 16) {
-    const __bf16* const from = p.q + x.t * p.q_ts + (int64_t)(x.head * p.group + min(h0 + c, p.group - 1)) * p.q_hs + 8 * g;
-    s16x8 q[kSteps];
+    for (int h0 = 0; h0 < p.group; h0 += 16) {
+      const __bf16* const from = p.q + x.t * p.q_ts + (int64_t)(x.head * p.group + min(h0 + c, p.group - 1)) * p.q_hs + 8 * g;
+      s16x8 q[kSteps];
 #pragma unroll
-    for (int k = 0; k < kSteps; ++k) q[k] = *reinterpret_cast<const s16x8*>(from + 32 * k);
-    f32x4 sum[TILES], mass[TILES];
+      for (int k = 0; k < kSteps; ++k) q[k] = *reinterpret_cast<const s16x8*>(from + 32 * k);
+      f32x4 sum[TILES], mass[TILES];
 #pragma unroll
-    for (int i = 0; i < TILES; ++i) sum[i] = mass[i] = f32x4{};
+      for (int i = 0; i < TILES; ++i) sum[i] = mass[i] = f32x4{};
 #pragma unroll
-    for (int k = 0; k < kSteps; ++k) {
-      const s16x8 below = q[k] >> 15;  // all bits where q is below zero
-      const auto bf = [](s16x8 v) __attribute__((always_inline)) { return __builtin_bit_cast(bf16x8, v); };
-      const auto magnitude = [&](bf16x8 v) __attribute__((always_inline)) { return bf(__builtin_bit_cast(s16x8, v) & (short)0x7fff); };
-      const bf16x8 up = bf(q[k] & ~below), down = bf(q[k] & below), down_size = magnitude(down);
+      for (int k = 0; k < kSteps; ++k) {
+        const s16x8 below = q[k] >> 15;  // all bits where q is below zero
+        const auto bf = [](s16x8 v) __attribute__((always_inline)) { return __builtin_bit_cast(bf16x8, v); };
+        const auto magnitude = [&](bf16x8 v) __attribute__((always_inline)) { return bf(__builtin_bit_cast(s16x8, v) & (short)0x7fff); };
+        const bf16x8 up = bf(q[k] & ~below), down = bf(q[k] & below), down_size = magnitude(down);
 #pragma unroll
-      for (int i = 0; i < TILES; ++i) {
-        sum[i] = mfma16(up, largest[i][k], mfma16(down, least[i][k], sum[i]));
-        mass[i] = mfma16(up, magnitude(largest[i][k]), mfma16(down_size, magnitude(least[i][k]), mass[i]));
+        for (int i = 0; i < TILES; ++i) {
+          sum[i] = mfma16(up, largest[i][k], mfma16(down, least[i][k], sum[i]));
+          mass[i] = mfma16(up, magnitude(largest[i][k]), mfma16(down_size, magnitude(least[i][k]), mass[i]));
+        }
       }
+#pragma unroll
+      for (int i = 0; i < TILES; ++i)
+#pragma unroll
+        for (int v = 0; v < 4; ++v) {
+          out[i].x = fmaxf(out[i].x, sum[i][v]);
+          out[i].y = fmaxf(out[i].y, mass[i][v] < INFINITY ? mass[i][v] : INFINITY);
+        }
     }
 #pragma unroll
-    for (int i = 0; i < TILES; ++i)
-#pragma unroll
-      for (int v = 0; v < 4; ++v) {
-        out[i].x = fmaxf(out[i].x, sum[i][v]);
-        out[i].y = fmaxf(out[i].y, mass[i][v] < INFINITY ? mass[i][v] : INFINITY);
-      }
+    for (int i = 0; i < TILES; ++i) out[i] = make_float2(quad_max(out[i].x), quad_max(out[i].y));
   }
-#pragma unroll
-  for (int i = 0; i < TILES; ++i) out[i] = make_float2(quad_max(out[i].x), quad_max(out[i].y));
-}
+};
 
 // A page's score in fp64, by a whole wavefront: eight lanes a head, eight heads at a time.
 template <int D>
@@ -164,16 +181,32 @@ __device__ __forceinline__ float exact_score(const KVSelectParams& p, const Item
   return best;
 }
 
+// A workgroup: kChunk pages of a head, for p.tokens tokens, whose bounds are read once for all of a sequence.
 template <int D>
 __global__ __launch_bounds__(kThreads) void kv_score_kernel(KVSelectParams p) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int chunk = blockIdx.x % p.chunks, item = blockIdx.x / p.chunks;
-  const Item x = item_of(p, item, lane);
-  const int scored = x.pages - 1, first = chunk * kChunk + 32 * wave;  // (the token's own page is not scored)
-  if (x.pages <= p.keep || first >= scored) return;
-  float2 found[2];
-  score_pages<D, 2>(p, x, first, scored, lane, found);
-  if (lane < 32) reinterpret_cast<float2*>(p.pages_of)[item * p.row + first + lane] = lane < 16 ? found[0] : found[1];  // (of those behind the last: not read)
+  const int chunk = blockIdx.x % p.chunks, part = blockIdx.x / p.chunks, t0 = part / p.heads * p.tokens, head = part % p.heads;
+  const int first = chunk * kChunk + 32 * wave;
+  PageBounds<D, 2> bounds;
+  int loaded = -1;  // sequence
+  Item x;
+  x.end = 0;
+#pragma unroll 1
+  for (int t = t0; t < min(t0 + p.tokens, p.T); ++t) {
+    const int item = t * p.heads + head;
+    if (t < x.end) {
+      x.t = t;
+      see(p, x);
+    } else {
+      x = item_of(p, item, lane);
+    }
+    if (x.pages <= p.keep || first >= x.pages - 1) continue;  // (the token's own page is not scored)
+    if (x.seq != loaded) bounds.load(p, x, first, pages_of(p, x.length), lane);
+    loaded = x.seq;
+    float2 found[2];
+    bounds.score(p, x, lane, found);
+    if (lane < 32) reinterpret_cast<float2*>(p.pages_of)[item * p.row + first + lane] = lane < 16 ? found[0] : found[1];  // (of those behind the last: not read)
+  }
 }
 
 // Sums and maxima over a workgroup, one barrier each (the other half of what is shared is still being read from the call before).
@@ -402,7 +435,9 @@ __global__ __launch_bounds__(kThreads) void kv_pick_few_kernel(KVSelectParams p)
 #pragma unroll 1
   for (int first = 32 * wave; first < n; first += kChunk) {
     float2 found[2];
-    score_pages<D, 2>(p, x, first, n, lane, found);
+    PageBounds<D, 2> bounds;
+    bounds.load(p, x, first, n, lane);
+    bounds.score(p, x, lane, found);
     const float2 mine = lane < 16 ? found[0] : found[1];
     const bool real = lane < 32 && first + lane < n;
     const float s = settle_unknown<D>(p, x, first, real, mine, lane);
@@ -469,7 +504,13 @@ extern "C" int pith_kv_select(const pith_kv_select_args* a, pith_stream_t stream
       kv_pick_few_kernel<D><<<items, kThreads, 0, s>>>(p);
       return;
     }
-    if (a->keep > 1 && a->table_width > a->keep) kv_score_kernel<D><<<items * (unsigned)p.chunks, kThreads, 0, s>>>(p);  // (else nothing is scored)
+    if (a->keep > 1 && a->table_width > a->keep) {  // (else nothing is scored)
+      // Tokens of a workgroup: those that a sequence has on average, up to four, as long as there are two workgroups for every compute unit. us of the whole call with
+      // 1 / 2 / 4 / 8: 22 sequences of 7 over up to 674 pages, heads of 64 / 4, 53 / 46 / 44 / 46; 8 of 4 over up to 2048 39 / 33 / 31 / 31; 108 of 2 46 / 40 / 40 / 41.
+      const int64_t each = (a->T + a->B - 1) / a->B, most = items * (int64_t)p.chunks / (2 * compute_units_or_default());
+      p.tokens = (int)std::max<int64_t>(std::min<int64_t>({each, most, 4}), 1);
+      kv_score_kernel<D><<<(unsigned)((a->T + p.tokens - 1) / p.tokens * p.heads * p.chunks), kThreads, 0, s>>>(p);
+    }
     if (a->table_width <= kSomePages) kv_pick_kernel<D, 512, kSomePages / 512><<<items, 512, 0, s>>>(p);
     else kv_pick_kernel<D, 1024, kMostPages / 1024><<<items, 1024, 0, s>>>(p);
   };

@@ -3,8 +3,9 @@
 // Everything is prefix sums over the requests: offsets are sums of the counts; pages that ended requests return go behind the pool's at sums of what they
 // held; pages that are taken come off its top at sums of what is needed. A request is served if what is needed up to it and it included does not exceed the
 // pool, or it needs nothing: sums only grow, so the served ones that need pages are a beginning of the list, and the order decides, not the schedule.
-// One workgroup does that; few tokens are its work too, many go to a second launch. All of it is latency: a step of 32 requests moves 1 KB. Up to 64
-// requests are a lane each and need no barrier for their sums: 32 tokens FIGURE.
+// One workgroup does that; up to 8192 tokens are its work too, more go to a second launch. All of it is latency: a step of 32 requests moves 1 KB. Up to 64
+// requests are a lane each and need no barrier for their sums; up to 1024 are a thread each, with three barriers and sums of 32 bits. us of a call, launch
+// included: 32 requests of a token each 7.1, 423 8.7 (12.2 in the loop for any number, whose sums have 64 bits), 1000 11.8 (16.2); 16 prompts, 16384 tokens, 10.
 #include "cache_attn.h"
 #include "pith_kv.h"
 
@@ -12,7 +13,7 @@ namespace pith {
 namespace {
 
 constexpr int kThreads = 1024, kWaves = kThreads / 64;
-constexpr int kInOne = 1024;  // requests whose sums stay in LDS
+constexpr int kInOne = kThreads;  // requests whose sums stay in LDS
 
 struct PlanParams {
   const int32_t* counts;
@@ -62,6 +63,16 @@ __device__ __forceinline__ int64_t block_scan(int64_t x, int64_t* waves, int64_t
   return before + x;
 }
 
+// The same of 32 bits, with room of its own for every call: one barrier.
+__device__ __forceinline__ int block_scan(int x, int* waves) {
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  x = wave_scan(x);
+  if (lane == 63) waves[wave] = x;
+  __syncthreads();
+  const int sums = wave_scan(lane < wave ? waves[lane] : 0);
+  return x + __builtin_amdgcn_readlane(sums, 63);
+}
+
 // Position and slot of token t; the first row of a page that was taken brings it into the table. `cu(i)`, `request(i)`: of request i.
 template <typename C, typename R>
 __device__ __forceinline__ void place_token(const PlanParams& p, int64_t t, int64_t top, const C& cu, const R& request) {
@@ -93,13 +104,11 @@ __device__ __forceinline__ void place_token(const PlanParams& p, int64_t t, int6
   p.slots[t] = slot;
 }
 
-// TOKENS: at most kInOne requests, and the tokens' places in the same launch.
-template <bool TOKENS>
+// Any number of requests; the tokens are for the next launch.
 __global__ __launch_bounds__(kThreads) void plan_kernel(PlanParams p) {
   __shared__ int64_t waves[kWaves];
   __shared__ int64_t base[kInOne];
-  __shared__ int32_t held_of[kInOne], cu_of[kInOne + 1];
-  __shared__ Request request_of[TOKENS ? kInOne : 1];
+  __shared__ int32_t held_of[kInOne];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int64_t page_size = (int64_t)1 << p.page_shift, most = p.table_width << p.page_shift;
   const auto length_of = [&](int i) { return (int32_t)min(max((int64_t)p.lengths[i], (int64_t)0), most); };
@@ -148,16 +157,10 @@ __global__ __launch_bounds__(kThreads) void plan_kernel(PlanParams p) {
       p.granted[i] = served ? (int32_t)rows : 0;
       p.lengths_out[i] = count < 0 ? 0 : length + (served ? (int32_t)rows : 0);
       p.cu_q[i + 1] = (int32_t)last;
-      const Request r = {length, served, needed - need};
-      if constexpr (TOKENS) {
-        request_of[tid] = r;
-        cu_of[tid + 1] = (int32_t)last;
-      } else {
-        p.requests[i] = r;
-      }
+      p.requests[i] = Request{length, served, needed - need};
     }
   }
-  if (tid == 0) p.cu_q[0] = cu_of[0] = 0;
+  if (tid == 0) p.cu_q[0] = 0;
 #pragma unroll
   for (int d = 1; d < 64; d <<= 1) taken = max(taken, (int64_t)__shfl_xor(taken, d));
   __syncthreads();
@@ -166,11 +169,62 @@ __global__ __launch_bounds__(kThreads) void plan_kernel(PlanParams p) {
   if (tid == 0) {
     for (int w = 0; w < kWaves; ++w) taken = max(taken, waves[w]);
     p.free_count_out[0] = (int32_t)(top - taken);
-    if constexpr (!TOKENS) *p.top = top;
+    *p.top = top;
   }
-  if constexpr (TOKENS)
-    for (int64_t t = tid; t < p.T; t += kThreads)
-      place_token(p, t, top, [&](int i) { return (int64_t)cu_of[i]; }, [&](int i) { return request_of[i]; });
+}
+
+// Up to kInOne requests, a thread each, and up to kTokensInOne tokens in the same launch: 32 bits hold all sums but those of the pages that come back.
+constexpr int64_t kTokensInOne = 8192;
+__global__ __launch_bounds__(kThreads) void plan_some_kernel(PlanParams p) {
+  __shared__ int64_t back_sums[kWaves];
+  __shared__ int64_t base[kInOne];
+  __shared__ int32_t held_of[kInOne], cu_of[kInOne + 1], row_sums[kWaves], page_sums[kWaves], most_taken[kWaves];
+  __shared__ Request request_of[kInOne];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int page = 1 << p.page_shift, most = (int)(p.table_width << p.page_shift), tokens = (int)p.T;
+  const bool some = tid < p.B;
+  const int count = some ? p.counts[tid] : 0;
+  const int length = some ? min(max(p.lengths[tid], 0), most) : 0;
+  const int64_t had = min(max((int64_t)p.free_count[0], (int64_t)0), p.pool);
+  const auto pages_of = [&](int rows) { return (int)(((unsigned)rows + page - 1) >> p.page_shift); };
+  const int held = pages_of(length);
+
+  int64_t back = 0;
+  if (__syncthreads_or(count < 0)) {  // (the barrier is also for those that have yet to read what is written below)
+    const int64_t mine = count < 0 ? held : 0;
+    base[tid] = had + block_scan(mine, back_sums, back) - mine;
+    held_of[tid] = (int)mine;
+    __syncthreads();
+    for (int r = wave; r < p.B; r += kWaves) {  // a wave each
+      const int n = held_of[r];
+      for (int k = lane; k < n; k += 64)
+        if (base[r] + k < p.pool) p.free_pages[base[r] + k] = p.table[r * p.table_rs + k];
+    }
+  }
+  const int64_t top = min(had + back, p.pool);
+
+  const int wanted = min(max(count, 0), tokens);
+  const int upto = block_scan(wanted, row_sums), first = min(upto - wanted, tokens), last = min(upto, tokens), rows = last - first;
+  const bool fits = count >= 0 && rows <= most - length;
+  const int need = fits ? pages_of(length + rows) - held : 0;
+  const int needed = block_scan(need, page_sums);
+  const bool served = fits && (need == 0 || needed <= top);
+  const int taken = wave_scan_max(served && need > 0 ? needed : 0);
+  if (lane == 63) most_taken[wave] = taken;
+  if (some) {
+    p.granted[tid] = served ? rows : 0;
+    p.lengths_out[tid] = count < 0 ? 0 : length + (served ? rows : 0);
+    p.cu_q[tid + 1] = cu_of[tid + 1] = last;
+    request_of[tid] = Request{length, served, needed - need};
+  }
+  if (tid == 0) p.cu_q[0] = cu_of[0] = 0;
+  __syncthreads();  // (and what was laid on the pool is there)
+  if (wave == 0) {
+    const int all = wave_scan_max(lane < kWaves ? most_taken[lane] : 0);
+    if (lane == 63) p.free_count_out[0] = (int32_t)(top - all);
+  }
+  for (int t = tid; t < tokens; t += kThreads)
+    place_token(p, t, top, [&](int i) { return (int64_t)cu_of[i]; }, [&](int i) { return request_of[i]; });
 }
 
 __global__ __launch_bounds__(256) void place_kernel(PlanParams p) {
@@ -260,7 +314,6 @@ __global__ __launch_bounds__(kThreads) void plan_few_kernel(PlanParams p) {
   }
 }
 
-constexpr int64_t kTokensInOne = 8192;
 bool in_one(const pith_plan_step_args* a) { return a->B <= kInOne && a->T <= kTokensInOne; }
 
 int check_plan(const pith_plan_step_args* a, const char* who) {
@@ -311,12 +364,12 @@ extern "C" int pith_plan_step(const pith_plan_step_args* a, pith_stream_t stream
     const int64_t threads = (a->T + 63) & ~(int64_t)63;
     plan_few_kernel<<<1, (unsigned)(threads < 64 ? 64 : threads > kThreads ? kThreads : threads), 0, s>>>(p);
   } else if (one) {
-    plan_kernel<true><<<1, kThreads, 0, s>>>(p);
+    plan_some_kernel<<<1, kThreads, 0, s>>>(p);
   } else {
     p.top = (int64_t*)a->workspace;
     p.requests = (Request*)((char*)a->workspace + 16);
     if (a->B <= 64 && a->T <= 1 << 24) plan_few_kernel<<<1, 256, 0, s>>>(p);
-    else plan_kernel<false><<<1, kThreads, 0, s>>>(p);
+    else plan_kernel<<<1, kThreads, 0, s>>>(p);
     if (a->T > 0) place_kernel<<<(unsigned)((a->T + 255) / 256), 256, 0, s>>>(p);
   }
   return check_launch(who);
