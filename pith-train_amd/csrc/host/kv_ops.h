@@ -66,11 +66,13 @@ Six plan_step(const Tensor& counts, const Tensor& lengths, const Tensor& table, 
         is_index(free_pages, counts, at::kInt, {a.pool_size}) && is_index(free_count, counts, at::kInt, {1})) {
       // one allocation for all results and the workspace: six of them would take longer than the kernel
       a.workspace_bytes = pith_plan_step_workspace_bytes(&a);
-      const int64_t ints = a.workspace_bytes + 16 * tokens;
-      const Tensor whole = fresh(counts, {ints + 4 * (3 * a.B + 2)}, at::kByte);
-      const Tensor positions = part_of(whole, a.workspace_bytes, tokens, at::kLong), slots = part_of(whole, a.workspace_bytes + 8 * tokens, tokens, at::kLong),
-                   cu_q = part_of(whole, ints, a.B + 1, at::kInt), after = part_of(whole, ints + 4 * (a.B + 1), a.B, at::kInt),
-                   granted = part_of(whole, ints + 4 * (2 * a.B + 1), a.B, at::kInt), count = part_of(whole, ints + 4 * (3 * a.B + 1), 1, at::kInt);
+      // (their parts begin at multiples of 16 bytes, which compiled graphs expect of a result)
+      int64_t end = a.workspace_bytes;
+      const auto place = [&](int64_t n, int64_t size) { return std::exchange(end, (end + n * size + 15) & ~(int64_t)15); };
+      const int64_t at_positions = place(tokens, 8), at_slots = place(tokens, 8), at_cu = place(a.B + 1, 4), at_after = place(a.B, 4), at_granted = place(a.B, 4), at_count = place(1, 4);
+      const Tensor whole = fresh(counts, {end}, at::kByte);
+      const Tensor positions = part_of(whole, at_positions, tokens, at::kLong), slots = part_of(whole, at_slots, tokens, at::kLong), cu_q = part_of(whole, at_cu, a.B + 1, at::kInt),
+                   after = part_of(whole, at_after, a.B, at::kInt), granted = part_of(whole, at_granted, a.B, at::kInt), count = part_of(whole, at_count, 1, at::kInt);
       a.workspace = whole.data_ptr();
       a.counts = counts.data_ptr<int32_t>(); a.lengths = lengths.data_ptr<int32_t>();
       a.page_table = table.data_ptr<int32_t>();

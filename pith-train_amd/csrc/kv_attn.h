@@ -59,7 +59,7 @@ struct KVAttnParams {
   int max_len;      // table_width * page_size
   float kappa;      // scale * log2(e)
   int whole;        // steps of the longest row block where none is cut, else 0
-  int parts;        // of every row block, where all are cut alike, else 0
+  int parts;        // of every row block, where all are cut alike (into two or more), else 0
   // workspace (not used where none is cut)
   int* items;        // number of row blocks of this call
   KVJoin* joins;     // [row blocks]
@@ -201,7 +201,7 @@ struct KVWalk {
     return false;
   }
   __device__ __forceinline__ int n_steps() const { return min(s.steps - step, end - at); }  // (a part without keys: 0 or less)
-  __device__ __forceinline__ bool whole(const KVAttnParams& p) const { return p.parts ? p.parts == 1 : n_steps() == s.steps; }
+  __device__ __forceinline__ bool whole(const KVAttnParams& p) const { return !p.parts && n_steps() == s.steps; }
   __device__ __forceinline__ int slot(const KVAttnParams& p) const { return p.parts ? range : 2 * range + (at == begin ? 0 : 1); }
   // Who ends a row block says how it was cut.
   __device__ __forceinline__ void leave_join(const KVAttnParams& p, int row0, int head, int rows) const {
@@ -344,7 +344,6 @@ __device__ __forceinline__ void wait_tiles(int later) {
   else if (SLOTS >= 2 && later >= 1) wait_loads<kAll + EXTRA>();
   else wait_loads<EXTRA>();
 }
-
 
 // Operand A over 32 keys, features 16 n ..; `first`: lds_address of the values + the lane's place. Element 4 h + v: key 16 h + 4 g + v.
 template <int D, bool FP8>

@@ -92,7 +92,7 @@ struct KVPlan {
   int row_groups;  // of 16 query rows, to a row block
   int workgroups;  // a multiple of 8
   int whole;       // steps of the longest row block where none is cut, else 0
-  int parts;       // of every row block, where all are cut alike, else 0
+  int parts;       // of every row block, where all are cut alike (into two or more), else 0
   int64_t max_items;
   int64_t joins_at, stats_at, results_at, bytes;  // workspace
 };
@@ -119,17 +119,20 @@ KVPlan plan_of(const pith_kv_attn_args* a) {
   pl.max_items = items(m);
   // No row block is cut where that would gain less than the join's launch costs (4 us), as long as there are few enough of them to begin at once, one on a compute unit: one
   // sequence of 517 rows, 4 heads, 8.8 us whole and 10.6 cut, 8 x 1024 rows, 8 tokens 12 / 17, 23 x 71 rows 10 / 13; but 64 x 900 rows (384 row blocks) 28 / 25, 86 x 2 14.6 / 13.1.
-  if (steps * pl.row_groups <= 8 && pl.max_items <= units) {
-    pl.whole = (int)steps;
-    pl.workgroups = (int)((pl.max_items + 7) & ~(int64_t)7);
-    pl.bytes = 256;
-    return pl;
-  }
+  bool whole = steps * pl.row_groups <= 8 && pl.max_items <= units;
   pl.workgroups = std::min(per_unit * units, kMaxGroups);
   if (a->head_tables) {
     pl.max_items = (group + m - 1) / m * a->cache.heads * a->B;
     pl.parts = (int)std::min(std::max<int64_t>(pl.workgroups / pl.max_items, 1), steps);
     pl.workgroups = (int)((pl.max_items * pl.parts + 7) & ~(int64_t)7);
+    whole = whole || pl.parts == 1;
+  }
+  if (whole) {
+    pl.whole = (int)steps;
+    pl.parts = 0;
+    pl.workgroups = (int)((pl.max_items + 7) & ~(int64_t)7);
+    pl.bytes = 256;
+    return pl;
   }
   const auto up = [](int64_t x) { return (x + 255) & ~(int64_t)255; };
   const int64_t slot_rows = (pl.parts ? 1 : 2) * (int64_t)pl.workgroups * m;
@@ -206,7 +209,7 @@ extern "C" int pith_kv_attn(const pith_kv_attn_args* a, pith_stream_t stream) {
   begin_launch();
   if (dim == 128) launch_kv_attn_d128(p, fp8, pl.row_groups, pl.workgroups, s);
   else launch_kv_attn_d64(p, fp8, pl.row_groups, pl.workgroups, s);
-  if (!pl.whole && pl.parts != 1) {
+  if (!pl.whole) {
     const dim3 grid((unsigned)pl.max_items, (unsigned)(16 * pl.row_groups / kJoinRows));
     if (dim == 128) kv_join_kernel<128><<<grid, kJoinThreads, 0, s>>>(p, 16 * pl.row_groups);
     else kv_join_kernel<64><<<grid, kJoinThreads, 0, s>>>(p, 16 * pl.row_groups);

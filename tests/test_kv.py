@@ -196,7 +196,7 @@ CALLS = {
         (dict(q=None), NULL), (dict(bounds=None), NULL), (dict(table_out=None), NULL), (dict(workspace=None), NULL), (dict(H=3), SHAPE), (dict(heads=0), SHAPE), (dict(dim=32), UNSUPPORTED),
         (dict(keep=0), SHAPE), (dict(keep=1 << 21), SHAPE), (dict(pages=0), SHAPE), (dict(page_size=20), SHAPE), (dict(bounds_ps=504), SHAPE), (dict(q_ts=120), SHAPE), (dict(q=264), ALIGN),
         (dict(q_hs=132), ALIGN), (dict(bounds_ps=516), ALIGN), (dict(workspace=128), ALIGN), (dict(workspace_bytes=64), SHAPE),
-        (dict(T=1 << 20, heads=128, H=128, bounds_ps=128 * 256, table_width=64, table_rs=64), UNSUPPORTED)]),
+        (dict(T=1 << 20, heads=128, H=128, bounds_ps=128 * 256, table_width=64, table_rs=64), UNSUPPORTED), (dict(table_width=16385, table_rs=16385), UNSUPPORTED)]),
 }  # fmt: skip
 
 

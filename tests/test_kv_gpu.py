@@ -574,6 +574,28 @@ def test_selection_from_more_pages_than_stay_in_lds(gpu):
     _selection(gpu, [16 * 9001 + 5, 16 * 8193], (2, 1, 64), 77, seed=6)
 
 
+@pytest.mark.parametrize("heads, counts, lengths, extra", [
+    ((4, 2, 128), [7] * 40 + [0, 1, 20, 0], [16 * (270 + i) + i for i in range(40)] + [5, 16 * 300, 16 * 310 + 3, 0], 5), ((6, 1, 64), [600], [16 * 700 + 9], 0), ((3, 3, 64), [2] * 200, [16 * 260 + i for i in range(200)], 1)],
+    ids=["drafts", "prompt", "pairs"])  # fmt: skip
+def test_selection_where_bounds_serve_several_tokens(gpu, heads, counts, lengths, extra):
+    _selection(gpu, lengths, heads, 9, counts=counts, seed=11, extra=extra)
+
+
+def test_selection_from_the_widest_tables(gpu):
+    _selection(gpu, [16 * 16382, 16 * 2048, 7], (2, 1, 64), 30, seed=12)
+
+
+def test_selection_reads_slices_and_bounds_of_one_layer_of_several(gpu):
+    g = torch.Generator().manual_seed(13)
+    b = Batch(gpu, [1, 3], [16 * 300, 16 * 280 + 5], (4, 2, 64), page=16, seed=13)
+    bounds = torch.randn(b.kv[0].shape[0], 3, 2, 2, 64, generator=g).sort(dim=3).values.to(BF).to(gpu)
+    wide = torch.randn(4, 8, 64, generator=g).to(BF).to(gpu)
+    for pages, q in ((bounds[:, 1], wide[:, 2:6]), (bounds[:, 2], b.q)):
+        got = K.kv_select_pages(q, pages, b.table, b.lens, b.cu_q, 16, 20)
+        want = K.kv_select_pages(q.contiguous(), pages.contiguous(), b.table, b.lens, b.cu_q, 16, 20)
+        assert torch.equal(got.page_table, want.page_table) and torch.equal(got.lengths, want.lengths)
+
+
 def test_equal_scores_go_to_the_pages_that_come_first(gpu):
     g = torch.Generator().manual_seed(7)
     bounds = torch.randint(0, 2, (102, 2, 2, 64), generator=g).to(BF)  # few different scores
@@ -632,7 +654,7 @@ def _plan_case(gpu, counts, lengths, page, tokens, spare, width, seed=0, into=Fa
 
 
 @pytest.mark.parametrize("into", [False, True])
-@pytest.mark.parametrize("b", [1, 5, 64, 300, 1500])
+@pytest.mark.parametrize("b", [1, 5, 64, 300, 1500, 65, 1024, 1025])
 @pytest.mark.parametrize("scarce", [False, True])
 def test_plans_are_the_oracles(gpu, b, scarce, into):
     g = torch.Generator().manual_seed(b)
@@ -658,12 +680,21 @@ def test_plans_of_long_prompts(gpu):
     assert plan.cu_q.tolist() == [0] and plan.slots.tolist() == [-1, -1] and plan.free_count.tolist() == [3]
 
 
+@pytest.mark.parametrize("b, tokens", [(3, 5), (70, 9001), (1100, 7)])
+def test_the_results_of_a_plan_lie_apart_and_aligned(gpu, b, tokens):
+    i32 = lambda *s: torch.zeros(*s, dtype=I32, device=gpu)  # noqa: E731
+    plan = paging.plan_step(i32(b), i32(b), i32(b, 4), paging.PagePool.full(3, gpu), 16, tokens)
+    assert [tuple(t.shape) for t in plan] == [(b + 1,), (b,), (tokens,), (tokens,), (b,), (1,)]
+    spans = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()) for t in plan)
+    assert all(t.data_ptr() % 16 == 0 and t.is_contiguous() for t in plan) and all(x[1] <= y[0] for x, y in zip(spans, spans[1:]))
+
+
 def test_nonsense_in_a_plan_stays_in_memory(gpu):
     i32 = lambda x: torch.tensor(x, dtype=I32, device=gpu)  # noqa: E731
     big = 2**31 - 1
     for count in (-5, big):
-        for lengths, counts in (([big, -big, 3], [1, 2, 3]), ([big, big, big], [-1, -7, big]), ([5, 5, 5], [big, big, big])):
-            table, free = torch.full((3, 4), big, dtype=I32, device=gpu), torch.full((6,), -big, dtype=I32, device=gpu)
+        for lengths, counts in (([big, -big, 3], [1, 2, 3]), ([big, big, big], [-1, -7, big]), ([5, 5, 5], [big, big, big]), ([big, -5, 3] * 30, [big, -1, big] * 30), ([big, 1] * 600, [-1, big] * 600)):
+            table, free = torch.full((len(counts), 4), big, dtype=I32, device=gpu), torch.full((6,), -big, dtype=I32, device=gpu)
             plan = paging.plan_step(i32(counts), i32(lengths), table, paging.PagePool(free, i32([count])), 16, 9)
             assert 0 <= int(plan.free_count) <= 6 and int(plan.cu_q[-1]) <= 9
             paging.plan_step(i32(counts), i32(lengths), table, paging.PagePool(free, i32([count])), 16, 20000)
@@ -803,6 +834,170 @@ def test_on_another_stream(gpu):
         plan = paging.plan_step(torch.ones(2, dtype=I32, device=gpu), b.lens, b.table.clone(), paging.PagePool.full(3, gpu), 64, 2)
     s.synchronize()
     assert all(torch.equal(x, y) for one in got for x, y in zip(one, want)) and plan.cu_q.tolist() == [0, 1, 2]
+
+
+def test_two_streams_at_once(gpu):
+    """Calls in flight on two streams have workspaces of their own."""
+    batches = [Batch(gpu, [1, 1, 2], [9000, 7000, 400], (8, 2, 128), page=16, seed=s) for s in (50, 51)]
+    bounds = [torch.randn(b.kv[0].shape[0], 2, 2, 128, generator=torch.Generator().manual_seed(s)).sort(dim=2).values.to(BF).to(gpu) for s, b in enumerate(batches)]
+
+    def calls(b, pages):
+        selected = K.kv_select_pages(b.q, pages, b.table, b.lens, b.cu_q, 16, 40)
+        return [*b.attention(), *selected, *K.kv_attention(b.q, b.cache, *selected, None, b.scale)]
+
+    want = [calls(*x) for x in zip(batches, bounds)]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = [[], []]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    for _ in range(10):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(calls(batches[i], bounds[i]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for one in got[i]:
+            assert all(torch.equal(x, y) for x, y in zip(one, want[i]))
+
+
+@BOTH
+def test_a_captured_sparse_step_is_the_eager_one(gpu, fp8):
+    """A whole step in a graph (plan, append, bounds, selection, attention to the selected pages), replayed beside the same steps run eagerly on tensors of their own."""
+    h, hkv, d, page, pages, b, width, tokens, keep = 8, 2, 64, 16, 200, 3, 60, 12, 4
+    g = torch.Generator().manual_seed(52)
+    cos, sin = (x.to(gpu) for x in _tables(d, 1000))
+    counts, qkv = torch.zeros(b, dtype=I32, device=gpu), torch.zeros(tokens, h + 2 * hkv, d, dtype=BF, device=gpu)
+
+    class State:
+        def __init__(self):
+            mk = lambda n, t=I32: torch.zeros(n, dtype=t, device=gpu)  # noqa: E731
+            self.cache = K.KVCache.empty(pages, hkv, d, page, L.FP8 if fp8 else BF, gpu)
+            for x in self.cache:
+                if x is not None:
+                    x.view(torch.uint8).zero_()
+            self.bounds = self.cache.empty_bounds().zero_()
+            self.pool, self.table, self.lengths = paging.PagePool.full(pages, gpu), torch.full((b, width), -1, dtype=I32, device=gpu), mk(b)
+            self.plan = paging.StepPlan(mk(b + 1), self.lengths, mk(tokens, I64), mk(tokens, I64), mk(b), self.pool.count)
+
+        def step(self):
+            p = self.plan
+            paging.plan_step_into(counts, self.lengths, self.table, self.pool, page, p)
+            return K.kv_decode(*qkv.split((h, hkv, hkv), 1), None, None, cos, sin, p.position_ids, p.slots, self.cache, self.table, self.lengths, p.cu_q, d**-0.5, bounds=self.bounds, keep=keep)
+
+        def all(self):
+            return [x for x in (*self.cache, self.bounds, *self.pool, self.table, *self.plan) if x is not None]
+
+    eager, captured = State(), State()
+    eager.step(), captured.step()  # (no tokens)
+    graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.graph(graph, stream=side):
+        out = captured.step()
+    for new in [[4, 4, 4]] * 20 + [[1, 1, 1], [2, -1, 3], [1, 9, 1], [-1, -1, 8]] + [[1, 1, 1]] * 6:
+        counts.copy_(torch.tensor(new, dtype=I32))
+        qkv.copy_(torch.randn(tokens, h + 2 * hkv, d, generator=g).to(BF))
+        graph.replay()
+        want = eager.step()
+        torch.cuda.synchronize()
+        n = sum(max(c, 0) for c in new)
+        assert torch.equal(out[:n], want[:n]) and int(eager.plan.cu_q[-1]) == n
+        assert all(torch.equal(x.view(torch.uint8), y.view(torch.uint8)) for x, y in zip(captured.all(), eager.all())), new
+
+
+@BOTH
+def test_a_compiled_step_writes_the_cache(gpu, fp8):
+    """The same results and the same rows in the cache as the eager step's, whose tensors the compiled one changes in place."""
+    g = torch.Generator().manual_seed(53)
+    qkv = torch.randn(6, 8, 64, generator=g).to(BF).to(gpu)
+    w = (1 + 0.1 * torch.randn(64, generator=g)).to(BF).to(gpu)
+    cos, sin = (x.to(gpu) for x in _tables(64, 60))
+    counts, lengths = torch.tensor([4, 2], dtype=I32, device=gpu), torch.tensor([30, 0], dtype=I32, device=gpu)
+
+    def step(table, free, count, bounds, *cache):
+        cache = K.KVCache(*cache)
+        plan = paging.plan_step(counts, lengths, table, paging.PagePool(free, count), 16, 6)
+        o = K.kv_decode(*qkv.split((4, 2, 2), 1), w, w, cos, sin, plan.position_ids, plan.slots, cache, table, plan.lengths, plan.cu_q, 0.125, bounds=bounds, keep=2)
+        return o, K.kv_attention(qkv[:, :4].contiguous(), cache, table, plan.lengths, plan.cu_q, 0.125)[0] * 2, plan.slots + 1
+
+    states = []
+    for _ in range(2):
+        cache = K.KVCache.empty(6, 2, 64, 16, L.FP8 if fp8 else BF, gpu)
+        pool = paging.PagePool.full(6, gpu)
+        state = [torch.tensor([[4, 5, -1], [-1, -1, -1]], dtype=I32, device=gpu), pool.free.flip(0).contiguous(), pool.count, cache.empty_bounds(), *(x for x in cache if x is not None)]
+        for x in state[3:]:
+            x.view(torch.uint8).zero_()
+        state[2].fill_(4)
+        states.append(state)
+    with torch.no_grad():
+        want = step(*states[0])
+        got = torch.compile(step, backend="aot_eager", fullgraph=True)(*states[1])
+    assert all(torch.equal(x, y) for x, y in zip(got, want)) and want[2].tolist() == [16 * 5 + 15, 16 * 5 + 16, 16 * 3 + 1, 16 * 3 + 2, 16 * 2 + 1, 16 * 2 + 2]
+    for x, y in zip(*states):
+        assert torch.equal(x.view(torch.uint8), y.view(torch.uint8)) and y.view(torch.uint8).any()
+
+
+# ---------------------------------------------------------------------------------------------
+# Far apart and long
+
+
+def _apart(x, gap):
+    buffer = torch.empty((x.shape[0] - 1) * gap + x[0].numel(), dtype=x.dtype, device=x.device)
+    y = buffer.as_strided(x.shape, (gap, *x.stride()[1:]))
+    for a, b in zip(y, x):
+        a.copy_(b)
+    return y
+
+
+@BOTH
+def test_pages_that_lie_further_apart_than_32_bits_count(gpu, fp8):
+    b = Batch(gpu, [2, 1], [100, 30], (4, 2, 64), page=64, fp8=fp8, seed=54)
+    far = K.KVCache(*(None if x is None else _apart(x, (1 << 30) + 64 if x.dtype == torch.float32 else (1 << 31) + 64) for x in b.cache))
+    for x, y in zip(K.kv_attention(b.q, far, b.table, b.lens, b.cu_q, b.scale), b.attention()):
+        assert torch.equal(x, y)
+    new, table = torch.randn(3, 8, 64, generator=torch.Generator().manual_seed(55)).to(BF).to(gpu), _tables(64, 10)
+    last = b.kv[0].shape[0] - 1
+    slots = torch.tensor([64 * last + 63, 64 * last, 5], device=gpu)
+    bounds, far_bounds = (f(b.cache.empty_bounds().zero_()) for f in (lambda x: x, lambda x: _apart(x, (1 << 31) + 64)))
+    pages, lens = torch.tensor([[last]], dtype=I32, device=gpu), torch.tensor([64], dtype=I32, device=gpu)
+    for cache, edges in ((b.cache, bounds), (far, far_bounds)):
+        K.kv_cache_append(*new.split((4, 2, 2), 1), None, None, *(x.to(gpu) for x in table), torch.arange(3, device=gpu), slots, cache)
+        K.kv_page_bounds(cache, edges, pages, lens, None, 1)
+    for x, y in zip((*b.cache, bounds), (*far, far_bounds)):
+        assert x is None or torch.equal(x.view(torch.uint8), y.contiguous().view(torch.uint8))
+    assert bounds[last].any() and not bounds[:last].any()
+    wide = torch.arange(last, -1, -1, dtype=I32, device=gpu).repeat(1, 80)[:, :300].contiguous()
+    finite = bounds.clone().copy_(torch.randn(bounds.shape, generator=torch.Generator().manual_seed(56)).sort(dim=2).values)
+    far_bounds.copy_(finite)
+    lens.fill_(64 * wide.shape[1])
+    for x, y in zip(*(K.kv_select_pages(b.q[:1], x, wide, lens, None, 64, 30) for x in (finite, far_bounds))):
+        assert torch.equal(x, y)
+    del far, far_bounds, cache, edges, x, y
+    torch.cuda.empty_cache()
+
+
+def _repeated(gpu, page, entries, heads, seed):
+    """One sequence whose table names the pages of another again and again: every row counts as often."""
+    b = Batch(gpu, [1], [page * 2], heads, page=page, fp8=True, seed=seed)
+    table, times = b.table[:, :2].repeat(1, entries // 2), entries // 2
+    lens = torch.tensor([2 * page * times], dtype=I32, device=gpu)
+    o, lse = K.kv_attention(b.q, b.cache, table, lens, None, b.scale)
+    want, want_lse, mass, spread = O.attention(b.q.cpu(), *b.rows(b.table[0], 2 * page), O.sees(1, 2 * page, None), b.scale)
+    e = (b.d + 8) * 2.0**-24 * spread
+    # sums of n rows on top. A row's keys are dealt to 256 workgroups of four waves at least, and a lane adds the weights of 8 of 32 of them: n / 4096 steps, each off by
+    # 2^-24 of a sum that never exceeds the whole; the products take 32 keys a step, with four roundings at most: n / 8192. Then 2048 such sums meet.
+    n = 2 * page * times
+    more = (n / 4096 + 2048) * 2.0**-24
+    _within(o, want, U * want.abs() + (U + 2 * (e[..., None] * math.log(2) + 2.0**-16 + more)) * mass, "o")
+    _within(lse, want_lse + math.log2(times), e.T + 2.0**-17 + 2 * more, "lse")
+
+
+def test_a_page_that_a_table_names_again_and_again(gpu):
+    _repeated(gpu, 16, 1 << 17, (8, 2, 64), 57)
+
+
+def test_the_longest_sequence(gpu):
+    """Almost 2^31 rows."""
+    _repeated(gpu, 1 << 16, 32766, (4, 1, 64), 58)
 
 
 def test_a_captured_call_follows_lengths_and_tables(gpu):
