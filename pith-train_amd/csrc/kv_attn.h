@@ -3,11 +3,13 @@
 //   S = kappa Q K^T,  O = softmax(S) V        for the query heads that share a key-value head
 //
 // Work list. The query rows of a sequence and key-value head (row = token * group + head of the group, n tokens: n * group rows) are cut into row blocks of
-// M = 16, 32 or 64 rows, each of which goes through all of the sequence's keys in steps of 128; the steps of all row blocks, one behind the other, are dealt
+// M = 16, 32 or 64 rows, each of which goes through the sequence's keys in steps of 128; the steps of all row blocks, one behind the other, are dealt
 // to the workgroups in equal ranges. Lengths are read on the device, so nothing depends on the host knowing them: a captured call follows its sequences as
 // they grow, and one long sequence among short ones is spread over as many workgroups as its share of the steps. Where there are fewer row blocks than
 // workgroups, ranges may be a little longer and each lie in one row block (to begin one costs queries, a first tile and a part). An XCD's workgroups take
 // ranges that follow one another, so that row blocks of one head find each other's keys in its cache.
+// Steps that no row of a block sees (of a prompt's first tokens, behind them) are dealt like the others but not taken; the row blocks' order puts the first and the
+// last beside each other, so that ranges of two or more are as much work all the same (4 prompts of 2048 tokens, heads of 32 / 4: 782 us without either, 476 with).
 // Two kinds of calls need no such list. Where page tables are so short that no row block is worth cutting, every workgroup takes one, whole, and there is
 // nothing to join. And tables of the heads (selected pages) are nearly full for whoever has a long context, so their row blocks are cut into the same
 // number of parts each, as many as there are workgroups for.
@@ -494,14 +496,16 @@ __global__ __launch_bounds__(kKVThreads, (KVRing<D, FP8, R>::kPerUnit)) void kv_
     } else {
       const int per_head = (s.n * p.group + M - 1) / M;
       head = __builtin_amdgcn_readfirstlane(walk.block / per_head);
-      row0 = (walk.block - head * per_head) * M;
+      const int i = walk.block - head * per_head;
+      row0 = (i & 1 ? per_head - 1 - (i >> 1) : i >> 1) * M;  // first, last, second, last but one: of a prompt these see as much two by two
       entries = p.table + walk.seq * p.table_rs;
     }
     const int rows = min(s.n * p.group - row0, M);
+    const int seen_by_any = p.tree ? s.len : min(max(s.len - s.n + __builtin_amdgcn_readfirstlane((row0 + rows - 1) / p.group) + 1, 0), s.len);  // keys that any row sees
     const ScalarTable table = (ScalarTable)(uintptr_t)entries;
     const int last = max(s.len - 1, 0);
     const int tile0 = walk.step * kKVWaves + wave;  // this wave's first
-    const int tiles = min((s.len + kTileKeys - 1) / kTileKeys, (walk.step + walk.n_steps()) * kKVWaves);
+    const int tiles = min((seen_by_any + kTileKeys - 1) / kTileKeys, (walk.step + walk.n_steps()) * kKVWaves);
     const int n_tiles = tiles > tile0 ? (tiles - tile0 + kKVWaves - 1) / kKVWaves : 0;
 
     bf16x8 q[R][kSteps];

@@ -104,22 +104,26 @@ KVPlan plan_of(const pith_kv_attn_args* a) {
   const int64_t steps = (a->table_width * a->cache.page_size + kStepKeys - 1) / kStepKeys, sequences = std::min(a->B, a->T);
   const auto items = [&](int64_t m) { return ((rows + m - 1) / m + sequences) * a->cache.heads; };
   // Rows of a row block. Fewer bytes and products with more of them, but every workgroup begins and ends with them more slowly, and rows that are not there are
-  // computed all the same: so 16 for sequences of no more, and while a compute unit has few steps with blocks of 16 and full page tables. us at 16 / 32 rows, heads
-  // of 32 / 4: 8 tokens, e4m3, 8 x 4096 rows (20 steps) 24 / 26, bf16, 16 x 2048 (20) 23 / 24, 8 x 8192 (40) 38 / 33, 16 x 8192 (80) 114 / 53; 16 tokens, e4m3, 16 x
-  // 2048 (36) 41 / 37; 2 tokens, 32 x 8192 75 / 76. And 64 for bf16 heads of 128 where that halves the row blocks and keys and values are more than the caches hold
-  // well: 8 tokens, 32 x 8192 (360 MB) 115 at 32 rows and 92 at 64, 16 tokens, 4 x 16384 45 / 39, but 512 tokens behind 8192 rows (17 MB) 107 / 117, 64 tokens, 4 x
-  // 8192 (67 MB) 65 / 69. (With e4m3 and with heads of 64 the 64 rows lost everywhere: 16 tokens, 16 x 8192 e4m3 77 / 80.)
+  // computed all the same: so 16 for sequences of no more, and while with blocks of 16 and full page tables a compute unit has few steps (32) and few row blocks
+  // (2.5; heads of 64, which have half the bytes and products, twice of both). us at 16 / 32 rows, heads of 32 / 4: 8 tokens, e4m3, 8 x 4096
+  // rows (20 steps) 24 / 26, bf16, 16 x 2048 (20) 23 / 24, 8 x 8192 (40) 38 / 33, 16 x 8192 (80) 114 / 53; 16 tokens, e4m3, 16 x 2048 (36) 41 / 37; 2 tokens, 32 x 8192
+  // 75 / 76; heads of 64 / 4, 8 tokens, 35 x 131 22 / 19 (few steps, but 3 row blocks); of 16 / 2 with 64 features, 14 tokens, 75 x 1530 (56 steps, 4.7 row blocks) 44 / 49.
+  // And 64 for bf16 heads of 128 where that halves the row blocks, which are long, and keys and values are more than the caches hold well: 8 tokens, 32 x 8192 (360 MB)
+  // 115 at 32 rows and 92 at 64, 16 tokens, 4 x 16384 45 / 39, 6 tokens, 64 x 2048 67 / 65, but 64 x 1024 42 / 53, 512 tokens behind 8192 rows (17 MB) 107 / 117, 64
+  // tokens, 4 x 8192 (67 MB) 65 / 69. (64 rows of e4m3 or of heads of 64 lose, or gain 7 % at most: 16 tokens, 16 x 8192 e4m3 77 / 80, 8, 32 x 8192, 64 features 62 / 58.)
   const double work = (double)items(16) * steps / units, bytes = (double)sequences * steps * kStepKeys * a->cache.heads * 512;
   const int64_t each = (rows + sequences - 1) / sequences;
+  const bool small = work * a->cache.dim <= 32 * 128 && 2 * items(16) * a->cache.dim <= 5 * units * 128;
   const bool halved = 19 * ((each + 63) / 64) <= 10 * ((each + 31) / 32);
-  if (rows <= 16 * a->B || work <= 28) pl.row_groups = 1;
-  else pl.row_groups = a->cache.dtype == PITH_BF16 && a->cache.dim == 128 && halved && bytes >= (96 << 20) ? 4 : 2;
+  if (rows <= 16 * a->B || small) pl.row_groups = 1;
+  else pl.row_groups = a->cache.dtype == PITH_BF16 && a->cache.dim == 128 && halved && steps >= 32 && bytes >= (96 << 20) ? 4 : 2;
   const int64_t m = 16 * pl.row_groups;
   const int per_unit = pl.row_groups <= 2 ? 2 : 1;  // workgroups (KVRing)
   pl.max_items = items(m);
-  // No row block is cut where that would gain less than the join's launch costs (4 us), as long as there are few enough of them to begin at once, one on a compute unit: one
-  // sequence of 517 rows, 4 heads, 8.8 us whole and 10.6 cut, 8 x 1024 rows, 8 tokens 12 / 17, 23 x 71 rows 10 / 13; but 64 x 900 rows (384 row blocks) 28 / 25, 86 x 2 14.6 / 13.1.
-  bool whole = steps * pl.row_groups <= 8 && pl.max_items <= units;
+  // No row block is cut where that would gain less than the join's launch costs (4 us), as long as all of them begin at once, and long ones do not share a compute unit: one
+  // sequence of 517 rows, 4 heads, 8.8 us whole and 10.6 cut, 8 x 1024 rows, 8 tokens 12 / 17, 23 x 71 rows (460 row blocks) 10 / 13; but 64 x 900 (384) 28 / 25, 86 x 2
+  // (688) 14.6 / 13.1.
+  bool whole = (steps * pl.row_groups <= 8 && pl.max_items <= units) || (steps * pl.row_groups <= 2 && pl.max_items <= per_unit * units);
   pl.workgroups = std::min(per_unit * units, kMaxGroups);
   if (a->head_tables) {
     pl.max_items = (group + m - 1) / m * a->cache.heads * a->B;
