@@ -61,16 +61,4 @@ inline int check_table(int64_t T, int64_t B, int64_t heads, int64_t table_width,
   return PITH_OK;
 }
 
-// The sequence of token t by the ends of all, looked up by a whole wavefront (64 ends at a time; wave-uniform). Where tokens and offsets contradict each
-// other, some sequence.
-__device__ __forceinline__ int sequence_of(const int32_t* cu_q, int B, int t, int lane) {
-  if (!cu_q) return t;
-  int seq = 0;
-  for (int b0 = 0; b0 < B; b0 += 64) {
-    const int end = b0 + lane < B ? cu_q[b0 + lane + 1] : 0x7fffffff;
-    seq += __popcll(__ballot(end <= t));
-  }
-  return min(seq, B - 1);
-}
-
 }  // namespace pith

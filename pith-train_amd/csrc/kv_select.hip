@@ -10,8 +10,9 @@
 // pages). With v the score of the last one chosen by these, a page above v + 2 E is in (whoever may exceed it is above v, too), one below v - 2 E is out, and
 // the few between are summed in fp64, if they are more than there are places. v is found by histograms of 256 equal parts of the range that it lies in, two most
 // often, to within 2 E. Infinities and NaN have no bound of the error: a page with one is summed in fp64 at once. NaN counts above all.
-// All of it is latency: 32 tokens with heads of 32 / 4 over up to 128 pages 12 us, one launch; 8 over up to 2048 pages 23 us, of which the scores are 9 (27 MB of bounds,
-// 3 TB/s) and the choice 10 (two histograms, one barrier a step, and the few pages in fp64).
+// All of it is latency: 32 tokens with heads of 32 / 4 over up to 128 pages 12 us, one launch; 8 over up to 2048 pages 23 us, three launches with the
+// bounds of the pages that the step filled: scores 8 (27 MB of bounds, 3.4 TB/s; four loads that wait for each other begin it), the choice 7 to 9 (1 until it knows what
+// it is about, 0.5 for the scores, 2.3 for the histograms, 1.3 for the few pages in fp64, 1.6 to rank and write).
 #include "cache_attn.h"
 #include "kv_common.h"
 
@@ -50,9 +51,21 @@ __device__ __forceinline__ Item item_of(const KVSelectParams& p, int item, int l
   Item x;
   x.t = item / p.heads;
   x.head = item - x.t * p.heads;
-  x.seq = sequence_of(p.cu_q, p.B, x.t, lane);
-  x.length = min(max(p.lengths[x.seq], 0), p.table_width << p.page_shift);
-  x.end = p.cu_q ? p.cu_q[x.seq + 1] : x.t + 1;
+  if (!p.cu_q) {
+    x.seq = x.t, x.end = x.t + 1, x.length = p.lengths[x.t];
+  } else {  // 64 sequences at a time: the first that ends behind the token, whose length has come along
+    x.seq = p.B - 1, x.end = 0, x.length = 0;  // (a token that is nobody's sees nothing)
+    for (int b0 = 0; b0 < p.B; b0 += 64) {
+      const int b = min(b0 + lane, p.B - 1), end = p.cu_q[b + 1], length = p.lengths[b];
+      const uint64_t behind = __ballot(end > x.t);
+      if (behind != 0) {
+        const int i = __builtin_ctzll(behind);
+        x.seq = min(b0 + i, p.B - 1), x.end = __builtin_amdgcn_readlane(end, i), x.length = __builtin_amdgcn_readlane(length, i);
+        break;
+      }
+    }
+  }
+  x.length = min(max(x.length, 0), p.table_width << p.page_shift);
   x.table = p.table + x.seq * p.table_rs;
   see(p, x);
   return x;
@@ -252,9 +265,9 @@ struct Team {
 __device__ __forceinline__ float in_range(float x) { return x != x ? 1e37f : fminf(fmaxf(x, -1e37f), 1e37f); }
 
 // Of the n pages of a token and head the `want` (fewer) with the largest scores: their numbers to out, in their order. score: in_range, of pages tid + THREADS e;
-// mass: the largest S of this thread's; memory: room for n. By a whole workgroup.
+// number: the table's entries of those; mass: the largest S of this thread's; memory: room for n. By a whole workgroup.
 template <int D, int THREADS, int E>
-__device__ __forceinline__ void choose(const KVSelectParams& p, const Item& x, Team<THREADS, E>& team, const float (&score)[E], float mass, int n, int want, uint2* memory, int32_t* out) {
+__device__ __forceinline__ void choose(const KVSelectParams& p, const Item& x, Team<THREADS, E>& team, const float (&score)[E], const int32_t (&number)[E], float mass, int n, int want, uint2* memory, int32_t* out) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   auto& shared = team.shared;
   const auto each = [&](const auto& f) __attribute__((always_inline)) {
@@ -358,7 +371,7 @@ __device__ __forceinline__ void choose(const KVSelectParams& p, const Item& x, T
       before += c;
     }
     const uint64_t mine = __ballot((is_in >> e) & 1);
-    if ((is_in >> e) & 1) out[here + __popcll(mine & ((1ull << lane) - 1))] = x.table[tid + THREADS * e];
+    if ((is_in >> e) & 1) out[here + __popcll(mine & ((1ull << lane) - 1))] = number[e];
   }
 }
 
@@ -399,8 +412,10 @@ __global__ __launch_bounds__(THREADS) void kv_pick_kernel(KVSelectParams p) {
   uint2* const memory = p.pages_of + item * p.row;
   const int n = x.pages - 1;
   float score[E], s[E], mass = 0.f;
+  int32_t number[E];
 #pragma unroll
   for (int e = 0; e < E; ++e) {
+    number[e] = x.table[min((int)threadIdx.x + THREADS * e, n - 1)];
     const float2 found = reinterpret_cast<const float2*>(memory)[min((int)threadIdx.x + THREADS * e, n - 1)];
     score[e] = found.x, s[e] = found.y;
   }
@@ -417,7 +432,7 @@ __global__ __launch_bounds__(THREADS) void kv_pick_kernel(KVSelectParams p) {
       score[e] = settle_unknown<D>(p, x, 64 * wave + THREADS * e, (int)threadIdx.x + THREADS * e < n, make_float2(score[e], s[e]), lane);
   }
   Team<THREADS, E> team(shared);
-  choose<D, THREADS, E>(p, x, team, score, mass, n, p.keep - 1, memory, out);
+  choose<D, THREADS, E>(p, x, team, score, number, mass, n, p.keep - 1, memory, out);
 }
 
 // Scores and choice in one launch, for tables of up to kFewPages pages.
@@ -431,6 +446,7 @@ __global__ __launch_bounds__(kThreads) void kv_pick_few_kernel(KVSelectParams p)
   int32_t* const out = p.table_out + (int64_t)item * p.keep;
   if (!begin_choice(p, x, item, out)) return;
   const int n = x.pages - 1;
+  const int32_t number[1] = {x.table[min((int)threadIdx.x, n - 1)]};
   float mass = 0.f;
 #pragma unroll 1
   for (int first = 32 * wave; first < n; first += kChunk) {
@@ -447,7 +463,7 @@ __global__ __launch_bounds__(kThreads) void kv_pick_few_kernel(KVSelectParams p)
   __syncthreads();
   const float score[1] = {scores[threadIdx.x]};
   Team<kThreads, 1> team(shared);
-  choose<D, kThreads, 1>(p, x, team, score, mass, n, p.keep - 1, p.pages_of + item * p.row, out);
+  choose<D, kThreads, 1>(p, x, team, score, number, mass, n, p.keep - 1, p.pages_of + item * p.row, out);
 }
 
 int check_select(const pith_kv_select_args* a, const char* who) {
