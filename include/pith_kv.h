@@ -152,11 +152,13 @@ int pith_kv_attn(const pith_kv_attn_args* args, pith_stream_t stream);
  *                    pith_kv_attn_args; append them first). Others keep what they hold.
  *   pith_kv_select   for token t, which sees n rows (as in the causal pith_kv_attn) in ceil(n / page_size) pages, and each key-value head: all of them if
  *                    they are at most `keep`; else the token's own, the last, and the keep - 1 of the others with the largest scores
- *                        max over the heads h of the group of sum_d max(q[t,h,d] * least_d, q[t,h,d] * largest_d)   (no q . k of the page exceeds it)
+ *                        max over the heads h of the group of sum_d max(q[t,h,d] * least_d, q[t,h,d] * largest_d)   (no q . k of the page exceeds
+ *                        it, but for the rounding of bounds of e4m3 keys)
  *                    summed in fp64, rounded to fp32 and compared so; equal scores in favour of the page that comes first, NaN above all. Their numbers go, in
  *                    the order of the sequence, to table_out [T, heads, keep] int32 (contiguous; -1 behind the last) and the rows they make to lengths_out
  *                    [T, heads]: a call of pith_kv_attn with head_tables and without cu_q. Tokens behind cu_q[B] and those that see nothing get no page.
- * q [T, H, dim] bf16 as in pith_kv_attn_args. keep >= 1. workspace of pith_kv_select: pith_kv_select_workspace_bytes, 256-byte aligned. */
+ * q [T, H, dim] bf16 as in pith_kv_attn_args. keep >= 1; pith_kv_select takes page tables of up to 16384 pages. Its workspace:
+ * pith_kv_select_workspace_bytes, 256-byte aligned. */
 typedef struct {
   pith_kv_cache cache;
   void* bounds;

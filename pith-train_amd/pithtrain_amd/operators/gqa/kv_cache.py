@@ -326,8 +326,9 @@ def kv_select_pages(
 ) -> SelectedPages:  # fmt: skip
     """The pages that every token and key-value head attends to: its own (the last one that it sees), and the keep - 1 others that score highest, in the order
     of the sequence; all of them where there are no more than keep. A page's score is the largest over the query heads of the group of
-    sum_d max(q_d least_d, q_d largest_d), which no q . k of the page exceeds; equal scores go to the page that comes first, NaN is above all. q [T, h, d]
-    are rotated queries, bounds kv_page_bounds', page_table, lengths, cu_q as in kv_attention (causal). Tokens from cu_q[b] on get no page and no row."""
+    sum_d max(q_d least_d, q_d largest_d), which no q . k of the page exceeds (but for the rounding of an e4m3 cache's bounds); equal scores go to the page that
+    comes first, NaN is above all. q [T, h, d] are rotated queries, bounds kv_page_bounds', page_table (up to 16384 pages wide), lengths, cu_q as in kv_attention
+    (causal). Tokens from cu_q[b] on get no page and no row."""
     return SelectedPages(*_select_op(q, bounds, page_table, lengths, cu_q, page_size, keep))
 
 
@@ -338,7 +339,8 @@ def kv_decode(
 ) -> torch.Tensor:  # fmt: skip
     """The layer between its projections for new tokens, o [T, h, d]: their rows go into the cache, then they attend to the cached rows of their sequences
     (lengths count the new rows). With bounds (KVCache.empty_bounds, which every step of the sequences must have been given) they are kept up to date, and
-    with keep too a token attends to that many pages only. Arguments as in the functions above. Rows of o from cu_q[b] on hold nothing."""
+    with keep too a token attends to that many pages only. Arguments as in the functions above, each looked at when its turn comes: where the attention's are
+    refused, the rows have been written. Rows of o from cu_q[b] on hold nothing."""
     assert keep is None or (bounds is not None and tree_mask is None), "keep needs bounds, and goes with causal attention"
     q = kv_cache_append(q, k, v, q_weight, k_weight, cos, sin, position_ids, slots, cache, eps)
     if bounds is not None:
