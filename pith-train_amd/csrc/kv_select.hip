@@ -3,8 +3,8 @@
 //
 //   score(page) = max over the heads of the group of sum_d max(q_d least_d, q_d largest_d)
 //
-// A choice must not depend on the order of a sum, or the same scores would choose differently elsewhere: products of two bf16 values are exact in fp32, and
-// their sum in fp64 loses nothing that a rounding to fp32 would show. But only the pages around the last one chosen need that. So scores are formed by matrix
+// A choice must not depend on the order of a sum, or the same scores would choose differently elsewhere: products of two bf16 values are exact in fp64, and
+// their sum in it loses nothing that a rounding to fp32 would show. But only the pages around the last one chosen need that. So scores are formed by matrix
 // instructions first, sum_d q+_d largest_d + q-_d least_d with q+ and q- the parts of q above and below zero, in fp32, beside the same sum of absolute values,
 // S: 2 D terms, each addition off by at most 2^-23 of S, so that a score is off by at most E = 2^-14 S (twice what the additions can lose; the largest S of all
 // pages). With v the score of the last one chosen by these, a page above v + 2 E is in (whoever may exceed it is above v, too), one below v - 2 E is out, and
@@ -183,7 +183,7 @@ __device__ __forceinline__ float exact_score(const KVSelectParams& p, const Item
     for (int e = 0; e < E / 8; ++e) {
       const bf16x8 q = *reinterpret_cast<const bf16x8*>(row + 8 * e);
 #pragma unroll
-      for (int k = 0; k < 8; ++k) sum += (double)__builtin_elementwise_maximum((float)q[k] * (float)least[e][k], (float)q[k] * (float)largest[e][k]);  // (NaN stays)
+      for (int k = 0; k < 8; ++k) sum += __builtin_elementwise_maximum((double)q[k] * (double)least[e][k], (double)q[k] * (double)largest[e][k]);  // (NaN stays; in 32 bits they could overflow)
     }
 #pragma unroll
     for (int d = 1; d < 8; d <<= 1) sum += __shfl_xor(sum, d);

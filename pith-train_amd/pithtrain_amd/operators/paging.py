@@ -89,7 +89,8 @@ def plan_step(counts: torch.Tensor, lengths: torch.Tensor, page_table: torch.Ten
     Requests that ended give their ceil(length / page_size) pages back, and have length 0. The others get rows length .. length + count - 1, and the
     pages that these need beyond those they have, from the top of the pool, where ended requests have just laid theirs; or none of them, where the pool does not suffice for
     a request or for one in front of it, or its table is too narrow: then granted is 0, the length stays and its tokens have slots of -1, which an append
-    skips. Tokens behind the last request have position 0 and slot -1. page_table and pool.free are updated in place; lengths and pool.count are not: the
+    skips (what an attention to their requests gives them is of no use; other requests do not notice). Tokens behind the last request have position 0 and slot -1.
+    A page belongs to one request: one that two tables name would go back to the pool twice. page_table and pool.free are updated in place; lengths and pool.count are not: the
     values behind the step are in the result, and the same call again plans the same step (plan_step_into can write them back)."""
     return StepPlan(*_plan_op(counts, lengths, page_table, pool.free, pool.count, page_size, tokens))
 

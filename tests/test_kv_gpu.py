@@ -613,6 +613,20 @@ def test_scores_that_are_no_numbers(gpu):
     _selection(gpu, [16 * 100 - 1], (3, 1, 64), 60, seed=10, bounds=bounds)
 
 
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf, 3.0e38])
+def test_queries_that_are_no_numbers(gpu, monkeypatch, bad):
+    """Their scores are infinities and NaN, those of the other head and token are not."""
+    made = Batch.__init__
+
+    def with_bad_ones(self, *args, **kw):
+        made(self, *args, **kw)
+        self.q[0, 1, 5] = bad
+        self.q[2, 2] = bad
+
+    monkeypatch.setattr(Batch, "__init__", with_bad_ones)
+    _selection(gpu, [16 * 100 + 3, 16 * 300, 16 * 290 + 1], (4, 2, 64), 30, seed=14)
+
+
 def test_sparse_attention_of_all_pages_is_the_dense_call(gpu):
     b = Batch(gpu, [1, 1, 2], [200, 90, 333], page=16, seed=15)
     bounds = b.cache.empty_bounds().zero_()
@@ -794,6 +808,27 @@ def test_requests_that_come_and_go_over_all_their_pages(gpu):
 
 def test_a_captured_step_follows_its_requests(gpu):
     assert _answer(gpu, False, None, captured=True) == 24
+
+
+def test_a_request_without_pages_disturbs_no_other(gpu):
+    """Its tokens leave no row; what the others get is what they get without it."""
+    g = torch.Generator().manual_seed(33)
+    cos, sin = (x.to(gpu) for x in _tables(64, 60))
+    qkv = torch.randn(9, 8, 64, generator=g).to(BF).to(gpu)
+    results = []
+    for counts, spare in (([4, 4, 1], 3), ([4, 4, 1], 2)):
+        cache = K.KVCache.empty(8, 2, 64, 16, device=gpu)
+        cache.k.zero_(), cache.v.zero_()
+        table = torch.tensor([[6, 7, -1], [-1, -1, -1], [5, -1, -1]], dtype=I32, device=gpu)
+        pool = paging.PagePool(torch.tensor([0, 1, 2, -1, -1, -1], dtype=I32, device=gpu), torch.tensor([spare - 2], dtype=I32, device=gpu))
+        lengths = torch.tensor([20, 0, 3], dtype=I32, device=gpu)
+        plan = paging.plan_step(torch.tensor(counts, dtype=I32, device=gpu), lengths, table, pool, 16, 9)
+        o = K.kv_decode(*qkv.split((4, 2, 2), 1), None, None, cos, sin, plan.position_ids, plan.slots, cache, table, plan.lengths, plan.cu_q, 0.125)
+        results.append((plan, o, cache))
+    (all_, want, _), (denied, got, cache) = results
+    assert all_.granted.tolist() == [4, 4, 1] and denied.granted.tolist() == [4, 0, 1] and denied.lengths.tolist() == [24, 0, 4]
+    assert (denied.slots[4:8] == -1).all() and not cache.k[:5].any()
+    assert torch.equal(got[:4], want[:4]) and torch.equal(got[8:], want[8:])
 
 
 def test_the_latent_cache_takes_the_same_plan(gpu):
@@ -1038,3 +1073,66 @@ def test_empty_calls(gpu):
     assert K.kv_cache_append(b.q[:0], b.q[:0, :2], b.q[:0, :2], None, None, none(4, 64), none(4, 64), none(0, d=I64), none(0, d=I64), b.cache).shape == (0, 4, 64)
     selected = K.kv_select_pages(b.q, b.cache.empty_bounds(), b.table[:0], b.lens[:0], torch.zeros(1, dtype=I32, device=gpu), 64, 3)
     assert (selected.page_table == -1).all() and (selected.lengths == 0).all()
+
+
+# ---------------------------------------------------------------------------------------------
+# Refusals
+
+
+def test_wrong_arguments_are_refused(gpu):
+    b = Batch(gpu, [1, 2], [40, 50], (4, 2, 64), page=16, seed=40)
+    before = [x.clone() for x in b.kv]
+    z = lambda *s, d=BF: torch.zeros(*s, dtype=d, device=gpu)  # noqa: E731
+    k, v = b.kv
+    call = lambda **kw: K.kv_attention(*{**dict(q=b.q, c=b.cache, t=b.table, l=b.lens, cu=b.cu_q, s=0.1, m=None), **kw}.values())  # noqa: E731
+    for match, kw in [
+        ("q must be", dict(q=b.q.float())), ("q must be", dict(q=b.q[..., :32])), ("cu_q must be", dict(cu=b.cu_q[:2])), ("cu_q must be", dict(cu=b.cu_q.long())),
+        ("lengths must be", dict(l=b.lens.long())), ("page_table must be", dict(t=b.table[:1])), ("page_table must be", dict(t=b.table.long())), ("tree_mask must be", dict(m=z(2, d=I64))),
+        ("one token a sequence", dict(cu=None)), ("does not match cache.k", dict(c=K.KVCache(k, v[1:]))), ("does not match cache.k", dict(c=K.KVCache(k, v.to(L.FP8)))),
+        ("has no scales", dict(c=K.KVCache(k, v, z(*k.shape[:3], d=torch.float32)))), ("needs a float32", dict(c=K.KVCache(k.to(L.FP8), v.to(L.FP8)))),
+        ("is not contiguous", dict(c=K.KVCache(k.transpose(1, 2).contiguous().transpose(1, 2), v))), ("64 or 128", dict(c=K.KVCache(z(2, 2, 16, 96), z(2, 2, 16, 96)))),
+        ("lengths must be", dict(q=b.q[:2], t=z(2, 2, 3, d=I32), l=z(2, 3, d=I32), cu=None)), ("page_table must be", dict(q=b.q[:2], t=z(2, 1, 3, d=I32), l=z(2, 2, d=I32), cu=None)),
+        ("no cu_q", dict(t=z(2, 2, 3, d=I32), l=z(2, 2, d=I32))), ("one page table for all", dict(q=b.q[:2], t=z(2, 2, 3, d=I32), l=z(2, 2, d=I32), cu=None, m=z(2, d=I64))),
+    ]:  # fmt: skip
+        with pytest.raises(AssertionError, match=match):
+            call(**kw)
+    for match, kw in [("page size", dict(c=K.KVCache(k[:, :, :8].contiguous(), v[:, :, :8].contiguous()))), ("empty page table", dict(t=b.table[:, :0])), ("query heads", dict(q=z(3, 3, 64)))]:
+        with pytest.raises(_C.PithError, match=match):
+            call(**kw)
+    with pytest.raises(RuntimeError, match="different devices|need tensors on a GPU"):
+        call(l=b.lens.cpu())
+    with pytest.raises(AssertionError, match="wrong dtype or shape"):
+        K.kv_attention_into(b.q, b.cache, b.table, b.lens, b.cu_q, 0.1, None, torch.empty_like(b.q), z(4, 2, d=torch.float32))
+
+    new = dict(q=z(3, 4, 64), k=z(3, 2, 64), v=z(3, 2, 64), qw=z(64), kw=z(64), cos=z(8, 64), sin=z(8, 64), p=z(3, d=I64), s=z(3, d=I64), c=b.cache)
+    for match, kw in [("k must be", dict(k=z(3, 4, 64))), ("v has 2 tokens", dict(v=z(2, 2, 64))), ("given together", dict(qw=None)), ("tensors of one dtype", dict(qw=z(32))),
+                      ("tensors of one dtype", dict(qw=z(64, d=torch.float32))), ("cos and sin must be", dict(cos=z(8, 32), sin=z(8, 32))), ("slots must be", dict(s=z(3, d=I32))), ("position_ids must be", dict(p=z(2, d=I64)))]:  # fmt: skip
+        with pytest.raises(AssertionError, match=match):
+            K.kv_cache_append(*{**new, **kw}.values())
+    with pytest.raises(TypeError):
+        K.kv_cache_append(*{**new, "qw": z(64, d=torch.float16), "kw": z(64, d=torch.float16)}.values())
+
+    bounds = b.cache.empty_bounds()
+    for match, kw in [("bounds must be", dict(b=bounds[1:])), ("bounds must be", dict(b=bounds.float())), ("page_table must be", dict(t=b.table[:1])), ("tokens = -1", dict(n=-1)), ("one token a sequence", dict(cu=None, n=3))]:
+        with pytest.raises(AssertionError, match=match):
+            K.kv_page_bounds(*{**dict(c=b.cache, b=bounds, t=b.table, l=b.lens, cu=b.cu_q, n=3), **kw}.values())
+    select = lambda **kw: K.kv_select_pages(*{**dict(q=b.q, b=bounds, t=b.table, l=b.lens, cu=b.cu_q, p=16, k=2), **kw}.values())  # noqa: E731
+    for match, kw in [("bounds must be", dict(b=bounds[..., :32])), ("q must be", dict(q=b.q.float())), ("keep = 0", dict(k=0)), ("page_table must be", dict(l=b.lens[:1]))]:  # (b is what lengths say)
+        with pytest.raises(AssertionError, match=match):
+            select(**kw)
+    for match, kw in [("page size", dict(p=24)), ("query heads", dict(q=z(3, 3, 64))), ("at most 16384", dict(t=z(2, 16385, d=I32)))]:
+        with pytest.raises(_C.PithError, match=match):
+            select(**kw)
+    for kw in (dict(keep=2), dict(keep=2, bounds=bounds, tree_mask=z(3, d=I64))):
+        with pytest.raises(AssertionError, match="keep needs bounds"):
+            K.kv_decode(*new.values(), b.table, b.lens, b.cu_q, 0.1, **kw)
+
+    plan = dict(c=z(2, d=I32), l=z(2, d=I32), t=z(2, 3, d=I32), pool=paging.PagePool.full(4, gpu), p=16, n=3)
+    for match, kw in [("counts must be", dict(c=z(2, d=I64))), ("lengths must be", dict(l=z(3, d=I32))), ("page_table must be", dict(t=z(3, 3, d=I32))), ("tokens = -1", dict(n=-1)),
+                      ("pool.count must be", dict(pool=paging.PagePool(z(4, d=I32), z(2, d=I32)))), ("pool.free must be", dict(pool=paging.PagePool(z(8, d=I32)[::2], z(1, d=I32))))]:  # fmt: skip
+        with pytest.raises(AssertionError, match=match):
+            paging.plan_step(*{**plan, **kw}.values())
+    with pytest.raises(_C.PithError, match="page size"):
+        paging.plan_step(*{**plan, "p": 24}.values())
+    torch.cuda.synchronize()
+    assert all(torch.equal(x.view(torch.int16), y.view(torch.int16)) for x, y in zip(before, b.kv))
