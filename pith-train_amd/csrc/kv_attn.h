@@ -19,14 +19,14 @@
 //
 // The kernel. Memory bounds it: a key row and a value row of 512 bytes (bf16, 128 features) stand against 4 * 128 flop for each of the group's rows. So the four
 // wavefronts of a workgroup walk alone, each through every fourth tile of 32 keys, with no barrier until the segment ends: a wave brings its tiles global -> LDS by
-// direct loads into a ring of its own (128 KB of keys and values in flight on a compute unit, see KVRing) and waits with counted waits for its own requests only, for
-// the keys while the values are still under way. Products are 16x16x32 with the query row as the result's column, so a lane owns one row, and the scores of a lane are
+// direct loads into a ring of its own (see KVRing) and waits with counted waits for its own requests only, for the keys while the values are
+// still under way. Products are 16x16x32 with the query row as the result's column, so a lane owns one row, and the scores of a lane are
 // its part of operand B of the second product as they stand: key 4 g + v of either half tile is contracted at place 8 g + v or 8 g + 4 + v, and the values are read
 // (transposed, from LDS) in that order. No weight moves between lanes. The waves' results of a segment are joined through LDS.
 // A fragment that was read serves all 16-row groups of the block: 64 rows cost a tile's reads once. With M = 64 the products are 1024 of a tile's cycles, and
 // the tile still comes more slowly than that from memory.
 // Measured, heads of 32 / 4 with 128 features: 32 sequences of up to 8192 rows, bf16, one token each (303 MB) 64 us, 4.7 TB/s; 8 of up to 131072 rows, e4m3 (879 MB)
-// 164 us, 5.4 TB/s, where a copy reaches 4.9; 64 selected pages of 8 such sequences (34 MB) 15 us, of which the join's launch is 4 and beginnings and ends
+// 160 us, 5.5 TB/s, where a copy reaches 4.9; 64 selected pages of 8 such sequences (34 MB) 15 us, of which the join's launch is 4 and beginnings and ends
 // about 4; one sequence of 517 rows 8.8 us, a launch and 5 steps of waiting for memory.
 // The weights go into the second product as bf16, which is what the matrix cores take beside a cache of bf16 (or e4m3, widened exactly): half a step, 2^-8, of
 // each, while their sum is of the unrounded ones. With e4m3 a weight is rounded once, when its row's scale is in it.
@@ -275,13 +275,15 @@ struct KVTile {
 };
 
 // Tiles of a wave in flight, and workgroups of a compute unit. Two workgroups fill each other's gaps (their beginnings and ends, a wave's way from its keys to its
-// weights), with rings of 64 KB each; a ring of one tile is enough then, as its keys are asked for while the values before them are worked on and the other way
-// round. 64 rows fill the registers, and with them one workgroup has the compute unit. (us with one workgroup and rings of 128 KB / with two: 8 sequences of 64
-// selected pages, e4m3, 17.2 / 15.3; trees of 8 over 5001 rows, heads of 64, 16.8 / 15.5; 4 tokens, 32 x 1024 rows 23.2 / 18.6; long streams alike.)
+// weights), and a ring of one tile is enough then, as its keys are asked for while the values before them are worked on and the other way round; e4m3 with 32 rows
+// has two, for the queries to come through. 64 rows fill the registers, and with them one workgroup has the compute unit, with rings of 128 KB. (us with one workgroup
+// and rings of 128 KB / with two and 64 KB each / with two and one tile a wave: 8 sequences of 64 selected pages, e4m3, 17.2 / 15.3 / 15.2; trees of 8 over 5001 rows, heads
+// of 64, 16.8 / 15.9 / 15.6; 4 tokens, 32 x 1024 rows 23.2 / 18.6; 8 x 131072 rows, e4m3, 165 / 164 / 160, heads of 64 - / 95 / 88; 1 x 9094 - / 14.2 / 15.1. Three or four
+// workgroups, where their registers allow: 16.8 for the trees, 165 for the long rows.)
 template <int D, bool FP8, int R>
 struct KVRing {
   static constexpr int kPerUnit = R <= 2 ? 2 : 1;
-  static constexpr int kSlots = R > 2 ? 2 : FP8 && D == 64 ? 4 : FP8 || D == 64 ? 2 : 1;
+  static constexpr int kSlots = R > 2 || (FP8 && R == 2) ? 2 : 1;
   static constexpr int kBytes = kSlots * KVTile<D, FP8>::kSlot;
 };
 
@@ -340,10 +342,8 @@ __device__ __forceinline__ void stage_rows(const KVAttnParams& p, const KVWork& 
 // Until all but the last `later` tiles' requests and EXTRA more are there.
 template <int D, bool FP8, int SLOTS, int EXTRA>
 __device__ __forceinline__ void wait_tiles(int later) {
-  constexpr int kAll = KVTile<D, FP8>::kAll;
-  if (SLOTS == 4 && later >= 3) wait_loads<SLOTS == 4 ? 3 * kAll + EXTRA : 0>();
-  else if (SLOTS == 4 && later == 2) wait_loads<SLOTS == 4 ? 2 * kAll + EXTRA : 0>();
-  else if (SLOTS >= 2 && later >= 1) wait_loads<kAll + EXTRA>();
+  static_assert(SLOTS <= 2, "at most one tile behind");
+  if (SLOTS == 2 && later >= 1) wait_loads<KVTile<D, FP8>::kAll + EXTRA>();
   else wait_loads<EXTRA>();
 }
 
