@@ -82,8 +82,8 @@ typedef const __attribute__((address_space(4))) int32_t* ScalarTable;
 __device__ __forceinline__ float scaled(float weight, float scale) { return weight == 0.f ? 0.f : weight * scale; }
 
 // x *= f in place: as a plain product under a branch the accumulators are copied on the other way, which doubles their registers. The compiler does not
-// look into the statement for hazards: f may come from v_exp_f32 right before it (one wait state), and x from products of the tile before (two barriers
-// away).
+// look into the statement for hazards: f may come from v_exp_f32 right before it (one wait state), and x from products of the tile before, which have ended: they stand
+// two barriers away, or in front of the products whose scores f comes from.
 __device__ __forceinline__ void scale_in_place(f32x4& x, float f) {
   float a = x[0], b = x[1], c = x[2], d = x[3];
   asm("s_nop 1\n\tv_mul_f32 %0, %4, %0\n\tv_mul_f32 %1, %4, %1\n\tv_mul_f32 %2, %4, %2\n\tv_mul_f32 %3, %4, %3" : "+v"(a), "+v"(b), "+v"(c), "+v"(d) : "v"(f));

@@ -652,8 +652,13 @@ __global__ __launch_bounds__(kKVThreads, (KVRing<D, FP8, R>::kPerUnit)) void kv_
           l[r] += y[e];
         }
         if constexpr (FP8) {
+          if (partial) {  // (the scale of a row that is not seen may hold anything)
 #pragma unroll
-          for (int e = 0; e < 8; ++e) y[e] = scaled(y[e], v_scale[e]);
+            for (int e = 0; e < 8; ++e) y[e] = (seen[r] >> e) & 1 ? y[e] * v_scale[e] : 0.f;
+          } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) y[e] *= v_scale[e];
+          }
         }
         weight[r] = to_bf16x8(y[0], y[1], y[2], y[3], y[4], y[5], y[6], y[7]);
         if constexpr (R > 2) __builtin_amdgcn_sched_barrier(0);
