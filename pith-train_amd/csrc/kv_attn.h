@@ -63,11 +63,12 @@ struct KVAttnParams {
   int whole;        // steps of the longest row block where none is cut, else 0
   int parts;        // of every row block, where all are cut alike (into two or more), else 0
   // workspace (not used where none is cut)
-  int* items;        // number of row blocks of this call
-  KVJoin* joins;     // [row blocks]
+  int* items;        // number of entries of joins in this call
+  KVJoin* joins;     // one for every row block, or, where those may be more, for every workgroup that its range's first segment (no other can end a row block that is cut)
   float2* stats;     // [slots][M] reference (in bits) and sum
   float* results;    // [slots][M][D] of parts; slot 2 i: of workgroup i's that begins with its range, 2 i + 1: one that begins later (cut alike: slot i)
   int max_items;     // capacity of joins
+  int by_range;      // joins are the workgroups'
 };
 
 // A sequence, or a sequence's key-value head where these have tables of their own.
@@ -124,13 +125,16 @@ struct KVWalk {
     }
     KVWork x = {};
     int w = 0, k = 0, sw = 0, sk = 0, total = 0, blocks_total = 0;
-    int behind = 0;  // the sequences that were loaded: their last offset
-    const auto load = [&](int b0) __attribute__((always_inline)) {  // 64 sequences
-      if (b0 == 0) behind = kv_offset(p, 0);
+    int behind = kv_offset(p, 0);  // the sequences that were digested: their last offset
+    const auto fetch = [&](int b0, int& length, int& end) __attribute__((always_inline)) {  // of 64 sequences
+      const int b = min(b0 + lane, p.B - 1);
+      length = p.lengths[b];
+      end = kv_offset(p, b + 1);
+    };
+    const auto digest = [&](int b0, int length, int end) __attribute__((always_inline)) {
       const bool some = b0 + lane < p.B;
-      const int length = some ? p.lengths[b0 + lane] : 0;
-      const int c1 = max(wave_scan_max(some ? kv_offset(p, b0 + lane + 1) : 0), behind);  // (lanes without one: no tokens)
-      x = kv_work<M>(p, __builtin_amdgcn_update_dpp(behind, c1, 0x138, 0xf, 0xf, false), c1, length);  // from the lane below
+      const int c1 = max(wave_scan_max(some ? end : 0), behind);  // (lanes without one: no tokens)
+      x = kv_work<M>(p, __builtin_amdgcn_update_dpp(behind, c1, 0x138, 0xf, 0xf, false), c1, some ? length : 0);  // from the lane below
       behind = __builtin_amdgcn_readlane(c1, 63);
     };
     const auto sums = [&]() __attribute__((always_inline)) {
@@ -141,19 +145,25 @@ struct KVWalk {
     };
     single = p.whole != 0;
     per = p.whole;
-    if (p.whole) {
-      load(0);
-      sums();
-    } else {
+    // Lane i: steps, row blocks and last offset of the first i + 1 times 64 sequences (of the first 4096).
+    int steps_to = 0, blocks_to = 0, offset_to = 0;
 #pragma unroll 1
-      for (int b0 = 0; b0 < p.B; b0 += 64) {
-        load(b0);
-        sums();
-        total += __builtin_amdgcn_readlane(sw, 63);
-        blocks_total += __builtin_amdgcn_readlane(sk, 63);
-      }
-      // (named as global memory: with a store to anywhere behind it, all waits for LDS in the kernel would be waits for everything)
-      if (blockIdx.x == 0 && threadIdx.x == 0) *(__attribute__((address_space(1))) int*)(uintptr_t)p.items = min(blocks_total, p.max_items);
+    for (int b0 = 0; b0 < p.B; b0 += 256) {
+      int length[4], end[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) fetch(b0 + 64 * j, length[j], end[j]);  // (four loads at a time: those behind the last sequence are its own)
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (b0 + 64 * j < p.B) {
+          digest(b0 + 64 * j, length[j], end[j]);
+          sums();
+          total += __builtin_amdgcn_readlane(sw, 63);
+          blocks_total += __builtin_amdgcn_readlane(sk, 63);
+          const bool mine = lane == (b0 >> 6) + j;
+          steps_to = mine ? total : steps_to, blocks_to = mine ? blocks_total : blocks_to, offset_to = mine ? behind : offset_to;
+        }
+    }
+    if (!p.whole) {
       per = total <= groups ? 1 : uniform((total + groups - 1) / groups);  // (divisions leave the scalar registers)
       if (blocks_total < groups && p.B <= 64 && total < 1 << 30) {  // (more sequences are not looked up twice)
         const int most = per + kStart;
@@ -165,19 +175,36 @@ struct KVWalk {
             per = longer;
             single = true;
             if (per > 1) sums();
+            total = ranges * per;  // with what row blocks are taken for
             break;
           }
         }
       }
+      // (named as global memory: with a store to anywhere behind it, all waits for LDS in the kernel would be waits for everything)
+      if (blockIdx.x == 0 && threadIdx.x == 0)
+        *(__attribute__((address_space(1))) int*)(uintptr_t)p.items = min(p.by_range ? uniform((total + per - 1) / per) : blocks_total, p.max_items);
     }
     begin = at = range * per;
     end = at + per;  // (the host has bounded total + gridDim.x)
-    int before = 0;  // steps in front of the sequence
+    int before = 0, b0 = 0;  // steps in front of the sequence; the first of the 64 that it may be among
     item = 0;
+    if (p.B > 64) {
+      const int chunks = min(__popcll(__ballot(steps_to <= at && 64 * lane < p.B)), 63);  // (steps only grow; lanes without sequences are behind)
+      if (chunks > 0) {
+        before = __builtin_amdgcn_readlane(steps_to, chunks - 1);
+        item = __builtin_amdgcn_readlane(blocks_to, chunks - 1);
+        behind = __builtin_amdgcn_readlane(offset_to, chunks - 1);
+        b0 = 64 * chunks;
+      } else {
+        behind = kv_offset(p, 0);
+      }
+    }
 #pragma unroll 1
-    for (int b0 = 0; b0 < p.B; b0 += 64) {
+    for (; b0 < p.B; b0 += 64) {
       if (p.B > 64) {
-        load(b0);
+        int length, end;
+        fetch(b0, length, end);
+        digest(b0, length, end);
         sums();
       }
       const uint64_t beyond = __ballot(before + sw > at);
@@ -205,23 +232,25 @@ struct KVWalk {
   __device__ __forceinline__ int n_steps() const { return min(s.steps - step, end - at); }  // (a part without keys: 0 or less)
   __device__ __forceinline__ bool whole(const KVAttnParams& p) const { return !p.parts && n_steps() == s.steps; }
   __device__ __forceinline__ int slot(const KVAttnParams& p) const { return p.parts ? range : 2 * range + (at == begin ? 0 : 1); }
-  // Who ends a row block says how it was cut.
+  // Who ends a row block says how it was cut; by ranges, everybody says once whether it has ended one.
   __device__ __forceinline__ void leave_join(const KVAttnParams& p, int row0, int head, int rows) const {
-    if (p.whole || threadIdx.x != 0 || item + block >= p.max_items) return;
+    const int index = p.by_range ? range : item + block;
+    if (p.whole || threadIdx.x != 0 || index >= p.max_items || (p.by_range && at != begin)) return;
     KVJoin join = {row0, s.tok0, head, rows, 0, 0, 0, 1};
     if (p.parts) {
       if (step != 0) return;
       join.first = range, join.second = range + 1, join.stride = 1, join.parts = p.parts;
-    } else {
-      if (step + n_steps() != s.steps) return;
+    } else if (step + n_steps() == s.steps) {
       if (!whole(p)) {
         const int from = at - step;  // of the row block in the work list
         const int id = from / per;
         join.first = 2 * id + (from == id * per ? 0 : 1);
         join.second = 2 * id + 2, join.stride = 2, join.parts = range - id + 1;
       }
+    } else if (!p.by_range) {
+      return;
     }
-    p.joins[item + block] = join;
+    p.joins[index] = join;
   }
   // On to the next segment. False: the range is done.
   __device__ __forceinline__ bool next(const KVAttnParams& p) {
@@ -283,7 +312,7 @@ struct KVTile {
 template <int D, bool FP8, int R>
 struct KVRing {
   static constexpr int kPerUnit = R <= 2 ? 2 : 1;
-  static constexpr int kSlots = R > 2 || (FP8 && R == 2) ? 2 : 1;
+  static constexpr int kSlots = R > 2 ? 2 : 1;
   static constexpr int kBytes = kSlots * KVTile<D, FP8>::kSlot;
 };
 
@@ -326,18 +355,22 @@ struct KVLoads {
   __device__ __forceinline__ void values(const KVAttnParams& p, char* slot, int source) const { rows(p.cache.v, p.cache.v_ps, slot + T::kBytes, source); }
 };
 
-// Query rows row0 .. of a sequence and head into LDS, laid out like keys of bf16: 1 KB a request, every lane from an address of its own. (Loads of the compiler's
-// would make it wait for everything that is under way at their first use, in every turn of the loop.) Rows behind the block's last one are that one.
+// Query rows row0 .. of a sequence and head into LDS, laid out like keys of bf16: 1 KB a request, every lane from an address of its own, the waves in turn. (Loads of the
+// compiler's would make it wait for everything that is under way at their first use, in every turn of the loop.) Rows behind the block's last one are that one.
 template <int D, int R>
-__device__ __forceinline__ void stage_rows(const KVAttnParams& p, const KVWork& s, int head, int row0, int rows, char* area, int lane) {
-  using T = KVTile<D, false>;
+struct KVQueries {
+  static constexpr int kBytes = 16 * R * 2 * D, kAll = kBytes / 1024, kEach = kAll > kKVWaves ? kAll / kKVWaves : 1;  // requests; of a wave (fewer than waves: some twice)
+  static __device__ __forceinline__ void stage(const KVAttnParams& p, const KVWork& s, int head, int row0, int rows, char* area, int wave, int lane) {
+    using T = KVTile<D, false>;
 #pragma unroll
-  for (int n = 0; n < R * D / 32; ++n) {
-    const int row = (1024 * n + 16 * lane) / T::kRow, piece = (lane % (T::kRow / 16)) ^ (kv_swizzle<T::kRow>(row));
-    const int at = row0 + min(row, rows - 1), tok = at / p.group;
-    load_lds16_at(p.q + (int64_t)(s.tok0 + tok) * p.q_ts + (int64_t)(head * p.group + at - tok * p.group) * p.q_hs + 8 * piece, area + 1024 * n);
+    for (int j = 0; j < kEach; ++j) {
+      const int n = (wave * kEach + j) % kAll;
+      const int row = (1024 * n + 16 * lane) / T::kRow, piece = (lane % (T::kRow / 16)) ^ (kv_swizzle<T::kRow>(row));
+      const int at = row0 + min(row, rows - 1), tok = at / p.group;
+      load_lds16_at(p.q + (int64_t)(s.tok0 + tok) * p.q_ts + (int64_t)(head * p.group + at - tok * p.group) * p.q_hs + 8 * piece, area + 1024 * n);
+    }
   }
-}
+};
 
 // Until all but the last `later` tiles' requests and EXTRA more are there.
 template <int D, bool FP8, int SLOTS, int EXTRA>
@@ -473,6 +506,7 @@ __global__ __launch_bounds__(kKVThreads, (KVRing<D, FP8, R>::kPerUnit)) void kv_
   constexpr int M = 16 * R, kSteps = D / 32;  // of the score's contraction
   constexpr int kRegion = kRing > M * D * 4 ? kRing : M * D * 4;  // of a wave: its tiles, then its results
   __shared__ __attribute__((aligned(1024))) char lds[kKVWaves * kRegion];
+  __shared__ __attribute__((aligned(1024))) char queries[KVQueries<D, R>::kBytes];
   __shared__ float2 wave_stats[kKVWaves][M];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int c = lane & 15, g = lane >> 4;
@@ -535,42 +569,27 @@ __global__ __launch_bounds__(kKVThreads, (KVRing<D, FP8, R>::kPerUnit)) void kv_
       loads.keys(p, ring + i * T::kSlot, source, lane);
       loads.values(p, ring + i * T::kSlot, source);
     };
-    // The queries come through the end of the ring, in front of its first tiles in the queue and read before its last ones are asked for.
-    const auto read_queries = [&](const char* staged) __attribute__((always_inline)) {
-#pragma unroll
-      for (int r = 0; r < R; ++r)
-#pragma unroll
-        for (int i = 0; i < kSteps; ++i) {  // e4m3 keys are read 16 features at a time: steps 2 i, 2 i + 1 contract features 64 i + 16 g + {0..7, 8..15}
-          const int piece = FP8 ? 8 * (i >> 1) + 2 * g + (i & 1) : 4 * i + g;
-          q[r][i] = *reinterpret_cast<const bf16x8*>(staged + KVTile<D, false>::place(16 * r + c, piece));
-        }
-      __builtin_amdgcn_s_waitcnt(0xC07F);  // the queries have been read
-      asm volatile("" ::: "memory");
-    };
-    if (n_tiles > 0) {
-      if constexpr (kSlots == 1) {  // the only tile's values wait for them
-        static_assert(M * 2 * D <= T::kBytes, "the queries lie where the values will");
-        stage_rows<D, R>(p, s, head, row0, rows, ring + T::kBytes, lane);
-        look_up(0);
-        const Loads loads(p, pages, key_of_tile(0), last, head);
-        loads.keys(p, ring, source, lane);
-        wait_loads<T::kScaleLoads + T::kLoads>();
-        read_queries(ring + T::kBytes);
-        loads.values(p, ring, source);
-      } else {
-        constexpr int kQuerySlots = (M * 2 * D + T::kSlot - 1) / T::kSlot, kFirst = kSlots - kQuerySlots;
-        static_assert(kFirst >= 1, "a tile beside the queries");
-        char* const staged = ring + kFirst * T::kSlot;
-        stage_rows<D, R>(p, s, head, row0, rows, staged, lane);
+    // The queries stand in front of the first tiles in the queue.
+    KVQueries<D, R>::stage(p, s, head, row0, rows, queries, wave, lane);
+    const int ahead = min(kSlots, n_tiles);
 #pragma unroll 1
-        for (int i = 0; i < min(kFirst, n_tiles); ++i) request(i);
-        wait_tiles<D, FP8, kSlots, 0>(min(kFirst, n_tiles));
-        read_queries(staged);
-#pragma unroll 1
-        for (int i = kFirst; i < min(kSlots, n_tiles); ++i) request(i);
+    for (int i = 0; i < ahead; ++i) request(i);
+    if (kSlots == 2 && ahead == 2) wait_loads<2 * T::kAll>();
+    else if (ahead == 1) wait_loads<T::kAll>();
+    else wait_loads<0>();
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();  // (the tiles stay under way)
+    asm volatile("" ::: "memory");
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+      for (int i = 0; i < kSteps; ++i) {  // e4m3 keys are read 16 features at a time: steps 2 i, 2 i + 1 contract features 64 i + 16 g + {0..7, 8..15}
+        const int piece = FP8 ? 8 * (i >> 1) + 2 * g + (i & 1) : 4 * i + g;
+        q[r][i] = *reinterpret_cast<const bf16x8*>(queries + KVTile<D, false>::place(16 * r + c, piece));
       }
-      look_up(kSlots);
-    }
+    __builtin_amdgcn_s_waitcnt(0xC07F);  // the queries have been read
+    asm volatile("" ::: "memory");
+    if (n_tiles > 0) look_up(kSlots);
     int slot_at = 0;
 #pragma unroll 1
     for (int i = 0; i < n_tiles; ++i) {

@@ -13,7 +13,7 @@ namespace {
 constexpr int kJoinThreads = 512, kJoinRows = 4;
 constexpr int kMaxGroups = 512;  // workgroups of the attention kernel, at most, where row blocks are cut: kMaxGroups + 1 parts of one
 
-// Joins the parts of a row block: o = sum_i w_i O_i / sum_i w_i l_i, w_i = 2^(m_i - max m). blockIdx.x: row block, blockIdx.y: four rows of it. A wave forms
+// Joins the parts of a row block: o = sum_i w_i O_i / sum_i w_i l_i, w_i = 2^(m_i - max m). blockIdx.x: entry of the joins, blockIdx.y: four rows of it. A wave forms
 // the weights of a row; then groups of threads, a piece of four features each, take every so many-th part and meet in LDS.
 template <int D>
 __global__ __launch_bounds__(kJoinThreads) void kv_join_kernel(KVAttnParams p, int m) {
@@ -93,7 +93,8 @@ struct KVPlan {
   int workgroups;  // a multiple of 8
   int whole;       // steps of the longest row block where none is cut, else 0
   int parts;       // of every row block, where all are cut alike (into two or more), else 0
-  int64_t max_items;
+  bool by_range;   // joins are the workgroups'
+  int64_t max_items;  // row blocks, or joins
   int64_t joins_at, stats_at, results_at, bytes;  // workspace
 };
 
@@ -138,6 +139,9 @@ KVPlan plan_of(const pith_kv_attn_args* a) {
     pl.bytes = 256;
     return pl;
   }
+  // A join for each workgroup where the row blocks are more: 1024 sequences of up to 200 rows, 4096 row blocks, of which 512 at most are cut: FIG us / FIG.
+  pl.by_range = !pl.parts && pl.max_items > pl.workgroups;
+  if (pl.by_range) pl.max_items = pl.workgroups;
   const auto up = [](int64_t x) { return (x + 255) & ~(int64_t)255; };
   const int64_t slot_rows = (pl.parts ? 1 : 2) * (int64_t)pl.workgroups * m;
   pl.joins_at = 256;
@@ -208,6 +212,7 @@ extern "C" int pith_kv_attn(const pith_kv_attn_args* a, pith_stream_t stream) {
   p.stats = (float2*)(ws + pl.stats_at);
   p.results = (float*)(ws + pl.results_at);
   p.max_items = (int)pl.max_items;
+  p.by_range = pl.by_range;
   hipStream_t s = (hipStream_t)stream;
   const bool fp8 = a->cache.dtype == PITH_FP8_E4M3;
   begin_launch();
