@@ -9,7 +9,7 @@
 // workgroups, ranges may be a little longer and each lie in one row block (to begin one costs queries, a first tile and a part). An XCD's workgroups take
 // ranges that follow one another, so that row blocks of one head find each other's keys in its cache.
 // Steps that no row of a block sees (of a prompt's first tokens, behind them) are dealt like the others but not taken; the row blocks' order puts the first and the
-// last beside each other, so that ranges of two or more are as much work all the same (4 prompts of 2048 tokens, heads of 32 / 4: 782 us without either, 476 with).
+// last beside each other, so that ranges of two or more are as much work all the same (4 prompts of 2048 tokens, heads of 32 / 4: 782 us without either, 476 with, when both came).
 // Two kinds of calls need no such list. Where page tables are so short that no row block is worth cutting, every workgroup takes one, whole, and there is
 // nothing to join. And tables of the heads (selected pages) are nearly full for whoever has a long context, so their row blocks are cut into the same
 // number of parts each, as many as there are workgroups for.
@@ -147,21 +147,32 @@ struct KVWalk {
     per = p.whole;
     // Lane i: steps, row blocks and last offset of the first i + 1 times 64 sequences (of the first 4096).
     int steps_to = 0, blocks_to = 0, offset_to = 0;
+    const auto add = [&]() __attribute__((always_inline)) {
+      sums();
+      total += __builtin_amdgcn_readlane(sw, 63);
+      blocks_total += __builtin_amdgcn_readlane(sk, 63);
+    };
+    if (p.B <= 64) {
+      int length, end;
+      fetch(0, length, end);
+      digest(0, length, end);
+      add();
+    } else {
 #pragma unroll 1
-    for (int b0 = 0; b0 < p.B; b0 += 256) {
-      int length[4], end[4];
+      for (int b0 = 0; b0 < p.B; b0 += 256) {
+        int length[4], end[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) fetch(b0 + 64 * j, length[j], end[j]);  // (four loads at a time: those behind the last sequence are its own)
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (b0 + 64 * j < p.B) {
-          digest(b0 + 64 * j, length[j], end[j]);
-          sums();
-          total += __builtin_amdgcn_readlane(sw, 63);
-          blocks_total += __builtin_amdgcn_readlane(sk, 63);
+        for (int j = 0; j < 4; ++j) fetch(b0 + 64 * j, length[j], end[j]);  // (four loads at a time: those behind the last sequence are its own)
+#pragma unroll 1
+        for (int j = 0; j < 4 && b0 + 64 * j < p.B; ++j) {
+          digest(b0 + 64 * j, length[0], end[0]);
+          add();
           const bool mine = lane == (b0 >> 6) + j;
           steps_to = mine ? total : steps_to, blocks_to = mine ? blocks_total : blocks_to, offset_to = mine ? behind : offset_to;
+          length[0] = length[1], length[1] = length[2], length[2] = length[3];
+          end[0] = end[1], end[1] = end[2], end[2] = end[3];
         }
+      }
     }
     if (!p.whole) {
       per = total <= groups ? 1 : uniform((total + groups - 1) / groups);  // (divisions leave the scalar registers)
@@ -304,8 +315,8 @@ struct KVTile {
 };
 
 // Tiles of a wave in flight, and workgroups of a compute unit. Two workgroups fill each other's gaps (their beginnings and ends, a wave's way from its keys to its
-// weights), and a ring of one tile is enough then, as its keys are asked for while the values before them are worked on and the other way round; e4m3 with 32 rows
-// has two, for the queries to come through. 64 rows fill the registers, and with them one workgroup has the compute unit, with rings of 128 KB. (us with one workgroup
+// weights), and a ring of one tile is enough then, as its keys are asked for while the values before them are worked on and the other way round. 64 rows fill the
+// registers, and with them one workgroup has the compute unit, with rings of 128 KB. (us with one workgroup
 // and rings of 128 KB / with two and 64 KB each / with two and one tile a wave: 8 sequences of 64 selected pages, e4m3, 17.2 / 15.3 / 15.2; trees of 8 over 5001 rows, heads
 // of 64, 16.8 / 15.9 / 15.6; 4 tokens, 32 x 1024 rows 23.2 / 18.6; 8 x 131072 rows, e4m3, 165 / 164 / 160, heads of 64 - / 95 / 88; 1 x 9094 - / 14.2 / 15.1. Three or four
 // workgroups, where their registers allow: 16.8 for the trees, 165 for the long rows.)

@@ -179,6 +179,17 @@ def test_attention_of_more_sequences_than_a_wavefront_scans_at_once(gpu):
     b.check(*b.attention())
 
 
+@BOTH
+@pytest.mark.parametrize("wide", [False, True])
+@pytest.mark.parametrize("b, every, most", [(150, 1, 1), (300, 2, 3), (4300, 9, 1), (4300, 50, 2), (4200, 4150, 1)], ids=str)
+def test_attention_of_many_sequences_of_which_few_have_tokens(gpu, monkeypatch, b, every, most, wide, fp8):
+    if wide:
+        monkeypatch.setitem(globals(), "MIN_WIDTH", 256)
+    counts = [1 + i % most if i % every == every - 1 else 0 for i in range(b)]
+    x = Batch(gpu, counts, [(7 * i) % 130 for i in range(b)], (4, 2, 64), page=16, fp8=fp8, seed=21, extra_tokens=2)
+    x.check(*x.attention())
+
+
 def test_attention_of_more_row_blocks_than_workgroups(gpu):
     b = Batch(gpu, [1] * 300, [7 + i % 200 for i in range(300)], (8, 4, 64), page=16, seed=6)
     b.check(*b.attention())
