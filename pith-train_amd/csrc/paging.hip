@@ -173,8 +173,9 @@ __global__ __launch_bounds__(kThreads) void plan_kernel(PlanParams p) {
   }
 }
 
-// Up to kInOne requests, a thread each, and up to kTokensInOne tokens in the same launch: 32 bits hold all sums but those of the pages that come back.
-constexpr int64_t kTokensInOne = 8192;
+// Up to kInOne requests, a thread each, and up to kTokensInOne tokens in the same launch, or up to kTokensIn32 in the next: 32 bits hold all sums but those of the pages that
+// come back.
+constexpr int64_t kTokensInOne = 8192, kTokensIn32 = 1 << 20;
 __global__ __launch_bounds__(kThreads) void plan_some_kernel(PlanParams p) {
   __shared__ int64_t back_sums[kWaves];
   __shared__ int64_t base[kInOne];
@@ -222,6 +223,11 @@ __global__ __launch_bounds__(kThreads) void plan_some_kernel(PlanParams p) {
   if (wave == 0) {
     const int all = wave_scan_max(lane < kWaves ? most_taken[lane] : 0);
     if (lane == 63) p.free_count_out[0] = (int32_t)(top - all);
+  }
+  if (p.requests) {  // (the tokens are for the next launch)
+    if (some) p.requests[tid] = request_of[tid];
+    if (tid == 0) *p.top = top;
+    return;
   }
   for (int t = tid; t < tokens; t += kThreads)
     place_token(p, t, top, [&](int i) { return (int64_t)cu_of[i]; }, [&](int i) { return request_of[i]; });
@@ -369,6 +375,7 @@ extern "C" int pith_plan_step(const pith_plan_step_args* a, pith_stream_t stream
     p.top = (int64_t*)a->workspace;
     p.requests = (Request*)((char*)a->workspace + 16);
     if (a->B <= 64 && a->T <= 1 << 24) plan_few_kernel<<<1, 256, 0, s>>>(p);
+    else if (a->B <= kInOne && a->T <= kTokensIn32) plan_some_kernel<<<1, kThreads, 0, s>>>(p);
     else plan_kernel<<<1, kThreads, 0, s>>>(p);
     if (a->T > 0) place_kernel<<<(unsigned)((a->T + 255) / 256), 256, 0, s>>>(p);
   }

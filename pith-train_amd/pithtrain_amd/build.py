@@ -44,7 +44,7 @@ HIPCC_FLAGS = [
 # without a mask 43.8 / 47.8).
 # Attention to the key-value cache: with 512 registers a lane at hand the compiler would keep the results of matrix instructions in the accumulators' half of
 # the file, and move them out and back around every rescaling that may come; with 64 query rows it then spills inside the loop, whose reloads wait for every tile
-# under way. In the common half nothing spills (32 sequences of 8 tokens over up to 8192 rows, 64 query rows: 118 us without the flag, 92 with it; the rest 0 to 4 % faster).
+# under way. In the common half nothing spills there (32 sequences of 8 tokens over up to 8192 rows, 64 query rows: 118 us without the flag, 92 with it; the rest 0 to 4 % faster).
 KV_ATTN_FLAGS = ["-mllvm", "-amdgpu-mfma-vgpr-form"]
 SOURCE_FLAGS = {"attn_bwd_chunks.hip": ["-falign-loops=64"], "kv_attn.hip": KV_ATTN_FLAGS, "kv_attn_d64.hip": KV_ATTN_FLAGS}
 

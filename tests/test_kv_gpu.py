@@ -696,6 +696,8 @@ def test_plans_of_long_prompts(gpu):
     """Tokens in a launch of their own; a table that is too narrow; fewer tokens than the counts say; nothing at all."""
     _plan_case(gpu, [9000, 0, 3000, 7], [5, 70, 16, 64], 16, 12007, 800, 700, seed=1)
     _plan_case(gpu, [9000, 0, 3000, 7], [5, 70, 16, 64], 16, 12007, 560, 700, seed=1, into=True)
+    for into in (False, True):
+        _plan_case(gpu, [90 + i % 40 - 200 * (i % 7 == 6) for i in range(150)], [i % 90 for i in range(150)], 16, 14000, 900, 20, seed=4, into=into)
     want = _plan_case(gpu, [40, 17, 3], [5, 0, 16], 16, 60, 50, 2, seed=2)
     assert want["granted"] == [0, 17, 3]
     _plan_case(gpu, [20, 30, 4], [1, 2, 3], 16, 33, 50, 8, seed=3)
