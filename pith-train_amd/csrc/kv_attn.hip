@@ -109,15 +109,16 @@ KVPlan plan_of(const pith_kv_attn_args* a) {
   // (2.5; heads of 64, which have half the bytes and products, twice of both). us at 16 / 32 rows, heads of 32 / 4: 8 tokens, e4m3, 8 x 4096
   // rows (20 steps) 24 / 26, bf16, 16 x 2048 (20) 23 / 24, 8 x 8192 (40) 38 / 33, 16 x 8192 (80) 114 / 53; 16 tokens, e4m3, 16 x 2048 (36) 41 / 37; 2 tokens, 32 x 8192
   // 75 / 76; heads of 64 / 4, 8 tokens, 35 x 131 22 / 19 (few steps, but 3 row blocks); of 16 / 2 with 64 features, 14 tokens, 75 x 1530 (56 steps, 4.7 row blocks) 44 / 49.
-  // And 64 for bf16 heads of 128 where that halves the row blocks, which are long, and keys and values are more than the caches hold well: 8 tokens, 32 x 8192 (360 MB)
-  // 115 at 32 rows and 92 at 64, 16 tokens, 4 x 16384 45 / 39, 6 tokens, 64 x 2048 67 / 65, but 64 x 1024 42 / 53, 512 tokens behind 8192 rows (17 MB) 107 / 117, 64
-  // tokens, 4 x 8192 (67 MB) 65 / 69. (64 rows of e4m3 or of heads of 64 lose, or gain 7 % at most: 16 tokens, 16 x 8192 e4m3 77 / 80, 8, 32 x 8192, 64 features 62 / 58.)
+  // And 64 for bf16 heads of 128 where that makes the row blocks fewer by a quarter and keys and values are about as much as the last-level cache holds, or more: 8 tokens,
+  // 32 x 8192 (540 MB) 115 at 32 rows and 92 at 64, 18, 55 x 1771 (200 MB) 91 / 76, 6, 64 x 2048 (270 MB) 65 / 65, but 8 tokens, 8 x 8192 (130 MB) 30 / 33, 64 x 1024 (130 MB)
+  // 43 / 53, 512 behind 8192 rows (17 MB) 109 / 119. (64 rows of e4m3 or of heads of 64 lose, or gain 7 % at most: 16 tokens, 16 x 8192 e4m3 77 / 80, 8, 32 x 8192, 64
+  // features 62 / 58.)
   const double work = (double)items(16) * steps / units, bytes = (double)sequences * steps * kStepKeys * a->cache.heads * 512;
   const int64_t each = (rows + sequences - 1) / sequences;
   const bool small = work * a->cache.dim <= 32 * 128 && 2 * items(16) * a->cache.dim <= 5 * units * 128;
-  const bool halved = 19 * ((each + 63) / 64) <= 10 * ((each + 31) / 32);
+  const bool fewer = 4 * ((each + 63) / 64) <= 3 * ((each + 31) / 32);
   if (rows <= 16 * a->B || small) pl.row_groups = 1;
-  else pl.row_groups = a->cache.dtype == PITH_BF16 && a->cache.dim == 128 && halved && steps >= 32 && bytes >= (96 << 20) ? 4 : 2;
+  else pl.row_groups = a->cache.dtype == PITH_BF16 && a->cache.dim == 128 && fewer && bytes >= (192 << 20) ? 4 : 2;
   const int64_t m = 16 * pl.row_groups;
   const int per_unit = pl.row_groups <= 2 ? 2 : 1;  // workgroups (KVRing)
   pl.max_items = items(m);

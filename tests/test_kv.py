@@ -244,8 +244,8 @@ def test_rows_of_a_row_block_go_by_the_rows_of_a_sequence_and_the_work_list():
     wide = dict(table_width=65536, table_rs=65536)
     assert rows(T=16, lse_hs=16, **wide) == 16  # sixteen rows a sequence and key-value head
     assert rows(T=17, lse_hs=17, **wide) == 32 and rows(T=32, lse_hs=32, **wide) == 32
-    assert rows(T=33, lse_hs=33, **wide) == 64  # where that halves the row blocks
-    assert rows(T=33, lse_hs=33, cache=_cache(**FP8), **wide) == 32 and rows(T=72, lse_hs=72, **wide) == 32
+    assert rows(T=33, lse_hs=33, **wide) == rows(T=72, lse_hs=72, **wide) == 64  # where that makes the row blocks fewer by a quarter
+    assert rows(T=33, lse_hs=33, cache=_cache(**FP8), **wide) == 32 and rows(T=33, lse_hs=33, cache=_cache(dim=64, k_ps=64 * 128, v_ps=64 * 128), **wide) == 32
     assert rows(T=256, lse_hs=256, **wide) == 64 and rows(T=256, lse_hs=256, table_width=512, table_rs=512) == 32  # and there is so much to read
     assert rows(T=64, lse_hs=64, table_width=16, table_rs=16) == 16  # and a work list of some length
 
