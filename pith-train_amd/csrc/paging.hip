@@ -4,7 +4,7 @@
 // held; pages that are taken come off its top at sums of what is needed. A request is served if what is needed up to it and it included does not exceed the
 // pool, or it needs nothing: sums only grow, so the served ones that need pages are a beginning of the list, and the order decides, not the schedule.
 // One workgroup does that; up to 8192 tokens are its work too, more go to a second launch. All of it is latency: a step of 32 requests moves 1 KB. Up to 64
-// requests are a lane each and need no barrier for their sums; up to 1024 are a thread each, with three barriers and sums of 32 bits. us of a call, launch
+// requests are a lane each and need no barrier for their sums; up to 1024 are a thread each, with four barriers (three more where pages come back) and sums of 32 bits. us of a call, launch
 // included: 32 requests of a token each 7.1, 423 8.7 (12.2 in the loop for any number, whose sums have 64 bits), 1000 11.8 (16.2); 16 prompts, 16384 tokens, 10.
 #include "cache_attn.h"
 #include "pith_kv.h"
@@ -238,8 +238,8 @@ __global__ __launch_bounds__(256) void place_kernel(PlanParams p) {
   if (t < p.T) place_token(p, t, *p.top, [&](int i) { return (int64_t)p.cu_q[i]; }, [&](int i) { return p.requests[i]; });
 }
 
-// The same for up to 64 requests, a lane each: every wave forms all sums by itself, and looks a token's request up among its lanes. (LDS and barriers only
-// where pages come back.)
+// The same for up to 64 requests, a lane each: every wave forms all sums by itself, and looks a token's request up among its lanes. No LDS; a barrier behind
+// what all waves read and the first writes, and another where pages come back.
 __global__ __launch_bounds__(kThreads) void plan_few_kernel(PlanParams p) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
   const int page = 1 << p.page_shift;
@@ -303,7 +303,9 @@ __global__ __launch_bounds__(kThreads) void plan_few_kernel(PlanParams p) {
     for (int d = 32; d > 0; d >>= 1)
       if (__shfl(last, r + d - 1) <= t) r += d;
     r = min(r, 63);
-    const int position = __shfl(length, r) + t - __shfl(first, r), index = position >> p.page_shift, in_page = position & (page - 1);
+    const int before = __shfl(length, r), into = t - __shfl(first, r);
+    const int position = (int)((unsigned)before + (unsigned)into);  // (of a request that is served: below 2^31)
+    const int index = position >> p.page_shift, in_page = position & (page - 1);
     const int beyond = index - __shfl(held, r);
     const int64_t at = top - 1 - __shfl(taken, r) - beyond;
     int64_t slot = -1;
@@ -314,7 +316,7 @@ __global__ __launch_bounds__(kThreads) void plan_few_kernel(PlanParams p) {
       slot = ((int64_t)number << p.page_shift) + in_page;
     }
     if (t < tokens) {
-      p.positions[t] = t < end ? position : 0;
+      p.positions[t] = t < end ? (int64_t)before + into : 0;
       p.slots[t] = slot;
     }
   }
