@@ -149,14 +149,15 @@ int pith_kv_attn(const pith_kv_attn_args* args, pith_stream_t stream);
  * Which pages a token attends to. bounds [pages, heads, 2, dim] bf16 (page stride bounds_ps, a multiple of 8) beside a cache hold the least and the largest
  * value of each key feature over the rows of a page (of e4m3: value * scale; rounded to bf16; NaN where a key has one).
  *   pith_kv_bounds   writes those of every page whose last row is one of the newest tokens of its sequence (T, B, cu_q, lengths, page_table as in
- *                    pith_kv_attn_args; append them first). Others keep what they hold.
+ *                    pith_kv_attn_args, offsets counted likewise; append them first). Others keep what they hold.
  *   pith_kv_select   for token t, which sees n rows (as in the causal pith_kv_attn) in ceil(n / page_size) pages, and each key-value head: all of them if
  *                    they are at most `keep`; else the token's own, the last, and the keep - 1 of the others with the largest scores
  *                        max over the heads h of the group of sum_d max(q[t,h,d] * least_d, q[t,h,d] * largest_d)   (no q . k of the page exceeds
  *                        it, but for the rounding of bounds of e4m3 keys)
  *                    summed in fp64, rounded to fp32 and compared so; equal scores in favour of the page that comes first, NaN above all. Their numbers go, in
  *                    the order of the sequence, to table_out [T, heads, keep] int32 (contiguous; -1 behind the last) and the rows they make to lengths_out
- *                    [T, heads]: a call of pith_kv_attn with head_tables and without cu_q. Tokens behind cu_q[B] and those that see nothing get no page.
+ *                    [T, heads]: a call of pith_kv_attn with head_tables and without cu_q. Tokens that are no sequence's (in front of
+ *                    cu_q[0], behind cu_q[B]) and those that see nothing get no page.
  * q [T, H, dim] bf16 as in pith_kv_attn_args. keep >= 1; pith_kv_select takes page tables of up to 16384 pages. Its workspace:
  * pith_kv_select_workspace_bytes, 256-byte aligned. */
 typedef struct {

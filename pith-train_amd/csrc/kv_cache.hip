@@ -172,7 +172,11 @@ __global__ __launch_bounds__(kThreads) void kv_bounds_kernel(KVBoundsParams p) {
   const int b = blockIdx.x, head = blockIdx.y;
   const int page_size = 1 << p.cache.page_shift;
   const int length = min(max(p.lengths[b], 0), p.table_width << p.cache.page_shift);
-  const int n = p.cu_q ? min(max(p.cu_q[b + 1] - p.cu_q[b], 0), p.T) : 1;
+  int n = 1;
+  if (p.cu_q) {
+    const int end = min(max(p.cu_q[b + 1], 0), p.T), begin = offset_so_far(p.cu_q, b, p.T, threadIdx.x & 63);
+    n = max(end - begin, 0);
+  }
   for (int i = (max(length - n, 0) >> p.cache.page_shift) + blockIdx.z; i < length >> p.cache.page_shift; i += gridDim.z) {
     const int64_t page = safe_page(p.table[b * p.table_rs + i], p.cache.pages);
     float lo[8], hi[8];

@@ -1,6 +1,7 @@
 // What the kernels of the key-value cache (include/pith_kv.h) share.
 #pragma once
 
+#include "cache_attn.h"
 #include "latent_common.h"
 #include "pith_kv.h"
 
@@ -24,6 +25,20 @@ inline KVCache to_device(const pith_kv_cache& c) {
   d.pages = (int)c.pages; d.heads = (int)c.heads;
   d.page_shift = __builtin_ctzll((unsigned long long)c.page_size);
   return d;
+}
+
+// Token offsets count as their maximum so far, from 0 to T, so that whatever they hold no token belongs to two sequences. The offset of sequence b, by a whole
+// wavefront: the largest of the first b + 1, 256 of them under way at a time.
+__device__ __forceinline__ int offset_so_far(const int32_t* cu_q, int b, int T, int lane) {
+  int most = 0;
+  for (int i0 = 0; i0 <= b; i0 += 256) {
+    int x[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) x[k] = cu_q[min(i0 + 64 * k + lane, b)];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) most = max(most, x[k]);
+  }
+  return min(__builtin_amdgcn_readlane(wave_scan_max(most), 63), T);
 }
 
 // Sizes of pages, heads and features, of a cache or of the bounds beside one.

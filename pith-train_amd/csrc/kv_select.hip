@@ -54,16 +54,18 @@ __device__ __forceinline__ Item item_of(const KVSelectParams& p, int item, int l
   if (!p.cu_q) {
     x.seq = x.t, x.end = x.t + 1, x.length = p.lengths[x.t];
   } else {  // 64 sequences at a time: the first that ends behind the token, whose length has come along
-    x.seq = p.B - 1, x.end = 0, x.length = 0;  // (a token that is nobody's sees nothing)
+    x.seq = p.B - 1, x.end = 0, x.length = 0;  // (a token that is nobody's sees nothing: in front of the first offset, or behind all)
+    const int first = p.cu_q[0];
     for (int b0 = 0; b0 < p.B; b0 += 64) {
       const int b = min(b0 + lane, p.B - 1), end = p.cu_q[b + 1], length = p.lengths[b];
       const uint64_t behind = __ballot(end > x.t);
       if (behind != 0) {
         const int i = __builtin_ctzll(behind);
-        x.seq = min(b0 + i, p.B - 1), x.end = __builtin_amdgcn_readlane(end, i), x.length = __builtin_amdgcn_readlane(length, i);
+        x.seq = min(b0 + i, p.B - 1), x.end = min(__builtin_amdgcn_readlane(end, i), p.T), x.length = __builtin_amdgcn_readlane(length, i);
         break;
       }
     }
+    if (x.t < first) x.end = 0, x.length = 0;
   }
   x.length = min(max(x.length, 0), p.table_width << p.page_shift);
   x.table = p.table + x.seq * p.table_rs;

@@ -328,7 +328,7 @@ def kv_select_pages(
     of the sequence; all of them where there are no more than keep. A page's score is the largest over the query heads of the group of
     sum_d max(q_d least_d, q_d largest_d), which no q . k of the page exceeds (but for the rounding of an e4m3 cache's bounds); equal scores go to the page that
     comes first, NaN is above all. q [T, h, d] are rotated queries, bounds kv_page_bounds', page_table (up to 16384 pages wide), lengths, cu_q as in kv_attention
-    (causal). Tokens from cu_q[b] on get no page and no row."""
+    (causal). Tokens in front of cu_q[0] and from cu_q[b] on get no page and no row."""
     return SelectedPages(*_select_op(q, bounds, page_table, lengths, cu_q, page_size, keep))
 
 
