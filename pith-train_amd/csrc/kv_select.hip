@@ -6,10 +6,13 @@
 // A choice must not depend on the order of a sum, or the same scores would choose differently elsewhere: products of two bf16 values are exact in fp64, and
 // their sum in it loses nothing that a rounding to fp32 would show. But only the pages around the last one chosen need that. So scores are formed by matrix
 // instructions first, sum_d q+_d largest_d + q-_d least_d with q+ and q- the parts of q above and below zero, in fp32, beside the same sum of absolute values,
-// S: 2 D terms, each addition off by at most 2^-23 of S, so that a score is off by at most E = 2^-14 S (twice what the additions can lose; the largest S of all
-// pages). With v the score of the last one chosen by these, a page above v + 2 E is in (whoever may exceed it is above v, too), one below v - 2 E is out, and
-// the few between are summed in fp64, if they are more than there are places. v is found by histograms of 256 equal parts of the range that it lies in, two most
-// often, to within 2 E. Infinities and NaN have no bound of the error: a page with one is summed in fp64 at once. NaN counts above all.
+// S: 2 D terms, each addition off by at most 2^-23 of S, so that a page's score is off by at most E = 2^-14 S (twice what the additions can lose). The score v
+// of the last one chosen by these is found by histograms of 256 equal parts of the range that it lies in, two most often, to within 2 E of an average page. The
+// score of the last one that has to be chosen then lies above the least that a page from v on may have and below the most that one up to v may: a page that is above
+// the latter with its E taken off is in, one below the former with its E added is out, and the few between are summed in fp64, if they are more than there are places.
+// A page of another size is in question by itself alone. Infinities and NaN have no bound of the error: a page with one is summed in fp64 at once. NaN counts above all.
+// Of equal scores all are in question. Up to 128 are ranked by comparing each with all; more by the bytes of their keys, a wave summing its own pages one after the
+// other: 8 tokens over 2000 pages of one score 370 us, over 16000 2450 (18 and 70 where scores differ); one such token holds the call up.
 // All of it is latency: 32 tokens with heads of 32 / 4 over up to 128 pages 12 us, one launch; 8 over up to 2048 pages 23 us, three launches with the
 // bounds of the pages that the step filled: scores 8 (27 MB of bounds, 3.4 TB/s; four loads that wait for each other begin it), the choice 7 to 9 (1 until it knows what
 // it is about, 0.5 for the scores, 2.3 for the histograms, 1.3 for the few pages in fp64, 1.6 to rank and write).
@@ -230,16 +233,17 @@ struct Team {
   static constexpr int kGroups = THREADS / 64, kListed = 128;
   struct Shared {
     int2 sums[2][kGroups];
+    float4 survey[kGroups];
     __attribute__((aligned(16))) int histogram[2][256];
-    int chosen[E * kGroups];
+    __attribute__((aligned(16))) int chosen[E * kGroups];
     int listed;
     uint2 list[kListed];
   };
   Shared& shared;
   int turn;
   __device__ __forceinline__ explicit Team(Shared& s) : shared(s), turn(0) {}
+  static __device__ __forceinline__ float wave_max(float x) { return quad_max(group_reduce<16>(x, [](float y, float z) { return fmaxf(y, z); })); }
   __device__ __forceinline__ float2 most(float a, float b) {
-    const auto wave_max = [](float x) __attribute__((always_inline)) { return quad_max(group_reduce<16>(x, [](float y, float z) { return fmaxf(y, z); })); };
     a = wave_max(a), b = wave_max(b);
     if ((threadIdx.x & 63) == 63) shared.sums[turn][threadIdx.x >> 6] = make_int2(__float_as_int(a), __float_as_int(b));
     __syncthreads();
@@ -250,6 +254,20 @@ struct Team {
     }
     turn ^= 1;
     return make_float2(a, b);
+  }
+  // Once: the largest a, b and c, and the sum of d (added in one order: of all threads the same).
+  __device__ __forceinline__ float4 survey(float a, float b, float c, float d) {
+    a = wave_max(a), b = wave_max(b), c = wave_max(c);
+    d = quad_sum(group_reduce<16>(d, [](float y, float z) { return y + z; }));
+    if ((threadIdx.x & 63) == 63) shared.survey[threadIdx.x >> 6] = make_float4(a, b, c, d);
+    __syncthreads();
+    d = 0.f;
+#pragma unroll
+    for (int w = 0; w < kGroups; ++w) {
+      const float4 s = shared.survey[w];
+      a = fmaxf(a, s.x), b = fmaxf(b, s.y), c = fmaxf(c, s.z), d += s.w;
+    }
+    return make_float4(a, b, c, d);
   }
   __device__ __forceinline__ int2 sums(int x, int y) {
     x = wave_scan(x), y = wave_scan(y);
@@ -266,10 +284,32 @@ struct Team {
 // A score as the search for v sees it: infinities and what comes near them become large numbers, in the same order.
 __device__ __forceinline__ float in_range(float x) { return x != x ? 1e37f : fminf(fmaxf(x, -1e37f), 1e37f); }
 
+// How far a score of the matrix instructions may be off (S: the sum of the absolute values, infinity where the score is that of exact_score) and terms that are
+// below the normal range.
+__device__ __forceinline__ float error_of(float mass) { return (mass < INFINITY ? mass * 0x1p-14f : 0.f) + 0x1p-60f; }
+
+// The part of a histogram, from the highest, in which the left-th lies; `left` becomes its rank in there. Every wave looks it up, four parts a lane.
+__device__ __forceinline__ int part_with(const int* histogram, int lane, int& left) {
+  const int4 h = *reinterpret_cast<const int4*>(&histogram[252 - 4 * lane]);
+  const int mine = h.x + h.y + h.z + h.w, upto = wave_scan(mine);
+  const int j = __builtin_ctzll(__ballot(upto >= left));
+  left -= __builtin_amdgcn_readlane(upto - mine, j);
+  const int hw = __builtin_amdgcn_readlane(h.w, j), hz = __builtin_amdgcn_readlane(h.z, j), hy = __builtin_amdgcn_readlane(h.y, j);
+  int part = 255 - 4 * j;
+  if (left > hw) {
+    left -= hw, --part;
+    if (left > hz) {
+      left -= hz, --part;
+      if (left > hy) left -= hy, --part;
+    }
+  }
+  return part;
+}
+
 // Of the n pages of a token and head the `want` (fewer) with the largest scores: their numbers to out, in their order. score: in_range, of pages tid + THREADS e;
-// number: the table's entries of those; mass: the largest S of this thread's; memory: room for n. By a whole workgroup.
-template <int D, int THREADS, int E>
-__device__ __forceinline__ void choose(const KVSelectParams& p, const Item& x, Team<THREADS, E>& team, const float (&score)[E], const int32_t (&number)[E], float mass, int n, int want, uint2* memory, int32_t* out) {
+// error(e): how far each may be off; number(e): the table's entries of those; memory: room for n. By a whole workgroup.
+template <int D, int THREADS, int E, typename F, typename N>
+__device__ __forceinline__ void choose(const KVSelectParams& p, const Item& x, Team<THREADS, E>& team, const float (&score)[E], const F& error, const N& number, int n, int want, uint2* memory, int32_t* out) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   auto& shared = team.shared;
   const auto each = [&](const auto& f) __attribute__((always_inline)) {
@@ -279,14 +319,16 @@ __device__ __forceinline__ void choose(const KVSelectParams& p, const Item& x, T
   };
   if (tid < 256) shared.histogram[0][tid] = 0;
   if (tid == 0) shared.listed = 0;
-  float a = -INFINITY, b = -INFINITY;
-  each([&](int, float s) __attribute__((always_inline)) { a = fmaxf(a, s), b = fmaxf(b, -s); });
-  float2 r = team.most(a, b);
-  float high = r.x, low = -r.y;  // v lies between
-  const float off = 2.f * (team.most(mass, 0.f).x * 0x1p-14f + 0x1p-60f);  // 2 E (and terms that are below the normal range)
+  float a = -INFINITY, b = -INFINITY, top = 0.f, sum = 0.f;
+  const float share = 1.f / (float)n;
+  each([&](int e, float s) __attribute__((always_inline)) { a = fmaxf(a, s), b = fmaxf(b, -s), top = fmaxf(top, error(e)), sum += error(e) * share; });
+  const float4 about = team.survey(a, b, top, sum);
+  float high = about.x, low = -about.y;  // v lies between
+  const float worst = about.z, off = 2.f * about.w;  // the largest error, twice the mean: v need not be known better
   int left = want;  // v is the how many-th of those between them
+  int turn = 0;
 #pragma unroll 1
-  for (int turn = 0; high - low > off; turn ^= 1) {
+  for (; high - low > off; turn ^= 1) {
     const float scale = 255.f / (high - low);
     const auto part_of = [&](float s) __attribute__((always_inline)) { return min((int)((s - low) * scale), 255); };  // (low: 0, high: another)
     if (tid < 256) shared.histogram[turn ^ 1][tid] = 0;
@@ -294,49 +336,68 @@ __device__ __forceinline__ void choose(const KVSelectParams& p, const Item& x, T
       if (s >= low && s <= high) atomicAdd(&shared.histogram[turn][part_of(s)], 1);
     });
     __syncthreads();
-    // every wave looks the part up: four parts a lane, from the highest
-    const int4 h = *reinterpret_cast<const int4*>(&shared.histogram[turn][252 - 4 * lane]);
-    const int mine = h.x + h.y + h.z + h.w, upto = wave_scan(mine);
-    const int j = __builtin_ctzll(__ballot(upto >= left));
-    left -= __builtin_amdgcn_readlane(upto - mine, j);
-    const int hw = __builtin_amdgcn_readlane(h.w, j), hz = __builtin_amdgcn_readlane(h.z, j), hy = __builtin_amdgcn_readlane(h.y, j);
-    int part = 255 - 4 * j;
-    if (left > hw) {
-      left -= hw, --part;
-      if (left > hz) {
-        left -= hz, --part;
-        if (left > hy) left -= hy, --part;
-      }
-    }
+    const int part = part_with(shared.histogram[turn], lane, left);
     a = b = -INFINITY;
     each([&](int, float s) __attribute__((always_inline)) {
       if (s >= low && s <= high && part_of(s) == part) a = fmaxf(a, s), b = fmaxf(b, -s);
     });
-    r = team.most(a, b);
+    const float2 r = team.most(a, b);
     high = r.x, low = -r.y;
   }
 
+  // The score of the last one chosen, in fp64, lies between the least that any page from `low` on may have (`want` pages at least are there) and the most that any up to
+  // `high` may (fewer than `want` are not among these). Where errors are much alike, the largest stands for all of them, which saves a barrier (0.4 us).
   int in = 0, open = 0;
   uint32_t is_in = 0, is_open = 0;  // bit e
-  each([&](int e, float s) __attribute__((always_inline)) {
-    const bool yes = s > high + off, no = s < low - off;
+  const auto sort_out = [&](int e, float s, float off, float least, float most) __attribute__((always_inline)) {
+    const bool yes = s - off > most, no = s + off < least;
     in += yes, open += !yes && !no;
     is_in |= (uint32_t)yes << e, is_open |= (uint32_t)(!yes && !no) << e;
-  });
+  };
+  if (worst <= 2.f * off) {  // (uniform)
+    each([&](int e, float s) __attribute__((always_inline)) { sort_out(e, s, worst, low - worst, high + worst); });
+  } else {
+    a = b = -INFINITY;
+    each([&](int e, float s) __attribute__((always_inline)) {
+      const float off = error(e);
+      a = s >= low ? fmaxf(a, off - s) : a;
+      b = s <= high ? fmaxf(b, s + off) : b;
+    });
+    const float2 r = team.most(a, b);
+    each([&](int e, float s) __attribute__((always_inline)) { sort_out(e, s, error(e), -r.x, r.y); });
+  }
   const int2 all = team.sums(in, open);
   const int places = want - all.x;  // for those in question
+  // f(e, how many of those that `mine` says come before the thread's page e), in the pages' order: of all waves' counts four a lane, and their sums so far.
+  const auto place = [&](const auto& mine, const auto& f) __attribute__((always_inline)) {
+    constexpr int kWaves = THREADS / 64;
+    static_assert(kWaves % 4 == 0 && E * kWaves <= 256, "four counts a lane");
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const uint64_t bits = __ballot(mine(e));
+      if (lane == 0) shared.chosen[e * kWaves + wave] = __popcll(bits);
+    }
+    __syncthreads();
+    const int4 c = lane < E * kWaves / 4 ? *reinterpret_cast<const int4*>(&shared.chosen[4 * lane]) : make_int4(0, 0, 0, 0);
+    const int four = c.x + c.y + c.z + c.w, nth = wave & 3;
+    const int upto = wave_scan(four) - four + (nth > 0 ? c.x : 0) + (nth > 1 ? c.y : 0) + (nth > 2 ? c.z : 0);
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const uint64_t bits = __ballot(mine(e));
+      f(e, __builtin_amdgcn_readlane(upto, e * (kWaves / 4) + __builtin_amdgcn_readfirstlane(wave >> 2)) + __popcll(bits & ((1ull << lane) - 1)));
+    }
+  };
   if (all.y == places) {
     is_in |= is_open;
-  } else {  // (uniform)
-    uint2* const list = all.y <= Team<THREADS, E>::kListed ? shared.list : memory;
+  } else if (all.y <= Team<THREADS, E>::kListed) {  // (uniform)
 #pragma unroll
     for (int e = 0; e < E; ++e)
-      if ((is_open >> e) & 1) list[atomicAdd(&shared.listed, 1)].x = tid + THREADS * e;  // (in any order: what follows goes by the pages' numbers)
+      if ((is_open >> e) & 1) shared.list[atomicAdd(&shared.listed, 1)].x = tid + THREADS * e;  // (in any order: what follows goes by the pages' numbers)
     __syncthreads();
 #pragma unroll 1
     for (int k = wave; k < all.y; k += THREADS / 64) {
-      const float exact = exact_score<D>(p, x, __builtin_amdgcn_readfirstlane(list[k].x), lane);
-      if (lane == 0) list[k].y = sort_key(exact);
+      const float exact = exact_score<D>(p, x, __builtin_amdgcn_readfirstlane(shared.list[k].x), lane);
+      if (lane == 0) shared.list[k].y = sort_key(exact);
     }
     __syncthreads();
     // a page in question is in if fewer than `places` of the others are in front of it
@@ -345,36 +406,62 @@ __device__ __forceinline__ void choose(const KVSelectParams& p, const Item& x, T
       if (__any((is_open >> e) & 1)) {
         const uint32_t i = tid + THREADS * e;
         uint32_t key = 0;
-        for (int k = 0; k < all.y; ++k) key = list[k].x == i ? list[k].y : key;
+        for (int k = 0; k < all.y; ++k) key = shared.list[k].x == i ? shared.list[k].y : key;
         int rank = 0;
         for (int k = 0; k < all.y; ++k) {
-          const uint2 other = list[k];
+          const uint2 other = shared.list[k];
           rank += other.y > key || (other.y == key && other.x < i);
         }
         is_in |= (uint32_t)(((is_open >> e) & 1) && rank < places) << e;
       }
     }
-  }
-  // their places: of the wave's pages for each e, then of all in front
-#pragma unroll
-  for (int e = 0; e < E; ++e) {
-    const uint64_t mine = __ballot((is_in >> e) & 1);
-    if (lane == 0) shared.chosen[e * (THREADS / 64) + wave] = __popcll(mine);
-  }
-  __syncthreads();
-  int before = 0;
-#pragma unroll
-  for (int e = 0; e < E; ++e) {
-    int here = before;
-#pragma unroll
-    for (int w = 0; w < THREADS / 64; ++w) {
-      const int c = shared.chosen[e * (THREADS / 64) + w];
-      here += w < wave ? c : 0;
-      before += c;
+  } else {
+    // Many, equal ones most often: a wave sums its own pages, the key of the last one chosen is found by histograms of its bytes, and of those that have it the first are in.
+#pragma unroll 1
+    for (int e = 0; e < E; ++e) {
+      uint64_t mine = __ballot((is_open >> e) & 1);
+      while (mine != 0) {
+        const int j = __builtin_ctzll(mine);
+        mine &= mine - 1;
+        const float exact = exact_score<D>(p, x, __builtin_amdgcn_readfirstlane(64 * wave + THREADS * e + j), lane);
+        if (lane == j) memory[tid + THREADS * e].y = sort_key(exact);
+      }
     }
-    const uint64_t mine = __ballot((is_in >> e) & 1);
-    if ((is_in >> e) & 1) out[here + __popcll(mine & ((1ull << lane) - 1))] = number[e];
+    uint32_t border = 0;
+    left = places;
+#pragma unroll 1
+    for (int shift = 24; shift >= 0; shift -= 8) {
+      int* const histogram = shared.histogram[turn];
+      __syncthreads();  // the round before has been read
+      if (tid < 256) histogram[tid] = 0;
+      __syncthreads();
+#pragma unroll 1
+      for (int e = 0; e < E; ++e)
+        if ((is_open >> e) & 1) {
+          const uint32_t key = memory[tid + THREADS * e].y;
+          if (shift == 24 || (key ^ border) >> (shift + 8) == 0) atomicAdd(&histogram[(key >> shift) & 255], 1);
+        }
+      __syncthreads();
+      border |= (uint32_t)part_with(histogram, lane, left) << shift;
+    }
+    uint32_t is_equal = 0;
+#pragma unroll 1
+    for (int e = 0; e < E; ++e)
+      if ((is_open >> e) & 1) {
+        const uint32_t key = memory[tid + THREADS * e].y;
+        is_in |= (uint32_t)(key > border) << e, is_equal |= (uint32_t)(key == border) << e;
+      }
+    const auto equal = [&](int e) __attribute__((always_inline)) { return (is_equal >> e) & 1; };
+    uint32_t first = 0;
+    place(equal, [&](int e, int rank) __attribute__((always_inline)) { first |= (uint32_t)(rank < left) << e; });
+    is_in |= is_equal & first;
+    __syncthreads();  // the counts have been read
   }
+  // their places
+  const auto chosen = [&](int e) __attribute__((always_inline)) { return (is_in >> e) & 1; };
+  place(chosen, [&](int e, int at) __attribute__((always_inline)) {
+    if (chosen(e)) out[at] = number(e);
+  });
 }
 
 // A page whose S is not known gets its score in fp64 (`index`: of lane 0's page; by a whole wavefront).
@@ -413,11 +500,12 @@ __global__ __launch_bounds__(THREADS) void kv_pick_kernel(KVSelectParams p) {
   if (!begin_choice(p, x, item, out)) return;
   uint2* const memory = p.pages_of + item * p.row;
   const int n = x.pages - 1;
-  float score[E], s[E], mass = 0.f;
-  int32_t number[E];
+  float score[E], s[E];
+  constexpr bool kEarly = E <= 4;  // the table's entries come with the scores, and stay with the errors in registers (which do not hold 16 of each: read when they are wanted)
+  int32_t early[kEarly ? E : 1];
 #pragma unroll
   for (int e = 0; e < E; ++e) {
-    number[e] = x.table[min((int)threadIdx.x + THREADS * e, n - 1)];
+    if constexpr (kEarly) early[e] = x.table[min((int)threadIdx.x + THREADS * e, n - 1)];
     const float2 found = reinterpret_cast<const float2*>(memory)[min((int)threadIdx.x + THREADS * e, n - 1)];
     score[e] = found.x, s[e] = found.y;
   }
@@ -425,16 +513,29 @@ __global__ __launch_bounds__(THREADS) void kv_pick_kernel(KVSelectParams p) {
 #pragma unroll
   for (int e = 0; e < E; ++e) {
     known = known && s[e] < INFINITY;
-    mass = s[e] < INFINITY ? fmaxf(mass, s[e]) : mass;
     score[e] = known ? in_range(score[e]) : score[e];
   }
-  if (__any(!known)) {  // (rare)
+  if (__any(!known)) {  // (rare; by way of the memory, so that the loop has one body)
+    float2* const mine = reinterpret_cast<float2*>(memory) + threadIdx.x;
+#pragma unroll 1
+    for (int e = 0; e < E; ++e) {
+      const bool real = (int)threadIdx.x + THREADS * e < n;
+      const float settled = settle_unknown<D>(p, x, 64 * wave + THREADS * e, real, real ? mine[THREADS * e] : make_float2(0.f, 0.f), lane);
+      if (real) mine[THREADS * e].x = settled;
+    }
 #pragma unroll
-    for (int e = 0; e < E; ++e)
-      score[e] = settle_unknown<D>(p, x, 64 * wave + THREADS * e, (int)threadIdx.x + THREADS * e < n, make_float2(score[e], s[e]), lane);
+    for (int e = 0; e < E; ++e) score[e] = (int)threadIdx.x + THREADS * e < n ? mine[THREADS * e].x : 0.f;
   }
   Team<THREADS, E> team(shared);
-  choose<D, THREADS, E>(p, x, team, score, number, mass, n, p.keep - 1, memory, out);
+  const auto error = [&](int e) __attribute__((always_inline)) {
+    if constexpr (kEarly) return error_of(s[e]);
+    else return error_of(reinterpret_cast<const float2*>(memory)[threadIdx.x + THREADS * e].y);
+  };
+  const auto number = [&](int e) __attribute__((always_inline)) {
+    if constexpr (kEarly) return early[e];
+    else return x.table[threadIdx.x + THREADS * e];
+  };
+  choose<D, THREADS, E>(p, x, team, score, error, number, n, p.keep - 1, memory, out);
 }
 
 // Scores and choice in one launch, for tables of up to kFewPages pages.
@@ -442,14 +543,13 @@ constexpr int kFewPages = 256, kSomePages = 2048, kMostPages = 16384;
 template <int D>
 __global__ __launch_bounds__(kThreads) void kv_pick_few_kernel(KVSelectParams p) {
   __shared__ typename Team<kThreads, 1>::Shared shared;
-  __shared__ float scores[kFewPages];
+  __shared__ float2 scores[kFewPages];  // and how far they may be off
   const int item = blockIdx.x, lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const Item x = item_of(p, item, lane);
   int32_t* const out = p.table_out + (int64_t)item * p.keep;
   if (!begin_choice(p, x, item, out)) return;
   const int n = x.pages - 1;
-  const int32_t number[1] = {x.table[min((int)threadIdx.x, n - 1)]};
-  float mass = 0.f;
+  const int32_t number = x.table[min((int)threadIdx.x, n - 1)];
 #pragma unroll 1
   for (int first = 32 * wave; first < n; first += kChunk) {
     float2 found[2];
@@ -459,13 +559,13 @@ __global__ __launch_bounds__(kThreads) void kv_pick_few_kernel(KVSelectParams p)
     const float2 mine = lane < 16 ? found[0] : found[1];
     const bool real = lane < 32 && first + lane < n;
     const float s = settle_unknown<D>(p, x, first, real, mine, lane);
-    if (real) scores[first + lane] = s;
-    mass = real && mine.y < INFINITY ? fmaxf(mass, mine.y) : mass;
+    if (real) scores[first + lane] = make_float2(s, error_of(mine.y));
   }
   __syncthreads();
-  const float score[1] = {scores[threadIdx.x]};
+  const float score[1] = {scores[threadIdx.x].x}, error = scores[threadIdx.x].y;
   Team<kThreads, 1> team(shared);
-  choose<D, kThreads, 1>(p, x, team, score, number, mass, n, p.keep - 1, p.pages_of + item * p.row, out);
+  choose<D, kThreads, 1>(
+      p, x, team, score, [&](int) __attribute__((always_inline)) { return error; }, [&](int) __attribute__((always_inline)) { return number; }, n, p.keep - 1, p.pages_of + item * p.row, out);
 }
 
 int check_select(const pith_kv_select_args* a, const char* who) {

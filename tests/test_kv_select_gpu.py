@@ -1,4 +1,5 @@
-"""Selection of pages on the GPU with token offsets that do not begin at 0 or that fall. test_kv_gpu.py has the ordinary calls."""
+"""Selection of pages on the GPU where many pages are close to the border of the choice, where one has bounds of another size than the rest, and with token offsets
+that do not begin at 0 or that fall. The choice is exact: it has to be the oracle's. test_kv_gpu.py has the ordinary calls."""
 
 import pytest
 import test_kv_gpu as G
@@ -8,6 +9,94 @@ from pithtrain_amd.operators.gqa import kv_cache as K
 
 pytestmark = pytest.mark.gpu
 BF, I32 = G.BF, G.I32
+
+
+# ---------------------------------------------------------------------------------------------
+# Many pages in question
+
+
+def _close(pages, heads, values, seed):
+    """Bounds whose scores differ by less than a sum of 32 bits over the features is known to: 1 (or -1) in all features but the last, which is one of `values`."""
+    g = torch.Generator().manual_seed(seed)
+    bounds = torch.ones(pages, heads, 2, 64) * (-1 if max(values) < 0 else 1)
+    last = torch.tensor(values)[torch.randint(0, len(values), (pages, heads), generator=g)]
+    bounds[..., 0, 63], bounds[..., 1, 63] = last, last
+    return bounds.to(BF)
+
+
+def _ones(monkeypatch):
+    made = G.Batch.__init__
+
+    def of_ones(self, *args, **kw):
+        made(self, *args, **kw)
+        self.q.fill_(1.0)
+
+    monkeypatch.setattr(G.Batch, "__init__", of_ones)
+
+
+# sums of absolute values are 63 and a little: scores that lie 2^-8 apart, E, may stand in either order
+VALUES = {"equal": [0.5], "two": [0.0, 2.0**-17], "many": [2.0**-9 * (1 + i / 128) for i in range(128)], "below": [-(2.0**-9) * (1 + i / 128) for i in range(128)]}
+# tables of one launch, of up to 2048 pages and of more
+WIDTHS = [(250, 200), (250, 3), (254, 129), (1999, 700), (1999, 5), (16381, 4000), (9001, 77)]
+
+
+@pytest.mark.parametrize("values", VALUES)
+@pytest.mark.parametrize("pages, keep", WIDTHS, ids=str)
+def test_choices_among_many_pages_in_question(gpu, monkeypatch, pages, keep, values):
+    _ones(monkeypatch)
+    lengths = [16 * pages, 16 * (pages - 7) + 3]
+    _selection_of(gpu, lengths, keep, _close(2 * (pages + 2), 2, VALUES[values], pages))
+
+
+@pytest.mark.parametrize("pages, keep", WIDTHS, ids=str)
+def test_choices_among_pages_without_anything_in_them(gpu, pages, keep):
+    """A cache of zeros: all scores are 0 exactly."""
+    _selection_of(gpu, [16 * pages - 5], keep, torch.zeros(pages + 2, 2, 2, 64, dtype=BF))
+
+
+def _selection_of(gpu, lengths, keep, bounds):
+    G._selection(gpu, lengths, (4, 2, 64), keep, seed=3, bounds=bounds)
+
+
+@pytest.mark.parametrize("pages, keep", [(250, 60), (2000, 64), (16000, 64)])
+@pytest.mark.parametrize("size", [30.0, 1000.0, 1e30])
+def test_choices_beside_a_page_with_bounds_of_another_size(gpu, pages, keep, size):
+    g = torch.Generator().manual_seed(pages)
+    x = torch.randn(pages + 2, 2, 2, 64, generator=g)
+    x[::97] *= size
+    bounds = torch.stack((x.amin(2), x.amax(2)), 2).to(BF)
+    _selection_of(gpu, [16 * pages - 3], keep, bounds)
+    bounds[:, :, 1] = bounds[:, :, 0]  # and of scores on both sides of the others'
+    _selection_of(gpu, [16 * pages - 3], keep, bounds)
+
+
+def _us(call, calls=20):
+    call()
+    first, last = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+    first.record()
+    for _ in range(calls):
+        call()
+    last.record()
+    torch.cuda.synchronize()
+    return first.elapsed_time(last) * 1000 / calls
+
+
+@pytest.mark.parametrize("pages", [2000, 16000])
+def test_one_page_of_another_size_or_equal_scores_do_not_take_a_call_out_of_proportion(gpu, pages):
+    """Only pages whose own sums may be off by what separates them from the border are summed anew: one page with bounds ten thousand times as large as the rest makes no more
+    of them. Equal scores do, and a page is summed and counted, not compared with all others: the time grows like the pages, not like their square. (us measured: 2000 pages 18,
+    21 and 370, 16000 pages 70, 90 and 2450, for eight tokens.)"""
+    g = torch.Generator().manual_seed(1)
+    x = torch.randn(pages, 4, 2, 64, generator=g)
+    ordinary = torch.stack((x.amin(2), x.amax(2)), 2).to(BF).to(gpu)
+    outlying, equal = ordinary.clone(), torch.ones_like(ordinary)
+    outlying[pages // 2] *= 10000
+    q = torch.randn(2, 8, 64, generator=g).to(BF).to(gpu)
+    table, lens = torch.arange(pages, dtype=I32, device=gpu).repeat(2, 1), torch.tensor([16 * pages - 1] * 2, dtype=I32, device=gpu)
+    us = {name: _us(lambda: K.kv_select_pages(q, bounds, table, lens, None, 16, 64)) for name, bounds in (("ordinary", ordinary), ("outlying", outlying), ("equal", equal))}
+    print(us)
+    assert us["outlying"] < 10 * us["ordinary"], us
+    assert us["equal"] < 10 * us["ordinary"] + 0.5 * pages, us
 
 
 # ---------------------------------------------------------------------------------------------
