@@ -159,7 +159,7 @@ int pith_kv_attn(const pith_kv_attn_args* args, pith_stream_t stream);
  *                    [T, heads]: a call of pith_kv_attn with head_tables and without cu_q. Tokens that are no sequence's (in front of
  *                    cu_q[0], behind cu_q[B]) and those that see nothing get no page.
  * q [T, H, dim] bf16 as in pith_kv_attn_args. keep >= 1; pith_kv_select takes page tables of up to 16384 pages. Its workspace:
- * pith_kv_select_workspace_bytes, 256-byte aligned. */
+ * pith_kv_select_workspace_bytes (64 MB at most, or what one token needs: more tokens than that serves are taken in parts), 256-byte aligned. */
 typedef struct {
   pith_kv_cache cache;
   void* bounds;

@@ -32,9 +32,10 @@ struct KVSelectParams {
   const __bf16 *q, *bounds;
   const int32_t *table, *lengths, *cu_q;
   int32_t *table_out, *lengths_out;
-  uint2* pages_of;  // workspace, [T * heads][row]: score and S of each page, then the pages in question
+  uint2* pages_of;  // workspace, [tokens of the part * heads][row]: score and S of each page, then the keys of those in question
   int64_t q_ts, q_hs, table_rs, bounds_ps, row;
   int T, B, heads, group, pages, page_shift, table_width, keep, chunks, tokens;
+  int first, last;  // the part's tokens
 };
 
 // A token and key-value head.
@@ -203,14 +204,14 @@ __device__ __forceinline__ float exact_score(const KVSelectParams& p, const Item
 template <int D>
 __global__ __launch_bounds__(kThreads) void kv_score_kernel(KVSelectParams p) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int chunk = blockIdx.x % p.chunks, part = blockIdx.x / p.chunks, t0 = part / p.heads * p.tokens, head = part % p.heads;
+  const int chunk = blockIdx.x % p.chunks, part = blockIdx.x / p.chunks, t0 = p.first + part / p.heads * p.tokens, head = part % p.heads;
   const int first = chunk * kChunk + 32 * wave;
   PageBounds<D, 2> bounds;
   int loaded = -1;  // sequence
   Item x;
   x.end = 0;
 #pragma unroll 1
-  for (int t = t0; t < min(t0 + p.tokens, p.T); ++t) {
+  for (int t = t0; t < min(t0 + p.tokens, p.last); ++t) {
     const int item = t * p.heads + head;
     if (t < x.end) {
       x.t = t;
@@ -223,7 +224,7 @@ __global__ __launch_bounds__(kThreads) void kv_score_kernel(KVSelectParams p) {
     loaded = x.seq;
     float2 found[2];
     bounds.score(p, x, lane, found);
-    if (lane < 32) reinterpret_cast<float2*>(p.pages_of)[item * p.row + first + lane] = lane < 16 ? found[0] : found[1];  // (of those behind the last: not read)
+    if (lane < 32) reinterpret_cast<float2*>(p.pages_of)[(item - p.first * p.heads) * p.row + first + lane] = lane < 16 ? found[0] : found[1];  // (of those behind the last: not read)
   }
 }
 
@@ -494,11 +495,11 @@ __device__ __forceinline__ bool begin_choice(const KVSelectParams& p, const Item
 template <int D, int THREADS, int E>
 __global__ __launch_bounds__(THREADS) void kv_pick_kernel(KVSelectParams p) {
   __shared__ typename Team<THREADS, E>::Shared shared;
-  const int item = blockIdx.x, lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int item = p.first * p.heads + blockIdx.x, lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const Item x = item_of(p, item, lane);
   int32_t* const out = p.table_out + (int64_t)item * p.keep;
   if (!begin_choice(p, x, item, out)) return;
-  uint2* const memory = p.pages_of + item * p.row;
+  uint2* const memory = p.pages_of + blockIdx.x * p.row;
   const int n = x.pages - 1;
   float score[E], s[E];
   constexpr bool kEarly = E <= 4;  // the table's entries come with the scores, and stay with the errors in registers (which do not hold 16 of each: read when they are wanted)
@@ -544,7 +545,7 @@ template <int D>
 __global__ __launch_bounds__(kThreads) void kv_pick_few_kernel(KVSelectParams p) {
   __shared__ typename Team<kThreads, 1>::Shared shared;
   __shared__ float2 scores[kFewPages];  // and how far they may be off
-  const int item = blockIdx.x, lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int item = p.first * p.heads + blockIdx.x, lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const Item x = item_of(p, item, lane);
   int32_t* const out = p.table_out + (int64_t)item * p.keep;
   if (!begin_choice(p, x, item, out)) return;
@@ -565,7 +566,7 @@ __global__ __launch_bounds__(kThreads) void kv_pick_few_kernel(KVSelectParams p)
   const float score[1] = {scores[threadIdx.x].x}, error = scores[threadIdx.x].y;
   Team<kThreads, 1> team(shared);
   choose<D, kThreads, 1>(
-      p, x, team, score, [&](int) __attribute__((always_inline)) { return error; }, [&](int) __attribute__((always_inline)) { return number; }, n, p.keep - 1, p.pages_of + item * p.row, out);
+      p, x, team, score, [&](int) __attribute__((always_inline)) { return error; }, [&](int) __attribute__((always_inline)) { return number; }, n, p.keep - 1, p.pages_of + blockIdx.x * p.row, out);
 }
 
 int check_select(const pith_kv_select_args* a, const char* who) {
@@ -582,6 +583,14 @@ int check_select(const pith_kv_select_args* a, const char* who) {
 
 int64_t chunks_of(const pith_kv_select_args* a) { return (a->table_width + kChunk - 1) / kChunk; }
 
+// Tokens are taken in parts of as many as 64 MB of scores serve (one at least), one behind the other: a prompt of 8192 tokens over 2048 pages, 4 heads, has 512 MB of them
+// (2.91 ms in eight parts, 2.82 at once).
+constexpr int64_t kPartBytes = 64 << 20;
+int64_t part_of(const pith_kv_select_args* a) {
+  const int64_t each = a->heads * chunks_of(a) * kChunk * (int64_t)sizeof(uint2);
+  return std::max<int64_t>(std::min(a->T, each > 0 ? kPartBytes / each : a->T), 1);
+}
+
 }  // namespace
 }  // namespace pith
 
@@ -589,7 +598,7 @@ using namespace pith;
 
 extern "C" int64_t pith_kv_select_workspace_bytes(const pith_kv_select_args* a) {
   if (check_select(a, "pith_kv_select_workspace_bytes") != PITH_OK || a->B == 0) return 0;
-  return a->T * a->heads * chunks_of(a) * kChunk * (int64_t)sizeof(uint2);
+  return a->T == 0 ? 0 : part_of(a) * a->heads * chunks_of(a) * kChunk * (int64_t)sizeof(uint2);
 }
 
 extern "C" int pith_kv_select(const pith_kv_select_args* a, pith_stream_t stream) {
@@ -615,9 +624,10 @@ extern "C" int pith_kv_select(const pith_kv_select_args* a, pith_stream_t stream
   p.pages = (int)a->pages; p.page_shift = __builtin_ctzll((unsigned long long)a->page_size); p.table_width = (int)a->table_width; p.keep = (int)a->keep;
   hipStream_t s = (hipStream_t)stream;
   begin_launch();
-  const unsigned items = (unsigned)(a->T * a->heads);
   const auto launch = [&](auto d) {
     constexpr int D = decltype(d)::value;
+    const int tokens = p.last - p.first;
+    const unsigned items = (unsigned)(tokens * p.heads);
     if (a->table_width <= kFewPages) {
       kv_pick_few_kernel<D><<<items, kThreads, 0, s>>>(p);
       return;
@@ -627,12 +637,15 @@ extern "C" int pith_kv_select(const pith_kv_select_args* a, pith_stream_t stream
       // 1 / 2 / 4 / 8: 22 sequences of 7 over up to 674 pages, heads of 64 / 4, 53 / 46 / 44 / 46; 8 of 4 over up to 2048 39 / 33 / 31 / 31; 108 of 2 46 / 40 / 40 / 41.
       const int64_t each = (a->T + a->B - 1) / a->B, most = items * (int64_t)p.chunks / (2 * compute_units_or_default());
       p.tokens = (int)std::max<int64_t>(std::min<int64_t>({each, most, 4}), 1);
-      kv_score_kernel<D><<<(unsigned)((a->T + p.tokens - 1) / p.tokens * p.heads * p.chunks), kThreads, 0, s>>>(p);
+      kv_score_kernel<D><<<(unsigned)((tokens + p.tokens - 1) / p.tokens * p.heads * p.chunks), kThreads, 0, s>>>(p);
     }
     if (a->table_width <= kSomePages) kv_pick_kernel<D, 512, kSomePages / 512><<<items, 512, 0, s>>>(p);
     else kv_pick_kernel<D, 1024, kMostPages / 1024><<<items, 1024, 0, s>>>(p);
   };
-  if (a->dim == 128) launch(std::integral_constant<int, 128>());
-  else launch(std::integral_constant<int, 64>());
+  for (const int64_t part = part_of(a); p.first < p.T; p.first = p.last) {
+    p.last = (int)std::min<int64_t>(p.first + part, p.T);
+    if (a->dim == 128) launch(std::integral_constant<int, 128>());
+    else launch(std::integral_constant<int, 64>());
+  }
   return check_launch(who);
 }

@@ -238,6 +238,15 @@ def test_workspaces():
     assert select() == 4 * 2 * 128 * 8 and select(T=0) == select(keep=0) == 0 and select(table_width=129) == 2 * select()
 
 
+def test_the_workspace_of_a_selection_is_bounded():
+    """64 MB, or what one token needs, however many tokens there are."""
+    select = lambda **kw: _C.lib().pith_kv_select_workspace_bytes(ctypes.byref(_select(**kw)))  # noqa: E731
+    prompt = dict(heads=4, H=32, table_width=2048, table_rs=2048, bounds_ps=1024)
+    assert select(T=1, **prompt) == 4 * 2048 * 8 and select(T=1024, **prompt) == 64 << 20
+    assert [select(T=t, **prompt) for t in (1025, 8192, 100000)] == [64 << 20] * 3
+    assert select(T=9, heads=1024, H=1024, table_width=16384, table_rs=16384, bounds_ps=1 << 18) == 1024 * 16384 * 8
+
+
 def test_rows_of_a_row_block_go_by_the_rows_of_a_sequence_and_the_work_list():
     rows = lambda **kw: _C.lib().pith_kv_attn_rows(ctypes.byref(_attn(**kw)))  # noqa: E731
     assert rows(T=0) == rows(B=0) == rows(H=3) == 0  # nothing to launch, or what pith_kv_attn rejects

@@ -1,10 +1,11 @@
-"""Selection of pages on the GPU where many pages are close to the border of the choice, where one has bounds of another size than the rest, and with token offsets
-that do not begin at 0 or that fall. The choice is exact: it has to be the oracle's. test_kv_gpu.py has the ordinary calls."""
+"""Selection of pages on the GPU where many pages are close to the border of the choice, where one has bounds of another size than the rest, for more tokens than
+are taken at a time, and with token offsets that do not begin at 0 or that fall. The choice is exact: it has to be the oracle's. test_kv_gpu.py has the ordinary calls."""
 
 import pytest
 import test_kv_gpu as G
 import torch
 
+from oracle import kv_oracle as O
 from pithtrain_amd.operators.gqa import kv_cache as K
 
 pytestmark = pytest.mark.gpu
@@ -132,3 +133,50 @@ def test_offsets_count_as_their_maximum_so_far_in_all_operators(gpu, offsets, sa
         for at in range(same[i], same[i + 1]):
             assert (rows[at] == int(lens[i]) - same[i + 1] + at + 1 - page * (-(-(int(lens[i]) - same[i + 1] + at + 1) // page) - 5)).all()
     assert (chosen[~mine] == -1).all() and (rows[~mine] == 0).all() and (o[~mine] == 7).all() and (chosen[mine] >= 0).all() and (o[mine] != 7).any()
+
+
+# ---------------------------------------------------------------------------------------------
+# Many tokens
+
+
+def test_many_tokens_are_chosen_for_in_parts(gpu):
+    """More tokens than one part of the workspace holds: the choice for each is the one that it gets in a call of few."""
+    g = torch.Generator().manual_seed(2)
+    pages, page, t = 2048, 16, 2300
+    x = torch.randn(pages, 4, 2, 64, generator=g)
+    bounds = torch.stack((x.amin(2), x.amax(2)), 2).to(BF).to(gpu)
+    q = torch.randn(t, 8, 64, generator=g).to(BF).to(gpu)
+    table = torch.randperm(pages, generator=g).to(I32).view(1, pages).repeat(2, 1).to(gpu)
+    counts = [1900, 390]  # and ten that are nobody's
+    lens, cu_q = [page * 2040 + 7, page * pages], torch.tensor([0, 1900, 2290], dtype=I32, device=gpu)
+    chosen, rows = K.kv_select_pages(q, bounds, table, torch.tensor(lens, dtype=I32, device=gpu), cu_q, page, 30)
+    for i, (first, n) in enumerate(zip((0, 1900), counts)):
+        for at in range(0, n, 100):
+            few = min(100, n - at)
+            visible = torch.tensor([lens[i] - n + at + few], dtype=I32, device=gpu)
+            want = K.kv_select_pages(q[first + at : first + at + few], bounds, table[i : i + 1], visible, torch.tensor([0, few], dtype=I32, device=gpu), page, 30)
+            assert torch.equal(chosen[first + at : first + at + few], want.page_table) and torch.equal(rows[first + at : first + at + few], want.lengths), (i, at)
+    assert (chosen[2290:] == -1).all() and (rows[2290:] == 0).all()
+    some = 1234
+    want = O.select(q[some].cpu(), bounds[table[0].long()].cpu(), lens[0] - 1900 + some + 1, page, 30)
+    assert all(torch.equal(chosen[some, j].cpu(), table[0].cpu()[want[j]]) for j in range(4))
+
+
+def test_a_captured_choice_for_many_tokens(gpu):
+    g = torch.Generator().manual_seed(4)
+    x = torch.randn(700, 16, 2, 64, generator=g)
+    bounds = torch.stack((x.amin(2), x.amax(2)), 2).to(BF).to(gpu)
+    q, table = torch.randn(1500, 16, 64, generator=g).to(BF).to(gpu), torch.arange(700, dtype=I32, device=gpu).view(1, -1)
+    lens, cu_q = torch.tensor([16 * 700], dtype=I32, device=gpu), torch.tensor([0, 1500], dtype=I32, device=gpu)
+    call = lambda: K.kv_select_pages(q, bounds, table, lens, cu_q, 16, 9)  # noqa: E731
+    call()
+    graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.graph(graph, stream=side):
+        got = call()
+    for length in (16 * 700, 1600, 16 * 650 + 5, 16 * 700):
+        lens.fill_(length)
+        graph.replay()
+        want = call()
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for x, y in zip(got, want))
