@@ -141,7 +141,8 @@ typedef struct {
 
 int64_t pith_kv_attn_workspace_bytes(const pith_kv_attn_args* args);
 /* Query rows to a row block of the kernel that such a call takes, 16, 32 or 64; 0 for a call that launches nothing or is rejected for its sizes. A row's
- * keys are cut, and its sums ordered, by that and by the lengths of all sequences of the call. */
+ * keys are cut, and its sums ordered, by that and by the lengths of all sequences of the call. In blocks of 16 rows a softmax weight keeps 16 bits in the product with
+ * the values (2^-15 of it is lost at most), in those of 32 and 64 the 8 of a bf16 number (2^-8). */
 int pith_kv_attn_rows(const pith_kv_attn_args* args);
 int pith_kv_attn(const pith_kv_attn_args* args, pith_stream_t stream);
 

@@ -28,8 +28,13 @@
 // Measured, heads of 32 / 4 with 128 features: 32 sequences of up to 8192 rows, bf16, one token each (303 MB) 64 us, 4.7 TB/s; 8 of up to 131072 rows, e4m3 (879 MB)
 // 160 us, 5.5 TB/s, where a copy reaches 4.9; 64 selected pages of 8 such sequences (34 MB) 15 us, of which the join's launch is 4 and beginnings and ends
 // about 4; one sequence of 517 rows 8.8 us, a launch and 5 steps of waiting for memory.
-// The weights go into the second product as bf16, which is what the matrix cores take beside a cache of bf16 (or e4m3, widened exactly): half a step, 2^-8, of
-// each, while their sum is of the unrounded ones. With e4m3 a weight is rounded once, when its row's scale is in it.
+// The matrix cores take weights as bf16 beside a cache of bf16 (or e4m3, widened exactly; a weight then has its row's scale in it). In blocks of 16 rows, where these
+// products are few beside the bytes, a weight goes in as two numbers, its upper half and the rest rounded, and keeps 16 bits of its fraction: 2^-15 of it is lost at
+// most, and the outputs are off by what their own rounding does (norm of the difference from 64 bits by the norm: 0.0016; 0.0023 with one number). It takes, us with one
+// number / two: one sequence of 517 rows 8.9 / 9.7 (eight more products and 20 instructions a tile in a chain of five), 32 of up to 8192 63.0 / 63.5, 8 of up to
+// 131072, e4m3, 158.2 / 158.8, 1024 of up to 200 73.1 / 74.9, 64 selected pages 15.2 / 15.2. Blocks of 32 and 64 rows take one number, half a step, 2^-8, of each: there the
+// second costs 2 to 19 % (8 tokens, 32 x 8192 rows 111.5 / 114.1, 16, 16 x 8192, e4m3, 78.9 / 84.7, 512 behind 8192 111 / 133, 4 prompts of 2048 227 / 255, half of them cached).
+// The sum of the weights is of the unrounded ones everywhere.
 #pragma once
 
 #include "cache_attn.h"
@@ -443,6 +448,22 @@ __device__ __forceinline__ uint32_t seen_keys(const KVAttnParams& p, const KVWor
   return seen;
 }
 
+// Weights as the sum of two bf16 numbers, the upper 16 bits of each and the rounded rest of it: off by 2^-15 of the weight at most. The rest has 2^-20 of the weight on
+// top, so that it is 0 only where the weight is: a value that is infinite stays so in the products with both. (Of infinite weights, which come of scales that are, the
+// rest is NaN.)
+__device__ __forceinline__ bf16x8 upper_halves(const float (&y)[8]) {
+  u32x4 u;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) u[e] = __builtin_amdgcn_perm(__float_as_uint(y[2 * e + 1]), __float_as_uint(y[2 * e]), 0x07060302u);
+  return __builtin_bit_cast(bf16x8, u);
+}
+__device__ __forceinline__ bf16x8 rests(const float (&y)[8]) {
+  float x[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) x[e] = fmaf(y[e], 1.f + 0x1p-20f, -__uint_as_float(__float_as_uint(y[e]) & 0xffff0000u));
+  return to_bf16x8(x[0], x[1], x[2], x[3], x[4], x[5], x[6], x[7]);
+}
+
 // Values that are not finite, in a tile that some rows see in part only: a row's weight of a key it does not see is 0, and must stay so against whatever the
 // key's value holds. What such a value makes of a row that does see it is an infinity or NaN whatever the rest: `up` and `down` note, for each of the lane's
 // features (bit 4 n + v), whether one above and one below all numbers was seen (NaN is both). Then it is 0 in LDS. Rare, and as slow as it likes to be.
@@ -652,7 +673,9 @@ __global__ __launch_bounds__(kKVThreads, (KVRing<D, FP8, R>::kPerUnit)) void kv_
             for (int v = 0; v < 4; ++v) k_scale[4 * h + v] = scales[h][v] * p.kappa, v_scale[4 * h + v] = scales[2 + h][v];
       }
       const bool partial = key0 + kTileKeys > s.len - s.n + (p.tree ? 0 : 1);  // some row may not see all of it
+      constexpr bool kSplit = R == 1;  // weights as two bf16 numbers
       bf16x8 weight[R];
+      float unrounded[8];  // weights of the row, if they go in as two numbers
       uint32_t seen[R];
 #pragma unroll
       for (int r = 0; r < R; ++r) {
@@ -690,7 +713,11 @@ __global__ __launch_bounds__(kKVThreads, (KVRing<D, FP8, R>::kPerUnit)) void kv_
             for (int e = 0; e < 8; ++e) y[e] *= v_scale[e];
           }
         }
-        weight[r] = to_bf16x8(y[0], y[1], y[2], y[3], y[4], y[5], y[6], y[7]);
+        if constexpr (kSplit) {
+          weight[r] = upper_halves(y);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) unrounded[e] = y[e];
+        } else weight[r] = to_bf16x8(y[0], y[1], y[2], y[3], y[4], y[5], y[6], y[7]);
         if constexpr (R > 2) __builtin_amdgcn_sched_barrier(0);
       }
       const Loads loads(p, pages, key_of_tile(i + kSlots), last, head);
@@ -714,6 +741,12 @@ __global__ __launch_bounds__(kKVThreads, (KVRing<D, FP8, R>::kPerUnit)) void kv_
         for (int n = 0; n < kAhead; ++n)
 #pragma unroll
           for (int r = 0; r < R; ++r) acc[r][n0 + n] = mfma16(v[n], weight[r], acc[r][n0 + n]);
+        if constexpr (kSplit) {
+          __builtin_amdgcn_sched_barrier(0);
+          const bf16x8 rest = rests(unrounded);
+#pragma unroll
+          for (int n = 0; n < kAhead; ++n) acc[0][n0 + n] = mfma16(v[n], rest, acc[0][n0 + n]);
+        }
       }
       if (more) {
         __builtin_amdgcn_s_waitcnt(0xC07F);  // the values have been read
