@@ -1,4 +1,4 @@
-// What the attention kernels to the two caches share: scans over the lanes of a wavefront, softmax references, e4m3.
+// What the kernels of the two caches share: scans and sums over the lanes of a wavefront, softmax references, e4m3.
 #pragma once
 
 #include "latent_common.h"
@@ -33,30 +33,6 @@ __device__ __forceinline__ int wave_scan_max(int x) {
   return max_dpp<0x143, 0xc>(x);
 }
 
-// A value of another lane of the row of 16.
-template <int CTRL>
-__device__ __forceinline__ float lane_dpp(float x) {
-  return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), CTRL, 0xf, 0xf, true));
-}
-constexpr int kDppXor1 = 0xB1, kDppXor2 = 0x4E, kDppHalfMirror = 0x141, kDppMirror = 0x140, kDppRotate8 = 0x128, kDppQuadMirror = 0x1B;
-// Over groups of 8 or 16 lanes; all of a group have the result. (Behind the first two steps lanes of a quad agree, so a mirrored half or row is as good as an
-// exchanged one.)
-template <int LANES, typename F>
-__device__ __forceinline__ float group_reduce(float x, const F& f) {
-  static_assert(LANES == 8 || LANES == 16, "rows of 64 or 128 features");
-  x = f(x, lane_dpp<kDppXor1>(x));
-  x = f(x, lane_dpp<kDppXor2>(x));
-  x = f(x, lane_dpp<kDppHalfMirror>(x));
-  if constexpr (LANES == 16) x = f(x, lane_dpp<kDppMirror>(x));
-  return x;
-}
-// Of the lane half a group away.
-template <int LANES>
-__device__ __forceinline__ float other_half(float x) {
-  if constexpr (LANES == 16) return lane_dpp<kDppRotate8>(x);
-  else return lane_dpp<kDppQuadMirror>(lane_dpp<kDppHalfMirror>(x));
-}
-
 // max / sum over the four lanes c, c + 16, c + 32, c + 48 that share a query row
 __device__ __forceinline__ float quad_max(float x) {
   const int i = __float_as_int(x);
@@ -78,9 +54,6 @@ __device__ __forceinline__ bf16x8 widen(uint32_t w0, uint32_t w1) {
 // Tables that nobody writes while the kernel runs, read as constant memory: by scalar loads, which the counted waits for tiles do not see.
 typedef const __attribute__((address_space(4))) int32_t* ScalarTable;
 
-// A weight times its row's scale; 0 stays 0, also against a scale that is not finite.
-__device__ __forceinline__ float scaled(float weight, float scale) { return weight == 0.f ? 0.f : weight * scale; }
-
 // x *= f in place: as a plain product under a branch the accumulators are copied on the other way, which doubles their registers. The compiler does not
 // look into the statement for hazards: f may come from v_exp_f32 right before it (one wait state), and x from products of the tile before, which have ended: they stand
 // two barriers away, or in front of the products whose scores f comes from.
@@ -88,13 +61,6 @@ __device__ __forceinline__ void scale_in_place(f32x4& x, float f) {
   float a = x[0], b = x[1], c = x[2], d = x[3];
   asm("s_nop 1\n\tv_mul_f32 %0, %4, %0\n\tv_mul_f32 %1, %4, %1\n\tv_mul_f32 %2, %4, %2\n\tv_mul_f32 %3, %4, %3" : "+v"(a), "+v"(b), "+v"(c), "+v"(d) : "v"(f));
   x = f32x4{a, b, c, d};
-}
-
-// A wave-uniform address that the compiler formed in vector registers.
-__device__ __forceinline__ const char* scalar_pointer(const void* x) {
-  const uint64_t a = reinterpret_cast<uint64_t>(x);
-  const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)a), hi = __builtin_amdgcn_readfirstlane((uint32_t)(a >> 32));
-  return reinterpret_cast<const char*>((uint64_t)hi << 32 | lo);
 }
 
 // Where a score may exceed the reference of its row's weights, in bits, before the reference is moved: weights stay below 2^8, far from the end of

@@ -99,7 +99,7 @@ __device__ __forceinline__ int kv_offset(const KVAttnParams& p, int b) { return 
 // A workgroup's way through its range of the work list, segment by segment (steps of one row block). Every wave walks for itself; all of it is wave-uniform.
 template <int M>
 struct KVWalk {
-  static constexpr int kStart = 2, kLeast = 1;
+  static constexpr int kStart = 2;  // steps that a range may be longer
   int range, per, begin, at, end;  // this workgroup's range, its length, begin, place, end
   int seq, item, block, step;      // sequence, row blocks in front of it, row block, first step of the segment
   bool single;                     // one segment a range
@@ -183,7 +183,7 @@ struct KVWalk {
       per = total <= groups ? 1 : uniform((total + groups - 1) / groups);  // (divisions leave the scalar registers)
       if (blocks_total < groups && p.B <= 64 && total < 1 << 30) {  // (more sequences are not looked up twice)
         const int most = per + kStart;
-        int longer = max(per, kLeast);
+        int longer = per;
 #pragma unroll 1
         for (int ranges; longer <= most; longer = max(longer + 1, uniform((int)(longer * ((float)ranges / groups))))) {
           ranges = __builtin_amdgcn_readlane(wave_scan(k * (longer > 1 ? (x.steps + longer - 1) / longer : x.steps)), 63);

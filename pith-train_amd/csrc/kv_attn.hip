@@ -2,7 +2,6 @@
 #include "kv_attn.h"
 
 #include <algorithm>
-#include <type_traits>
 
 namespace pith {
 

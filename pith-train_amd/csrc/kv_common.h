@@ -27,6 +27,30 @@ inline KVCache to_device(const pith_kv_cache& c) {
   return d;
 }
 
+// A value of another lane of the row of 16.
+template <int CTRL>
+__device__ __forceinline__ float lane_dpp(float x) {
+  return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), CTRL, 0xf, 0xf, true));
+}
+constexpr int kDppXor1 = 0xB1, kDppXor2 = 0x4E, kDppHalfMirror = 0x141, kDppMirror = 0x140, kDppRotate8 = 0x128, kDppQuadMirror = 0x1B;
+// Over groups of 8 or 16 lanes; all of a group have the result. (Behind the first two steps lanes of a quad agree, so a mirrored half or row is as good as an
+// exchanged one.)
+template <int LANES, typename F>
+__device__ __forceinline__ float group_reduce(float x, const F& f) {
+  static_assert(LANES == 8 || LANES == 16, "rows of 64 or 128 features");
+  x = f(x, lane_dpp<kDppXor1>(x));
+  x = f(x, lane_dpp<kDppXor2>(x));
+  x = f(x, lane_dpp<kDppHalfMirror>(x));
+  if constexpr (LANES == 16) x = f(x, lane_dpp<kDppMirror>(x));
+  return x;
+}
+// Of the lane half a group away.
+template <int LANES>
+__device__ __forceinline__ float other_half(float x) {
+  if constexpr (LANES == 16) return lane_dpp<kDppRotate8>(x);
+  else return lane_dpp<kDppQuadMirror>(lane_dpp<kDppHalfMirror>(x));
+}
+
 // Token offsets count as their maximum so far, from 0 to T, so that whatever they hold no token belongs to two sequences. The offset of sequence b, by a whole
 // wavefront: the largest of the first b + 1, 256 of them under way at a time.
 __device__ __forceinline__ int offset_so_far(const int32_t* cu_q, int b, int T, int lane) {

@@ -313,6 +313,9 @@ __device__ __forceinline__ void clean_tile(char* tile, int w, int lane) {
   }
 }
 
+// A weight times its row's scale; 0 stays 0, also against a scale that is not finite.
+__device__ __forceinline__ float scaled(float weight, float scale) { return weight == 0.f ? 0.f : weight * scale; }
+
 // Scores x[0 .. N-1] of keys key0 .. against a row of token tok: those of keys that it does not see -> -infinity. In the last tiles of a sequence only, so
 // what a token sees is looked up anew there. (In words and without branches: hipcc 7.2 lost the selected score behind nested conditions on a shift of
 // 64 bits.)
@@ -349,6 +352,13 @@ __device__ __forceinline__ int lane_here() {
   int lane;
   asm volatile("v_mbcnt_lo_u32_b32 %0, -1, 0\n\tv_mbcnt_hi_u32_b32 %0, -1, %0" : "=v"(lane));
   return lane;
+}
+
+// A wave-uniform address that the compiler formed in vector registers.
+__device__ __forceinline__ const char* scalar_pointer(const void* x) {
+  const uint64_t a = reinterpret_cast<uint64_t>(x);
+  const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)a), hi = __builtin_amdgcn_readfirstlane((uint32_t)(a >> 32));
+  return reinterpret_cast<const char*>((uint64_t)hi << 32 | lo);
 }
 
 // Query rows row0 .. of the walk's row block into LDS, laid out like the rows of a bf16 tile of M keys: wave w brings rows 8 w .. 8 w + 7 (M = 16: the first
