@@ -29,7 +29,7 @@ class PagePool(NamedTuple):
 
 class StepPlan(NamedTuple):
     """What plan_step returns. cu_q [b + 1] int32: offsets of the requests' tokens; lengths [b] int32: cached rows behind the step; position_ids, slots [T]
-    int64; granted [b] int32: new rows that have pages; free_count [1] int32: of the pool behind the step."""
+    int64; granted [b] int32: new rows that have pages; free_count [1] int32: of the pool behind the step. They share one allocation: who keeps one for long clones it."""
 
     cu_q: torch.Tensor
     lengths: torch.Tensor
@@ -90,7 +90,8 @@ def plan_step(counts: torch.Tensor, lengths: torch.Tensor, page_table: torch.Ten
     pages that these need beyond those they have, from the top of the pool, where ended requests have just laid theirs; or none of them, where the pool does not suffice for
     a request or for one in front of it, or its table is too narrow: then granted is 0, the length stays and its tokens have slots of -1, which an append
     skips (what an attention to their requests gives them is of no use; other requests do not notice). Tokens behind the last request have position 0 and slot -1.
-    A page belongs to one request: one that two tables name would go back to the pool twice. page_table and pool.free are updated in place; lengths and pool.count are not: the
+    A request holds the ceil(length / page_size) first pages of its row: where lengths are lowered between steps (drafts that were not taken), the pages
+    behind those are the caller's to lay on the pool again, or to keep the length for. A page belongs to one request: one that two tables name would go back to the pool twice. page_table and pool.free are updated in place; lengths and pool.count are not: the
     values behind the step are in the result, and the same call again plans the same step (plan_step_into can write them back)."""
     return StepPlan(*_plan_op(counts, lengths, page_table, pool.free, pool.count, page_size, tokens))
 
