@@ -171,12 +171,13 @@ __global__ __launch_bounds__(kThreads) void kv_bounds_kernel(KVBoundsParams p) {
   const int sub = threadIdx.x % kLanes, group = threadIdx.x / kLanes;
   const int b = blockIdx.x, head = blockIdx.y;
   const int page_size = 1 << p.cache.page_shift;
-  const int length = min(max(p.lengths[b], 0), p.table_width << p.cache.page_shift);
-  int n = 1;
+  int cached, n;
   if (p.cu_q) {
-    const int end = min(max(p.cu_q[b + 1], 0), p.T), begin = offset_so_far(p.cu_q, b, p.T, threadIdx.x & 63);
-    n = max(end - begin, 0);
+    n = new_tokens(p.cu_q, b, p.T, p.lengths, threadIdx.x & 63, cached);
+  } else {
+    n = 1, cached = p.lengths[b];
   }
+  const int length = min(max(cached, 0), p.table_width << p.cache.page_shift);
   for (int i = (max(length - n, 0) >> p.cache.page_shift) + blockIdx.z; i < length >> p.cache.page_shift; i += gridDim.z) {
     const int64_t page = safe_page(p.table[b * p.table_rs + i], p.cache.pages);
     float lo[8], hi[8];

@@ -59,7 +59,9 @@ __device__ __forceinline__ Item item_of(const KVSelectParams& p, int item, int l
     x.seq = x.t, x.end = x.t + 1, x.length = p.lengths[x.t];
   } else {  // 64 sequences at a time: the first that ends behind the token, whose length has come along
     x.seq = p.B - 1, x.end = 0, x.length = 0;  // (a token that is nobody's sees nothing: in front of the first offset, or behind all)
-    const int first = p.cu_q[0];
+    int at_first = 0;
+    asm("" : "+v"(at_first));  // (by a vector load, which is under way together with those below)
+    const int first = p.cu_q[at_first];
     for (int b0 = 0; b0 < p.B; b0 += 64) {
       const int b = min(b0 + lane, p.B - 1), end = p.cu_q[b + 1], length = p.lengths[b];
       const uint64_t behind = __ballot(end > x.t);
@@ -69,7 +71,7 @@ __device__ __forceinline__ Item item_of(const KVSelectParams& p, int item, int l
         break;
       }
     }
-    if (x.t < first) x.end = 0, x.length = 0;
+    if (x.t < __builtin_amdgcn_readfirstlane(first)) x.end = 0, x.length = 0;
   }
   x.length = min(max(x.length, 0), p.table_width << p.page_shift);
   x.table = p.table + x.seq * p.table_rs;
