@@ -86,3 +86,36 @@ def test_native_and_python_bodies_agree(gpu, name):
     assert not called, f"an ordinary call went through the Python body of {called}"
     for x, y in zip(*results):
         assert torch.equal(x.view(torch.uint8), y.view(torch.uint8)) and x.dtype == y.dtype
+
+
+@G.BOTH
+@pytest.mark.parametrize("made_inside", [False, True])
+def test_steps_in_inference_mode(gpu, made_inside, fp8):
+    """The same rows and results as under no_grad, with tensors made inside or outside."""
+    g = torch.Generator().manual_seed(8)
+    qkv = torch.randn(3, 41, 8, 64, generator=g).to(BF).to(gpu)
+    cos, sin = (x.to(gpu) for x in G._tables(64))
+
+    def state():
+        cache = K.KVCache.empty(9, 2, 64, 16, G.L.FP8 if fp8 else BF, gpu)
+        for x in cache:
+            if x is not None:
+                x.view(torch.uint8).zero_()
+        return cache, cache.empty_bounds().zero_(), torch.full((2, 6), -1, dtype=I32, device=gpu), paging.PagePool.full(9, gpu), torch.zeros(2, dtype=I32, device=gpu)
+
+    def steps(cache, bounds, table, pool, lengths):
+        results = []
+        for i, counts in enumerate(([40, 1], [1, 17], [3, -1])):
+            plan = paging.plan_step(torch.tensor(counts, dtype=I32, device=gpu), lengths, table, pool, 16, 41)
+            lengths, pool = plan.lengths, paging.PagePool(pool.free, plan.free_count)
+            n = sum(max(c, 0) for c in counts)
+            o = K.kv_decode(*qkv[i].split((4, 2, 2), 1), None, None, cos, sin, plan.position_ids, plan.slots, cache, table, lengths, plan.cu_q, 0.125, bounds=bounds, keep=2)
+            results += [o[:n], *plan]
+        return results + [x for x in (*cache, bounds, table, pool.free) if x is not None]
+
+    with torch.no_grad():
+        want = steps(*state())
+    outside = state()
+    with torch.inference_mode():
+        got = steps(*(state() if made_inside else outside))
+    assert all(torch.equal(x.view(torch.uint8), y.view(torch.uint8)) for x, y in zip(got, want))
