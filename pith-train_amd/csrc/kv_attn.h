@@ -27,7 +27,7 @@
 // the tile still comes more slowly than that from memory.
 // Measured, heads of 32 / 4 with 128 features: 32 sequences of up to 8192 rows, bf16, one token each (303 MB) 64 us, 4.7 TB/s; 8 of up to 131072 rows, e4m3 (879 MB)
 // 160 us, 5.5 TB/s, where a copy reaches 4.9; 64 selected pages of 8 such sequences (34 MB) 15 us, of which the join's launch is 4 and beginnings and ends
-// about 4; one sequence of 517 rows 8.8 us, a launch and 5 steps of waiting for memory.
+// about 4; one sequence of 517 rows 9.7 us, a launch and 5 steps, each of which waits for memory.
 // The matrix cores take weights as bf16 beside a cache of bf16 (or e4m3, widened exactly; a weight then has its row's scale in it). In blocks of 16 rows, where these
 // products are few beside the bytes, a weight goes in as two numbers, its upper half and the rest rounded, and keeps 16 bits of its fraction: 2^-15 of it is lost at
 // most, and the outputs are off by what their own rounding does (norm of the difference from 64 bits by the norm: 0.0016; 0.0023 with one number). It takes, us with one

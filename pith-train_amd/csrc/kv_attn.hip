@@ -122,7 +122,7 @@ KVPlan plan_of(const pith_kv_attn_args* a) {
   const int per_unit = pl.row_groups <= 2 ? 2 : 1;  // workgroups (KVRing)
   pl.max_items = items(m);
   // No row block is cut where that would gain less than the join's launch costs (4 us), as long as all of them begin at once, and long ones do not share a compute unit: one
-  // sequence of 517 rows, 4 heads, 8.8 us whole and 10.6 cut, 8 x 1024 rows, 8 tokens 12 / 17, 23 x 71 rows (460 row blocks) 10 / 13; but 64 x 900 (384) 28 / 25, 86 x 2
+  // sequence of 517 rows, 4 heads, 8.8 us whole and 10.6 cut (with weights of 8 bits), 8 x 1024 rows, 8 tokens 12 / 17, 23 x 71 rows (460 row blocks) 10 / 13; but 64 x 900 (384) 28 / 25, 86 x 2
   // (688) 14.6 / 13.1.
   bool whole = (steps * pl.row_groups <= 8 && pl.max_items <= units) || (steps * pl.row_groups <= 2 && pl.max_items <= per_unit * units);
   pl.workgroups = std::min(per_unit * units, kMaxGroups);

@@ -13,8 +13,8 @@
 // A page of another size is in question by itself alone. Infinities and NaN have no bound of the error: a page with one is summed in fp64 at once. NaN counts above all.
 // Of equal scores all are in question. Up to 128 are ranked by comparing each with all; more by the bytes of their keys, a wave summing its own pages one after the
 // other: 8 tokens over 2000 pages of one score 370 us, over 16000 2450 (18 and 70 where scores differ); one such token holds the call up.
-// All of it is latency: 32 tokens with heads of 32 / 4 over up to 128 pages 12 us, one launch; 8 over up to 2048 pages 23 us, three launches with the
-// bounds of the pages that the step filled: scores 8 (27 MB of bounds, 3.4 TB/s; four loads that wait for each other begin it), the choice 7 to 9 (1 until it knows what
+// All of it is latency: 32 tokens with heads of 32 / 4 over up to 128 pages 12 us, one launch; 8 over up to 2048 pages 24 us, three launches with the
+// bounds of the pages that the step filled: scores 10 (27 MB of bounds, 2.7 TB/s; four loads that wait for each other begin it), the choice 7 to 9 (1 until it knows what
 // it is about, 0.5 for the scores, 2.3 for the histograms, 1.3 for the few pages in fp64, 1.6 to rank and write).
 #include "cache_attn.h"
 #include "kv_common.h"
