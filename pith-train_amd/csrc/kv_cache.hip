@@ -7,6 +7,8 @@
 #include "cache_attn.h"
 #include "kv_common.h"
 
+#include <algorithm>
+
 namespace pith {
 namespace {
 
@@ -162,6 +164,42 @@ struct KVBoundsParams {
 __device__ __forceinline__ float least(float a, float b) { return __builtin_elementwise_minimum(a, b); }
 __device__ __forceinline__ float largest(float a, float b) { return __builtin_elementwise_maximum(a, b); }
 
+// Pages first .. last - 1 of sequence b that its new tokens filled. Token offsets count as their maximum so far, from 0 to T, so that whatever they hold no token belongs
+// to two sequences: the largest of the first b + 1, by a whole wavefront, 256 of them at a time, and more than that only if those and the sequence's own two do not say already
+// that there is no page (they can only say too many).
+struct Filled {
+  int first, last;
+};
+__device__ __forceinline__ Filled filled_pages(const KVBoundsParams& p, int b, int lane) {
+  const int shift = p.cache.page_shift;
+  const auto pages = [&](int cached, int n) __attribute__((always_inline)) {
+    const int length = min(max(cached, 0), p.table_width << shift);
+    return Filled{max(length - n, 0) >> shift, length >> shift};
+  };
+  if (!p.cu_q) return pages(p.lengths[b], 1);
+  const auto load = [&](int i0, int (&x)[4]) __attribute__((always_inline)) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) x[k] = p.cu_q[min(i0 + 64 * k + lane, b)];
+  };
+  int x[4], end = p.cu_q[b + 1], most = p.cu_q[b], cached = p.lengths[b];
+  load(0, x);
+  asm volatile("" : "+s"(end), "+s"(most), "+s"(cached), "+v"(x[0]), "+v"(x[1]), "+v"(x[2]), "+v"(x[3]));  // one wait for all of them, not one each where they are used
+  const auto by = [&](int most_) __attribute__((always_inline)) {
+    const int begin = __builtin_amdgcn_readlane(wave_scan_max(max(max(max(x[0], x[1]), max(x[2], x[3])), max(most_, 0))), 63);
+    return pages(cached, max(min(max(end, 0), p.T) - min(begin, p.T), 0));
+  };
+  Filled f = by(most);
+  if (b >= 256 && f.first < f.last) {
+    int more = max(max(x[0], x[1]), max(x[2], x[3]));
+    for (int i0 = 256; i0 <= b; i0 += 256) {
+      load(i0, x);
+      more = max(more, max(max(x[0], x[1]), max(x[2], x[3])));
+    }
+    f = by(more);
+  }
+  return f;
+}
+
 // blockIdx.x: sequence, blockIdx.y: key-value head, blockIdx.z: every how many-th of the pages that its new tokens filled. A group of lanes takes every
 // 256 / kLanes-th row; what the groups found meets in LDS.
 template <int D, bool FP8>
@@ -171,14 +209,8 @@ __global__ __launch_bounds__(kThreads) void kv_bounds_kernel(KVBoundsParams p) {
   const int sub = threadIdx.x % kLanes, group = threadIdx.x / kLanes;
   const int b = blockIdx.x, head = blockIdx.y;
   const int page_size = 1 << p.cache.page_shift;
-  int cached, n;
-  if (p.cu_q) {
-    n = new_tokens(p.cu_q, b, p.T, p.lengths, threadIdx.x & 63, cached);
-  } else {
-    n = 1, cached = p.lengths[b];
-  }
-  const int length = min(max(cached, 0), p.table_width << p.cache.page_shift);
-  for (int i = (max(length - n, 0) >> p.cache.page_shift) + blockIdx.z; i < length >> p.cache.page_shift; i += gridDim.z) {
+  const Filled filled = filled_pages(p, b, threadIdx.x & 63);
+  for (int i = filled.first + blockIdx.z; i < filled.last; i += gridDim.z) {
     const int64_t page = safe_page(p.table[b * p.table_rs + i], p.cache.pages);
     float lo[8], hi[8];
 #pragma unroll
@@ -305,7 +337,10 @@ extern "C" int pith_kv_bounds(const pith_kv_bounds_args* a, pith_stream_t stream
   p.table_rs = a->B > 1 ? a->table_rs : 0; p.bounds_ps = c.pages > 1 ? a->bounds_ps : 0;
   p.T = (int)a->T; p.table_width = (int)a->table_width;
   const int64_t most = a->T / c.page_size + 1;  // pages that the tokens of one sequence can fill
-  const dim3 grid((unsigned)a->B, (unsigned)c.heads, (unsigned)(most < 64 ? most : 64));
+  // Workgroups of a sequence and head, which share its pages: up to 64 where there are few of them, 8 where they are thousands, one each of which could be a prompt (us of a
+  // decoding step over heads of 128, 4 of them, 1024 sequences, with 17 / 8 19 / 10, 4096 with 64 / 8 262 / 36).
+  const int64_t z = std::max<int64_t>(4096 / (a->B * c.heads), 8);
+  const dim3 grid((unsigned)a->B, (unsigned)c.heads, (unsigned)std::min<int64_t>({most, z, 64}));
   hipStream_t s = (hipStream_t)stream;
   begin_launch();
   const bool fp8 = c.dtype == PITH_FP8_E4M3;

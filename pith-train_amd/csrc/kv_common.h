@@ -51,27 +51,6 @@ __device__ __forceinline__ float other_half(float x) {
   else return lane_dpp<kDppQuadMirror>(lane_dpp<kDppHalfMirror>(x));
 }
 
-// Token offsets count as their maximum so far, from 0 to T, so that whatever they hold no token belongs to two sequences. The new tokens of sequence b, by a whole
-// wavefront, from the largest of the first b + 1 offsets, 256 of them at a time; its cached rows, as they stand in `lengths`, come along.
-__device__ __forceinline__ int new_tokens(const int32_t* cu_q, int b, int T, const int32_t* lengths, int lane, int& cached) {
-  const auto most_of = [&](const int (&x)[4]) __attribute__((always_inline)) { return max(max(x[0], x[1]), max(x[2], x[3])); };
-  const auto load = [&](int i0, int (&x)[4]) __attribute__((always_inline)) {
-#pragma unroll
-    for (int k = 0; k < 4; ++k) x[k] = cu_q[min(i0 + 64 * k + lane, b)];
-  };
-  int x[4], end = cu_q[b + 1];
-  cached = lengths[b];
-  load(0, x);
-  asm volatile("" : "+s"(end), "+s"(cached), "+v"(x[0]), "+v"(x[1]), "+v"(x[2]), "+v"(x[3]));  // one wait for all of them, not one each where they are used
-  int most = max(most_of(x), 0);
-  for (int i0 = 256; i0 <= b; i0 += 256) {
-    load(i0, x);
-    most = max(most, most_of(x));
-  }
-  const int begin = min(__builtin_amdgcn_readlane(wave_scan_max(most), 63), T);
-  return max(min(max(end, 0), T) - begin, 0);
-}
-
 // Sizes of pages, heads and features, of a cache or of the bounds beside one.
 inline int check_pages(int64_t pages, int64_t page_size, int64_t heads, int64_t dim, const char* who) {
   if (page_size < 16 || page_size > 65536 || (page_size & (page_size - 1)))

@@ -135,6 +135,26 @@ def test_offsets_count_as_their_maximum_so_far_in_all_operators(gpu, offsets, sa
     assert (chosen[~mine] == -1).all() and (rows[~mine] == 0).all() and (o[~mine] == 7).all() and (chosen[mine] >= 0).all() and (o[mine] != 7).any()
 
 
+@G.BOTH
+@pytest.mark.parametrize("b, prompt", [(1, 1500), (700, 1500), (700, 200), (1500, 40)])
+def test_bounds_of_a_prompt_among_many_sequences(gpu, b, prompt, fp8):
+    """More pages than workgroups of a sequence, behind more sequences than are looked at together."""
+    page, at = 16, b - 1
+    counts = [1] * b
+    counts[at] = prompt
+    lengths = [1 + (5 * i) % 40 for i in range(b)]
+    lengths[at] = prompt + 21
+    x = G.Batch(gpu, counts, lengths, (4, 2, 64), page=page, fp8=fp8, seed=b)
+    bounds = torch.full_like(x.cache.empty_bounds(), 3.0)
+    K.kv_page_bounds(x.cache, bounds, x.table, x.lens, x.cu_q, sum(counts))
+    filled = torch.cat([x.table[i, (n - c) // page : n // page].cpu() for i, (c, n) in enumerate(zip(counts, lengths))]).long()
+    keys = x.kv[0][filled.to(gpu)].float() * (1.0 if x.scales[0] is None else x.scales[0][filled.to(gpu)][..., None])
+    assert len(filled) > prompt // page and torch.equal(bounds[filled.to(gpu)], torch.stack((keys.amin(2), keys.amax(2)), 2).to(BF))
+    others = torch.ones(len(bounds), dtype=torch.bool)
+    others[filled] = False
+    assert (bounds[others.to(gpu)] == 3).all()
+
+
 # ---------------------------------------------------------------------------------------------
 # Many tokens
 
